@@ -1,4 +1,5 @@
-"""ctypes binding of libcertex_c.so, the C API of the index (include/cuvs/neighbors/certex.h).
+"""ctypes binding of libcertex_c.so, the C API of the index (include/cuvs/neighbors/certex.h) and of the
+attention operators (include/cuvs/neighbors/certex_attention.h).
 
 Python reaches the index only through these C entry points; tensors cross as DLPack v1.0 structs
 that borrow torch's memory (no deleter is called). The library must have been built
@@ -7,6 +8,7 @@ that borrow torch's memory (no deleter is called). The library must have been bu
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -71,6 +73,20 @@ class IndexParams(ctypes.Structure):
 
 class SearchParams(ctypes.Structure):
     _fields_ = [("anchors", ctypes.c_int32), ("batch_size", ctypes.c_int32), ("probe_lists", ctypes.c_int32)]
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("rotary_dim", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("base", ctypes.c_double),
+        ("scaling", ctypes.c_int32),
+        ("factor", ctypes.c_double),
+        ("original_length", ctypes.c_double),
+        ("ramp_low", ctypes.c_double),
+        ("ramp_high", ctypes.c_double),
+        ("magnitude", ctypes.c_double),
+    ]
 
 
 class IndexHandle(ctypes.Structure):
@@ -182,6 +198,21 @@ def lib():
                     "cuvsCertexTimingBegin": [],
                     "cuvsCertexTimingEnd": [P(ctypes.c_double), P(i64)],
                 }
+                st = ctypes.c_size_t
+                sig |= {
+                    "cuvsCertexRotaryParamsCreate": [P(P(RotaryParams))],
+                    "cuvsCertexRotaryParamsDestroy": [P(RotaryParams)],
+                    "cuvsCertexRotaryFrequencies": [P(RotaryParams), P(ctypes.c_double), P(ctypes.c_double)],
+                    "cuvsCertexRotaryCreate": [st, P(RotaryParams), P(st)],
+                    "cuvsCertexRotaryDestroy": [st],
+                    # tensors as addresses of DLManagedTensors (views())
+                    "cuvsCertexRotate": [st, st, vp, vp, vp, ctypes.c_bool],
+                    "cuvsCertexAppendPages": [st, st] + [vp] * 9,
+                    "cuvsCertexPagedAttentionWorkspace": [vp, vp, vp, vp, i64, P(i64)],
+                    "cuvsCertexPagedAttention": [st] + [vp] * 5 + [ctypes.c_float, i64] + [vp] * 3,
+                    "cuvsCertexSelectedAttentionWorkspace": [vp, vp, vp, P(i64)],
+                    "cuvsCertexSelectedAttention": [st] + [vp] * 4 + [ctypes.c_float] + [vp] * 3,
+                }
                 for name, args in sig.items():
                     fn = getattr(L, name)
                     fn.argtypes = args
@@ -231,6 +262,41 @@ class Borrowed:
 
 
 _tls = threading.local()
+
+_VIEW = struct.Struct("=QiiiBBHQQQQQ4q4q")  # a DLManagedTensor, then its extents and strides
+_VIEWS = 12  # of a call
+
+
+class _Views:
+    """DLManagedTensors of one call's tensors, strides included, written into memory of the calling thread
+    that the next call reuses: a fraction of the time that ctypes structures take to fill."""
+
+    def __init__(self):
+        self.buffer = ctypes.create_string_buffer(_VIEWS * _VIEW.size)
+        self.base, self.n = ctypes.addressof(self.buffer), 0
+
+    def __call__(self, t):
+        """The address of a tensor of the caller's (None: NULL), valid until the thread's next views()."""
+        if t is None:
+            return None
+        at = self.n * _VIEW.size
+        self.n += 1
+        address, ndim = self.base + at, t.ndim
+        code, bits = _DL[t.dtype]
+        pad = (0,) * (4 - ndim)
+        device = t.device
+        _VIEW.pack_into(self.buffer, at, t.data_ptr(), kDLROCM if t.is_cuda else kDLCPU, device.index or 0, ndim, code,
+                        bits, 1, address + 64, address + 96, 0, 0, 0, *t.shape, *pad, *t.stride(), *pad)
+        return address
+
+
+def views():
+    """The calling thread's _Views, empty."""
+    v = getattr(_tls, "views", None)
+    if v is None:
+        v = _tls.views = _Views()
+    v.n = 0
+    return v
 
 
 def resources():

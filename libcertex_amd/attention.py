@@ -8,6 +8,7 @@ on equal scores, the lower key id first.
 import torch
 
 from .index import Index, _require
+from .paged import selected_attention
 
 def _stride(n, k):
     """An anchor stride between 1 and 16 (the reference picks one from n and k,
@@ -167,6 +168,14 @@ class KeyCache:
         scores = D.reshape(H, m, k)
         ids = I.reshape(H, m, k)
         return (scores[:, 0], ids[:, 0]) if single else (scores, ids)
+
+    def attend(self, q, values, k=None, scale=None, page_table=None, batch=None):
+        """Sparse attention: softmax over the exact top k of every query, times the values of those keys. q as in
+        topk; values (n_kv_heads, n, value_dim) in key order, or with page_table the pages of this sequence (see
+        selected_attention); scale defaults to head_dim ** -0.5. Returns (n_heads, m, value_dim) or (n_heads, value_dim)
+        in the values' type."""
+        scores, ids = self.topk(q, k, batch)
+        return selected_attention(scores, ids, values, self.head_dim**-0.5 if scale is None else scale, page_table)
 
 
 def topk(q, keys, k):

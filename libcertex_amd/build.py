@@ -26,6 +26,10 @@ SOURCES = [
     "kernels/encode.hip",
     "kernels/partition.hip",
     "kernels/lists.hip",
+    "attention/rotate.hip",
+    "attention/attend.hip",
+    "attention/select.hip",
+    "attention/c_api.cpp",
     "device_memory.cpp",
     "certex.cpp",
     "c_api.cpp",

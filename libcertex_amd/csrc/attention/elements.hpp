@@ -1,0 +1,30 @@
+// Elements of the attention operators' tensors: float32, float16 and bfloat16, computed in float32.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace certex_amd::attention {
+
+using f16_t  = _Float16;
+using bf16_t = __bf16;
+
+/** N elements that one load or store moves. */
+template <typename T, int N>
+struct alignas(sizeof(T) * N) pack {
+  T e[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ pack<T, N> load(const T* p)
+{
+  return *reinterpret_cast<const pack<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, pack<T, N> const& v)
+{
+  *reinterpret_cast<pack<T, N>*>(p) = v;
+}
+
+}  // namespace certex_amd::attention

@@ -1,0 +1,180 @@
+// Rotation by position, and its fusion with the append to a paged cache.
+//
+// Position p turns pair i of a head by the angle p f_i: (a, b) -> m (a cos - b sin, a sin + b cos).
+// The frequencies are kept in turns as 64-bit fixed point, so p f_i modulo one turn is the low half
+// of one integer product: exact for every position, where a float32 product loses the angle (at
+// position 131,072 it is 0.008 radians off), and nothing is read from a table. The top 32 bits of
+// the fraction go to sin and cos of half turns: the angle is within 2^-24 of itself.
+#include "attention.hpp"
+#include "elements.hpp"
+
+#include <algorithm>
+#include <numeric>
+#include <stdexcept>
+
+namespace certex_amd::attention {
+namespace {
+
+constexpr int kThreads = 256;
+
+/**
+ * One thread: one vector of V elements of a row (of both halves in the half layout), over
+ * heads_per_thread heads of one token. Blocks are dealt to the jobs in order.
+ */
+template <typename T, int V, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
+{
+  int64_t block = blockIdx.x;
+  int j         = 0;
+  while (j + 1 < a.jobs && block >= a.job[j].blocks) { block -= a.job[j++].blocks; }
+  const turn_job& b = a.job[j];
+  const uint64_t at = uint64_t(block) * kThreads + threadIdx.x;
+  uint32_t item, group;
+  uint64_t token;
+  if (b.blocks < (int64_t(1) << 23)) {  // 32-bit quotients
+    const uint32_t row = uint32_t(at) / uint32_t(b.items);
+    item               = uint32_t(at) - row * uint32_t(b.items);
+    token              = row / uint32_t(b.groups);
+    group              = row - uint32_t(token) * uint32_t(b.groups);
+  } else {
+    const uint64_t row = at / uint64_t(b.items);
+    item               = uint32_t(at - row * uint64_t(b.items));
+    token              = row / uint64_t(b.groups);
+    group              = uint32_t(row - token * uint64_t(b.groups));
+  }
+  if (token >= uint64_t(a.tokens)) { return; }
+  const uint64_t outer = a.inner == a.tokens ? 0 : token / uint64_t(a.inner);
+  const uint64_t inner = token - outer * uint64_t(a.inner);
+  const int64_t p      = a.positions[int64_t(token)];
+
+  const T* src = static_cast<const T*>(b.src) + int64_t(outer) * b.src_outer + int64_t(inner) * b.src_token;
+  T* dst       = static_cast<T*>(b.dst);
+  if (b.paged) {
+    const int64_t s = a.sequences.p != nullptr ? a.sequences[int64_t(token)] : int64_t(token);
+    if (s < 0 || s >= a.pages.sequences || p < 0 || p >= int64_t(a.pages.width) * a.pages.page) { return; }
+    const uint32_t entry = uint32_t(p) / uint32_t(a.pages.page);
+    const uint32_t slot  = uint32_t(p) - entry * uint32_t(a.pages.page);
+    const int32_t page   = a.pages.table[s * a.pages.width + entry];
+    if (page < 0 || page >= a.pages.n_pages) { return; }
+    dst += int64_t(page) * b.dst_outer + int64_t(slot) * b.dst_token;
+  } else {
+    dst += int64_t(outer) * b.dst_outer + int64_t(inner) * b.dst_token;
+  }
+  const int h0 = int(group) * a.heads_per_thread;
+  const int h1 = min(h0 + a.heads_per_thread, b.heads);
+
+  if (item >= uint32_t(b.turned)) {  // the rest of the row
+    const int at_row = b.rotary + int(item - uint32_t(b.turned)) * V;
+#pragma unroll 4
+    for (int h = h0; h < h1; ++h) {
+      store<T, V>(dst + h * b.dst_head + at_row, load<T, V>(src + h * b.src_head + at_row));
+    }
+    return;
+  }
+  constexpr int P = INTERLEAVED ? (V > 1 ? V / 2 : 1) : V;  // pairs of a thread
+  float c[P], s[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const uint64_t turns = uint64_t(p) * a.frequencies[int(item) * P + i];
+    sincospif(float(int32_t(turns >> 32)) * 0x1p-31f, &s[i], &c[i]);
+    c[i] *= a.magnitude;
+    s[i] *= a.transpose ? -a.magnitude : a.magnitude;
+  }
+  if constexpr (INTERLEAVED && V > 1) {
+    const int at_row = int(item) * V;
+#pragma unroll 4
+    for (int h = h0; h < h1; ++h) {
+      auto x = load<T, V>(src + h * b.src_head + at_row);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float u = float(x.e[2 * i]), w = float(x.e[2 * i + 1]);
+        x.e[2 * i]     = T(__builtin_fmaf(u, c[i], -(w * s[i])));
+        x.e[2 * i + 1] = T(__builtin_fmaf(u, s[i], w * c[i]));
+      }
+      store<T, V>(dst + h * b.dst_head + at_row, x);
+    }
+  } else {
+    const int first  = INTERLEAVED ? int(item) * 2 : int(item) * V;
+    const int second = INTERLEAVED ? first + 1 : first + b.rotary / 2;
+#pragma unroll 4
+    for (int h = h0; h < h1; ++h) {
+      auto x = load<T, V>(src + h * b.src_head + first);
+      auto y = load<T, V>(src + h * b.src_head + second);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float u = float(x.e[i]), w = float(y.e[i]);
+        x.e[i] = T(__builtin_fmaf(u, c[i], -(w * s[i])));
+        y.e[i] = T(__builtin_fmaf(u, s[i], w * c[i]));
+      }
+      store<T, V>(dst + h * b.dst_head + first, x);
+      store<T, V>(dst + h * b.dst_head + second, y);
+    }
+  }
+}
+
+template <typename T, int V, bool INTERLEAVED>
+void launch(turn_args& a, hipStream_t stream)
+{
+  int64_t blocks = 0, threads = 0;
+  for (int j = 0; j < a.jobs; ++j) {
+    turn_job& b = a.job[j];
+    // pairs of a thread: V of the half layout, V / 2 interleaved ones (V = 1: one pair)
+    b.turned = INTERLEAVED && V > 1 ? b.rotary / V : b.rotary / 2 / V;
+    b.items  = b.turned + (b.dim - b.rotary) / V;
+    threads += a.tokens * b.heads * b.items;
+  }
+  // one thread computes its sines and cosines once for up to 8 heads, unless that would leave
+  // fewer threads than the chip holds
+  a.heads_per_thread = int32_t(std::clamp<int64_t>(threads / (256 * 2048), 1, 8));
+  for (int j = 0; j < a.jobs; ++j) {
+    turn_job& b = a.job[j];
+    b.groups    = (b.heads + a.heads_per_thread - 1) / a.heads_per_thread;
+    b.blocks    = (a.tokens * b.groups * b.items + kThreads - 1) / kThreads;
+    blocks += b.blocks;
+  }
+  if (blocks >= (int64_t(1) << 24)) { throw std::invalid_argument("certex: too many elements to rotate in one call"); }
+  if (blocks > 0) { turn_kernel<T, V, INTERLEAVED><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a); }
+}
+
+template <typename T, int V>
+void launch(turn_args& a, hipStream_t stream)
+{
+  a.interleaved ? launch<T, V, true>(a, stream) : launch<T, V, false>(a, stream);
+}
+
+}  // namespace
+
+void turn(elem type, turn_args a, hipStream_t stream)
+{
+  // the widest vectors that every row, stride and base address is a multiple of
+  const int size = elem_bytes(type);
+  int64_t g      = 16 / size;
+  for (int j = 0; j < a.jobs; ++j) {
+    turn_job const& b = a.job[j];
+    for (int64_t x : {b.src_outer, b.src_token, b.src_head, b.dst_outer, b.dst_token, b.dst_head, int64_t(b.dim),
+                      a.interleaved ? int64_t(b.rotary) : int64_t(b.rotary / 2),
+                      int64_t(reinterpret_cast<uintptr_t>(b.src) / size),
+                      int64_t(reinterpret_cast<uintptr_t>(b.dst) / size)}) {
+      g = std::gcd(g, x);
+    }
+  }
+  const auto by_width = [&](auto tag) {
+    using T = decltype(tag);
+    if (g == 8) {
+      if constexpr (sizeof(T) == 2) { launch<T, 8>(a, stream); }
+    } else if (g == 4) {
+      launch<T, 4>(a, stream);
+    } else if (g == 2) {
+      launch<T, 2>(a, stream);
+    } else {
+      launch<T, 1>(a, stream);
+    }
+  };
+  switch (type) {
+    case elem::f32: by_width(float{}); break;
+    case elem::f16: by_width(f16_t{}); break;
+    case elem::bf16: by_width(bf16_t{}); break;
+  }
+}
+
+}  // namespace certex_amd::attention

@@ -53,6 +53,24 @@ auto resources::stream() const -> void* { return s_->stream; }
 
 void resources::set_stream(void* stream)
 {
+  // The scratch passes from one stream to the next, which waits for it. A stream that records a graph
+  // is not given it (a search waits on the host and cannot be recorded), and a wait here would break
+  // the recording: the stream before it is waited for by the first change after.
+  hipStreamCaptureStatus recording = hipStreamCaptureStatusNone;
+  if (stream != nullptr && !s_->owns_stream &&
+      hipStreamIsCapturing(static_cast<hipStream_t>(stream), &recording) != hipSuccess) {
+    (void)hipGetLastError();
+    recording = hipStreamCaptureStatusNone;
+  }
+  if (recording == hipStreamCaptureStatusActive) {
+    if (!s_->before_recording) { s_->before_recording = s_->stream; }
+    s_->stream = static_cast<hipStream_t>(stream);
+    return;
+  }
+  if (s_->before_recording) {
+    CERTEX_HIP_TRY(hipStreamSynchronize(*s_->before_recording));
+    s_->before_recording.reset();
+  }
   CERTEX_HIP_TRY(hipStreamSynchronize(s_->stream));
   if (s_->owns_stream) {
     CERTEX_HIP_TRY(hipStreamDestroy(s_->stream));
