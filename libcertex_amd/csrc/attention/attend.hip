@@ -1,8 +1,27 @@
 // Attention of one new token of every sequence over its pages of keys and values.
 //
-// out = sum_t p_t v_t / sum_t p_t with p_t = exp(scale q.k_t - m), m the largest exponent, over the
-// positions t of [max(0, len - window), len). One pass over the positions keeps m, the sum and the
+// out = sum_t p_t v_t / sum_t p_t with p_t = 2^(x_t - m), x_t = scale log2(e) q.k_t, over the positions t
+// of [max(0, len - window), len). One pass over the positions keeps a reference m, the sum and the
 // output in float32, and scales the last two where m grows.
+//
+// What bounds it: every key and value is read once and used by the heads / kv_heads query heads that share
+// it, a few operations per byte, so the rate at which memory is read. The kernel keeps the two products
+// off the critical path by giving them to the matrix cores in a form that needs no exchange between lanes
+// and no LDS:
+// - a wave takes 32 positions; S^T = K Q^T has the positions as rows and up to 16 query heads as columns, so that
+//   K rows go from memory to the operand registers as they lie (16 bytes of a row per lane);
+// - the rows of the two 16-position products are permuted such that a lane's 8 results are the 8
+//   consecutive positions that it holds as k-slots of O^T = V^T P^T: the weights never move;
+// - V^T is formed in registers: a lane loads 8 positions x 8 columns (16 bytes of a row each, whole rows per 16
+//   lanes) and swaps halfwords (v_perm), 32 instructions per 32 x 128 values;
+// - m, the sum and the scaling are per query head, that is per lane.
+// The loads of the next keys and of this tile's values are in flight during both products.
+//
+// Work is dealt on the device, from the lengths: tiles of 128 positions (32 per wave) of all sequences
+// and heads, in order, in equal shares to the workgroups, so that any mix of lengths fills the chip and the host reads
+// nothing back. A share that cuts a row of work leaves a partial (m, sum, output) in the workspace, and a second
+// launch joins them in order of position.
+#include "../kernels/lanes.hpp"
 #include "attention.hpp"
 #include "elements.hpp"
 
@@ -11,82 +30,585 @@
 namespace certex_amd::attention {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWaves   = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kTile    = 32;              // positions of a wave's step
+constexpr int kStep    = kTile * kWaves;  // of a workgroup's
+constexpr int kRows    = 16;              // query heads of a product
+constexpr int kShares  = 512;             // workgroups: two per compute unit at most
+constexpr float kLog2e = 1.44269504088896340736f;
 
-/** One workgroup per sequence and query head: 256 positions at a time, one per thread. */
-template <typename T>
-__global__ __launch_bounds__(kThreads) void attend_kernel(attend_args a)
+using f32x4  = __attribute__((ext_vector_type(4))) float;
+using u32x4  = __attribute__((ext_vector_type(4))) uint32_t;
+using u32x2  = __attribute__((ext_vector_type(2))) uint32_t;
+using f16x8  = __attribute__((ext_vector_type(8))) _Float16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+
+/** n / d for n < 2^28 by a product: m = ceil(2^(28 + s) / d) with 2^s >= d exceeds 2^(28 + s) / d by less than 1, so the
+ *  quotient's error n (m d - 2^(28 + s)) / d stays below 1 / d. */
+struct divisor {
+  uint32_t m, shift, d;
+  explicit divisor(uint32_t by) : d(by)
+  {
+    uint32_t s = 0;
+    while ((uint64_t(1) << s) < by) { ++s; }
+    shift = 28 + s;
+    m     = uint32_t(((uint64_t(1) << shift) + by - 1) / by);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> shift); }
+};
+
+struct attend_plan {
+  divisor page8;      // groups of 8 positions per page
+  int32_t row_tiles;  // products of 16 query heads per key head
+  int32_t group;      // query heads per key head
+  int32_t tables;     // key heads x row_tiles
+  int32_t shares;     // at most
+  float scale2;       // scale log2(e)
+  float* part_out;    // [2 kShares][kRows][vdim]
+  float* part_max;    // [2 kShares][kRows]
+  float* part_sum;
+};
+
+/** Positions [begin, end) of a sequence, and its tiles of kStep from begin rounded down to 8. */
+struct span {
+  int32_t begin, end, tiles;
+};
+
+__device__ __forceinline__ span span_of(attend_args const& a, int64_t b)
 {
-  __shared__ float s_q[kMaxHeadDim];
-  __shared__ float s_p[kThreads];
-  __shared__ int64_t s_v[kThreads];
-  __shared__ float s_part[kThreads / 64];
-  const int h = blockIdx.x, g = h / (a.heads / a.kv_heads), tid = threadIdx.x;
-  const int64_t b = blockIdx.y;
-  const T* q      = static_cast<const T*>(a.q) + b * a.q_seq + h * a.q_head;
-  for (int i = tid; i < a.dim; i += kThreads) { s_q[i] = float(q[i]); }
-  int64_t end         = a.lengths[b];
-  end                 = end < 0 ? 0 : min(end, int64_t(a.pages.width) * a.pages.page);
+  int64_t end = a.lengths[b];
+  end         = end < 0 ? 0 : min(end, int64_t(a.pages.width) * a.pages.page);
+  if (a.pages.n_pages == 0) { end = 0; }
   const int64_t begin = a.window > 0 && end > a.window ? end - a.window : 0;
-  float top = -INFINITY, total = 0.0f, acc = 0.0f;
-  for (int64_t t0 = begin; t0 < end; t0 += kThreads) {
-    const int64_t t = t0 + tid;
-    float x         = -INFINITY;
-    int64_t v_at    = -1;
-    __syncthreads();
-    if (t < end) {
-      const int32_t page = a.pages.table[b * a.pages.width + t / a.pages.page];
-      if (page >= 0 && page < a.pages.n_pages) {
-        const int64_t slot = t % a.pages.page;
-        const T* k = static_cast<const T*>(a.k) + page * a.k_page + slot * a.k_slot + g * a.k_head;
-        v_at       = page * a.v_page + slot * a.v_slot + g * a.v_head;
-        float dot  = 0.0f;
-        for (int i = 0; i < a.dim; ++i) { dot = __builtin_fmaf(s_q[i], float(k[i]), dot); }
-        x = dot * a.scale;
-      }
-    }
-    float m = x;
-    for (int d = 32; d > 0; d /= 2) { m = fmaxf(m, __shfl_xor(m, d)); }
-    if (tid % 64 == 0) { s_part[tid / 64] = m; }
-    __syncthreads();
-    m                 = fmaxf(fmaxf(s_part[0], s_part[1]), fmaxf(s_part[2], s_part[3]));
-    const float grown = fmaxf(top, m);
-    const float base  = grown == -INFINITY ? 0.0f : grown;
-    const float keep  = expf(top - base);  // 0 at first
-    const float p     = expf(x - base);
-    s_p[tid]          = p;
-    s_v[tid]          = v_at;
-    float sum         = p;
-    for (int d = 32; d > 0; d /= 2) { sum += __shfl_xor(sum, d); }
-    __syncthreads();
-    if (tid % 64 == 0) { s_part[tid / 64] = sum; }
-    __syncthreads();
-    total = total * keep + ((s_part[0] + s_part[1]) + (s_part[2] + s_part[3]));
-    top   = grown;
-    if (tid < a.vdim) {
-      acc         = acc * keep;
-      const int n = int(min(int64_t(kThreads), end - t0));
-      for (int i = 0; i < n; ++i) {
-        if (s_v[i] >= 0) { acc = __builtin_fmaf(s_p[i], float(static_cast<const T*>(a.v)[s_v[i] + tid]), acc); }
+  return {int32_t(begin), int32_t(end), int32_t((end - (begin & ~int64_t(7)) + kStep - 1) / kStep)};
+}
+
+/** All tiles of the call (the same on every lane). */
+__device__ __forceinline__ int64_t count_tiles(attend_args const& a)
+{
+  int64_t mine = 0;
+  for (int64_t b = threadIdx.x % 64; b < a.pages.sequences; b += 64) { mine += span_of(a, b).tiles; }
+  return lanes::sum<64>(mine);
+}
+
+/** The shares: share w takes the units [w units / n, (w + 1) units / n). */
+struct shares {
+  int64_t units, n;
+  __device__ __forceinline__ int64_t first(int64_t w) const { return w * units / n; }
+  __device__ __forceinline__ int64_t of(int64_t unit) const { return ((unit + 1) * n - 1) / units; }
+};
+
+__device__ __forceinline__ shares shares_of(attend_args const& a, attend_plan const& p)
+{
+  const int64_t units = count_tiles(a) * p.tables;
+  return {units, min(int64_t(p.shares), units)};
+}
+
+/** The elements of a lane's piece: 16 bytes of a row at any alignment of the elements (the memory takes
+ *  misaligned vector loads); TINY rows are shorter than a piece and read element by element. */
+template <typename T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) loose {
+  T e[N];
+};
+
+template <int BYTES, typename T>
+__device__ __forceinline__ auto piece(const T* p)
+{
+  if constexpr (BYTES == 16) {
+    u32x4 v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, sizeof(T)), 16);
+    return v;
+  } else {
+    u32x2 v;
+    __builtin_memcpy(&v, __builtin_assume_aligned(p, sizeof(T)), 8);
+    return v;
+  }
+}
+
+/** Keys, queries and values of a wave's step for elements T, head dimensions up to D. */
+template <typename T, int D>
+struct geometry {
+  static constexpr bool kWide = sizeof(T) == 4;
+  static constexpr int kPiece  = kWide ? 4 : 8;           // elements of a key piece (16 bytes)
+  static constexpr int kChunk  = 4 * kPiece;              // dimensions of a product's four lane groups
+  static constexpr int kChunks = D / kChunk;
+  static constexpr int kCols   = kWide || D <= 64 ? 4 : 8;  // columns of a value piece
+  static constexpr int kBlocks = D / (16 * kCols);          // pieces of a lane per value row
+  using key   = u32x4;
+  using value = std::conditional_t<kWide || D >= 128, u32x4, u32x2>;
+};
+
+__device__ __forceinline__ f32x4 mfma(f16_t, u32x4 a, u32x4 b, f32x4 c)
+{
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(bf16_t, u32x4 a, u32x4 b, f32x4 c)
+{
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+  const T v[2] = {T(lo), T(hi)};
+  uint32_t w;
+  __builtin_memcpy(&w, v, 4);
+  return w;
+}
+
+/** The weights' reference may lag the largest exponent by this much before the sums are rescaled, and weights are
+ *  multiplied by 2^kLift: float16 weights reach 2^15 and keep their precision down to 2^-28 of the largest. */
+template <typename T>
+constexpr float kSlack = 8.0f;
+template <>
+constexpr float kSlack<f16_t> = 2.0f;
+template <typename T>
+constexpr float kLift = 0.0f;
+template <>
+constexpr float kLift<f16_t> = 13.0f;
+
+/** Rows that fill the D elements of their tiles; shorter ones; rows of fewer than 8 elements. */
+enum class fit : int { full, part, tiny };
+
+/** Workgroups per compute unit: a wave holds 32 keys and values in registers. */
+template <typename T, int D>
+constexpr int kPerUnit = sizeof(T) * D <= 256 ? 2 : 1;
+
+template <typename T, int D, fit FIT>
+__global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(attend_args a, attend_plan plan)
+{
+  constexpr bool TINY    = FIT == fit::tiny;
+  constexpr bool FULL    = FIT == fit::full;
+  using G                = geometry<T, D>;
+  constexpr int kChunks  = G::kChunks, kPiece = G::kPiece, kCols = G::kCols, kBlocks = G::kBlocks;
+  constexpr int kOut     = kBlocks * kCols;  // accumulators of 16 columns
+  __shared__ float s_out[kWaves][kRows][D];
+  __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, r = lane % 16, g = lane / 16;
+  const int64_t share = blockIdx.x;
+
+  const shares sh = shares_of(a, plan);
+  // rows without a position
+  for (int64_t b = share; b < a.pages.sequences; b += gridDim.x) {
+    if (span_of(a, b).tiles == 0) {
+      T* out = static_cast<T*>(a.out) + b * a.heads * a.vdim;
+      for (int i = tid; i < a.heads * a.vdim; i += kThreads) { out[i] = T(0.0f); }
+      if (a.lse != nullptr) {
+        for (int i = tid; i < a.heads; i += kThreads) { a.lse[b * a.heads + i] = -INFINITY; }
       }
     }
   }
-  const int64_t row = b * a.heads + h;
-  if (tid < a.vdim) { static_cast<T*>(a.out)[row * a.vdim + tid] = T(total > 0.0f ? acc / total : total); }
-  if (tid == 0 && a.lse != nullptr) { a.lse[row] = total == 0.0f ? -INFINITY : top + logf(total); }
+  if (share >= sh.n) { return; }
+  int64_t unit       = sh.first(share);
+  const int64_t last = sh.first(share + 1);
+
+  // the sequence of the first unit
+  int64_t b = 0, before = 0;  // units of the sequences below b
+  for (int64_t b0 = 0;; b0 += 64) {
+    const int64_t mine = b0 + lane < a.pages.sequences ? span_of(a, b0 + lane).tiles : 0;
+    const int64_t incl = lanes::scan_incl(int(mine)) * int64_t(plan.tables);
+    const uint64_t up  = __ballot(before + incl > unit);
+    if (up != 0) {
+      const int at = __builtin_ctzll(up);
+      b            = b0 + at;
+      before += __shfl(incl - mine * plan.tables, at);
+      break;
+    }
+    before += __shfl(incl, 63);
+  }
+
+  const int key_off   = TINY ? 0 : FULL ? D : a.dim - kPiece;  // of the last whole piece of a row
+  const int value_off = TINY ? 0 : FULL ? D : a.vdim - kCols;
+  const int dim = FULL ? D : a.dim, vdim = FULL ? D : a.vdim;
+  bool first          = true;
+  for (; unit < last; first = false) {
+    const span sp = span_of(a, b);
+    if (sp.tiles == 0) {
+      ++b;
+      continue;
+    }
+    const int table = int((unit - before) / sp.tiles), t0 = int(unit - before - int64_t(table) * sp.tiles);
+    const int t1    = int(min(int64_t(sp.tiles), t0 + last - unit));
+    const int kv    = table / plan.row_tiles, row0 = (table - kv * plan.row_tiles) * kRows;
+    const int rows  = min(kRows, plan.group - row0);
+    const int h0    = kv * plan.group + row0;
+
+    // the queries: column r, pieces of the dimensions that this lane's group holds
+    u32x4 q[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int dim0 = (c * 4 + g) * kPiece;
+      T e[kPiece];
+#pragma unroll
+      for (int j = 0; j < kPiece; ++j) {
+        // the piece that a row ends in is taken from the row's end: dimensions that an earlier piece holds are 0
+        const int at = TINY ? dim0 + j : min(dim0, key_off) + j;
+        const bool in = r < rows && at >= dim0 && at < dim;
+        e[j]          = in ? static_cast<const T*>(a.q)[b * a.q_seq + (h0 + r) * a.q_head + at] : T(0.0f);
+      }
+      __builtin_memcpy(&q[c], e, 16);
+    }
+
+    const int32_t* pages = a.pages.table + b * a.pages.width;
+    const int start8     = sp.begin / 8;
+    const int last8      = (sp.end - 1) / 8;
+    const T* k_head      = static_cast<const T*>(a.k) + kv * a.k_head;
+    const T* v_head      = static_cast<const T*>(a.v) + kv * a.v_head;
+
+    f32x4 o[kOut];
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) { o[i] = f32x4{0, 0, 0, 0}; }
+    float top = -INFINITY, limit = -INFINITY, base = 0.0f, total = 0.0f;
+
+    // group of 8 positions, its page entry and the first position's slot
+    struct place {
+      int32_t page, slot;
+    };
+    const auto entry = [&](int group8) {
+      const int at   = min(group8, last8);
+      const int e    = int(plan.page8(uint32_t(at)));
+      return place{pages[e], (at - e * int(plan.page8.d)) * 8};
+    };
+    u32x4 k[2][kChunks];
+    const auto load_keys = [&](place at) {
+      const int page  = uint32_t(at.page) < uint32_t(a.pages.n_pages) ? at.page : 0;
+      const T* k_page = k_head + int64_t(page) * a.k_page;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const T* row = k_page + int64_t(at.slot + half * 4 + r % 4) * a.k_slot;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int dim0 = (c * 4 + g) * kPiece;
+          if constexpr (TINY) {
+            T e[kPiece];
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j) { e[j] = dim0 + j < dim ? row[dim0 + j] : T(0.0f); }
+            __builtin_memcpy(&k[half][c], e, 16);
+          } else {
+            k[half][c] = piece<16>(row + (FULL ? dim0 : min(dim0, key_off)));
+          }
+        }
+      }
+    };
+
+    // a wave's tiles: one in every workgroup tile of the segment that reaches it
+    int group8       = start8 + (t0 * kWaves + wave) * (kTile / 8);
+    const int stop8  = min(start8 + t1 * kWaves * (kTile / 8), last8 + 1);
+    place k_at{}, v_at{};
+    if (group8 < stop8) {
+      k_at = entry(group8 + r / 4);
+      v_at = entry(group8 + g);
+      load_keys(k_at);
+    }
+    while (group8 < stop8) {
+      const int next8 = group8 + kWaves * (kTile / 8);
+      // values of this step: positions group8 * 8 + g * 8 + 0..7
+      const bool have = uint32_t(v_at.page) < uint32_t(a.pages.n_pages);
+      const T* v_page = v_head + int64_t(have ? v_at.page : 0) * a.v_page + int64_t(v_at.slot) * a.v_slot;
+      typename G::value v[8][kBlocks];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const T* row = v_page + j * a.v_slot;
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) {
+          const int col = (n * 16 + r) * kCols;
+          if constexpr (TINY) {
+            T e[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) { e[i] = col + i < vdim ? row[col + i] : T(0.0f); }
+            __builtin_memcpy(&v[j][n], e, sizeof(e));
+          } else {
+            v[j][n] = piece<sizeof(T) * kCols>(row + (FULL ? col : min(col, value_off)));
+          }
+        }
+      }
+      if (FIT == fit::part) {
+        // dimensions past the row, or held by an earlier piece: 0 (an infinity there would meet the query's 0)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int dim0 = (c * 4 + g) * kPiece;
+          const int skip = dim0 - min(dim0, key_off);  // leading elements of the piece that do not count
+          if constexpr (G::kWide) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              k[0][c][w] = skip > w ? 0u : k[0][c][w];
+              k[1][c][w] = skip > w ? 0u : k[1][c][w];
+            }
+          } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t mask = skip > 2 * w + 1 ? 0u : skip > 2 * w ? 0xffff0000u : 0xffffffffu;
+              k[0][c][w] &= mask;
+              k[1][c][w] &= mask;
+            }
+          }
+        }
+      }
+      f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        if constexpr (G::kWide) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              s[half] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, uint32_t(k[half][c][w])),
+                                                             __builtin_bit_cast(float, uint32_t(q[c][w])), s[half], 0, 0, 0);
+            }
+          }
+        } else {
+          s[0] = mfma(T{}, k[0][c], q[c], s[0]);
+          s[1] = mfma(T{}, k[1][c], q[c], s[1]);
+        }
+      }
+      // the next step's pages and keys
+      if (next8 < stop8) {
+        k_at = entry(next8 + r / 4);
+        v_at = entry(next8 + g);
+        load_keys(k_at);
+      }
+      // weights: lane group g holds positions (group8 + g) * 8 + 0..7 of query r
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { x[j] = s[j / 4][j % 4] * plan.scale2; }
+      const int t      = (group8 + g) * 8;
+      const bool whole = have && t >= sp.begin && t + 8 <= sp.end;
+      if (!__all(whole)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = have && t + j >= sp.begin && t + j < sp.end;
+          x[j]          = in ? x[j] : -INFINITY;
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+            for (int w = 0; w < int(sizeof(v[j][n]) / 4); ++w) { v[j][n][w] = in ? v[j][n][w] : 0u; }
+          }
+        }
+      }
+      float high = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) { high = fmaxf(high, x[j]); }
+      if (__any(high > limit)) {
+        const auto larger = [](float u, float w) { return fmaxf(u, w); };
+        high              = lanes::fold16(lanes::fold32(high, larger), larger);
+        const float grown = fmaxf(top, high);
+        const float keep  = grown == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - grown);
+        total *= keep;
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) { o[i] *= keep; }
+        top   = grown;
+        limit = grown + kSlack<T>;
+        base  = grown == -INFINITY ? 0.0f : grown - kLift<T>;
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { p[j] = __builtin_amdgcn_exp2f(x[j] - base); }
+      total += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+
+      if constexpr (G::kWide) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) {
+              o[n * kCols + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, uint32_t(v[j][n][e])), p[j],
+                                                                     o[n * kCols + e], 0, 0, 0);
+            }
+          }
+        }
+      } else {
+        // bfloat16 weights enter as value and remainder: 8 bits alone would cost as much as the output's own
+        // rounding. float16 weights are rounded once (11 bits).
+        u32x4 hi, lo;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          hi[w] = pack2<T>(p[2 * w], p[2 * w + 1]);
+          if constexpr (std::is_same_v<T, bf16_t>) {
+            lo[w] = pack2<T>(p[2 * w] - __builtin_bit_cast(float, hi[w] << 16),
+                             p[2 * w + 1] - __builtin_bit_cast(float, hi[w] & 0xffff0000u));
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+          for (int e = 0; e < kCols; ++e) {
+            u32x4 vt;  // column (n 16 + r) kCols + e of the 8 positions
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              vt[w] = __builtin_amdgcn_perm(v[2 * w + 1][n][e / 2], v[2 * w][n][e / 2], e % 2 == 0 ? 0x05040100u : 0x07060302u);
+            }
+            o[n * kCols + e] = mfma(T{}, vt, hi, o[n * kCols + e]);
+            if constexpr (std::is_same_v<T, bf16_t>) { o[n * kCols + e] = mfma(T{}, vt, lo, o[n * kCols + e]); }
+          }
+        }
+      }
+      group8 = next8;
+    }
+
+    // join the waves
+    total = lanes::fold32(total, [](float u, float w) { return u + w; });
+    total = lanes::fold16(total, [](float u, float w) { return u + w; });
+    __syncthreads();
+    if (r < rows) {
+      if (g == 0) {
+        s_max[wave][r] = top;
+        s_sum[wave][r] = total;
+      }
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = (n * 16 + g * 4 + i) * kCols;
+          if (col < vdim) {
+            const int at = FIT != fit::part ? col : min(col, value_off);
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) { s_out[wave][r][at + e] = o[n * kCols + e][i]; }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const bool done    = t0 == 0 && t1 == sp.tiles;
+    const int64_t slot = 2 * share + (first ? 0 : 1);
+    const int col      = tid % D;
+    for (int row = tid / D; row < rows; row += kThreads / D) {
+      float m = s_max[0][row];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) { m = fmaxf(m, s_max[w][row]); }
+      float sum = 0.0f, acc = 0.0f;
+      if (m != -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const float f = __builtin_amdgcn_exp2f(s_max[w][row] - m);
+          sum += f * s_sum[w][row];
+          acc += f * s_out[w][row][col];
+        }
+      }
+      if (done) {
+        const int64_t at = b * a.heads + h0 + row;
+        if (col < vdim) { static_cast<T*>(a.out)[at * vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum); }
+        if (col == 0 && a.lse != nullptr) {
+          a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
+        }
+      } else {
+        if (col < vdim) { plan.part_out[(slot * kRows + row) * vdim + col] = acc; }
+        if (col == 0) {
+          plan.part_max[slot * kRows + row] = m;
+          plan.part_sum[slot * kRows + row] = sum;
+        }
+      }
+    }
+    unit += t1 - t0;
+    if (t1 == sp.tiles && table + 1 == plan.tables) {
+      before += int64_t(sp.tiles) * plan.tables;
+      ++b;
+    }
+  }
+}
+
+/** One workgroup per sequence and product of query heads: joins the partials of a row of work that shares cut. */
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(attend_args a, attend_plan plan)
+{
+  const int table = blockIdx.x;
+  const int64_t b = blockIdx.y;
+  const shares sh = shares_of(a, plan);
+  const int tiles = span_of(a, b).tiles;
+  if (tiles == 0) { return; }
+  int64_t before = 0;
+  for (int64_t i = threadIdx.x % 64; i < b; i += 64) { before += span_of(a, i).tiles; }
+  before                = lanes::sum<64>(before) * plan.tables;
+  const int64_t unit    = before + int64_t(table) * tiles;
+  const int64_t w0      = sh.of(unit), w1 = sh.of(unit + tiles - 1);
+  if (w0 == w1) { return; }
+  const int kv = table / plan.row_tiles, row0 = (table - kv * plan.row_tiles) * kRows;
+  const int rows = min(kRows, plan.group - row0), h0 = kv * plan.group + row0;
+  const int64_t slot0 = 2 * w0 + (sh.first(w0) == unit ? 0 : 1);  // the later shares begin inside: their first slot
+  for (int i = threadIdx.x; i < rows * a.vdim; i += kThreads) {
+    const int row = i / a.vdim, col = i - row * a.vdim;
+    float m = plan.part_max[slot0 * kRows + row];
+    for (int64_t w = w0 + 1; w <= w1; ++w) { m = fmaxf(m, plan.part_max[2 * w * kRows + row]); }
+    float sum = 0.0f, acc = 0.0f;
+    if (m != -INFINITY) {
+      for (int64_t w = w0; w <= w1; ++w) {
+        const int64_t at = (w == w0 ? slot0 : 2 * w) * kRows + row;
+        const float f    = __builtin_amdgcn_exp2f(plan.part_max[at] - m);
+        sum += f * plan.part_sum[at];
+        acc += f * plan.part_out[at * a.vdim + col];
+      }
+    }
+    const int64_t at                              = b * a.heads + h0 + row;
+    static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
+    if (col == 0 && a.lse != nullptr) {
+      a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
+    }
+  }
+}
+
+int row_tiles_of(attend_args const& a) { return (a.heads / a.kv_heads + kRows - 1) / kRows; }
+
+/** Whether a row of work can be longer than one tile, so that shares can cut it. */
+bool can_split(attend_args const& a)
+{
+  int64_t most = int64_t(a.pages.width) * a.pages.page;
+  if (a.window > 0) { most = std::min(most, a.window + 7); }
+  return most > kStep;
 }
 
 }  // namespace
 
-size_t attend_workspace(elem, attend_args const&) { return 0; }
+size_t attend_workspace(elem, attend_args const& a)
+{
+  return can_split(a) ? sizeof(float) * 2 * kShares * kRows * (a.vdim + 2) : 0;
+}
 
 void attend(elem type, attend_args const& a, hipStream_t stream)
 {
-  const dim3 grid(uint32_t(a.heads), uint32_t(a.pages.sequences));
+  attend_plan plan{divisor(uint32_t(a.pages.page / kPageUnit))};
+  plan.row_tiles = row_tiles_of(a);
+  plan.group     = a.heads / a.kv_heads;
+  plan.tables    = a.kv_heads * plan.row_tiles;
+  plan.scale2    = a.scale * kLog2e;
+  plan.part_out  = static_cast<float*>(a.workspace);
+  plan.part_max  = plan.part_out + int64_t(2) * kShares * kRows * a.vdim;
+  plan.part_sum  = plan.part_max + 2 * kShares * kRows;
+  const bool split    = can_split(a);
+  const int dim       = std::max(a.dim, a.vdim);
+  const auto launched = [&](auto tag, auto bucket, auto how) {
+    using T         = decltype(tag);
+    constexpr int D = decltype(bucket)::value;
+    plan.shares     = 256 * kPerUnit<T, D>;
+    // without splitting there is at most one tile per sequence and table
+    const int64_t most = split ? plan.shares : std::min<int64_t>(plan.shares, a.pages.sequences * plan.tables);
+    attend_kernel<T, D, decltype(how)::value><<<dim3(uint32_t(most)), kThreads, 0, stream>>>(a, plan);
+    if (split) {
+      join_kernel<T><<<dim3(uint32_t(plan.tables), uint32_t(a.pages.sequences)), kThreads, 0, stream>>>(a, plan);
+    }
+  };
+  const auto sized = [&](auto tag) {
+    using full = std::integral_constant<fit, fit::full>;
+    using part = std::integral_constant<fit, fit::part>;
+    using tiny = std::integral_constant<fit, fit::tiny>;
+    const auto bucket = [&](auto d) {
+      constexpr int D = decltype(d)::value;
+      a.dim == D && a.vdim == D ? launched(tag, d, full{}) : launched(tag, d, part{});
+    };
+    if (std::min(a.dim, a.vdim) < 8) {
+      dim <= 64 ? launched(tag, std::integral_constant<int, 64>{}, tiny{}) : launched(tag, std::integral_constant<int, 256>{}, tiny{});
+    } else if (dim <= 64) {
+      bucket(std::integral_constant<int, 64>{});
+    } else if (dim <= 128) {
+      bucket(std::integral_constant<int, 128>{});
+    } else {
+      bucket(std::integral_constant<int, 256>{});
+    }
+  };
   switch (type) {
-    case elem::f32: attend_kernel<float><<<grid, kThreads, 0, stream>>>(a); break;
-    case elem::f16: attend_kernel<f16_t><<<grid, kThreads, 0, stream>>>(a); break;
-    case elem::bf16: attend_kernel<bf16_t><<<grid, kThreads, 0, stream>>>(a); break;
+    case elem::f32: sized(float{}); break;
+    case elem::f16: sized(f16_t{}); break;
+    case elem::bf16: sized(bf16_t{}); break;
   }
 }
 
