@@ -22,6 +22,13 @@ typedef uintptr_t cuvsResources_t;
 /** Create resources on the current device with a stream of their own (default priority). */
 CUVS_EXPORT cuvsError_t cuvsResourcesCreate(cuvsResources_t* res);
 
+/**
+ * Create resources on the current device and a stream of the caller's (a hipStream_t; NULL: the null stream).
+ * Nothing is allocated on the device until a search or an update uses them, so that they can be made while the stream
+ * records a graph; calls that only queue kernels (certex_attention.h) may share them between threads.
+ */
+CUVS_EXPORT cuvsError_t cuvsResourcesCreateOnStream(cuvsResources_t* res, void* stream);
+
 /** Free resources; waits for the work queued on their stream. */
 CUVS_EXPORT cuvsError_t cuvsResourcesDestroy(cuvsResources_t res);
 

@@ -30,6 +30,13 @@ class resources {
  public:
   /** Resources on the current device; stream nullptr: a new stream owned by the resources. */
   explicit resources(void* stream = nullptr);
+  /** Resources on the current device and a stream of the caller's (nullptr: the null stream). Nothing is
+   *  allocated until a search or an update uses them, so that they can be made while the stream
+   *  records a graph; calls that only take the stream may share them between threads. */
+  struct on_stream {
+    void* stream;
+  };
+  explicit resources(on_stream s);
   ~resources();
   resources(resources const&)            = delete;
   resources& operator=(resources const&) = delete;

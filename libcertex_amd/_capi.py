@@ -200,6 +200,7 @@ def lib():
                 }
                 st = ctypes.c_size_t
                 sig |= {
+                    "cuvsResourcesCreateOnStream": [P(st), vp],
                     "cuvsCertexRotaryParamsCreate": [P(P(RotaryParams))],
                     "cuvsCertexRotaryParamsDestroy": [P(RotaryParams)],
                     "cuvsCertexRotaryFrequencies": [P(RotaryParams), P(ctypes.c_double), P(ctypes.c_double)],
@@ -315,3 +316,23 @@ def resources():
         check(lib().cuvsStreamSet(entry[0], ctypes.c_void_p(stream)))
         entry[1] = stream
     return entry[0]
+
+
+_streams = {}
+
+
+def stream_resources():
+    """C resources of torch's current stream, shared by all threads: for calls that only queue kernels on it. A
+    change of stream waits for nothing, and the resources of a stream can be made while it records a graph."""
+    dev = torch.cuda.current_device()
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    res = _streams.get((dev, stream))
+    if res is None:
+        L = lib()
+        with _lock:
+            res = _streams.get((dev, stream))
+            if res is None:
+                h = ctypes.c_size_t(0)
+                check(L.cuvsResourcesCreateOnStream(ctypes.byref(h), ctypes.c_void_p(stream)))
+                res = _streams[dev, stream] = h.value
+    return res

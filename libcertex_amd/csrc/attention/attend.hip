@@ -36,6 +36,8 @@ constexpr int kTile    = 32;              // positions of a wave's step
 constexpr int kStep    = kTile * kWaves;  // of a workgroup's
 constexpr int kRows    = 16;              // query heads of a product
 constexpr int kShares  = 512;             // workgroups: two per compute unit at most
+constexpr int kJoinThreads = 512;
+static_assert(kShares <= kJoinThreads, "a thread per partial");
 constexpr float kLog2e = 1.44269504088896340736f;
 
 using f32x4  = __attribute__((ext_vector_type(4))) float;
@@ -478,13 +480,11 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) { m = fmaxf(m, s_max[w][row]); }
       float sum = 0.0f, acc = 0.0f;
-      if (m != -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const float f = __builtin_amdgcn_exp2f(s_max[w][row] - m);
-          sum += f * s_sum[w][row];
-          acc += f * s_out[w][row][col];
-        }
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = factor_of(s_max[w][row], m);
+        sum += f * s_sum[w][row];
+        acc += f * s_out[w][row][col];
       }
       if (done) {
         const int64_t at = b * a.heads + h0 + row;
@@ -508,40 +508,64 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
   }
 }
 
-/** One workgroup per sequence and product of query heads: joins the partials of a row of work that shares cut. */
+/**
+ * One workgroup per sequence and query head: joins the partials of a row of work that shares cut. Their factors
+ * first, in LDS; then a thread per column and quarter of the partials.
+ */
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(attend_args a, attend_plan plan)
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(attend_args a, attend_plan plan)
 {
-  const int table = blockIdx.x;
+  __shared__ float s_factor[kShares];
+  __shared__ float s_out[kJoinThreads];
+  __shared__ float s_part[kJoinThreads / 64];
+  const int h = blockIdx.x, tid = threadIdx.x;
   const int64_t b = blockIdx.y;
+  const int kv = h / plan.group, in_group = h - kv * plan.group;
+  const int table = kv * plan.row_tiles + in_group / kRows, row = in_group % kRows;
   const shares sh = shares_of(a, plan);
   const int tiles = span_of(a, b).tiles;
   if (tiles == 0) { return; }
   int64_t before = 0;
-  for (int64_t i = threadIdx.x % 64; i < b; i += 64) { before += span_of(a, i).tiles; }
-  before                = lanes::sum<64>(before) * plan.tables;
-  const int64_t unit    = before + int64_t(table) * tiles;
-  const int64_t w0      = sh.of(unit), w1 = sh.of(unit + tiles - 1);
+  for (int64_t i = tid % 64; i < b; i += 64) { before += span_of(a, i).tiles; }
+  before             = lanes::sum<64>(before) * plan.tables;
+  const int64_t unit = before + int64_t(table) * tiles;
+  const int64_t w0 = sh.of(unit), w1 = sh.of(unit + tiles - 1);
   if (w0 == w1) { return; }
-  const int kv = table / plan.row_tiles, row0 = (table - kv * plan.row_tiles) * kRows;
-  const int rows = min(kRows, plan.group - row0), h0 = kv * plan.group + row0;
-  const int64_t slot0 = 2 * w0 + (sh.first(w0) == unit ? 0 : 1);  // the later shares begin inside: their first slot
-  for (int i = threadIdx.x; i < rows * a.vdim; i += kThreads) {
-    const int row = i / a.vdim, col = i - row * a.vdim;
-    float m = plan.part_max[slot0 * kRows + row];
-    for (int64_t w = w0 + 1; w <= w1; ++w) { m = fmaxf(m, plan.part_max[2 * w * kRows + row]); }
-    float sum = 0.0f, acc = 0.0f;
-    if (m != -INFINITY) {
-      for (int64_t w = w0; w <= w1; ++w) {
-        const int64_t at = (w == w0 ? slot0 : 2 * w) * kRows + row;
-        const float f    = __builtin_amdgcn_exp2f(plan.part_max[at] - m);
-        sum += f * plan.part_sum[at];
-        acc += f * plan.part_out[at * a.vdim + col];
-      }
-    }
-    const int64_t at                              = b * a.heads + h0 + row;
-    static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
-    if (col == 0 && a.lse != nullptr) {
+  const int n = int(w1 - w0) + 1;
+  // the later shares begin inside the row of work: their first slot
+  const int64_t slot0 = 2 * w0 + (sh.first(w0) == unit ? 0 : 1);
+  const auto slot     = [&](int i) { return (i == 0 ? slot0 : 2 * (w0 + i)) * kRows + row; };
+
+  const float mine = tid < n ? plan.part_max[slot(tid)] : -INFINITY;
+  float m          = lanes::max<64>(mine);
+  if (tid % 64 == 0) { s_part[tid / 64] = m; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 64; ++w) { m = fmaxf(m, s_part[w]); }
+  const float f = factor_of(mine, m);
+  if (tid < n) { s_factor[tid] = f; }
+  const float weighed = lanes::sum<64>(tid < n ? f * plan.part_sum[slot(tid)] : 0.0f);
+  __syncthreads();
+  if (tid % 64 == 0) { s_part[tid / 64] = weighed; }
+  __syncthreads();
+  float sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 64; ++w) { sum += s_part[w]; }
+
+  const int cols = a.vdim <= 64 ? 64 : a.vdim <= 128 ? 128 : 256;
+  const int col = tid % cols, part = tid / cols, parts = kJoinThreads / cols;
+  float acc = 0.0f;
+  if (col < a.vdim) {
+#pragma unroll 8
+    for (int i = part; i < n; i += parts) { acc = __builtin_fmaf(s_factor[i], plan.part_out[slot(i) * a.vdim + col], acc); }
+  }
+  s_out[tid] = acc;
+  __syncthreads();
+  if (tid < a.vdim) {
+    for (int i = 1; i < parts; ++i) { acc += s_out[i * cols + tid]; }
+    const int64_t at = b * a.heads + h;
+    static_cast<T*>(a.out)[at * a.vdim + tid] = T(sum == 0.0f ? 0.0f : acc / sum);
+    if (tid == 0 && a.lse != nullptr) {
       a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
     }
   }
@@ -584,7 +608,7 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     const int64_t most = split ? plan.shares : std::min<int64_t>(plan.shares, a.pages.sequences * plan.tables);
     attend_kernel<T, D, decltype(how)::value><<<dim3(uint32_t(most)), kThreads, 0, stream>>>(a, plan);
     if (split) {
-      join_kernel<T><<<dim3(uint32_t(plan.tables), uint32_t(a.pages.sequences)), kThreads, 0, stream>>>(a, plan);
+      join_kernel<T><<<dim3(uint32_t(a.heads), uint32_t(a.pages.sequences)), kJoinThreads, 0, stream>>>(a, plan);
     }
   };
   const auto sized = [&](auto tag) {

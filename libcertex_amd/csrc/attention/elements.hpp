@@ -27,4 +27,11 @@ __device__ __forceinline__ void store(T* p, pack<T, N> const& v)
   *reinterpret_cast<pack<T, N>*>(p) = v;
 }
 
+/** What sums taken relative to the maximum `part` count relative to `whole` >= part (both in powers of 2). Where nothing
+ *  was counted both are -inf, and the sums are 0, or NaN of NaN scores: they pass as they are. */
+__device__ __forceinline__ float factor_of(float part, float whole)
+{
+  return whole == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(part - whole);
+}
+
 }  // namespace certex_amd::attention

@@ -16,6 +16,7 @@ namespace certex_amd::attention {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch   = 4;
 
 /**
  * One thread: one vector of V elements of a row (of both halves in the half layout), over
@@ -63,15 +64,23 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
   const int h0 = int(group) * a.heads_per_thread;
   const int h1 = min(h0 + a.heads_per_thread, b.heads);
 
+  // the rows of kBatch heads are in flight together
   if (item >= uint32_t(b.turned)) {  // the rest of the row
-    const int at_row = b.rotary + int(item - uint32_t(b.turned)) * V;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      store<T, V>(dst + h * b.dst_head + at_row, load<T, V>(src + h * b.src_head + at_row));
+    src += b.rotary + int(item - uint32_t(b.turned)) * V;
+    dst += b.rotary + int(item - uint32_t(b.turned)) * V;
+    for (int h = h0; h < h1; h += kBatch) {
+      pack<T, V> x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) { x[i] = load<T, V>(src + min(h + i, h1 - 1) * b.src_head); }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (h + i < h1) { store<T, V>(dst + (h + i) * b.dst_head, x[i]); }
+      }
     }
     return;
   }
-  constexpr int P = INTERLEAVED ? (V > 1 ? V / 2 : 1) : V;  // pairs of a thread
+  constexpr bool kAdjacent = INTERLEAVED && V > 1;        // pairs within a vector; else two vectors
+  constexpr int P          = kAdjacent ? V / 2 : V;       // pairs of a thread
   float c[P], s[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
@@ -80,34 +89,32 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
     c[i] *= a.magnitude;
     s[i] *= a.transpose ? -a.magnitude : a.magnitude;
   }
-  if constexpr (INTERLEAVED && V > 1) {
-    const int at_row = int(item) * V;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      auto x = load<T, V>(src + h * b.src_head + at_row);
+  const int first  = INTERLEAVED && V == 1 ? int(item) * 2 : int(item) * V;
+  const int second = INTERLEAVED ? 1 : b.rotary / 2;  // from the first
+  src += first;
+  dst += first;
+  for (int h = h0; h < h1; h += kBatch) {
+    pack<T, V> x[kBatch], y[kBatch];
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const float u = float(x.e[2 * i]), w = float(x.e[2 * i + 1]);
-        x.e[2 * i]     = T(__builtin_fmaf(u, c[i], -(w * s[i])));
-        x.e[2 * i + 1] = T(__builtin_fmaf(u, s[i], w * c[i]));
-      }
-      store<T, V>(dst + h * b.dst_head + at_row, x);
+    for (int i = 0; i < kBatch; ++i) {
+      const T* row = src + min(h + i, h1 - 1) * b.src_head;
+      x[i]         = load<T, V>(row);
+      if constexpr (!kAdjacent) { y[i] = load<T, V>(row + second); }
     }
-  } else {
-    const int first  = INTERLEAVED ? int(item) * 2 : int(item) * V;
-    const int second = INTERLEAVED ? first + 1 : first + b.rotary / 2;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      auto x = load<T, V>(src + h * b.src_head + first);
-      auto y = load<T, V>(src + h * b.src_head + second);
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const float u = float(x.e[i]), w = float(y.e[i]);
-        x.e[i] = T(__builtin_fmaf(u, c[i], -(w * s[i])));
-        y.e[i] = T(__builtin_fmaf(u, s[i], w * c[i]));
+    for (int i = 0; i < kBatch; ++i) {
+      if (h + i >= h1) { break; }
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        T& u          = kAdjacent ? x[i].e[2 * j] : x[i].e[j];
+        T& w          = kAdjacent ? x[i].e[2 * j + 1] : y[i].e[j];
+        const float f = float(u), g = float(w);
+        u = T(__builtin_fmaf(f, c[j], -(g * s[j])));
+        w = T(__builtin_fmaf(f, s[j], g * c[j]));
       }
-      store<T, V>(dst + h * b.dst_head + first, x);
-      store<T, V>(dst + h * b.dst_head + second, y);
+      T* row = dst + (h + i) * b.dst_head;
+      store<T, V>(row, x[i]);
+      if constexpr (!kAdjacent) { store<T, V>(row + second, y[i]); }
     }
   }
 }

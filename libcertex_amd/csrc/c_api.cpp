@@ -180,6 +180,14 @@ cuvsError_t cuvsResourcesCreate(cuvsResources_t* res)
   return translate([=] { *res = reinterpret_cast<cuvsResources_t>(new cuvs::resources()); });
 }
 
+cuvsError_t cuvsResourcesCreateOnStream(cuvsResources_t* res, void* stream)
+{
+  return translate([=] {
+    certex::expects(res != nullptr, "certex: NULL argument");
+    *res = reinterpret_cast<cuvsResources_t>(new cuvs::resources(cuvs::resources::on_stream{stream}));
+  });
+}
+
 cuvsError_t cuvsResourcesDestroy(cuvsResources_t res)
 {
   return translate([=] { delete reinterpret_cast<cuvs::resources*>(res); });

@@ -31,10 +31,13 @@ resources::resources(void* stream) : s_(std::make_unique<detail::resources_state
     CERTEX_HIP_TRY(hipStreamCreateWithFlags(&s_->stream, hipStreamNonBlocking));
     s_->owns_stream = true;
   }
-  // written by kernels while they run (publish_args): coherent
-  CERTEX_HIP_TRY(hipHostMalloc(&s_->host_small, 64, hipHostMallocMapped | hipHostMallocCoherent));
-  std::memset(s_->host_small, 0, 64);
-  CERTEX_HIP_TRY(hipEventCreateWithFlags(&s_->staged, hipEventDisableTiming));
+  (void)state();
+}
+
+resources::resources(on_stream s) : s_(std::make_unique<detail::resources_state>())
+{
+  CERTEX_HIP_TRY(hipGetDevice(&s_->device));
+  s_->stream = static_cast<hipStream_t>(s.stream);
 }
 
 resources::~resources()
@@ -53,24 +56,6 @@ auto resources::stream() const -> void* { return s_->stream; }
 
 void resources::set_stream(void* stream)
 {
-  // The scratch passes from one stream to the next, which waits for it. A stream that records a graph
-  // is not given it (a search waits on the host and cannot be recorded), and a wait here would break
-  // the recording: the stream before it is waited for by the first change after.
-  hipStreamCaptureStatus recording = hipStreamCaptureStatusNone;
-  if (stream != nullptr && !s_->owns_stream &&
-      hipStreamIsCapturing(static_cast<hipStream_t>(stream), &recording) != hipSuccess) {
-    (void)hipGetLastError();
-    recording = hipStreamCaptureStatusNone;
-  }
-  if (recording == hipStreamCaptureStatusActive) {
-    if (!s_->before_recording) { s_->before_recording = s_->stream; }
-    s_->stream = static_cast<hipStream_t>(stream);
-    return;
-  }
-  if (s_->before_recording) {
-    CERTEX_HIP_TRY(hipStreamSynchronize(*s_->before_recording));
-    s_->before_recording.reset();
-  }
   CERTEX_HIP_TRY(hipStreamSynchronize(s_->stream));
   if (s_->owns_stream) {
     CERTEX_HIP_TRY(hipStreamDestroy(s_->stream));
@@ -101,7 +86,16 @@ void resources::trim() const
 
 void resources::set_scratch_cap(size_t bytes) const { s_->slot_cap = bytes; }
 
-auto resources::state() const -> detail::resources_state& { return *s_; }
+auto resources::state() const -> detail::resources_state&
+{
+  if (s_->host_small == nullptr) {
+    // written by kernels while they run (publish_args): coherent
+    CERTEX_HIP_TRY(hipHostMalloc(&s_->host_small, 64, hipHostMallocMapped | hipHostMallocCoherent));
+    std::memset(s_->host_small, 0, 64);
+  }
+  if (s_->staged == nullptr) { CERTEX_HIP_TRY(hipEventCreateWithFlags(&s_->staged, hipEventDisableTiming)); }
+  return *s_;
+}
 
 }  // namespace cuvs
 

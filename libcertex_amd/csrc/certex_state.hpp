@@ -7,7 +7,6 @@
 
 #include <cstdint>
 #include <mutex>
-#include <optional>
 #include <shared_mutex>
 #include <stdexcept>
 #include <string>
@@ -132,7 +131,6 @@ struct resources_state {
   int device          = 0;
   hipStream_t stream  = nullptr;
   bool owns_stream    = false;
-  std::optional<hipStream_t> before_recording;  // the last stream, while the present one records a graph
   int64_t bucket_cap  = 1024;  // survivors per query kept by the last searches
   bool spill_pool     = false;  // a screen's LDS survivor lists overflowed: provide a spill pool
   // float searches of k <= 64: k times the rows per anchor from which the latest batch had buckets

@@ -116,7 +116,7 @@ class Rotary:
                 h = self._handles.get(device)
                 if h is None:
                     out = ctypes.c_size_t()
-                    C.check(C.lib().cuvsCertexRotaryCreate(C.resources(), ctypes.byref(self._params), ctypes.byref(out)))
+                    C.check(C.lib().cuvsCertexRotaryCreate(C.stream_resources(), ctypes.byref(self._params), ctypes.byref(out)))
                     h = self._handles[device] = out.value
         return h
 
@@ -146,7 +146,7 @@ class Rotary:
         if out is None and y.stride(-1) != 1:  # a dense tensor in another order of dimensions
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         _require(y.shape == x.shape, "out must have the shape of x")
-        res, view = C.resources(), C.views()
+        res, view = C.stream_resources(), C.views()
         C.check(C.lib().cuvsCertexRotate(res, self._handle(x.device.index), view(x), view(positions), view(y), transpose))
         return y
 
@@ -173,7 +173,7 @@ def append_pages(k, v, k_pages, v_pages, page_table, positions, sequences=None, 
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if rotary is not None:
         _require(rotary.head_dim == k.shape[-1], f"this rotation is of heads of {rotary.head_dim}, not {k.shape[-1]}")
-    res, view = C.resources(), C.views()
+    res, view = C.stream_resources(), C.views()
     C.check(C.lib().cuvsCertexAppendPages(
         res, 0 if rotary is None else rotary._handle(k.device.index), view(k), view(v), view(k_pages), view(v_pages),
         view(table), view(positions), view(sequences), view(q), view(out)))
@@ -204,7 +204,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
     window = 0 if window is None else int(window)
     out = torch.empty((q.shape[0], q.shape[1], v_pages.shape[3]), dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    L, res, view = C.lib(), C.resources(), C.views()
+    L, res, view = C.lib(), C.stream_resources(), C.views()
     qv, kv, vv, tv = view(q), view(k_pages), view(v_pages), view(table)
     need = ctypes.c_int64()
     C.check(L.cuvsCertexPagedAttentionWorkspace(qv, kv, vv, tv, window, ctypes.byref(need)))
@@ -240,7 +240,7 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     scores = scores.contiguous()
     out = torch.empty((*scores.shape[:2], values.shape[-1]), dtype=values.dtype, device=values.device)
     lse = torch.empty(scores.shape[:2], dtype=torch.float32, device=values.device) if return_lse else None
-    L, res, view = C.lib(), C.resources(), C.views()
+    L, res, view = C.lib(), C.stream_resources(), C.views()
     sv, vv, tv = view(scores), view(values), view(page_table)
     need = ctypes.c_int64()
     C.check(L.cuvsCertexSelectedAttentionWorkspace(sv, vv, tv, ctypes.byref(need)))

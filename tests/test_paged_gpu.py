@@ -305,6 +305,17 @@ def test_attend_nan_is_seen(gpu):
     out = certex.paged_attention(rand(2, 4, 64, dtype=torch.bfloat16), kp, vp, table, ints([50, 50]))
     assert out[0, 2:].isnan().all() and not out[0, :2].isnan().any() and not out[1].isnan().any()
 
+    q = rand(2, 4, 64, dtype=torch.bfloat16)
+    q[1, 3] = float("nan")  # every score of a row
+    for lens in ([50, 50], [50, 5000]):
+        kp, vp, table, *_ = paged(lens, 16, 2, 64, 64, torch.bfloat16, seed=14)
+        out, lse = certex.paged_attention(q, kp, vp, table, ints(lens), return_lse=True)
+        assert out[1, 3].isnan().all() and lse[1, 3].isnan() and not out[0].isnan().any() and not out[1, :3].isnan().any()
+    scores = torch.full((2, 1, 3000), float("nan"), device="cuda")
+    scores[1] = 1.0
+    out = certex.selected_attention(scores, torch.zeros((2, 1, 3000), dtype=torch.int64, device="cuda"), rand(2, 4, 64), 1.0)
+    assert out[0].isnan().all() and not out[1].isnan().any()
+
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_attend_unaligned_queries(gpu, dtype):
