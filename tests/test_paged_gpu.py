@@ -396,6 +396,30 @@ def test_selected(gpu, dtype, k, dv, heads, kv, m):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [512, 700, 2048, 2100, 4097])
+@pytest.mark.parametrize("dv", [128, 62, 200])
+def test_selected_shared_rows(gpu, dtype, k, dv):
+    """Queries of a head that select more rows than it has, of more than a die's cache; ids repeated within a query; all in
+    one range."""
+    n, heads, kv, m = 35_000, 4, 2, 64
+    values = rand(kv, n, dv, dtype=dtype)
+    scores = rand(heads, m, k, scale=5.0)
+    ids = torch.randint(0, n, (heads, m, k), device="cuda")
+    ids[0, 1] = 17
+    ids[0, 2] = ids[0, 2] % 500
+    ids[1, 0] = -1
+    ids[1, 1, ::2] = n
+    ids[1, 2, 1:] = -1
+    ids[2, 3, : k // 2] = -5
+    scores[3, 4] = scores[3, 4].sort(descending=True).values * 100
+    out, lse = certex.selected_attention(scores, ids, values, 0.3, return_lse=True)
+    host = values.double().cpu()
+    few = [0, 1, 2, 3, 4, m - 1]
+    check_selected(scores[:, few], ids[:, few], lambda j: host[j], heads, kv, 0.3, out[:, few], lse[:, few])
+    assert torch.equal(out, certex.selected_attention(scores, ids, values, 0.3))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_selected_missing(gpu, dtype):
     """-1 and ids past the values, scores of -inf, rows of none; values that nobody selected hold NaN."""
     values = rand(2, 500, 64, dtype=dtype)
