@@ -8,7 +8,7 @@
 // it, a few operations per byte, so the rate at which memory is read. The kernel keeps the two products
 // off the critical path by giving them to the matrix cores in a form that needs no exchange between lanes
 // and no LDS:
-// - a wave takes 32 positions; S^T = K Q^T has the positions as rows and up to 16 query heads as columns, so that
+// - a wave takes 32 positions (float32: 16); S^T = K Q^T has the positions as rows and up to 16 query heads as columns, so that
 //   K rows go from memory to the operand registers as they lie (16 bytes of a row per lane);
 // - the rows of the two 16-position products are permuted such that a lane's 8 results are the 8
 //   consecutive positions that it holds as k-slots of O^T = V^T P^T: the weights never move;
@@ -17,10 +17,11 @@
 // - m, the sum and the scaling are per query head, that is per lane.
 // The loads of the next keys and of this tile's values are in flight during both products.
 //
-// Work is dealt on the device, from the lengths: tiles of 128 positions (32 per wave) of all sequences
-// and heads, in order, in equal shares to the workgroups, so that any mix of lengths fills the chip and the host reads
-// nothing back. A share that cuts a row of work leaves a partial (m, sum, output) in the workspace, and a second
-// launch joins them in order of position.
+// Work is dealt on the device, from the lengths: the tiles of all sequences, one after the other, in equal shares, each
+// share to one workgroup per key head. So any mix of lengths fills the chip and the host reads nothing back, and the
+// heads of a position are read at about the same time (they are neighbours in memory where a slot holds all heads). A
+// share that cuts a sequence leaves a partial (m, sum, output) in the workspace, and a second launch joins them in order of
+// position.
 #include "../kernels/lanes.hpp"
 #include "attention.hpp"
 #include "elements.hpp"
@@ -32,12 +33,9 @@ namespace {
 
 constexpr int kWaves   = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kTile    = 32;              // positions of a wave's step
-constexpr int kStep    = kTile * kWaves;  // of a workgroup's
-constexpr int kRows    = 16;              // query heads of a product
-constexpr int kShares  = 512;             // workgroups: two per compute unit at most
-constexpr int kJoinThreads = 512;
-static_assert(kShares <= kJoinThreads, "a thread per partial");
+constexpr int kRows    = 16;   // query heads of a product
+constexpr int kUnits   = 256;  // compute units
+constexpr int kMaxShares = 2 * kUnits;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 using f32x4  = __attribute__((ext_vector_type(4))) float;
@@ -46,74 +44,75 @@ using u32x2  = __attribute__((ext_vector_type(2))) uint32_t;
 using f16x8  = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
-/** n / d for n < 2^28 by a product: m = ceil(2^(28 + s) / d) with 2^s >= d exceeds 2^(28 + s) / d by less than 1, so the
- *  quotient's error n (m d - 2^(28 + s)) / d stays below 1 / d. */
+/** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less than 1, so n m / 2^(29 + s)
+ *  exceeds n / d by less than 1 / d. */
 struct divisor {
   uint32_t m, shift, d;
   explicit divisor(uint32_t by) : d(by)
   {
     uint32_t s = 0;
     while ((uint64_t(1) << s) < by) { ++s; }
-    shift = 28 + s;
+    shift = 29 + s;
     m     = uint32_t(((uint64_t(1) << shift) + by - 1) / by);
   }
   __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> shift); }
 };
 
+/** Positions of a lane group in a step: its rows of the 16-position products (two of 16 bits, one of float32). */
+template <typename T>
+constexpr int kGroup = sizeof(T) == 4 ? 4 : 8;
+/** Positions of a wave's step, and of a workgroup's: a tile. */
+template <typename T>
+constexpr int kStep = 4 * kGroup<T>;
+template <typename T>
+constexpr int kTile = kStep<T> * kWaves;
+
 struct attend_plan {
-  divisor page8;      // groups of 8 positions per page
-  int32_t row_tiles;  // products of 16 query heads per key head
-  int32_t group;      // query heads per key head
-  int32_t tables;     // key heads x row_tiles
-  int32_t shares;     // at most
-  float scale2;       // scale log2(e)
-  float* part_out;    // [2 kShares][kRows][vdim]
-  float* part_max;    // [2 kShares][kRows]
+  divisor page_groups;  // lane groups' positions per page
+  int32_t row_tiles;    // products of 16 query heads per key head
+  int32_t group;        // query heads per key head
+  int32_t tables;       // key heads x row_tiles: table t is key head t % kv_heads, product t / kv_heads
+  int32_t shares;       // of a table's tiles, at most
+  bool one_die;         // the tables of a share run on one die
+  float scale2;         // scale log2(e)
+  float* part_out;      // [tables][2 shares][kRows][vdim]
+  float* part_max;      // [tables][2 shares][kRows]
   float* part_sum;
 };
 
-/** Positions [begin, end) of a sequence, and its tiles of kStep from begin rounded down to 8. */
+/** Positions [begin, end) of a sequence, and its tiles of TILE from begin rounded down to 8. */
 struct span {
   int32_t begin, end, tiles;
 };
 
+template <int TILE>
 __device__ __forceinline__ span span_of(attend_args const& a, int64_t b)
 {
   int64_t end = a.lengths[b];
   end         = end < 0 ? 0 : min(end, int64_t(a.pages.width) * a.pages.page);
   if (a.pages.n_pages == 0) { end = 0; }
   const int64_t begin = a.window > 0 && end > a.window ? end - a.window : 0;
-  return {int32_t(begin), int32_t(end), int32_t((end - (begin & ~int64_t(7)) + kStep - 1) / kStep)};
+  return {int32_t(begin), int32_t(end), int32_t((end - (begin & ~int64_t(7)) + TILE - 1) / TILE)};
 }
 
-/** All tiles of the call (the same on every lane). */
-__device__ __forceinline__ int64_t count_tiles(attend_args const& a)
-{
-  int64_t mine = 0;
-  for (int64_t b = threadIdx.x % 64; b < a.pages.sequences; b += 64) { mine += span_of(a, b).tiles; }
-  return lanes::sum<64>(mine);
-}
-
-/** The shares: share w takes the units [w units / n, (w + 1) units / n). */
+/** The shares of a table: share w takes the tiles [w tiles / n, (w + 1) tiles / n) of all sequences'. */
 struct shares {
-  int64_t units, n;
-  __device__ __forceinline__ int64_t first(int64_t w) const { return w * units / n; }
-  __device__ __forceinline__ int64_t of(int64_t unit) const { return ((unit + 1) * n - 1) / units; }
+  int64_t tiles, n;
+  __device__ __forceinline__ int64_t first(int64_t w) const { return w * tiles / n; }
+  __device__ __forceinline__ int64_t of(int64_t tile) const { return ((tile + 1) * n - 1) / tiles; }
 };
 
+template <int TILE>
 __device__ __forceinline__ shares shares_of(attend_args const& a, attend_plan const& p)
 {
-  const int64_t units = count_tiles(a) * p.tables;
-  return {units, min(int64_t(p.shares), units)};
+  int64_t mine = 0;
+  for (int64_t b = threadIdx.x % 64; b < a.pages.sequences; b += 64) { mine += span_of<TILE>(a, b).tiles; }
+  mine = lanes::sum<64>(mine);
+  return {mine, min(int64_t(p.shares), mine)};
 }
 
 /** The elements of a lane's piece: 16 bytes of a row at any alignment of the elements (the memory takes
  *  misaligned vector loads); TINY rows are shorter than a piece and read element by element. */
-template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) loose {
-  T e[N];
-};
-
 template <int BYTES, typename T>
 __device__ __forceinline__ auto piece(const T* p)
 {
@@ -128,6 +127,16 @@ __device__ __forceinline__ auto piece(const T* p)
   }
 }
 
+/** A value piece: read once by the call, so it is not kept in the caches. Measured: 64 sequences up to 8,192 184 -> 168 us, one of
+ *  131,072 103 -> 92 us. (Key pieces are half lines, whose other half is the next load's: 184 -> 181 us alone, 176 us together.) */
+template <int BYTES, typename T>
+__device__ __forceinline__ auto passing_piece(const T* p)
+{
+  using words = std::conditional_t<BYTES == 16, u32x4, u32x2>;
+  using loose = words __attribute__((aligned(sizeof(T))));
+  return words(__builtin_nontemporal_load(reinterpret_cast<const loose*>(p)));
+}
+
 /** Keys, queries and values of a wave's step for elements T, head dimensions up to D. */
 template <typename T, int D>
 struct geometry {
@@ -136,9 +145,11 @@ struct geometry {
   static constexpr int kChunk  = 4 * kPiece;              // dimensions of a product's four lane groups
   static constexpr int kChunks = D / kChunk;
   static constexpr int kCols   = kWide || D <= 64 ? 4 : 8;  // columns of a value piece
-  static constexpr int kBlocks = D / (16 * kCols);          // pieces of a lane per value row
+  static constexpr int kBlocks = (D + 16 * kCols - 1) / (16 * kCols);  // pieces of a lane per value row
+  static constexpr bool kWhole = D % (16 * kCols) == 0;                // no piece of a full row is past its end
+  static constexpr int kHalves = kGroup<T> / 4;             // 16-position products of a step
   using key   = u32x4;
-  using value = std::conditional_t<kWide || D >= 128, u32x4, u32x2>;
+  using value = std::conditional_t<kCols * sizeof(T) == 16, u32x4, u32x2>;
 };
 
 __device__ __forceinline__ f32x4 mfma(f16_t, u32x4 a, u32x4 b, f32x4 c)
@@ -173,9 +184,17 @@ constexpr float kLift<f16_t> = 13.0f;
 /** Rows that fill the D elements of their tiles; shorter ones; rows of fewer than 8 elements. */
 enum class fit : int { full, part, tiny };
 
-/** Workgroups per compute unit: a wave holds 32 keys and values in registers. */
+/** Workgroups per compute unit: a wave holds the keys and values of a step in registers. */
 template <typename T, int D>
-constexpr int kPerUnit = sizeof(T) * D <= 256 ? 2 : 1;
+constexpr int kPerUnit = D <= 128 ? 2 : 1;
+
+/** What of word w of a key or query piece counts when its first `skip` elements do not. */
+template <typename T>
+__device__ __forceinline__ uint32_t counted(int skip, int w)
+{
+  if constexpr (sizeof(T) == 4) { return skip > w ? 0u : 0xffffffffu; }
+  return skip > 2 * w + 1 ? 0u : skip > 2 * w ? 0xffff0000u : 0xffffffffu;
+}
 
 template <typename T, int D, fit FIT>
 __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(attend_args a, attend_plan plan)
@@ -185,15 +204,19 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
   using G                = geometry<T, D>;
   constexpr int kChunks  = G::kChunks, kPiece = G::kPiece, kCols = G::kCols, kBlocks = G::kBlocks;
   constexpr int kOut     = kBlocks * kCols;  // accumulators of 16 columns
+  constexpr int kGrp     = kGroup<T>, kHalves = G::kHalves, kTiles = kTile<T>;
   __shared__ float s_out[kWaves][kRows][D];
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, r = lane % 16, g = lane / 16;
-  const int64_t share = blockIdx.x;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, g = lane / 16;
+  // consecutive workgroups go to the 8 dies in turn: a share's tables to all of them, or to one
+  const int turn      = plan.one_die ? blockIdx.x / 8 : blockIdx.x;
+  const int table     = turn % plan.tables;
+  const int64_t share = plan.one_die ? int64_t(turn / plan.tables) * 8 + blockIdx.x % 8 : turn / plan.tables;
 
-  const shares sh = shares_of(a, plan);
+  const shares sh = shares_of<kTiles>(a, plan);
   // rows without a position
-  for (int64_t b = share; b < a.pages.sequences; b += gridDim.x) {
-    if (span_of(a, b).tiles == 0) {
+  for (int64_t b = blockIdx.x; b < a.pages.sequences; b += gridDim.x) {
+    if (span_of<kTiles>(a, b).tiles == 0) {
       T* out = static_cast<T*>(a.out) + b * a.heads * a.vdim;
       for (int i = tid; i < a.heads * a.vdim; i += kThreads) { out[i] = T(0.0f); }
       if (a.lse != nullptr) {
@@ -202,82 +225,84 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
     }
   }
   if (share >= sh.n) { return; }
-  int64_t unit       = sh.first(share);
+  int64_t tile       = sh.first(share);
   const int64_t last = sh.first(share + 1);
 
-  // the sequence of the first unit
-  int64_t b = 0, before = 0;  // units of the sequences below b
+  // the sequence of the first tile
+  int64_t b = 0, before = 0;  // tiles of the sequences below b
   for (int64_t b0 = 0;; b0 += 64) {
-    const int64_t mine = b0 + lane < a.pages.sequences ? span_of(a, b0 + lane).tiles : 0;
-    const int64_t incl = lanes::scan_incl(int(mine)) * int64_t(plan.tables);
-    const uint64_t up  = __ballot(before + incl > unit);
+    const int mine    = b0 + lane < a.pages.sequences ? span_of<kTiles>(a, b0 + lane).tiles : 0;
+    const int incl    = lanes::scan_incl(mine);
+    const uint64_t up = __ballot(before + incl > tile);
     if (up != 0) {
       const int at = __builtin_ctzll(up);
       b            = b0 + at;
-      before += __shfl(incl - mine * plan.tables, at);
+      before += __builtin_amdgcn_readlane(incl - mine, at);
       break;
     }
-    before += __shfl(incl, 63);
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
 
   const int key_off   = TINY ? 0 : FULL ? D : a.dim - kPiece;  // of the last whole piece of a row
-  const int value_off = TINY ? 0 : FULL ? D : a.vdim - kCols;
+  const int value_off = TINY ? 0 : (FULL ? D : a.vdim) - kCols;
   const int dim = FULL ? D : a.dim, vdim = FULL ? D : a.vdim;
-  bool first          = true;
-  for (; unit < last; first = false) {
-    const span sp = span_of(a, b);
+  const int kv = table % a.kv_heads, row0 = table / a.kv_heads * kRows;
+  const int rows = min(kRows, plan.group - row0), h0 = kv * plan.group + row0;
+  const T* k_head = static_cast<const T*>(a.k) + kv * a.k_head;
+  const T* v_head = static_cast<const T*>(a.v) + kv * a.v_head;
+  bool first      = true;
+  for (; tile < last; first = false) {
+    const span sp = span_of<kTiles>(a, b);
     if (sp.tiles == 0) {
       ++b;
       continue;
     }
-    const int table = int((unit - before) / sp.tiles), t0 = int(unit - before - int64_t(table) * sp.tiles);
-    const int t1    = int(min(int64_t(sp.tiles), t0 + last - unit));
-    const int kv    = table / plan.row_tiles, row0 = (table - kv * plan.row_tiles) * kRows;
-    const int rows  = min(kRows, plan.group - row0);
-    const int h0    = kv * plan.group + row0;
+    const int t0 = int(tile - before), t1 = int(min(int64_t(sp.tiles), t0 + last - tile));
 
     // the queries: column r, pieces of the dimensions that this lane's group holds
     u32x4 q[kChunks];
+    const T* q_row = static_cast<const T*>(a.q) + b * a.q_seq + (h0 + min(r, rows - 1)) * a.q_head;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int dim0 = (c * 4 + g) * kPiece;
-      T e[kPiece];
+      if constexpr (TINY) {
+        T e[kPiece];
 #pragma unroll
-      for (int j = 0; j < kPiece; ++j) {
+        for (int j = 0; j < kPiece; ++j) { e[j] = dim0 + j < dim ? q_row[dim0 + j] : T(0.0f); }
+        __builtin_memcpy(&q[c], e, 16);
+      } else {
         // the piece that a row ends in is taken from the row's end: dimensions that an earlier piece holds are 0
-        const int at = TINY ? dim0 + j : min(dim0, key_off) + j;
-        const bool in = r < rows && at >= dim0 && at < dim;
-        e[j]          = in ? static_cast<const T*>(a.q)[b * a.q_seq + (h0 + r) * a.q_head + at] : T(0.0f);
+        q[c] = piece<16>(q_row + (FULL ? dim0 : min(dim0, key_off)));
       }
-      __builtin_memcpy(&q[c], e, 16);
+      const int skip = FIT == fit::part ? dim0 - min(dim0, key_off) : 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) { q[c][w] = r < rows ? q[c][w] & counted<T>(skip, w) : 0u; }
     }
 
     const int32_t* pages = a.pages.table + b * a.pages.width;
-    const int start8     = sp.begin / 8;
-    const int last8      = (sp.end - 1) / 8;
-    const T* k_head      = static_cast<const T*>(a.k) + kv * a.k_head;
-    const T* v_head      = static_cast<const T*>(a.v) + kv * a.v_head;
+    const int start      = sp.begin / 8 * (8 / kGrp);  // in lane groups' positions
+    const int final      = (sp.end - 1) / kGrp;
 
     f32x4 o[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i) { o[i] = f32x4{0, 0, 0, 0}; }
     float top = -INFINITY, limit = -INFINITY, base = 0.0f, total = 0.0f;
 
-    // group of 8 positions, its page entry and the first position's slot
+    // the page of a group's positions, and the first one's slot
     struct place {
       int32_t page, slot;
     };
-    const auto entry = [&](int group8) {
-      const int at   = min(group8, last8);
-      const int e    = int(plan.page8(uint32_t(at)));
-      return place{pages[e], (at - e * int(plan.page8.d)) * 8};
+    const auto entry = [&](int group) {
+      const int at = min(group, final);
+      const int e  = int(plan.page_groups(uint32_t(at)));
+      return place{pages[e], (at - e * int(plan.page_groups.d)) * kGrp};
     };
-    u32x4 k[2][kChunks];
+    u32x4 k[kHalves][kChunks];
     const auto load_keys = [&](place at) {
       const int page  = uint32_t(at.page) < uint32_t(a.pages.n_pages) ? at.page : 0;
       const T* k_page = k_head + int64_t(page) * a.k_page;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < kHalves; ++half) {
         const T* row = k_page + int64_t(at.slot + half * 4 + r % 4) * a.k_slot;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
@@ -294,23 +319,23 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       }
     };
 
-    // a wave's tiles: one in every workgroup tile of the segment that reaches it
-    int group8       = start8 + (t0 * kWaves + wave) * (kTile / 8);
-    const int stop8  = min(start8 + t1 * kWaves * (kTile / 8), last8 + 1);
+    // a wave's steps: one in every tile of the segment that reaches it
+    int group      = start + (t0 * kWaves + wave) * 4;
+    const int stop = min(start + t1 * kWaves * 4, final + 1);
     place k_at{}, v_at{};
-    if (group8 < stop8) {
-      k_at = entry(group8 + r / 4);
-      v_at = entry(group8 + g);
+    if (group < stop) {
+      k_at = entry(group + r / 4);
+      v_at = entry(group + g);
       load_keys(k_at);
     }
-    while (group8 < stop8) {
-      const int next8 = group8 + kWaves * (kTile / 8);
-      // values of this step: positions group8 * 8 + g * 8 + 0..7
+    while (group < stop) {
+      const int next = group + kWaves * 4;
+      // values of this step: positions (group + g) * kGrp + 0..kGrp - 1
       const bool have = uint32_t(v_at.page) < uint32_t(a.pages.n_pages);
       const T* v_page = v_head + int64_t(have ? v_at.page : 0) * a.v_page + int64_t(v_at.slot) * a.v_slot;
-      typename G::value v[8][kBlocks];
+      typename G::value v[kGrp][kBlocks];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < kGrp; ++j) {
         const T* row = v_page + j * a.v_slot;
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) {
@@ -321,64 +346,57 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
             for (int i = 0; i < kCols; ++i) { e[i] = col + i < vdim ? row[col + i] : T(0.0f); }
             __builtin_memcpy(&v[j][n], e, sizeof(e));
           } else {
-            v[j][n] = piece<sizeof(T) * kCols>(row + (FULL ? col : min(col, value_off)));
+            v[j][n] = passing_piece<sizeof(T) * kCols>(row + (FULL && G::kWhole ? col : min(col, value_off)));
           }
         }
       }
-      if (FIT == fit::part) {
+      if (FIT == fit::part && dim < D) {
         // dimensions past the row, or held by an earlier piece: 0 (an infinity there would meet the query's 0)
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           const int dim0 = (c * 4 + g) * kPiece;
           const int skip = dim0 - min(dim0, key_off);  // leading elements of the piece that do not count
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t mask = counted<T>(skip, w);
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) { k[half][c][w] &= mask; }
+          }
+        }
+      }
+      f32x4 s[kHalves];
+#pragma unroll
+      for (int half = 0; half < kHalves; ++half) { s[half] = f32x4{0, 0, 0, 0}; }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half) {
           if constexpr (G::kWide) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              k[0][c][w] = skip > w ? 0u : k[0][c][w];
-              k[1][c][w] = skip > w ? 0u : k[1][c][w];
-            }
-          } else {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t mask = skip > 2 * w + 1 ? 0u : skip > 2 * w ? 0xffff0000u : 0xffffffffu;
-              k[0][c][w] &= mask;
-              k[1][c][w] &= mask;
-            }
-          }
-        }
-      }
-      f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        if constexpr (G::kWide) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
               s[half] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, uint32_t(k[half][c][w])),
                                                              __builtin_bit_cast(float, uint32_t(q[c][w])), s[half], 0, 0, 0);
             }
+          } else {
+            s[half] = mfma(T{}, k[half][c], q[c], s[half]);
           }
-        } else {
-          s[0] = mfma(T{}, k[0][c], q[c], s[0]);
-          s[1] = mfma(T{}, k[1][c], q[c], s[1]);
         }
       }
       // the next step's pages and keys
-      if (next8 < stop8) {
-        k_at = entry(next8 + r / 4);
-        v_at = entry(next8 + g);
+      if (next < stop) {
+        k_at = entry(next + r / 4);
+        v_at = entry(next + g);
         load_keys(k_at);
       }
-      // weights: lane group g holds positions (group8 + g) * 8 + 0..7 of query r
-      float x[8];
+      // weights: lane group g holds the positions t + 0..kGrp - 1 of query r
+      float x[kGrp];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { x[j] = s[j / 4][j % 4] * plan.scale2; }
-      const int t      = (group8 + g) * 8;
-      const bool whole = have && t >= sp.begin && t + 8 <= sp.end;
+      for (int j = 0; j < kGrp; ++j) { x[j] = s[j / 4][j % 4] * plan.scale2; }
+      const int t      = (group + g) * kGrp;
+      const bool whole = have && t >= sp.begin && t + kGrp <= sp.end;
       if (!__all(whole)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kGrp; ++j) {
           const bool in = have && t + j >= sp.begin && t + j < sp.end;
           x[j]          = in ? x[j] : -INFINITY;
 #pragma unroll
@@ -390,7 +408,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       }
       float high = x[0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) { high = fmaxf(high, x[j]); }
+      for (int j = 1; j < kGrp; ++j) { high = fmaxf(high, x[j]); }
       if (__any(high > limit)) {
         const auto larger = [](float u, float w) { return fmaxf(u, w); };
         high              = lanes::fold16(lanes::fold32(high, larger), larger);
@@ -403,14 +421,15 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         limit = grown + kSlack<T>;
         base  = grown == -INFINITY ? 0.0f : grown - kLift<T>;
       }
-      float p[8];
+      float p[kGrp];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) { p[j] = __builtin_amdgcn_exp2f(x[j] - base); }
-      total += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      for (int j = 0; j < kGrp; ++j) { p[j] = __builtin_amdgcn_exp2f(x[j] - base); }
+#pragma unroll
+      for (int j = 0; j < kGrp; j += 4) { total += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]); }
 
       if constexpr (G::kWide) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kGrp; ++j) {
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n) {
 #pragma unroll
@@ -446,7 +465,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
           }
         }
       }
-      group8 = next8;
+      group = next;
     }
 
     // join the waves
@@ -473,9 +492,10 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
     }
     __syncthreads();
     const bool done    = t0 == 0 && t1 == sp.tiles;
-    const int64_t slot = 2 * share + (first ? 0 : 1);
-    const int col      = tid % D;
-    for (int row = tid / D; row < rows; row += kThreads / D) {
+    const int64_t slot = (int64_t(table) * plan.shares + share) * 2 + (first ? 0 : 1);
+    constexpr int kOnce = kThreads / D;  // rows at a time
+    const int col       = tid % D;
+    for (int row = tid < kOnce * D ? tid / D : rows; row < rows; row += kOnce) {
       float m = s_max[0][row];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) { m = fmaxf(m, s_max[w][row]); }
@@ -500,115 +520,160 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         }
       }
     }
-    unit += t1 - t0;
-    if (t1 == sp.tiles && table + 1 == plan.tables) {
-      before += int64_t(sp.tiles) * plan.tables;
+    tile += t1 - t0;
+    if (t1 == sp.tiles) {
+      before += sp.tiles;
       ++b;
     }
   }
 }
 
 /**
- * One workgroup per sequence and query head: joins the partials of a row of work that shares cut. Their factors
- * first, in LDS; then a thread per column and quarter of the partials.
+ * One workgroup per sequence and query head: joins the partials of a sequence that shares cut. Their factors first, in
+ * LDS; then a thread per column and part of the partials.
  */
-template <typename T>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(attend_args a, attend_plan plan)
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void join_kernel(attend_args a, attend_plan plan)
 {
-  __shared__ float s_factor[kShares];
-  __shared__ float s_out[kJoinThreads];
-  __shared__ float s_part[kJoinThreads / 64];
+  constexpr int kTiles = kTile<T>;
+  __shared__ float s_factor[kMaxShares];
+  __shared__ float s_out[THREADS];
+  __shared__ float s_part[THREADS / 64];
   const int h = blockIdx.x, tid = threadIdx.x;
   const int64_t b = blockIdx.y;
   const int kv = h / plan.group, in_group = h - kv * plan.group;
-  const int table = kv * plan.row_tiles + in_group / kRows, row = in_group % kRows;
-  const shares sh = shares_of(a, plan);
-  const int tiles = span_of(a, b).tiles;
+  const int table = in_group / kRows * a.kv_heads + kv, row = in_group % kRows;
+  const int tiles = span_of<kTiles>(a, b).tiles;
+  int64_t before = 0, all = 0;
+  for (int64_t i = tid % 64; i < a.pages.sequences; i += 64) {
+    const int n = span_of<kTiles>(a, i).tiles;
+    before += i < b ? n : 0;
+    all += n;
+  }
+  before = lanes::sum<64>(before);
+  all    = lanes::sum<64>(all);
   if (tiles == 0) { return; }
-  int64_t before = 0;
-  for (int64_t i = tid % 64; i < b; i += 64) { before += span_of(a, i).tiles; }
-  before             = lanes::sum<64>(before) * plan.tables;
-  const int64_t unit = before + int64_t(table) * tiles;
-  const int64_t w0 = sh.of(unit), w1 = sh.of(unit + tiles - 1);
+  const shares sh{all, min(int64_t(plan.shares), all)};
+  const int64_t w0 = sh.of(before), w1 = sh.of(before + tiles - 1);
   if (w0 == w1) { return; }
   const int n = int(w1 - w0) + 1;
-  // the later shares begin inside the row of work: their first slot
-  const int64_t slot0 = 2 * w0 + (sh.first(w0) == unit ? 0 : 1);
-  const auto slot     = [&](int i) { return (i == 0 ? slot0 : 2 * (w0 + i)) * kRows + row; };
+  // the later shares begin inside the sequence: their first slot
+  const int64_t slot0 = 2 * w0 + (sh.first(w0) == before ? 0 : 1);
+  const auto slot     = [&](int i) {
+    return (int64_t(table) * plan.shares * 2 + (i == 0 ? slot0 : 2 * (w0 + i))) * kRows + row;
+  };
 
-  const float mine = tid < n ? plan.part_max[slot(tid)] : -INFINITY;
-  float m          = lanes::max<64>(mine);
+  float m = -INFINITY;
+  for (int i = tid; i < n; i += THREADS) {
+    s_factor[i] = plan.part_max[slot(i)];
+    m           = fmaxf(m, s_factor[i]);
+  }
+  m = lanes::max<64>(m);
   if (tid % 64 == 0) { s_part[tid / 64] = m; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kJoinThreads / 64; ++w) { m = fmaxf(m, s_part[w]); }
-  const float f = factor_of(mine, m);
-  if (tid < n) { s_factor[tid] = f; }
-  const float weighed = lanes::sum<64>(tid < n ? f * plan.part_sum[slot(tid)] : 0.0f);
-  __syncthreads();
-  if (tid % 64 == 0) { s_part[tid / 64] = weighed; }
+  for (int w = 0; w < THREADS / 64; ++w) { m = fmaxf(m, s_part[w]); }
   __syncthreads();
   float sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 64; ++w) { sum += s_part[w]; }
-
-  const int cols = a.vdim <= 64 ? 64 : a.vdim <= 128 ? 128 : 256;
-  const int col = tid % cols, part = tid / cols, parts = kJoinThreads / cols;
-  float acc = 0.0f;
-  if (col < a.vdim) {
-#pragma unroll 8
-    for (int i = part; i < n; i += parts) { acc = __builtin_fmaf(s_factor[i], plan.part_out[slot(i) * a.vdim + col], acc); }
+  for (int i = tid; i < n; i += THREADS) {
+    s_factor[i] = factor_of(s_factor[i], m);
+    sum += s_factor[i] * plan.part_sum[slot(i)];
   }
-  s_out[tid] = acc;
+  sum = lanes::sum<64>(sum);
+  if (tid % 64 == 0) { s_part[tid / 64] = sum; }
   __syncthreads();
-  if (tid < a.vdim) {
-    for (int i = 1; i < parts; ++i) { acc += s_out[i * cols + tid]; }
-    const int64_t at = b * a.heads + h;
-    static_cast<T*>(a.out)[at * a.vdim + tid] = T(sum == 0.0f ? 0.0f : acc / sum);
-    if (tid == 0 && a.lse != nullptr) {
-      a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) { sum += s_part[w]; }
+
+  const int64_t at = b * a.heads + h;
+  const int cols = min(THREADS, a.vdim <= 64 ? 64 : a.vdim <= 128 ? 128 : 256);
+  const int part = tid / cols, parts = THREADS / cols;
+  for (int col0 = 0; col0 < a.vdim; col0 += cols) {  // more than once only with one part
+    const int col = col0 + tid % cols;
+    float acc     = 0.0f;
+    if (col < a.vdim) {
+#pragma unroll 8
+      for (int i = part; i < n; i += parts) { acc = __builtin_fmaf(s_factor[i], plan.part_out[slot(i) * a.vdim + col], acc); }
     }
+    if (parts > 1) {
+      s_out[tid] = acc;
+      __syncthreads();
+    }
+    if (part == 0 && col < a.vdim) {
+      for (int i = 1; i < parts; ++i) { acc += s_out[i * cols + tid]; }
+      static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
+    }
+  }
+  if (tid == 0 && a.lse != nullptr) {
+    a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
   }
 }
 
 int row_tiles_of(attend_args const& a) { return (a.heads / a.kv_heads + kRows - 1) / kRows; }
 
-/** Whether a row of work can be longer than one tile, so that shares can cut it. */
-bool can_split(attend_args const& a)
+/** Most positions of a sequence, from begin rounded down to 8. */
+int64_t longest_of(attend_args const& a)
 {
-  int64_t most = int64_t(a.pages.width) * a.pages.page;
-  if (a.window > 0) { most = std::min(most, a.window + 7); }
-  return most > kStep;
+  const int64_t most = int64_t(a.pages.width) * a.pages.page;
+  return a.window > 0 ? std::min(most, a.window + 7) : most;
+}
+
+/** Whether tables read the same cache lines, so that one die's cache should serve them: several products of query heads
+ *  of a key head, or rows of heads that begin within a line. */
+bool shares_lines(attend_args const& a, int bytes)
+{
+  return row_tiles_of(a) > 1 || (a.kv_heads > 1 && (a.k_head * bytes % 128 != 0 || a.v_head * bytes % 128 != 0));
+}
+
+/** Shares of a table: one workgroup per place on the chip over all tables, two rounds where that would leave places
+ *  empty; no more than there can be tiles. */
+int shares_for(attend_args const& a, int tile, int per_unit)
+{
+  const int64_t places = int64_t(kUnits) * per_unit, tables = int64_t(a.kv_heads) * row_tiles_of(a);
+  int64_t n = std::max<int64_t>(1, places / tables);
+  if (n * tables * 4 < places * 3) { n = (2 * places + tables - 1) / tables; }
+  return int(std::min({n, int64_t(kMaxShares), std::max<int64_t>(1, a.pages.sequences * ((longest_of(a) + tile - 1) / tile))}));
 }
 
 }  // namespace
 
-size_t attend_workspace(elem, attend_args const& a)
+size_t attend_workspace(elem type, attend_args const& a)
 {
-  return can_split(a) ? sizeof(float) * 2 * kShares * kRows * (a.vdim + 2) : 0;
+  const int tile = type == elem::f32 ? kTile<float> : kTile<f16_t>;
+  if (longest_of(a) <= tile) { return 0; }  // nothing to cut
+  // the most shares that any variant takes
+  const size_t slots = size_t(2) * a.kv_heads * row_tiles_of(a) * std::max(shares_for(a, tile, 1), shares_for(a, tile, 2));
+  return sizeof(float) * slots * kRows * (a.vdim + 2);
 }
 
 void attend(elem type, attend_args const& a, hipStream_t stream)
 {
-  attend_plan plan{divisor(uint32_t(a.pages.page / kPageUnit))};
-  plan.row_tiles = row_tiles_of(a);
-  plan.group     = a.heads / a.kv_heads;
-  plan.tables    = a.kv_heads * plan.row_tiles;
-  plan.scale2    = a.scale * kLog2e;
-  plan.part_out  = static_cast<float*>(a.workspace);
-  plan.part_max  = plan.part_out + int64_t(2) * kShares * kRows * a.vdim;
-  plan.part_sum  = plan.part_max + 2 * kShares * kRows;
-  const bool split    = can_split(a);
   const int dim       = std::max(a.dim, a.vdim);
   const auto launched = [&](auto tag, auto bucket, auto how) {
     using T         = decltype(tag);
     constexpr int D = decltype(bucket)::value;
-    plan.shares     = 256 * kPerUnit<T, D>;
-    // without splitting there is at most one tile per sequence and table
-    const int64_t most = split ? plan.shares : std::min<int64_t>(plan.shares, a.pages.sequences * plan.tables);
-    attend_kernel<T, D, decltype(how)::value><<<dim3(uint32_t(most)), kThreads, 0, stream>>>(a, plan);
-    if (split) {
-      join_kernel<T><<<dim3(uint32_t(a.heads), uint32_t(a.pages.sequences)), kJoinThreads, 0, stream>>>(a, plan);
+    attend_plan plan{divisor(uint32_t(a.pages.page / kGroup<T>))};
+    plan.row_tiles  = row_tiles_of(a);
+    plan.group      = a.heads / a.kv_heads;
+    plan.tables     = a.kv_heads * plan.row_tiles;
+    plan.scale2     = a.scale * kLog2e;
+    plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
+    const int64_t slots = int64_t(2) * plan.tables * plan.shares * kRows;
+    plan.part_out   = static_cast<float*>(a.workspace);
+    plan.part_max   = plan.part_out + slots * a.vdim;
+    plan.part_sum   = plan.part_max + slots;
+    plan.one_die        = shares_lines(a, sizeof(T)) && plan.shares >= 8;
+    const int blocks    = (plan.one_die ? (plan.shares + 7) / 8 * 8 : plan.shares) * plan.tables;
+    attend_kernel<T, D, decltype(how)::value><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a, plan);
+    if (longest_of(a) > kTile<T>) {
+      const dim3 grid(uint32_t(a.heads), uint32_t(a.pages.sequences));
+      // a few partials per sequence, or many
+      if (plan.shares <= 8 * a.pages.sequences) {
+        join_kernel<T, 128><<<grid, 128, 0, stream>>>(a, plan);
+      } else {
+        join_kernel<T, 512><<<grid, 512, 0, stream>>>(a, plan);
+      }
     }
   };
   const auto sized = [&](auto tag) {
@@ -623,6 +688,8 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
       dim <= 64 ? launched(tag, std::integral_constant<int, 64>{}, tiny{}) : launched(tag, std::integral_constant<int, 256>{}, tiny{});
     } else if (dim <= 64) {
       bucket(std::integral_constant<int, 64>{});
+    } else if (dim <= 96) {
+      bucket(std::integral_constant<int, 96>{});
     } else if (dim <= 128) {
       bucket(std::integral_constant<int, 128>{});
     } else {
