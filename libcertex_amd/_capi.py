@@ -264,7 +264,9 @@ class Borrowed:
 
 _tls = threading.local()
 
-_VIEW = struct.Struct("=QiiiBBHQQQQQ4q4q")  # a DLManagedTensor, then its extents and strides
+# a DLManagedTensor of n dimensions, then its extents (64 bytes in) and strides (96 bytes in)
+_VIEW = [struct.Struct(f"=QiiiBBHQQQQQ{n}q{32 - 8 * n}x{n}q") for n in range(5)]
+_VIEW_BYTES = 128
 _VIEWS = 12  # of a call
 
 
@@ -273,21 +275,19 @@ class _Views:
     that the next call reuses: a fraction of the time that ctypes structures take to fill."""
 
     def __init__(self):
-        self.buffer = ctypes.create_string_buffer(_VIEWS * _VIEW.size)
+        self.buffer = ctypes.create_string_buffer(_VIEWS * _VIEW_BYTES)
         self.base, self.n = ctypes.addressof(self.buffer), 0
 
     def __call__(self, t):
         """The address of a tensor of the caller's (None: NULL), valid until the thread's next views()."""
         if t is None:
             return None
-        at = self.n * _VIEW.size
+        at = self.n * _VIEW_BYTES
         self.n += 1
-        address, ndim = self.base + at, t.ndim
+        address, ndim, device = self.base + at, t.ndim, t.get_device()  # -1: the host
         code, bits = _DL[t.dtype]
-        pad = (0,) * (4 - ndim)
-        device = t.device
-        _VIEW.pack_into(self.buffer, at, t.data_ptr(), kDLROCM if t.is_cuda else kDLCPU, device.index or 0, ndim, code,
-                        bits, 1, address + 64, address + 96, 0, 0, 0, *t.shape, *pad, *t.stride(), *pad)
+        _VIEW[ndim].pack_into(self.buffer, at, t.data_ptr(), kDLROCM if device >= 0 else kDLCPU, max(device, 0),
+                              ndim, code, bits, 1, address + 64, address + 96, 0, 0, 0, *t.shape, *t.stride())
         return address
 
 

@@ -47,6 +47,7 @@ struct turn_job {
   bool paged = false;
   // set by the launcher
   int32_t items = 0, turned = 0, groups = 0;  // vectors per row, those rotated, groups of heads
+  bool lines = false;                         // one load of a row reads whole cache lines
   int64_t blocks = 0;
 };
 

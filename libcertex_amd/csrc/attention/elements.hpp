@@ -21,6 +21,17 @@ __device__ __forceinline__ pack<T, N> load(const T* p)
 {
   return *reinterpret_cast<const pack<T, N>*>(p);
 }
+/** Elements that the call reads once: not kept in the caches. */
+template <typename T, int N>
+__device__ __forceinline__ pack<T, N> load_once(const T* p)
+{
+  if constexpr (sizeof(T) * N >= 4) {
+    using words = uint32_t __attribute__((ext_vector_type(sizeof(T) * N / 4)));
+    return __builtin_bit_cast(pack<T, N>, __builtin_nontemporal_load(reinterpret_cast<const words*>(p)));
+  } else {
+    return load<T, N>(p);
+  }
+}
 template <typename T, int N>
 __device__ __forceinline__ void store(T* p, pack<T, N> const& v)
 {

@@ -20,20 +20,28 @@ import torch
 from . import _capi as C
 from .index import _require
 
-_ROWS = (torch.float32, torch.float16, torch.bfloat16)
+_ROWS = frozenset((torch.float32, torch.float16, torch.bfloat16))
 _INTS = (torch.int32, torch.int64)
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {None: 0, "linear": 1, "base": 2, "ramp": 3}
 
 
-def _rows(t, what, ndim, like=None):
-    """A row tensor on the GPU of one of the element types, dense in its last dimension."""
+def _refuse_rows(t, what, ndim, like):
+    """Why t is no row tensor of these dimensions (nothing for a subclass that is one)."""
     _require(isinstance(t, torch.Tensor) and t.is_cuda, f"{what} must be a GPU tensor")
     if like is None:
         _require(t.dtype in _ROWS, f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
     else:
         _require(t.dtype == like.dtype, f"{what} must be {like.dtype} as the other tensors, not {t.dtype}")
     _require(t.ndim == ndim, f"{what} must have {ndim} dimensions, not shape {tuple(t.shape)}")
+
+
+def _rows(t, what, ndim, like=None):
+    """A row tensor on the GPU of one of the element types (of `like`'s, if given). The checks come once in one
+    expression: a call that passes spends a fraction of a microsecond on them."""
+    if not (type(t) is torch.Tensor and t.is_cuda and t.ndim == ndim
+            and (t.dtype in _ROWS if like is None else t.dtype == like.dtype)):
+        _refuse_rows(t, what, ndim, like)
     return t
 
 
@@ -44,15 +52,21 @@ def _read(t, what, ndim, like=None):
 
 
 def _ints(t, what, dtypes=_INTS):
-    _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes,
-             f"{what} must be a GPU tensor of " + " or ".join(str(d) for d in dtypes))
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes):
+        raise ValueError(f"{what} must be a GPU tensor of " + " or ".join(str(d) for d in dtypes))
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _no_gradient(*tensors):
     if torch.is_grad_enabled():
-        _require(not any(t is not None and t.requires_grad for t in tensors),
-                 "this operator has no gradient: call it under torch.no_grad()")
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("this operator has no gradient: call it under torch.no_grad()")
+
+
+def _output(like, shape):
+    """A dense tensor of like's type and device."""
+    return torch.empty_like(like) if like.is_contiguous() and like.shape == shape else like.new_empty(shape)
 
 
 class _Rotate(torch.autograd.Function):
@@ -137,11 +151,12 @@ class Rotary:
         return self._rotate(x, positions, bool(transpose), out)
 
     def _rotate(self, x, positions, transpose, out):
-        _require(isinstance(x, torch.Tensor) and x.ndim in (3, 4) and x.shape[-1] == self.head_dim,
-                 f"x must be a tensor (tokens, heads, {self.head_dim}) or (batch, tokens, heads, {self.head_dim})")
+        if not (isinstance(x, torch.Tensor) and x.ndim in (3, 4) and x.shape[-1] == self.head_dim):
+            raise ValueError(f"x must be a tensor (tokens, heads, {self.head_dim}) or (batch, tokens, heads, {self.head_dim})")
         x = _read(x, "x", x.ndim)
         positions = _ints(positions, "positions")
-        _require(positions.shape == x.shape[:-2], f"positions must have shape {tuple(x.shape[:-2])}, one entry per token")
+        if positions.shape != x.shape[:-2]:
+            raise ValueError(f"positions must have shape {tuple(x.shape[:-2])}, one entry per token")
         y = torch.empty_like(x) if out is None else _rows(out, "out", x.ndim, x)
         if out is None and y.stride(-1) != 1:  # a dense tensor in another order of dimensions
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -170,9 +185,9 @@ def append_pages(k, v, k_pages, v_pages, page_table, positions, sequences=None, 
         sequences = _ints(sequences, "sequences")
     if q is not None:
         q = _read(q, "q", 3, k)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if rotary is not None:
-        _require(rotary.head_dim == k.shape[-1], f"this rotation is of heads of {rotary.head_dim}, not {k.shape[-1]}")
+        out = _output(q, q.shape)
+    if rotary is not None and rotary.head_dim != k.shape[-1]:
+        raise ValueError(f"this rotation is of heads of {rotary.head_dim}, not {k.shape[-1]}")
     res, view = C.stream_resources(), C.views()
     C.check(C.lib().cuvsCertexAppendPages(
         res, 0 if rotary is None else rotary._handle(k.device.index), view(k), view(v), view(k_pages), view(v_pages),
@@ -200,9 +215,10 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
     _no_gradient(q, k_pages, v_pages)
     table = _ints(page_table, "page_table", (torch.int32,))
     lengths = _ints(lengths, "lengths")
-    _require(window is None or window >= 1, f"the window must be at least 1, not {window}")
+    if window is not None and window < 1:
+        raise ValueError(f"the window must be at least 1, not {window}")
     window = 0 if window is None else int(window)
-    out = torch.empty((q.shape[0], q.shape[1], v_pages.shape[3]), dtype=q.dtype, device=q.device)
+    out = _output(q, (*q.shape[:2], v_pages.shape[3]))
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     L, res, view = C.lib(), C.stream_resources(), C.views()
     qv, kv, vv, tv = view(q), view(k_pages), view(v_pages), view(table)
@@ -226,9 +242,9 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     _require(isinstance(scores, torch.Tensor) and scores.is_cuda and scores.dtype == torch.float32,
              "scores must be a float32 GPU tensor")
     ids = _ints(ids, "ids")
-    _require(scores.ndim in (2, 3) and scores.shape == ids.shape,
-             f"scores and ids must have one shape (n_heads, queries, k) or (n_heads, k), not {tuple(scores.shape)} "
-             f"and {tuple(ids.shape)}")
+    if scores.ndim not in (2, 3) or scores.shape != ids.shape:
+        raise ValueError(f"scores and ids must have one shape (n_heads, queries, k) or (n_heads, k), not "
+                         f"{tuple(scores.shape)} and {tuple(ids.shape)}")
     values = _read(values, "values", 3 if page_table is None else 4)
     _no_gradient(scores, values)
     if page_table is not None:
@@ -238,7 +254,7 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     if single:
         scores, ids = scores[:, None], ids[:, None]
     scores = scores.contiguous()
-    out = torch.empty((*scores.shape[:2], values.shape[-1]), dtype=values.dtype, device=values.device)
+    out = values.new_empty((*scores.shape[:2], values.shape[-1]))
     lse = torch.empty(scores.shape[:2], dtype=torch.float32, device=values.device) if return_lse else None
     L, res, view = C.lib(), C.stream_resources(), C.views()
     sv, vv, tv = view(scores), view(values), view(page_table)
