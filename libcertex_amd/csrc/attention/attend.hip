@@ -73,6 +73,7 @@ struct attend_plan {
   int32_t group;        // query heads per key head
   int32_t tables;       // key heads x row_tiles: table t is key head t % kv_heads, product t / kv_heads
   int32_t shares;       // of a table's tiles, at most
+  int32_t halve;        // half as many shares where each of those has this many tiles or more (0: never)
   bool one_die;         // the tables of a share run on one die
   float scale2;         // scale log2(e)
   float* part_out;      // [tables][2 shares][kRows][vdim]
@@ -102,13 +103,18 @@ struct shares {
   __device__ __forceinline__ int64_t of(int64_t tile) const { return ((tile + 1) * n - 1) / tiles; }
 };
 
+__device__ __forceinline__ shares split(attend_plan const& p, int64_t tiles)
+{
+  const int64_t half = p.shares / 2;
+  return {tiles, p.halve > 0 && half > 0 && tiles >= half * p.halve ? half : min(int64_t(p.shares), tiles)};
+}
+
 template <int TILE>
 __device__ __forceinline__ shares shares_of(attend_args const& a, attend_plan const& p)
 {
   int64_t mine = 0;
   for (int64_t b = threadIdx.x % 64; b < a.pages.sequences; b += 64) { mine += span_of<TILE>(a, b).tiles; }
-  mine = lanes::sum<64>(mine);
-  return {mine, min(int64_t(p.shares), mine)};
+  return split(p, lanes::sum<64>(mine));
 }
 
 /** The elements of a lane's piece: 16 bytes of a row at any alignment of the elements (the memory takes
@@ -553,7 +559,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(attend_args a, attend_pla
   before = lanes::sum<64>(before);
   all    = lanes::sum<64>(all);
   if (tiles == 0) { return; }
-  const shares sh{all, min(int64_t(plan.shares), all)};
+  const shares sh = split(plan, all);
   const int64_t w0 = sh.of(before), w1 = sh.of(before + tiles - 1);
   if (w0 == w1) { return; }
   const int n = int(w1 - w0) + 1;
@@ -616,7 +622,7 @@ int row_tiles_of(attend_args const& a) { return (a.heads / a.kv_heads + kRows - 
 int64_t longest_of(attend_args const& a)
 {
   const int64_t most = int64_t(a.pages.width) * a.pages.page;
-  return a.window > 0 ? std::min(most, a.window + 7) : most;
+  return a.window > 0 && a.window < most ? std::min(most, a.window + 7) : most;
 }
 
 /** Whether tables read the same cache lines, so that one die's cache should serve them: several products of query heads
@@ -659,6 +665,11 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.tables     = a.kv_heads * plan.row_tiles;
     plan.scale2     = a.scale * kLog2e;
     plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
+    // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and fewer streams are
+    // read faster: 64 sequences up to 8,192 168 -> 159 us, one of 131,072 91.6 -> 89.6 us. Short ones need the other
+    // workgroup while they begin and end (128 sequences up to 1,000: 57 and 65 us), as do smaller steps (heads of 64: 177
+    // and 200 us; float32: 156 and 182 us).
+    plan.halve          = sizeof(T) == 2 && D == 128 && plan.row_tiles == 1 ? 32 : 0;
     const int64_t slots = int64_t(2) * plan.tables * plan.shares * kRows;
     plan.part_out   = static_cast<float*>(a.workspace);
     plan.part_max   = plan.part_out + slots * a.vdim;
