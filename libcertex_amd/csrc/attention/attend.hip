@@ -338,11 +338,11 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       const int next = group + kWaves * 4;
       // values of this step: positions (group + g) * kGrp + 0..kGrp - 1
       const bool have = uint32_t(v_at.page) < uint32_t(a.pages.n_pages);
-      const T* v_page = v_head + int64_t(have ? v_at.page : 0) * a.v_page + int64_t(v_at.slot) * a.v_slot;
+      const T* v_page = v_head + int64_t(have ? v_at.page : 0) * a.v_page;
       typename G::value v[kGrp][kBlocks];
 #pragma unroll
       for (int j = 0; j < kGrp; ++j) {
-        const T* row = v_page + j * a.v_slot;
+        const T* row = v_page + int64_t(v_at.slot + j) * a.v_slot;
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) {
           const int col = (n * 16 + r) * kCols;
