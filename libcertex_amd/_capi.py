@@ -271,33 +271,34 @@ _VIEWS = 12  # of a call
 
 
 class _Views:
-    """DLManagedTensors of one call's tensors, strides included, written into memory of the calling thread
-    that the next call reuses: a fraction of the time that ctypes structures take to fill."""
+    """Memory of a thread for the DLManagedTensors of one call, which the next call reuses."""
 
     def __init__(self):
         self.buffer = ctypes.create_string_buffer(_VIEWS * _VIEW_BYTES)
-        self.base, self.n = ctypes.addressof(self.buffer), 0
-
-    def __call__(self, t):
-        """The address of a tensor of the caller's (None: NULL), valid until the thread's next views()."""
-        if t is None:
-            return None
-        at = self.n * _VIEW_BYTES
-        self.n += 1
-        address, ndim, device = self.base + at, t.ndim, t.get_device()  # -1: the host
-        code, bits = _DL[t.dtype]
-        _VIEW[ndim].pack_into(self.buffer, at, t.data_ptr(), kDLROCM if device >= 0 else kDLCPU, max(device, 0),
-                              ndim, code, bits, 1, address + 64, address + 96, 0, 0, 0, *t.shape, *t.stride())
-        return address
+        self.base = ctypes.addressof(self.buffer)
 
 
-def views():
-    """The calling thread's _Views, empty."""
+def views(*tensors, first=0):
+    """The addresses of DLManagedTensors of the tensors, strides included (None: NULL), valid until the calling thread's next
+    views() (of as many places or more, from `first` on). Written as bytes: ctypes structures take several times as long to
+    fill."""
     v = getattr(_tls, "views", None)
     if v is None:
         v = _tls.views = _Views()
-    v.n = 0
-    return v
+    buffer, base, at, out = v.buffer, v.base, first * _VIEW_BYTES, []
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        address, ndim, device = base + at, t.ndim, t.get_device()  # -1: the host
+        if ndim > 4:
+            raise ValueError(f"tensors have at most 4 dimensions, not shape {tuple(t.shape)}")
+        code, bits = _DL[t.dtype]
+        _VIEW[ndim].pack_into(buffer, at, t.data_ptr(), kDLROCM if device >= 0 else kDLCPU, device if device >= 0 else 0, ndim,
+                              code, bits, 1, address + 64, address + 96, 0, 0, 0, *t.shape, *t.stride())
+        out.append(address)
+        at += _VIEW_BYTES
+    return out
 
 
 def resources():

@@ -30,10 +30,13 @@ cuvsError_t translate(Fn fn)
   return CUVS_ERROR;
 }
 
-void expects(bool ok, std::string const& message)
-{
-  if (!ok) { throw std::invalid_argument("certex: " + message); }
-}
+[[noreturn]] void refuse(std::string const& message) { throw std::invalid_argument("certex: " + message); }
+
+/** The message is only put together where the check fails. */
+#define EXPECTS(ok, message)         \
+  do {                               \
+    if (!(ok)) { refuse(message); }  \
+  } while (0)
 
 constexpr int kMaxDims = 4;
 
@@ -61,28 +64,28 @@ struct tensor {
 
 auto tensor_of(DLManagedTensor* m, const char* name) -> tensor
 {
-  expects(m != nullptr, std::string(name) + " is NULL");
+  EXPECTS(m != nullptr, std::string(name) + " is NULL");
   DLTensor const& t = m->dl_tensor;
   tensor v;
   v.name = name;
   v.ndim = t.ndim;
-  expects(t.ndim >= 1 && t.ndim <= kMaxDims, std::string(name) + " has the wrong number of dimensions");
-  expects(t.shape != nullptr, std::string(name) + " has no shape");
+  EXPECTS(t.ndim >= 1 && t.ndim <= kMaxDims, std::string(name) + " has the wrong number of dimensions");
+  EXPECTS(t.shape != nullptr, std::string(name) + " has no shape");
   v.p      = static_cast<char*>(t.data) + t.byte_offset;
   v.type   = t.dtype;
   v.device = t.device;
-  expects(t.device.device_type == kDLROCM || t.device.device_type == kDLCUDA || t.device.device_type == kDLCUDAManaged,
+  EXPECTS(t.device.device_type == kDLROCM || t.device.device_type == kDLCUDA || t.device.device_type == kDLCUDAManaged,
           std::string(name) + " must be in device memory");
   int64_t dense = 1;
   for (int i = t.ndim - 1; i >= 0; --i) {
-    expects(t.shape[i] >= 0, std::string(name) + " has a negative extent");
+    EXPECTS(t.shape[i] >= 0, std::string(name) + " has a negative extent");
     v.shape[i]  = t.shape[i];
     v.stride[i] = t.strides != nullptr ? t.strides[i] : dense;
-    expects(v.stride[i] >= 0, std::string(name) + " has a negative stride");
+    EXPECTS(v.stride[i] >= 0, std::string(name) + " has a negative stride");
     if (v.shape[i] <= 1) { v.stride[i] = dense; }  // never stepped: keeps alignment rules simple
     dense *= std::max<int64_t>(1, t.shape[i]);
   }
-  expects(v.size() == 0 || t.data != nullptr, std::string(name) + " has no data");
+  EXPECTS(v.size() == 0 || t.data != nullptr, std::string(name) + " has no data");
   return v;
 }
 
@@ -96,19 +99,19 @@ void expects_shape(tensor const& t, std::initializer_list<int64_t> shape)
   if (ok) { return; }
   std::string text;
   for (int64_t n : shape) { text += (text.empty() ? "" : ", ") + std::to_string(n); }
-  expects(false, std::string(t.name) + " must have shape (" + text + ")");
+  refuse(std::string(t.name) + " must have shape (" + text + ")");
 }
 
 void expects_ndim(tensor const& t, int ndim)
 {
-  expects(t.ndim == ndim, std::string(t.name) + " must have " + std::to_string(ndim) + " dimensions");
+  EXPECTS(t.ndim == ndim, std::string(t.name) + " must have " + std::to_string(ndim) + " dimensions");
 }
 
 auto dense(tensor t) -> tensor
 {
   int64_t expect = 1;
   for (int i = t.ndim - 1; i >= 0; --i) {
-    expects(t.stride[i] == expect || t.size() == 0, std::string(t.name) + " must be dense and row major");
+    EXPECTS(t.stride[i] == expect || t.size() == 0, std::string(t.name) + " must be dense and row major");
     expect *= t.shape[i];
   }
   return t;
@@ -127,9 +130,9 @@ auto rows(tensor t, ops::elem* type, bool first) -> tensor
   } else {
     throw std::invalid_argument(std::string("certex: ") + t.name + " must be float32, float16 or bfloat16");
   }
-  expects(first || e == *type, std::string(t.name) + " must have the element type of the other tensors");
+  EXPECTS(first || e == *type, std::string(t.name) + " must have the element type of the other tensors");
   *type = e;
-  expects(t.stride[t.ndim - 1] == 1 || t.size() == 0, std::string(t.name) + " must be dense in its last dimension");
+  EXPECTS(t.stride[t.ndim - 1] == 1 || t.size() == 0, std::string(t.name) + " must be dense in its last dimension");
   return t;
 }
 
@@ -137,7 +140,7 @@ auto rows(tensor t, ops::elem* type, bool first) -> tensor
 auto written(tensor t) -> tensor
 {
   for (int i = 0; i < t.ndim; ++i) {
-    expects(t.stride[i] > 0 || t.size() == 0, std::string(t.name) + " is written and must not be broadcast");
+    EXPECTS(t.stride[i] > 0 || t.size() == 0, std::string(t.name) + " is written and must not be broadcast");
   }
   return t;
 }
@@ -145,7 +148,7 @@ auto written(tensor t) -> tensor
 auto integers(DLManagedTensor* m, const char* name) -> tensor
 {
   tensor t = dense(tensor_of(m, name));
-  expects(t.is(kDLInt, 32) || t.is(kDLInt, 64), std::string(name) + " must be int32 or int64");
+  EXPECTS(t.is(kDLInt, 32) || t.is(kDLInt, 64), std::string(name) + " must be int32 or int64");
   return t;
 }
 
@@ -153,7 +156,7 @@ auto int_vector_of(tensor const& t) -> ops::int_vector { return {t.p, t.is(kDLIn
 
 auto res_of(cuvsResources_t res) -> cuvs::resources&
 {
-  expects(res != 0, "the resources handle is NULL");
+  EXPECTS(res != 0, "the resources handle is NULL");
   return *reinterpret_cast<cuvs::resources*>(res);
 }
 
@@ -161,7 +164,7 @@ template <typename... Ts>
 void expects_device(cuvs::resources const& r, Ts const&... ts)
 {
   for (tensor const* t : {&ts...}) {
-    expects(t->p == nullptr || t->size() == 0 || t->device.device_id == r.device(),
+    EXPECTS(t->p == nullptr || t->size() == 0 || t->device.device_id == r.device(),
             std::string(t->name) + " is on another device than the resources");
   }
 }
@@ -173,10 +176,10 @@ void check_launch() { CERTEX_HIP_TRY(hipGetLastError()); }
 
 auto page_map_of(tensor const& table, int64_t sequences, tensor const& pages) -> ops::page_map
 {
-  expects(table.is(kDLInt, 32), std::string(table.name) + " must be int32");
+  EXPECTS(table.is(kDLInt, 32), std::string(table.name) + " must be int32");
   const int64_t width = table.shape[table.ndim - 1], page = pages.shape[1], n_pages = pages.shape[0];
-  expects(page >= 1, "pages must hold at least one position");
-  expects(n_pages < (int64_t(1) << 31) && page < (int64_t(1) << 31) && width < (int64_t(1) << 31) &&
+  EXPECTS(page >= 1, "pages must hold at least one position");
+  EXPECTS(n_pages < (int64_t(1) << 31) && page < (int64_t(1) << 31) && width < (int64_t(1) << 31) &&
             (page == 0 || width <= ((int64_t(1) << 31) - 1) / page),
           "a sequence's pages hold fewer than 2^31 positions");
   return {static_cast<const int32_t*>(table.p), sequences, int32_t(width), int32_t(n_pages), int32_t(page)};
@@ -192,31 +195,31 @@ struct rotary {
 
 auto rotary_of(cuvsCertexRotary_t r) -> rotary&
 {
-  expects(r != 0, "the rotary handle is NULL");
+  EXPECTS(r != 0, "the rotary handle is NULL");
   return *reinterpret_cast<rotary*>(r);
 }
 
 /** The scaled frequencies and the magnitude. */
 auto frequencies_of(cuvsCertexRotaryParams const& p, double* magnitude) -> std::vector<double>
 {
-  expects(p.rotary_dim >= 2 && p.rotary_dim % 2 == 0, "rotary_dim must be even and at least 2");
-  expects(p.layout == CERTEX_ROTARY_HALF || p.layout == CERTEX_ROTARY_INTERLEAVED, "unknown rotary layout");
-  expects(p.scaling >= CERTEX_ROTARY_NONE && p.scaling <= CERTEX_ROTARY_RAMP, "unknown rotary scaling");
-  expects(std::isfinite(p.base) && p.base >= 1.0, "the rotary base must be at least 1");
-  expects(p.scaling == CERTEX_ROTARY_NONE || (std::isfinite(p.factor) && p.factor >= 1.0),
+  EXPECTS(p.rotary_dim >= 2 && p.rotary_dim % 2 == 0, "rotary_dim must be even and at least 2");
+  EXPECTS(p.layout == CERTEX_ROTARY_HALF || p.layout == CERTEX_ROTARY_INTERLEAVED, "unknown rotary layout");
+  EXPECTS(p.scaling >= CERTEX_ROTARY_NONE && p.scaling <= CERTEX_ROTARY_RAMP, "unknown rotary scaling");
+  EXPECTS(std::isfinite(p.base) && p.base >= 1.0, "the rotary base must be at least 1");
+  EXPECTS(p.scaling == CERTEX_ROTARY_NONE || (std::isfinite(p.factor) && p.factor >= 1.0),
           "the rotary factor must be at least 1");
-  expects(std::isfinite(p.magnitude) && p.magnitude >= 0.0, "the rotary magnitude must not be negative");
+  EXPECTS(std::isfinite(p.magnitude) && p.magnitude >= 0.0, "the rotary magnitude must not be negative");
   const int pairs = p.rotary_dim / 2;
   double base     = p.base;
   if (p.scaling == CERTEX_ROTARY_BASE) {
-    expects(p.rotary_dim > 2, "scaling the base needs more than one pair");
+    EXPECTS(p.rotary_dim > 2, "scaling the base needs more than one pair");
     base *= std::pow(p.factor, double(p.rotary_dim) / (p.rotary_dim - 2));
   }
   const double two_pi = 2.0 * M_PI;
   std::vector<double> f(pairs);
   if (p.scaling == CERTEX_ROTARY_RAMP) {
-    expects(std::isfinite(p.original_length) && p.original_length > 0.0, "the ramp needs the original length");
-    expects(std::isfinite(p.ramp_low) && std::isfinite(p.ramp_high) && p.ramp_low < p.ramp_high,
+    EXPECTS(std::isfinite(p.original_length) && p.original_length > 0.0, "the ramp needs the original length");
+    EXPECTS(std::isfinite(p.ramp_low) && std::isfinite(p.ramp_high) && p.ramp_low < p.ramp_high,
             "the ramp must rise");
   }
   for (int i = 0; i < pairs; ++i) {
@@ -252,18 +255,18 @@ auto attend_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v
   a.kv_heads = int32_t(k->shape[2]);
   a.dim      = int32_t(q->shape[2]);
   a.vdim     = int32_t(v->shape[3]);
-  expects(q->shape[1] >= 1 && q->shape[1] <= 65535 && k->shape[2] >= 1 && q->shape[1] % k->shape[2] == 0,
+  EXPECTS(q->shape[1] >= 1 && q->shape[1] <= 65535 && k->shape[2] >= 1 && q->shape[1] % k->shape[2] == 0,
           "the query heads must be a multiple of the key heads (and at most 65535)");
-  expects(q->shape[0] <= 65535, "at most 65535 sequences");
-  expects(a.dim >= 1 && k->shape[3] == a.dim, "q and k_pages must have the same head dimension");
-  expects(q->shape[2] <= ops::kMaxHeadDim && v->shape[3] >= 1 && v->shape[3] <= ops::kMaxHeadDim,
+  EXPECTS(q->shape[0] <= 65535, "at most 65535 sequences");
+  EXPECTS(a.dim >= 1 && k->shape[3] == a.dim, "q and k_pages must have the same head dimension");
+  EXPECTS(q->shape[2] <= ops::kMaxHeadDim && v->shape[3] >= 1 && v->shape[3] <= ops::kMaxHeadDim,
           "head dimensions must be between 1 and " + std::to_string(ops::kMaxHeadDim));
   expects_shape(*v, {k->shape[0], k->shape[1], k->shape[2], v->shape[3]});
   expects_ndim(*table, 2);
-  expects(table->shape[0] == q->shape[0], "page_table must have one row per sequence");
-  expects(k->shape[1] % ops::kPageUnit == 0 && k->shape[1] >= ops::kPageUnit,
+  EXPECTS(table->shape[0] == q->shape[0], "page_table must have one row per sequence");
+  EXPECTS(k->shape[1] % ops::kPageUnit == 0 && k->shape[1] >= ops::kPageUnit,
           "the page size must be a multiple of " + std::to_string(ops::kPageUnit));
-  expects(window >= 0, "the window must not be negative");
+  EXPECTS(window >= 0, "the window must not be negative");
   a.pages  = page_map_of(*table, q->shape[0], *k);
   a.q      = q->p;
   a.q_seq  = q->stride[0];
@@ -285,7 +288,7 @@ auto select_args_of(DLManagedTensor* scores_, DLManagedTensor* values_, DLManage
 {
   *scores = dense(tensor_of(scores_, "scores"));
   *values = rows(tensor_of(values_, "values"), type, true);
-  expects(scores->is(kDLFloat, 32), "scores must be float32");
+  EXPECTS(scores->is(kDLFloat, 32), "scores must be float32");
   expects_ndim(*scores, 3);
   ops::select_args a;
   const bool paged = table_ != nullptr;
@@ -303,14 +306,14 @@ auto select_args_of(DLManagedTensor* scores_, DLManagedTensor* values_, DLManage
     a.n      = values->shape[1];
     a.v_head = values->stride[0];
     a.v_slot = values->stride[1];
-    expects(a.n < (int64_t(1) << 31), "values hold fewer than 2^31 rows a head");
+    EXPECTS(a.n < (int64_t(1) << 31), "values hold fewer than 2^31 rows a head");
   }
-  expects(scores->shape[0] >= 1 && kv_heads >= 1 && scores->shape[0] % kv_heads == 0,
+  EXPECTS(scores->shape[0] >= 1 && kv_heads >= 1 && scores->shape[0] % kv_heads == 0,
           "the query heads must be a multiple of the value heads");
-  expects(vdim >= 1 && vdim <= ops::kMaxHeadDim,
+  EXPECTS(vdim >= 1 && vdim <= ops::kMaxHeadDim,
           "head dimensions must be between 1 and " + std::to_string(ops::kMaxHeadDim));
-  expects(scores->shape[0] * scores->shape[1] < (int64_t(1) << 24), "at most 2^24 - 1 queries over all heads");
-  expects(scores->shape[2] < (int64_t(1) << 31), "fewer than 2^31 selected rows a query");
+  EXPECTS(scores->shape[0] * scores->shape[1] < (int64_t(1) << 24), "at most 2^24 - 1 queries over all heads");
+  EXPECTS(scores->shape[2] < (int64_t(1) << 31), "fewer than 2^31 selected rows a query");
   a.heads    = int32_t(scores->shape[0]);
   a.kv_heads = int32_t(kv_heads);
   a.vdim     = int32_t(vdim);
@@ -325,12 +328,12 @@ auto select_args_of(DLManagedTensor* scores_, DLManagedTensor* values_, DLManage
 auto workspace_of(cuvs::resources const& r, DLManagedTensor* m, size_t bytes) -> void*
 {
   if (bytes == 0) { return nullptr; }
-  expects(m != nullptr, "this call needs a workspace");
+  EXPECTS(m != nullptr, "this call needs a workspace");
   tensor t = dense(tensor_of(m, "workspace"));
   expects_ndim(t, 1);
-  expects(t.is(kDLUInt, 8), "workspace must be uint8");
-  expects(size_t(t.shape[0]) >= bytes, "the workspace is too small");
-  expects(reinterpret_cast<uintptr_t>(t.p) % 16 == 0, "the workspace must be aligned to 16 bytes");
+  EXPECTS(t.is(kDLUInt, 8), "workspace must be uint8");
+  EXPECTS(size_t(t.shape[0]) >= bytes, "the workspace is too small");
+  EXPECTS(reinterpret_cast<uintptr_t>(t.p) % 16 == 0, "the workspace must be aligned to 16 bytes");
   expects_device(r, t);
   return t.p;
 }
@@ -339,7 +342,7 @@ auto lse_of(cuvs::resources const& r, DLManagedTensor* m, int64_t rows_, int64_t
 {
   if (m == nullptr) { return nullptr; }
   tensor t = dense(tensor_of(m, "lse"));
-  expects(t.is(kDLFloat, 32), "lse must be float32");
+  EXPECTS(t.is(kDLFloat, 32), "lse must be float32");
   expects_shape(t, {rows_, cols});
   expects_device(r, t);
   return static_cast<float*>(t.p);
@@ -352,7 +355,7 @@ extern "C" {
 cuvsError_t cuvsCertexRotaryParamsCreate(cuvsCertexRotaryParams_t* params)
 {
   return translate([=] {
-    expects(params != nullptr, "NULL argument");
+    EXPECTS(params != nullptr, "NULL argument");
     *params = new cuvsCertexRotaryParams{128, CERTEX_ROTARY_HALF, 10000.0, CERTEX_ROTARY_NONE, 1.0, 8192.0,
                                          1.0, 32.0, 0.0};
   });
@@ -366,7 +369,7 @@ cuvsError_t cuvsCertexRotaryParamsDestroy(cuvsCertexRotaryParams_t params)
 cuvsError_t cuvsCertexRotaryFrequencies(cuvsCertexRotaryParams_t params, double* frequencies, double* magnitude)
 {
   return translate([=] {
-    expects(params != nullptr && frequencies != nullptr && magnitude != nullptr, "NULL argument");
+    EXPECTS(params != nullptr && frequencies != nullptr && magnitude != nullptr, "NULL argument");
     const auto f = frequencies_of(*params, magnitude);
     std::copy(f.begin(), f.end(), frequencies);
   });
@@ -375,7 +378,7 @@ cuvsError_t cuvsCertexRotaryFrequencies(cuvsCertexRotaryParams_t params, double*
 cuvsError_t cuvsCertexRotaryCreate(cuvsResources_t res, cuvsCertexRotaryParams_t params, cuvsCertexRotary_t* out)
 {
   return translate([=] {
-    expects(params != nullptr && out != nullptr, "NULL argument");
+    EXPECTS(params != nullptr && out != nullptr, "NULL argument");
     auto& r          = res_of(res);
     double magnitude = 1.0;
     const auto f     = frequencies_of(*params, &magnitude);
@@ -412,14 +415,14 @@ cuvsError_t cuvsCertexRotate(cuvsResources_t res,
     const tensor x = rows(tensor_of(x_, "x"), &type, true);
     const tensor y = written(rows(tensor_of(y_, "y"), &type, false));
     const tensor p = integers(positions_, "positions");
-    expects(x.ndim == 3 || x.ndim == 4, "x must have 3 or 4 dimensions");
+    EXPECTS(x.ndim == 3 || x.ndim == 4, "x must have 3 or 4 dimensions");
     const int o = x.ndim - 3;  // 1: a batch dimension
-    expects(y.ndim == x.ndim && std::equal(x.shape, x.shape + x.ndim, y.shape), "y must have the shape of x");
-    expects(p.ndim == 1 + o && std::equal(x.shape, x.shape + 1 + o, p.shape), "positions must have one entry per token");
-    expects(h.rotary_dim <= x.shape[2 + o], "the rotation is wider than the heads");
+    EXPECTS(y.ndim == x.ndim && std::equal(x.shape, x.shape + x.ndim, y.shape), "y must have the shape of x");
+    EXPECTS(p.ndim == 1 + o && std::equal(x.shape, x.shape + 1 + o, p.shape), "positions must have one entry per token");
+    EXPECTS(h.rotary_dim <= x.shape[2 + o], "the rotation is wider than the heads");
     expects_device(r, x, y, p);
-    expects(h.device == r.device(), "the rotary handle is on another device than the resources");
-    expects(x.shape[1 + o] < (1 << 30) && x.shape[2 + o] < (1 << 30), "x is too large");
+    EXPECTS(h.device == r.device(), "the rotary handle is on another device than the resources");
+    EXPECTS(x.shape[1 + o] < (1 << 30) && x.shape[2 + o] < (1 << 30), "x is too large");
     if (x.size() == 0) { return; }
     ops::turn_args a;
     a.frequencies = h.frequencies.as<uint64_t>();
@@ -472,15 +475,15 @@ cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
     expects_ndim(kp, 4);
     expects_ndim(table, 2);
     const int64_t tokens = k.shape[0], heads = k.shape[1];
-    expects(v.ndim == 3 && v.shape[0] == tokens && v.shape[1] == heads, "v must have the tokens and heads of k");
+    EXPECTS(v.ndim == 3 && v.shape[0] == tokens && v.shape[1] == heads, "v must have the tokens and heads of k");
     expects_shape(kp, {kp.shape[0], kp.shape[1], heads, k.shape[2]});
     expects_shape(vp, {kp.shape[0], kp.shape[1], heads, v.shape[2]});
     expects_shape(p, {tokens});
     expects_device(r, k, v, kp, vp, table, p);
-    expects(heads < (1 << 30) && k.shape[2] < (1 << 30) && v.shape[2] < (1 << 30), "k or v is too large");
+    EXPECTS(heads < (1 << 30) && k.shape[2] < (1 << 30) && v.shape[2] < (1 << 30), "k or v is too large");
     if (h != nullptr) {
-      expects(h->rotary_dim <= k.shape[2], "the rotation is wider than the heads");
-      expects(h->device == r.device(), "the rotary handle is on another device than the resources");
+      EXPECTS(h->rotary_dim <= k.shape[2], "the rotation is wider than the heads");
+      EXPECTS(h->device == r.device(), "the rotary handle is on another device than the resources");
     }
     ops::turn_args a;
     a.positions = int_vector_of(p);
@@ -490,7 +493,7 @@ cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
       expects_device(r, s);
       a.sequences = int_vector_of(s);
     } else {
-      expects(table.shape[0] >= tokens, "without sequences, page_table must have one row per token");
+      EXPECTS(table.shape[0] >= tokens, "without sequences, page_table must have one row per token");
     }
     if (h != nullptr) {
       a.frequencies = h->frequencies.as<uint64_t>();
@@ -521,7 +524,7 @@ cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
     if (q_ != nullptr) {
       const tensor q  = rows(tensor_of(q_, "q"), &type, false);
       const tensor qo = written(rows(tensor_of(q_out_, "q_out"), &type, false));
-      expects(q.ndim == 3 && q.shape[0] == tokens && q.shape[2] == k.shape[2], "q must have the tokens and head dimension of k");
+      EXPECTS(q.ndim == 3 && q.shape[0] == tokens && q.shape[2] == k.shape[2], "q must have the tokens and head dimension of k");
       expects_shape(qo, {q.shape[0], q.shape[1], q.shape[2]});
       expects_device(r, q, qo);
       add(q, qo, rotated, false);
@@ -540,7 +543,7 @@ cuvsError_t cuvsCertexPagedAttentionWorkspace(DLManagedTensor* q_,
                                               int64_t* bytes)
 {
   return translate([=] {
-    expects(bytes != nullptr, "NULL argument");
+    EXPECTS(bytes != nullptr, "NULL argument");
     ops::elem type{};
     tensor q, k, v, table;
     const auto a = attend_args_of(q_, k_pages_, v_pages_, page_table_, window, &type, &q, &k, &v, &table);
@@ -570,7 +573,7 @@ cuvsError_t cuvsCertexPagedAttention(cuvsResources_t res,
     const tensor out = dense(rows(tensor_of(out_, "out"), &type, false));
     expects_shape(out, {q.shape[0], q.shape[1], v.shape[3]});
     expects_device(r, q, k, v, table, lengths, out);
-    expects(std::isfinite(scale), "the scale must be finite");
+    EXPECTS(std::isfinite(scale), "the scale must be finite");
     a.lse = lse_of(r, lse_, q.shape[0], q.shape[1]);
     if (q.shape[0] == 0) { return; }
     a.lengths   = int_vector_of(lengths);
@@ -588,7 +591,7 @@ cuvsError_t cuvsCertexSelectedAttentionWorkspace(DLManagedTensor* scores_,
                                                  int64_t* bytes)
 {
   return translate([=] {
-    expects(bytes != nullptr, "NULL argument");
+    EXPECTS(bytes != nullptr, "NULL argument");
     ops::elem type{};
     tensor scores, values, table;
     const auto a = select_args_of(scores_, values_, page_table_, &type, &scores, &values, &table);
@@ -616,7 +619,7 @@ cuvsError_t cuvsCertexSelectedAttention(cuvsResources_t res,
     const tensor out = dense(rows(tensor_of(out_, "out"), &type, false));
     expects_shape(out, {scores.shape[0], scores.shape[1], int64_t(a.vdim)});
     expects_device(r, scores, ids, values, table, out);
-    expects(std::isfinite(scale), "the scale must be finite");
+    EXPECTS(std::isfinite(scale), "the scale must be finite");
     a.lse = lse_of(r, lse_, scores.shape[0], scores.shape[1]);
     if (a.queries == 0) { return; }
     a.ids       = int_vector_of(ids);

@@ -82,7 +82,9 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         (positions,) = ctx.saved_tensors
-        return _Rotate.apply(dy, positions, ctx.rope, not ctx.transpose), None, None, None
+        if torch.is_grad_enabled():  # a gradient of the gradient was asked for
+            return _Rotate.apply(dy, positions, ctx.rope, not ctx.transpose), None, None, None
+        return ctx.rope._rotate(dy, positions, not ctx.transpose, None), None, None, None
 
 
 class Rotary:
@@ -161,8 +163,8 @@ class Rotary:
         if out is None and y.stride(-1) != 1:  # a dense tensor in another order of dimensions
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         _require(y.shape == x.shape, "out must have the shape of x")
-        res, view = C.stream_resources(), C.views()
-        C.check(C.lib().cuvsCertexRotate(res, self._handle(x.device.index), view(x), view(positions), view(y), transpose))
+        C.check(C.lib().cuvsCertexRotate(C.stream_resources(), self._handle(x.get_device()), *C.views(x, positions, y),
+                                         transpose))
         return y
 
 
@@ -188,15 +190,10 @@ def append_pages(k, v, k_pages, v_pages, page_table, positions, sequences=None, 
         out = _output(q, q.shape)
     if rotary is not None and rotary.head_dim != k.shape[-1]:
         raise ValueError(f"this rotation is of heads of {rotary.head_dim}, not {k.shape[-1]}")
-    res, view = C.stream_resources(), C.views()
     C.check(C.lib().cuvsCertexAppendPages(
-        res, 0 if rotary is None else rotary._handle(k.device.index), view(k), view(v), view(k_pages), view(v_pages),
-        view(table), view(positions), view(sequences), view(q), view(out)))
+        C.stream_resources(), 0 if rotary is None else rotary._handle(k.get_device()),
+        *C.views(k, v, k_pages, v_pages, table, positions, sequences, q, out)))
     return out
-
-
-def _workspace(bytes_, device):
-    return torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
 
 
 def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window=None, return_lse=False):
@@ -220,14 +217,13 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
     window = 0 if window is None else int(window)
     out = _output(q, (*q.shape[:2], v_pages.shape[3]))
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    L, res, view = C.lib(), C.stream_resources(), C.views()
-    qv, kv, vv, tv = view(q), view(k_pages), view(v_pages), view(table)
-    need = ctypes.c_int64()
+    L, need = C.lib(), ctypes.c_int64()
+    qv, kv, vv, tv, lv, ov, ev = C.views(q, k_pages, v_pages, table, lengths, out, lse)
     C.check(L.cuvsCertexPagedAttentionWorkspace(qv, kv, vv, tv, window, ctypes.byref(need)))
-    work = _workspace(need.value, q.device)
-    C.check(L.cuvsCertexPagedAttention(res, qv, kv, vv, tv, view(lengths),
-                                       q.shape[2] ** -0.5 if scale is None else float(scale), window, view(work),
-                                       view(out), view(lse)))
+    work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    C.check(L.cuvsCertexPagedAttention(C.stream_resources(), qv, kv, vv, tv, lv,
+                                       q.shape[2] ** -0.5 if scale is None else float(scale), window,
+                                       *C.views(work, first=7), ov, ev))
     return (out, lse) if return_lse else out
 
 
@@ -256,12 +252,11 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     scores = scores.contiguous()
     out = values.new_empty((*scores.shape[:2], values.shape[-1]))
     lse = torch.empty(scores.shape[:2], dtype=torch.float32, device=values.device) if return_lse else None
-    L, res, view = C.lib(), C.stream_resources(), C.views()
-    sv, vv, tv = view(scores), view(values), view(page_table)
-    need = ctypes.c_int64()
+    L, need = C.lib(), ctypes.c_int64()
+    sv, iv, vv, tv, ov, ev = C.views(scores, ids, values, page_table, out, lse)
     C.check(L.cuvsCertexSelectedAttentionWorkspace(sv, vv, tv, ctypes.byref(need)))
-    work = _workspace(need.value, values.device)
-    C.check(L.cuvsCertexSelectedAttention(res, sv, view(ids), vv, tv, float(scale), view(work), view(out), view(lse)))
+    work = values.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    C.check(L.cuvsCertexSelectedAttention(C.stream_resources(), sv, iv, vv, tv, float(scale), *C.views(work, first=6), ov, ev))
     if single:
         out, lse = out[:, 0], None if lse is None else lse[:, 0]
     return (out, lse) if return_lse else out
