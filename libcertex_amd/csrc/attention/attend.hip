@@ -256,17 +256,59 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
   const int rows = min(kRows, plan.group - row0), h0 = kv * plan.group + row0;
   const T* k_head = static_cast<const T*>(a.k) + kv * a.k_head;
   const T* v_head = static_cast<const T*>(a.v) + kv * a.v_head;
-  bool first      = true;
-  for (; tile < last; first = false) {
-    const span sp = span_of<kTiles>(a, b);
-    if (sp.tiles == 0) {
-      ++b;
-      continue;
-    }
-    const int t0 = int(tile - before), t1 = int(min(int64_t(sp.tiles), t0 + last - tile));
 
+  // the page of a group's positions, and the first one's slot
+  struct place {
+    int32_t page, slot;
+  };
+  span sp{};
+  int t0 = 0, t1 = 0, group = 0, stop = 0, final = 0;
+  const int32_t* pages = nullptr;
+  place v_at{};
+  u32x4 q[kChunks], k[kHalves][kChunks];
+  const auto entry = [&](int group) {
+    const int at = min(group, final);
+    const int e  = int(plan.page_groups(uint32_t(at)));
+    return place{pages[e], (at - e * int(plan.page_groups.d)) * kGrp};
+  };
+  const auto load_keys = [&](place at) {
+    const int page  = uint32_t(at.page) < uint32_t(a.pages.n_pages) ? at.page : 0;
+    const T* k_page = k_head + int64_t(page) * a.k_page;
+#pragma unroll
+    for (int half = 0; half < kHalves; ++half) {
+      const T* row = k_page + int64_t(at.slot + half * 4 + r % 4) * a.k_slot;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int dim0 = (c * 4 + g) * kPiece;
+        if constexpr (TINY) {
+          T e[kPiece];
+#pragma unroll
+          for (int j = 0; j < kPiece; ++j) { e[j] = dim0 + j < dim ? row[dim0 + j] : T(0.0f); }
+          __builtin_memcpy(&k[half][c], e, 16);
+        } else {
+          // the piece that a row ends in is taken from the row's end: dimensions that an earlier piece holds come again
+          k[half][c] = piece<16>(row + (FULL ? dim0 : min(dim0, key_off)));
+        }
+      }
+    }
+  };
+  // the share's tiles of sequence b (or of the next that has any): their range, and the first step's loads
+  const auto begin = [&] {
+    for (sp = span_of<kTiles>(a, b); sp.tiles == 0; sp = span_of<kTiles>(a, b)) { ++b; }
+    t0              = int(tile - before);
+    t1              = int(min(int64_t(sp.tiles), t0 + last - tile));
+    pages           = a.pages.table + b * a.pages.width;
+    const int start = sp.begin / 8 * (8 / kGrp);  // in lane groups' positions
+    final           = (sp.end - 1) / kGrp;
+    // a wave's steps: one in every tile that reaches it
+    group = start + (t0 * kWaves + wave) * 4;
+    stop  = min(start + t1 * kWaves * 4, final + 1);
+    place k_at{};
+    if (group < stop) {
+      k_at = entry(group + r / 4);
+      v_at = entry(group + g);
+    }
     // the queries: column r, pieces of the dimensions that this lane's group holds
-    u32x4 q[kChunks];
     const T* q_row = static_cast<const T*>(a.q) + b * a.q_seq + (h0 + min(r, rows - 1)) * a.q_head;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
@@ -277,63 +319,27 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         for (int j = 0; j < kPiece; ++j) { e[j] = dim0 + j < dim ? q_row[dim0 + j] : T(0.0f); }
         __builtin_memcpy(&q[c], e, 16);
       } else {
-        // the piece that a row ends in is taken from the row's end: dimensions that an earlier piece holds are 0
         q[c] = piece<16>(q_row + (FULL ? dim0 : min(dim0, key_off)));
       }
+    }
+    if (group < stop) { load_keys(k_at); }
+  };
+
+  begin();
+  for (bool first = true;; first = false) {
+    // query heads that there are not, dimensions that come twice: 0
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int dim0 = (c * 4 + g) * kPiece;
       const int skip = FIT == fit::part ? dim0 - min(dim0, key_off) : 0;
 #pragma unroll
       for (int w = 0; w < 4; ++w) { q[c][w] = r < rows ? q[c][w] & counted<T>(skip, w) : 0u; }
     }
-
-    const int32_t* pages = a.pages.table + b * a.pages.width;
-    const int start      = sp.begin / 8 * (8 / kGrp);  // in lane groups' positions
-    const int final      = (sp.end - 1) / kGrp;
-
     f32x4 o[kOut];
 #pragma unroll
     for (int i = 0; i < kOut; ++i) { o[i] = f32x4{0, 0, 0, 0}; }
     float top = -INFINITY, limit = -INFINITY, base = 0.0f, total = 0.0f;
 
-    // the page of a group's positions, and the first one's slot
-    struct place {
-      int32_t page, slot;
-    };
-    const auto entry = [&](int group) {
-      const int at = min(group, final);
-      const int e  = int(plan.page_groups(uint32_t(at)));
-      return place{pages[e], (at - e * int(plan.page_groups.d)) * kGrp};
-    };
-    u32x4 k[kHalves][kChunks];
-    const auto load_keys = [&](place at) {
-      const int page  = uint32_t(at.page) < uint32_t(a.pages.n_pages) ? at.page : 0;
-      const T* k_page = k_head + int64_t(page) * a.k_page;
-#pragma unroll
-      for (int half = 0; half < kHalves; ++half) {
-        const T* row = k_page + int64_t(at.slot + half * 4 + r % 4) * a.k_slot;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int dim0 = (c * 4 + g) * kPiece;
-          if constexpr (TINY) {
-            T e[kPiece];
-#pragma unroll
-            for (int j = 0; j < kPiece; ++j) { e[j] = dim0 + j < dim ? row[dim0 + j] : T(0.0f); }
-            __builtin_memcpy(&k[half][c], e, 16);
-          } else {
-            k[half][c] = piece<16>(row + (FULL ? dim0 : min(dim0, key_off)));
-          }
-        }
-      }
-    };
-
-    // a wave's steps: one in every tile of the segment that reaches it
-    int group      = start + (t0 * kWaves + wave) * 4;
-    const int stop = min(start + t1 * kWaves * 4, final + 1);
-    place k_at{}, v_at{};
-    if (group < stop) {
-      k_at = entry(group + r / 4);
-      v_at = entry(group + g);
-      load_keys(k_at);
-    }
     while (group < stop) {
       const int next = group + kWaves * 4;
       // values of this step: positions (group + g) * kGrp + 0..kGrp - 1
@@ -390,8 +396,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       }
       // the next step's pages and keys
       if (next < stop) {
-        k_at = entry(next + r / 4);
-        v_at = entry(next + g);
+        const place k_at = entry(next + r / 4);
+        v_at             = entry(next + g);
         load_keys(k_at);
       }
       // weights: lane group g holds the positions t + 0..kGrp - 1 of query r
@@ -474,7 +480,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       group = next;
     }
 
-    // join the waves
+    // join the waves, while the next sequence's first loads are in flight
     total = lanes::fold32(total, [](float u, float w) { return u + w; });
     total = lanes::fold16(total, [](float u, float w) { return u + w; });
     __syncthreads();
@@ -496,8 +502,16 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         }
       }
     }
-    __syncthreads();
     const bool done    = t0 == 0 && t1 == sp.tiles;
+    const int64_t out0 = b * a.heads + h0;
+    tile += t1 - t0;
+    const bool more = tile < last;
+    if (t1 == sp.tiles) {
+      before += sp.tiles;
+      ++b;
+    }
+    if (more) { begin(); }
+    __syncthreads();
     const int64_t slot = (int64_t(table) * plan.shares + share) * 2 + (first ? 0 : 1);
     constexpr int kOnce = kThreads / D;  // rows at a time
     const int col       = tid % D;
@@ -513,7 +527,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         acc += f * s_out[w][row][col];
       }
       if (done) {
-        const int64_t at = b * a.heads + h0 + row;
+        const int64_t at = out0 + row;
         if (col < vdim) { static_cast<T*>(a.out)[at * vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum); }
         if (col == 0 && a.lse != nullptr) {
           a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
@@ -526,11 +540,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         }
       }
     }
-    tile += t1 - t0;
-    if (t1 == sp.tiles) {
-      before += sp.tiles;
-      ++b;
-    }
+    if (!more) { break; }
   }
 }
 
