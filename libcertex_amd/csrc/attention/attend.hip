@@ -75,7 +75,8 @@ struct attend_plan {
   int32_t shares;       // of a table's tiles, at most
   int32_t halve;        // half as many shares where each of those has this many tiles or more (0: never)
   bool one_die;         // the tables of a share run on one die
-  float scale2;         // scale log2(e)
+  float scale2;         // scale log2(e), and what that is rounded by
+  float scale2_rest;
   float* part_out;      // [tables][2 shares][kRows][vdim]
   float* part_max;      // [tables][2 shares][kRows]
   float* part_sum;
@@ -435,7 +436,13 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       }
       float p[kGrp];
 #pragma unroll
-      for (int j = 0; j < kGrp; ++j) { p[j] = __builtin_amdgcn_exp2f(x[j] - base); }
+      for (int j = 0; j < kGrp; ++j) {
+        // float32: the exponent is rounded once, after the subtraction, and the scale's own rounding is made up for
+        p[j] = __builtin_amdgcn_exp2f(
+          G::kWide && x[j] != -INFINITY
+            ? __builtin_fmaf(s[j / 4][j % 4], plan.scale2, __builtin_fmaf(s[j / 4][j % 4], plan.scale2_rest, -base))
+            : x[j] - base);
+      }
 #pragma unroll
       for (int j = 0; j < kGrp; j += 4) { total += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]); }
 
@@ -452,16 +459,14 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
           }
         }
       } else {
-        // bfloat16 weights enter as value and remainder: 8 bits alone would cost as much as the output's own
-        // rounding. float16 weights are rounded once (11 bits).
+        // the weights enter as value and remainder: rounded once, to 8 or 11 bits, they would cost as much as the
+        // output's own rounding, and the matrix cores wait for memory
         u32x4 hi, lo;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          hi[w] = pack2<T>(p[2 * w], p[2 * w + 1]);
-          if constexpr (std::is_same_v<T, bf16_t>) {
-            lo[w] = pack2<T>(p[2 * w] - __builtin_bit_cast(float, hi[w] << 16),
-                             p[2 * w + 1] - __builtin_bit_cast(float, hi[w] & 0xffff0000u));
-          }
+          const T even = T(p[2 * w]), odd = T(p[2 * w + 1]);
+          hi[w]       = pack2<T>(p[2 * w], p[2 * w + 1]);
+          lo[w]       = pack2<T>(p[2 * w] - float(even), p[2 * w + 1] - float(odd));
         }
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) {
@@ -473,7 +478,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
               vt[w] = __builtin_amdgcn_perm(v[2 * w + 1][n][e / 2], v[2 * w][n][e / 2], e % 2 == 0 ? 0x05040100u : 0x07060302u);
             }
             o[n * kCols + e] = mfma(T{}, vt, hi, o[n * kCols + e]);
-            if constexpr (std::is_same_v<T, bf16_t>) { o[n * kCols + e] = mfma(T{}, vt, lo, o[n * kCols + e]); }
+            o[n * kCols + e] = mfma(T{}, vt, lo, o[n * kCols + e]);
           }
         }
       }
@@ -673,7 +678,8 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.row_tiles  = row_tiles_of(a);
     plan.group      = a.heads / a.kv_heads;
     plan.tables     = a.kv_heads * plan.row_tiles;
-    plan.scale2     = a.scale * kLog2e;
+    plan.scale2      = float(double(a.scale) * M_LOG2E);
+    plan.scale2_rest = float(double(a.scale) * M_LOG2E - double(plan.scale2));
     plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
     // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and fewer streams are
     // read faster: 64 sequences up to 8,192 168 -> 159 us, one of 131,072 91.6 -> 89.6 us. Short ones need the other

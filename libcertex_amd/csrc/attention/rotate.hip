@@ -3,8 +3,9 @@
 // Position p turns pair i of a head by the angle p f_i: (a, b) -> m (a cos - b sin, a sin + b cos).
 // The frequencies are kept in turns as 64-bit fixed point, so p f_i modulo one turn is the low half
 // of one integer product: exact for every position, where a float32 product loses the angle (at
-// position 131,072 it is 0.008 radians off), and nothing is read from a table. The top 32 bits of
-// the fraction go to sin and cos of half turns: the angle is within 2^-24 of itself.
+// position 131,072 it is 0.008 radians off), and nothing is read from a table. The top 24 bits of
+// the fraction go to sin and cos of half turns as they are, the next 8 turn the result by their small angle, so that the
+// angle costs the sines less than their own rounding.
 #include "attention.hpp"
 #include "elements.hpp"
 
@@ -93,8 +94,12 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
   if (turned) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const uint64_t turns = uint64_t(p) * a.frequencies[int(item) * P + i];
-      sincospif(float(int32_t(turns >> 32)) * 0x1p-31f, &s[i], &c[i]);
+      const uint32_t turns = uint32_t((uint64_t(p) * a.frequencies[int(item) * P + i]) >> 32);
+      float sine, cosine;
+      sincospif(float(int32_t(turns & ~255u)) * 0x1p-31f, &sine, &cosine);
+      const float rest = float(turns & 255u) * float(M_PI * 0x1p-31);
+      s[i]             = __builtin_fmaf(cosine, rest, sine);
+      c[i]             = __builtin_fmaf(sine, -rest, cosine);
       c[i] *= a.magnitude;
       s[i] *= a.transpose ? -a.magnitude : a.magnitude;
     }
