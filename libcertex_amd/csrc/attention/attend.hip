@@ -8,20 +8,27 @@
 // it, a few operations per byte, so the rate at which memory is read. The kernel keeps the two products
 // off the critical path by giving them to the matrix cores in a form that needs no exchange between lanes
 // and no LDS:
-// - a wave takes 32 positions (float32: 16); S^T = K Q^T has the positions as rows and up to 16 query heads as columns, so that
-//   K rows go from memory to the operand registers as they lie (16 bytes of a row per lane);
+// - a wave takes 32 positions (float32: 16); S^T = K Q^T has the positions as rows and up to 16 query heads
+//   as columns, so that K rows go from memory to the operand registers as they lie (16 bytes per lane);
 // - the rows of the two 16-position products are permuted such that a lane's 8 results are the 8
 //   consecutive positions that it holds as k-slots of O^T = V^T P^T: the weights never move;
-// - V^T is formed in registers: a lane loads 8 positions x 8 columns (16 bytes of a row each, whole rows per 16
-//   lanes) and swaps halfwords (v_perm), 32 instructions per 32 x 128 values;
+// - V^T is formed in registers: a lane loads 8 positions x 8 columns (16 bytes of a row each, whole rows
+//   per 16 lanes) and swaps halfwords (v_perm), 32 instructions per 32 x 128 values (float32: as it lies);
 // - m, the sum and the scaling are per query head, that is per lane.
 // The loads of the next keys and of this tile's values are in flight during both products.
 //
-// Work is dealt on the device, from the lengths: the tiles of all sequences, one after the other, in equal shares, each
-// share to one workgroup per key head. So any mix of lengths fills the chip and the host reads nothing back, and the
-// heads of a position are read at about the same time (they are neighbours in memory where a slot holds all heads). A
-// share that cuts a sequence leaves a partial (m, sum, output) in the workspace, and a second launch joins them in order of
-// position.
+//
+// Work is dealt on the device, from the lengths: the tiles of all sequences, one after the other, in
+// equal shares, each share to one workgroup per key head. So any mix of lengths fills the chip and the
+// host reads nothing back, and the heads of a position are read at about the same time (they are
+// neighbours in memory where a slot holds all heads). A share that cuts a sequence leaves a partial
+// (m, sum, output) in the workspace, and a second launch joins them in order of position.
+//
+// Measured (8 key heads of 128 bfloat16, 32 query heads; reading alone reaches 6.4 TB/s): 64 sequences up
+// to 8,192, 0.94 GB of keys and values: 158 us with the 6 us of the join, 5.9 TB/s; one sequence of
+// 131,072, 0.54 GB: 88 us, 6.1 TB/s; four of up to 131,072: 6.3 TB/s. Heads of 64: 5.4 TB/s where a slot holds
+// all heads (128 bytes of a line pair each), 6.2 with the heads first. More workgroups or waves per
+// compute unit read slower (three: 193 us for the 64 sequences): the memory prefers fewer streams.
 #include "../kernels/lanes.hpp"
 #include "attention.hpp"
 #include "elements.hpp"
@@ -44,8 +51,8 @@ using u32x2  = __attribute__((ext_vector_type(2))) uint32_t;
 using f16x8  = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
-/** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less than 1, so n m / 2^(29 + s)
- *  exceeds n / d by less than 1 / d. */
+/** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less
+ *  than 1, so n m / 2^(29 + s) exceeds n / d by less than 1 / d. */
 struct divisor {
   uint32_t m, shift, d;
   explicit divisor(uint32_t by) : d(by)
@@ -61,11 +68,9 @@ struct divisor {
 /** Positions of a lane group in a step: its rows of the 16-position products (two of 16 bits, one of float32). */
 template <typename T>
 constexpr int kGroup = sizeof(T) == 4 ? 4 : 8;
-/** Positions of a wave's step, and of a workgroup's: a tile. */
+/** Positions of a workgroup's step: a tile. */
 template <typename T>
-constexpr int kStep = 4 * kGroup<T>;
-template <typename T>
-constexpr int kTile = kStep<T> * kWaves;
+constexpr int kTile = 4 * kGroup<T> * kWaves;
 
 struct attend_plan {
   divisor page_groups;  // lane groups' positions per page
@@ -134,8 +139,9 @@ __device__ __forceinline__ auto piece(const T* p)
   }
 }
 
-/** A value piece: read once by the call, so it is not kept in the caches. Measured: 64 sequences up to 8,192 184 -> 168 us, one of
- *  131,072 103 -> 92 us. (Key pieces are half lines, whose other half is the next load's: 184 -> 181 us alone, 176 us together.) */
+/** A value piece: read once by the call, so it is not kept in the caches. Measured: 64 sequences up to 8,192
+ *  184 -> 168 us, one of 131,072 103 -> 92 us. (Key pieces are half lines, whose other half is the next
+ *  load's: reading them past the caches 184 -> 181 us alone, 176 us together.) */
 template <int BYTES, typename T>
 __device__ __forceinline__ auto passing_piece(const T* p)
 {
@@ -155,7 +161,6 @@ struct geometry {
   static constexpr int kBlocks = (D + 16 * kCols - 1) / (16 * kCols);  // pieces of a lane per value row
   static constexpr bool kWhole = D % (16 * kCols) == 0;                // no piece of a full row is past its end
   static constexpr int kHalves = kGroup<T> / 4;             // 16-position products of a step
-  using key   = u32x4;
   using value = std::conditional_t<kCols * sizeof(T) == 16, u32x4, u32x2>;
 };
 
@@ -550,8 +555,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
 }
 
 /**
- * One workgroup per sequence and query head: joins the partials of a sequence that shares cut. Their factors first, in
- * LDS; then a thread per column and part of the partials.
+ * One workgroup per sequence and query head: joins the partials of a sequence that shares cut. Their
+ * factors first, in LDS; then a thread per column and part of the partials.
  */
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void join_kernel(attend_args a, attend_plan plan)
@@ -640,8 +645,9 @@ int64_t longest_of(attend_args const& a)
   return a.window > 0 && a.window < most ? std::min(most, a.window + 7) : most;
 }
 
-/** Whether tables read the same cache lines, so that one die's cache should serve them: several products of query heads
- *  of a key head, or rows of heads that begin within a line. */
+/** Whether tables read the same cache lines, so that one die's cache should serve them: several products of
+ *  query heads of a key head, or rows of heads that begin within a line. Measured, over all dies and on one: 32
+ *  query heads of one key head 147 and 114 us, heads of 80 145 and 131 us; of 128 168 and 174 us. */
 bool shares_lines(attend_args const& a, int bytes)
 {
   return row_tiles_of(a) > 1 || (a.kv_heads > 1 && (a.k_head * bytes % 128 != 0 || a.v_head * bytes % 128 != 0));
@@ -681,10 +687,10 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.scale2      = float(double(a.scale) * M_LOG2E);
     plan.scale2_rest = float(double(a.scale) * M_LOG2E - double(plan.scale2));
     plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
-    // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and fewer streams are
-    // read faster: 64 sequences up to 8,192 168 -> 159 us, one of 131,072 91.6 -> 89.6 us. Short ones need the other
-    // workgroup while they begin and end (128 sequences up to 1,000: 57 and 65 us), as do smaller steps (heads of 64: 177
-    // and 200 us; float32: 156 and 182 us).
+    // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and
+    // fewer streams are read faster: 64 sequences up to 8,192 168 -> 159 us, one of 131,072 91.6 -> 89.6 us.
+    // Short ones need the other workgroup while they begin and end (128 sequences up to 1,000: 57 and 65 us),
+    // as do smaller steps (heads of 64: 177 and 200 us; float32: 156 and 182 us).
     plan.halve          = sizeof(T) == 2 && D == 128 && plan.row_tiles == 1 ? 32 : 0;
     const int64_t slots = int64_t(2) * plan.tables * plan.shares * kRows;
     plan.part_out   = static_cast<float*>(a.workspace);

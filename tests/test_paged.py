@@ -3,6 +3,8 @@ the C entry points."""
 
 import ctypes
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -137,3 +139,12 @@ def test_selection_checks():
     ]:
         with pytest.raises(ValueError, match=match):
             need(**kw)
+
+
+def test_header_is_c():
+    """certex_attention.h compiles as C99, warnings as errors."""
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    source = "#include <cuvs/neighbors/certex_attention.h>\nint main(void) { return CERTEX_ROTARY_HALF; }\n"
+    r = subprocess.run(["gcc", "-std=c99", "-Wall", "-Wextra", "-Werror", "-fsyntax-only", "-I", include, "-x", "c", "-"],
+                       input=source, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
