@@ -701,7 +701,7 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     attend_kernel<T, D, decltype(how)::value><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a, plan);
     if (longest_of(a) > kTile<T>) {
       const dim3 grid(uint32_t(a.heads), uint32_t(a.pages.sequences));
-      // a few partials per sequence, or many
+      // a few partials per sequence, or many (64 sequences: 13 us with 512 threads, 6 with 128)
       if (plan.shares <= 8 * a.pages.sequences) {
         join_kernel<T, 128><<<grid, 128, 0, stream>>>(a, plan);
       } else {

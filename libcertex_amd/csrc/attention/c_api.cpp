@@ -86,6 +86,8 @@ auto tensor_of(DLManagedTensor* m, const char* name) -> tensor
     dense *= std::max<int64_t>(1, t.shape[i]);
   }
   EXPECTS(v.size() == 0 || t.data != nullptr, std::string(name) + " has no data");
+  EXPECTS(reinterpret_cast<uintptr_t>(v.p) % std::max(1, t.dtype.bits / 8) == 0,
+          std::string(name) + " must begin at a multiple of its element size");
   return v;
 }
 

@@ -21,6 +21,20 @@ __device__ __forceinline__ pack<T, N> load(const T* p)
 {
   return *reinterpret_cast<const pack<T, N>*>(p);
 }
+/** The same at any address of the elements: the memory takes misaligned vectors. */
+template <typename T, int N>
+__device__ __forceinline__ pack<T, N> load_loose(const T* p)
+{
+  pack<T, N> v;
+  __builtin_memcpy(&v, __builtin_assume_aligned(p, sizeof(T)), sizeof(v));
+  return v;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_loose(T* p, pack<T, N> const& v)
+{
+  __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &v, sizeof(v));
+}
+
 /** Elements that the call reads once: not kept in the caches. */
 template <typename T, int N>
 __device__ __forceinline__ pack<T, N> load_once(const T* p)

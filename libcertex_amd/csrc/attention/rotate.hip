@@ -24,11 +24,22 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBatch   = 4;
 
+/** x in the element type, rounded from its float32 value: the compiler would round some float16 results once from the
+ *  exact sum of products (v_fma_mixlo_f16) and others twice, so that the vector's width showed in the bits. */
+template <typename T>
+__device__ __forceinline__ T narrowed(float x)
+{
+  if constexpr (std::is_same_v<T, f16_t>) { asm("" : "+v"(x)); }
+  return T(x);
+}
+
 /**
  * One thread: one vector of V elements of a row (of both halves in the half layout), over
- * heads_per_thread heads of one token. Blocks are dealt to the jobs in order.
+ * heads_per_thread heads of one token. Blocks are dealt to the jobs in order. LOOSE: rows of any
+ * length and alignment; what is turned and what is copied each end in a vector that is moved back to fit and
+ * writes some elements a second time, as they were written the first.
  */
-template <typename T, int V, bool INTERLEAVED>
+template <typename T, int V, bool INTERLEAVED, bool LOOSE>
 __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
 {
   int64_t block = blockIdx.x;
@@ -73,8 +84,11 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
   constexpr bool kAdjacent = INTERLEAVED && V > 1;   // pairs within a vector; else two vectors
   constexpr int P          = kAdjacent ? V / 2 : V;  // pairs of a thread
   const bool turned        = item < uint32_t(b.turned);  // else a vector that is copied
-  const int first  = !turned ? b.rotary + int(item - uint32_t(b.turned)) * V : int(item) * (INTERLEAVED && V == 1 ? 2 : V);
-  const int second = INTERLEAVED ? 1 : b.rotary / 2;  // from the first
+  const int second         = INTERLEAVED ? 1 : b.rotary / 2;  // from the first
+  int first                = turned ? int(item) * (INTERLEAVED && V == 1 ? 2 : V) : int(item - uint32_t(b.turned)) * V;
+  if constexpr (LOOSE) { first = min(first, (turned ? (INTERLEAVED ? b.rotary : b.rotary / 2) : b.dim - b.rotary) - V); }
+  const int pair = INTERLEAVED ? first / 2 : first;
+  if (!turned) { first += b.rotary; }
   src += first;
   dst += first;
   // the rows of kBatch heads are in flight together
@@ -88,7 +102,9 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
     }
   };
   const auto take_heads = [&](int h) {
-    if (b.lines) {
+    if constexpr (LOOSE) {
+      take(h, [](const T* p) { return load_loose<T, V>(p); });
+    } else if (b.lines) {
       take(h, [](const T* p) { return load_once<T, V>(p); });
     } else {
       take(h, [](const T* p) { return load<T, V>(p); });
@@ -99,7 +115,7 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
   if (turned) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const uint32_t turns = uint32_t((uint64_t(p) * a.frequencies[int(item) * P + i]) >> 32);
+      const uint32_t turns = uint32_t((uint64_t(p) * a.frequencies[pair + i]) >> 32);
       float sine, cosine;
       sincospif(float(int32_t(turns & ~255u)) * 0x1p-31f, &sine, &cosine);
       const float rest = float(turns & 255u) * float(M_PI * 0x1p-31);
@@ -109,6 +125,13 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
       s[i] *= a.transpose ? -a.magnitude : a.magnitude;
     }
   }
+  const auto put = [](T* p, pack<T, V> const& v) {
+    if constexpr (LOOSE) {
+      store_loose<T, V>(p, v);
+    } else {
+      store<T, V>(p, v);
+    }
+  };
   for (int h = h0;;) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -120,12 +143,12 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
           T& u          = kAdjacent ? x[i].e[2 * j] : x[i].e[j];
           T& w          = kAdjacent ? x[i].e[2 * j + 1] : y[i].e[j];
           const float f = float(u), g = float(w);
-          u = T(__builtin_fmaf(f, c[j], -(g * s[j])));
-          w = T(__builtin_fmaf(f, s[j], g * c[j]));
+          u = narrowed<T>(__builtin_fmaf(f, c[j], -(g * s[j])));
+          w = narrowed<T>(__builtin_fmaf(f, s[j], g * c[j]));
         }
-        if constexpr (!kAdjacent) { store<T, V>(row + second, y[i]); }
+        if constexpr (!kAdjacent) { put(row + second, y[i]); }
       }
-      store<T, V>(row, x[i]);
+      put(row, x[i]);
     }
     h += kBatch;
     if (h >= h1) { break; }
@@ -133,18 +156,19 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
   }
 }
 
-template <typename T, int V, bool INTERLEAVED>
+template <typename T, int V, bool INTERLEAVED, bool LOOSE>
 void launch(turn_args& a, hipStream_t stream)
 {
   int64_t blocks = 0, threads = 0;
   for (int j = 0; j < a.jobs; ++j) {
     turn_job& b = a.job[j];
     // pairs of a thread: V of the half layout, V / 2 interleaved ones (V = 1: one pair)
-    b.turned = INTERLEAVED && V > 1 ? b.rotary / V : b.rotary / 2 / V;
-    b.items  = b.turned + (b.dim - b.rotary) / V;
+    const auto vectors = [](int n) { return (n + V - 1) / V; };
+    b.turned           = vectors(INTERLEAVED && V > 1 ? b.rotary : b.rotary / 2);
+    b.items            = b.turned + vectors(b.dim - b.rotary);
     threads += a.tokens * b.heads * b.items;
-    // what one load of a row reads begins and ends on lines: read past the caches. (Half a line would be fetched
-    // twice: heads of 64 with 32 turned 125 -> 177 us; whole lines: 131,072 x 8 x 128 keys 100 -> 83 us.)
+    // what one load of a row reads begins and ends on lines: read past the caches. (Half a line would be
+    // fetched twice: heads of 64 with 32 turned 125 -> 177 us; whole lines: 131,072 x 8 x 128 keys 100 -> 83 us.)
     const auto whole = [](int64_t elements) { return elements * int64_t(sizeof(T)) % 128 == 0; };
     b.lines = whole(INTERLEAVED ? b.dim : b.rotary / 2) && whole(b.dim) && whole(b.src_token) && whole(b.src_head) &&
               whole(b.src_outer) && reinterpret_cast<uintptr_t>(b.src) % 128 == 0;
@@ -159,20 +183,42 @@ void launch(turn_args& a, hipStream_t stream)
     blocks += b.blocks;
   }
   if (blocks >= (int64_t(1) << 24)) { throw std::invalid_argument("certex: too many elements to rotate in one call"); }
-  if (blocks > 0) { turn_kernel<T, V, INTERLEAVED><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a); }
+  if (blocks > 0) { turn_kernel<T, V, INTERLEAVED, LOOSE><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a); }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool LOOSE = false>
 void launch(turn_args& a, hipStream_t stream)
 {
-  a.interleaved ? launch<T, V, true>(a, stream) : launch<T, V, false>(a, stream);
+  a.interleaved ? launch<T, V, true, LOOSE>(a, stream) : launch<T, V, false, LOOSE>(a, stream);
+}
+
+/** Whether rows of vectors of v elements can end in one that is moved back: the vector fits what is turned and what is
+ *  copied, and no element is read after it may have been written. */
+bool can_move_back(turn_args const& a, int v, int size)
+{
+  for (int j = 0; j < a.jobs; ++j) {
+    turn_job const& b = a.job[j];
+    const int turned = a.interleaved ? b.rotary : b.rotary / 2, copied = b.dim - b.rotary;
+    if ((turned > 0 && turned < v) || (copied > 0 && copied < v)) { return false; }
+    const int64_t outer = a.inner > 0 ? a.tokens / a.inner : 1;
+    const auto last     = [&](int64_t o, int64_t so, int64_t t, int64_t st, int64_t sh) {
+      return ((o - 1) * so + (t - 1) * st + (b.heads - 1) * sh + b.dim) * size;
+    };
+    const auto src = reinterpret_cast<uintptr_t>(b.src), dst = reinterpret_cast<uintptr_t>(b.dst);
+    const auto src_end = src + last(outer, b.src_outer, a.inner, b.src_token, b.src_head);
+    const auto dst_end = dst + (b.paged ? last(a.pages.n_pages, b.dst_outer, a.pages.page, b.dst_token, b.dst_head)
+                                        : last(outer, b.dst_outer, a.inner, b.dst_token, b.dst_head));
+    if (src < dst_end && dst < src_end) { return false; }
+  }
+  return true;
 }
 
 }  // namespace
 
 void turn(elem type, turn_args a, hipStream_t stream)
 {
-  // the widest vectors that every row, stride and base address is a multiple of
+  // the widest vectors that every row, stride and base address is a multiple of; 16 bytes at any alignment where
+  // those are narrower
   const int size = elem_bytes(type);
   int64_t g      = 16 / size;
   for (int j = 0; j < a.jobs; ++j) {
@@ -184,9 +230,15 @@ void turn(elem type, turn_args a, hipStream_t stream)
       g = std::gcd(g, x);
     }
   }
+  const int full      = 16 / size;
+  // Measured, narrow vectors and moved ones, us: halves of 33 of 130 (bfloat16) 96 and 84, of 51 of 128 163 and 140, of 20
+  // of 80 113 and 98; interleaved, whose narrow vectors of a row follow one another, 102 of 128 109 and 120, 66 of 130 equal.
+  const bool loose    = g < (a.interleaved ? 2 : full) && can_move_back(a, full, size);
   const auto by_width = [&](auto tag) {
     using T = decltype(tag);
-    if (g == 8) {
+    if (loose) {
+      launch<T, 16 / sizeof(T), true>(a, stream);
+    } else if (g == 8) {
       if constexpr (sizeof(T) == 2) { launch<T, 8>(a, stream); }
     } else if (g == 4) {
       launch<T, 4>(a, stream);

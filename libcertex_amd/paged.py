@@ -99,8 +99,9 @@ class Rotary:
     scale the frequencies: "linear" divides them by `factor`; "base" takes the base times
     factor^(rotary_dim / (rotary_dim - 2)); "ramp" keeps pairs that turn more than ramp[1] times within original_length
     positions, divides those that turn less than ramp[0] times, and blends between, with the magnitude
-    0.1 ln(factor) + 1 unless given. Angles are exact at every position: the product of the position and
-    the frequency is reduced in 64-bit fixed point.
+    0.1 ln(factor) + 1 unless given. Any position goes: its product with the frequency (a double) is reduced to a turn
+    exactly, in 64-bit fixed point. The first use on a GPU puts the frequencies there, which waits for the GPU: before a
+    graph is recorded, call the rotation once.
     """
 
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, layout="half", scaling=None, factor=1.0,

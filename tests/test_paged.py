@@ -105,6 +105,18 @@ def test_attention_checks():
             _need(**kw)
 
 
+def test_misaligned_data_is_refused():
+    t = [_tensor((2, 8, 64), torch.float16), *[_tensor((4, 16, 2, 64), torch.float16) for _ in range(2)],
+         _tensor((2, 2), torch.int32)]
+    out = ctypes.c_int64()
+    for bad in range(4):
+        for x in t:
+            x.dl_tensor.byte_offset = 0
+        t[bad].dl_tensor.byte_offset = 1
+        with pytest.raises(ValueError, match="multiple of its element size"):
+            C.check(C.lib().cuvsCertexPagedAttentionWorkspace(*[ctypes.addressof(x) for x in t], 0, ctypes.byref(out)))
+
+
 def test_null_arguments_are_errors():
     L = C.lib()
     n = ctypes.c_int64()

@@ -577,3 +577,29 @@ def test_refusals(gpu):
     ]:
         with pytest.raises(ValueError, match=match):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("d, r", [(130, 66), (128, 102), (61, 34), (45, 44), (20, 18), (17, 16), (9, 8)])
+def test_rotate_moved_vectors(gpu, dtype, layout, d, r):
+    """Rows that are no whole vectors, aligned and not, written elsewhere and in place."""
+    rope = certex.Rotary(d, rotary_dim=r, layout=layout)
+    p = torch.arange(40, device="cuda") * 977
+    wide = rand(40, 3, d + 9, dtype=dtype)
+    for lo in (0, 3):
+        x = wide[..., lo : lo + d]
+        want = ref.rotate(x, p, rope.frequencies, layout, r)
+        y = rope(x, p)
+        ref.assert_rotated(y, x, want, layout, r)
+        held = wide.clone()
+        part = held[..., lo : lo + d]
+        assert rope(part, p, out=part) is part and torch.equal(part, y)
+        assert torch.equal(held[..., :lo], wide[..., :lo]) and torch.equal(held[..., lo + d :], wide[..., lo + d :])
+    kp = torch.zeros((6, 8, 3, d), dtype=dtype, device="cuda")
+    vp = torch.zeros((6, 8, 3, d + 9), dtype=dtype, device="cuda")
+    table = ints([[4, 0, 5, 1, 3]])
+    x, at = wide[..., 3 : 3 + d], torch.arange(40, device="cuda")
+    certex.append_pages(x, wide, kp, vp, table, at, sequences=torch.zeros_like(at), rotary=rope)
+    page, slot = table[0].long()[at // 8], at % 8
+    assert torch.equal(kp[page, slot], rope(x, at)) and torch.equal(vp[page, slot], wide)
