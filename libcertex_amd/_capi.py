@@ -8,7 +8,6 @@ that borrow torch's memory (no deleter is called). The library must have been bu
 
 import ctypes
 import os
-import struct
 import threading
 
 import torch
@@ -206,7 +205,7 @@ def lib():
                     "cuvsCertexRotaryFrequencies": [P(RotaryParams), P(ctypes.c_double), P(ctypes.c_double)],
                     "cuvsCertexRotaryCreate": [st, P(RotaryParams), P(st)],
                     "cuvsCertexRotaryDestroy": [st],
-                    # tensors as addresses of DLManagedTensors (views())
+                    # tensors as addresses of DLManagedTensors (describe())
                     "cuvsCertexRotate": [st, st, vp, vp, vp, ctypes.c_bool],
                     "cuvsCertexAppendPages": [st, st] + [vp] * 9,
                     "cuvsCertexPagedAttentionWorkspace": [vp, vp, vp, vp, i64, P(i64)],
@@ -264,41 +263,18 @@ class Borrowed:
 
 _tls = threading.local()
 
-# a DLManagedTensor of n dimensions, then its extents (64 bytes in) and strides (96 bytes in)
-_VIEW = [struct.Struct(f"=QiiiBBHQQQQQ{n}q{32 - 8 * n}x{n}q") for n in range(5)]
-_VIEW_BYTES = 128
-_VIEWS = 12  # of a call
 
-
-class _Views:
-    """Memory of a thread for the DLManagedTensors of one call, which the next call reuses."""
-
-    def __init__(self):
-        self.buffer = ctypes.create_string_buffer(_VIEWS * _VIEW_BYTES)
-        self.base = ctypes.addressof(self.buffer)
-
-
-def views(*tensors, first=0):
-    """The addresses of DLManagedTensors of the tensors, strides included (None: NULL), valid until the calling thread's next
-    views() (of as many places or more, from `first` on). Written as bytes: ctypes structures take several times as long to
-    fill."""
-    v = getattr(_tls, "views", None)
-    if v is None:
-        v = _tls.views = _Views()
-    buffer, base, at, out = v.buffer, v.base, first * _VIEW_BYTES, []
-    for t in tensors:
-        if t is None:
-            out.append(None)
-            continue
-        address, ndim, device = base + at, t.ndim, t.get_device()  # -1: the host
-        if ndim > 4:
-            raise ValueError(f"tensors have at most 4 dimensions, not shape {tuple(t.shape)}")
-        code, bits = _DL[t.dtype]
-        _VIEW[ndim].pack_into(buffer, at, t.data_ptr(), kDLROCM if device >= 0 else kDLCPU, device if device >= 0 else 0, ndim,
-                              code, bits, 1, address + 64, address + 96, 0, 0, 0, *t.shape, *t.stride())
-        out.append(address)
-        at += _VIEW_BYTES
-    return out
+def describe(first, *tensors):
+    """Addresses of DLManagedTensors of the tensors, strides included (None: NULL), in places `first` on of the calling
+    thread's; a later call of as many places overwrites them. Of the extension _describe, which takes this function's place
+    on the first call."""
+    global describe
+    try:
+        from . import _describe
+    except ImportError as e:
+        raise ImportError(f"{os.path.join(HERE, '_describe.so')}: build it with `python -m libcertex_amd.build`") from e
+    describe = _describe.describe
+    return describe(first, *tensors)
 
 
 def resources():

@@ -1,4 +1,5 @@
-"""Build libcertex_c.so (the C-ABI library with the gfx950 kernels) in this directory with hipcc.
+"""Build libcertex_c.so (the C-ABI library with the gfx950 kernels) in this directory with hipcc, and _describe.so (the
+Python extension that describes torch tensors to it) with g++.
 
     python -m libcertex_amd.build        # or: python libcertex_amd/build.py
 
@@ -10,6 +11,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -63,12 +65,30 @@ def _compile(src, obj_dir):
     return obj
 
 
+def _extension():
+    """_describe.so, against torch's headers (host code only)."""
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    lib = library_paths()[0]
+    out = os.path.join(HERE, "_describe.so")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
+           *[f"-I{p}" for p in include_paths()], os.path.join(CSRC, "attention", "describe.cpp"), "-o", out + ".tmp",
+           f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the tensor descriptions' extension failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(out + ".tmp", out)
+
+
 def build(verbose=False):
     obj_dir = os.path.join(HERE, "_build")
     os.makedirs(obj_dir, exist_ok=True)
     workers = min(len(SOURCES), max(1, min(8, os.cpu_count() or 1)))
     with concurrent.futures.ThreadPoolExecutor(workers) as ex:
+        extension = ex.submit(_extension)
         objs = list(ex.map(lambda s: _compile(s, obj_dir), SOURCES))
+        extension.result()
     tmp = OUT + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)

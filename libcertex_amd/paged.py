@@ -164,7 +164,7 @@ class Rotary:
         if out is None and y.stride(-1) != 1:  # a dense tensor in another order of dimensions
             y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         _require(y.shape == x.shape, "out must have the shape of x")
-        C.check(C.lib().cuvsCertexRotate(C.stream_resources(), self._handle(x.get_device()), *C.views(x, positions, y),
+        C.check(C.lib().cuvsCertexRotate(C.stream_resources(), self._handle(x.get_device()), *C.describe(0, x, positions, y),
                                          transpose))
         return y
 
@@ -193,7 +193,7 @@ def append_pages(k, v, k_pages, v_pages, page_table, positions, sequences=None, 
         raise ValueError(f"this rotation is of heads of {rotary.head_dim}, not {k.shape[-1]}")
     C.check(C.lib().cuvsCertexAppendPages(
         C.stream_resources(), 0 if rotary is None else rotary._handle(k.get_device()),
-        *C.views(k, v, k_pages, v_pages, table, positions, sequences, q, out)))
+        *C.describe(0, k, v, k_pages, v_pages, table, positions, sequences, q, out)))
     return out
 
 
@@ -219,12 +219,12 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
     out = _output(q, (*q.shape[:2], v_pages.shape[3]))
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     L, need = C.lib(), ctypes.c_int64()
-    qv, kv, vv, tv, lv, ov, ev = C.views(q, k_pages, v_pages, table, lengths, out, lse)
+    qv, kv, vv, tv, lv, ov, ev = C.describe(0, q, k_pages, v_pages, table, lengths, out, lse)
     C.check(L.cuvsCertexPagedAttentionWorkspace(qv, kv, vv, tv, window, ctypes.byref(need)))
     work = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
     C.check(L.cuvsCertexPagedAttention(C.stream_resources(), qv, kv, vv, tv, lv,
                                        q.shape[2] ** -0.5 if scale is None else float(scale), window,
-                                       *C.views(work, first=7), ov, ev))
+                                       *C.describe(7, work), ov, ev))
     return (out, lse) if return_lse else out
 
 
@@ -254,10 +254,10 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     out = values.new_empty((*scores.shape[:2], values.shape[-1]))
     lse = torch.empty(scores.shape[:2], dtype=torch.float32, device=values.device) if return_lse else None
     L, need = C.lib(), ctypes.c_int64()
-    sv, iv, vv, tv, ov, ev = C.views(scores, ids, values, page_table, out, lse)
+    sv, iv, vv, tv, ov, ev = C.describe(0, scores, ids, values, page_table, out, lse)
     C.check(L.cuvsCertexSelectedAttentionWorkspace(sv, vv, tv, ctypes.byref(need)))
     work = values.new_empty(need.value, dtype=torch.uint8) if need.value else None
-    C.check(L.cuvsCertexSelectedAttention(C.stream_resources(), sv, iv, vv, tv, float(scale), *C.views(work, first=6), ov, ev))
+    C.check(L.cuvsCertexSelectedAttention(C.stream_resources(), sv, iv, vv, tv, float(scale), *C.describe(6, work), ov, ev))
     if single:
         out, lse = out[:, 0], None if lse is None else lse[:, 0]
     return (out, lse) if return_lse else out
