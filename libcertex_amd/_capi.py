@@ -205,7 +205,7 @@ def lib():
                     "cuvsCertexRotaryFrequencies": [P(RotaryParams), P(ctypes.c_double), P(ctypes.c_double)],
                     "cuvsCertexRotaryCreate": [st, P(RotaryParams), P(st)],
                     "cuvsCertexRotaryDestroy": [st],
-                    # tensors as addresses of DLManagedTensors (describe())
+                    # called by the extension _attention; here for callers with DLManagedTensors of their own
                     "cuvsCertexRotate": [st, st, vp, vp, vp, ctypes.c_bool],
                     "cuvsCertexAppendPages": [st, st] + [vp] * 9,
                     "cuvsCertexPagedAttentionWorkspace": [vp, vp, vp, vp, i64, P(i64)],
@@ -264,19 +264,6 @@ class Borrowed:
 _tls = threading.local()
 
 
-def describe(first, *tensors):
-    """Addresses of DLManagedTensors of the tensors, strides included (None: NULL), in places `first` on of the calling
-    thread's; a later call of as many places overwrites them. Of the extension _describe, which takes this function's place
-    on the first call."""
-    global describe
-    try:
-        from . import _describe
-    except ImportError as e:
-        raise ImportError(f"{os.path.join(HERE, '_describe.so')}: build it with `python -m libcertex_amd.build`") from e
-    describe = _describe.describe
-    return describe(first, *tensors)
-
-
 def resources():
     """Per-thread, per-device C resources bound to torch's current stream."""
     dev = torch.cuda.current_device()
@@ -313,3 +300,21 @@ def stream_resources():
                 check(L.cuvsResourcesCreateOnStream(ctypes.byref(h), ctypes.c_void_p(stream)))
                 res = _streams[dev, stream] = h.value
     return res
+
+
+_operators = None
+
+
+def operators():
+    """The extension _attention, which calls the attention operators' C entry points (an error if it was not built)."""
+    global _operators
+    if _operators is None:
+        lib()
+        try:
+            from . import _attention
+        except ImportError as e:
+            path = os.path.join(HERE, "_attention.so")
+            raise ImportError(f"{path} is missing or does not load: build it with `python -m libcertex_amd.build`") from e
+        _attention.init(CertexError, torch.OutOfMemoryError)
+        _operators = _attention
+    return _operators

@@ -1,5 +1,5 @@
-"""Build libcertex_c.so (the C-ABI library with the gfx950 kernels) in this directory with hipcc, and _describe.so (the
-Python extension that describes torch tensors to it) with g++.
+"""Build libcertex_c.so (the C-ABI library with the gfx950 kernels) in this directory with hipcc, and _attention.so (the
+attention operators' Python binding) with g++.
 
     python -m libcertex_amd.build        # or: python libcertex_amd/build.py
 
@@ -65,19 +65,21 @@ def _compile(src, obj_dir):
     return obj
 
 
-def _extension():
-    """_describe.so, against torch's headers (host code only)."""
+def _binding(out):
+    """_attention.so from csrc/attention/binding.cpp, host code against torch's headers; it calls libcertex_c.so, which has to
+    be there and is found next to it."""
     from torch.utils.cpp_extension import include_paths, library_paths
 
     lib = library_paths()[0]
-    out = os.path.join(HERE, "_describe.so")
+    rocm = os.path.dirname(os.path.dirname(HIPCC))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
-           *[f"-I{p}" for p in include_paths()], os.path.join(CSRC, "attention", "describe.cpp"), "-o", out + ".tmp",
-           f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"]
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", "-I", os.path.join(ROOT, "include"),
+           "-I", sysconfig.get_paths()["include"], *[f"-I{p}" for p in include_paths()], "-I", os.path.join(rocm, "include"),
+           os.path.join(CSRC, "attention", "binding.cpp"), "-o", out + ".tmp", f"-L{lib}", "-ltorch_python", "-ltorch_cpu",
+           "-lc10", "-lc10_hip", f"-L{HERE}", "-l:" + os.path.basename(OUT), f"-Wl,-rpath,{lib}", "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"the tensor descriptions' extension failed:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"the operators' binding failed:\n{r.stdout}\n{r.stderr}")
     os.replace(out + ".tmp", out)
 
 
@@ -86,15 +88,14 @@ def build(verbose=False):
     os.makedirs(obj_dir, exist_ok=True)
     workers = min(len(SOURCES), max(1, min(8, os.cpu_count() or 1)))
     with concurrent.futures.ThreadPoolExecutor(workers) as ex:
-        extension = ex.submit(_extension)
         objs = list(ex.map(lambda s: _compile(s, obj_dir), SOURCES))
-        extension.result()
     tmp = OUT + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, OUT)
+    _binding(os.path.join(HERE, "_attention.so"))
     if verbose:
         print(f"built {OUT}")
     return OUT

@@ -603,3 +603,46 @@ def test_rotate_moved_vectors(gpu, dtype, layout, d, r):
     certex.append_pages(x, wide, kp, vp, table, at, sequences=torch.zeros_like(at), rotary=rope)
     page, slot = table[0].long()[at // 8], at % 8
     assert torch.equal(kp[page, slot], rope(x, at)) and torch.equal(vp[page, slot], wide)
+
+
+def test_gradient_outlives_its_rotation(gpu):
+    """A graph keeps the frequencies that its backward needs."""
+    x, p = rand(9, 2, 32).requires_grad_(), torch.arange(9, device="cuda") * 5
+    rope = certex.Rotary(32)
+    f = rope.frequencies
+    y = rope(x, p)
+    del rope
+    dy = rand(9, 2, 32, seed=1)
+    y.backward(dy)
+    ref.assert_rotated(x.grad, dy, ref.rotate(dy, p, f, "half", 32, transpose=True), "half", 32)
+
+
+def test_threads(gpu):
+    """Calls of several threads at once, each on a stream of its own; the rotation and its frequencies are shared."""
+    import threading
+
+    lens = [900, 40]
+    kp, vp, table, *_ = paged(lens, 16, 2, 64, 64, torch.bfloat16, seed=18)
+    rope, pos = certex.Rotary(64), ints([899, 39])
+    qs = [rand(2, 8, 64, dtype=torch.bfloat16, seed=100 + i) for i in range(4)]
+    want = [certex.paged_attention(rope(q, pos), kp, vp, table, ints(lens)) for q in qs]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(50):
+                    got = certex.paged_attention(rope(qs[i], pos), kp, vp, table, ints(lens))
+                    if not torch.equal(got, want[i]):
+                        failed.append(i)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
