@@ -37,8 +37,9 @@ class Rotary:
     factor^(rotary_dim / (rotary_dim - 2)); "ramp" keeps pairs that turn more than ramp[1] times within original_length
     positions, divides those that turn less than ramp[0] times, and blends between, with the magnitude
     0.1 ln(factor) + 1 unless given. Any position goes: its product with the frequency (a double) is reduced to a turn
-    exactly, in 64-bit fixed point. The first use on a GPU puts the frequencies there, which waits for the GPU: before a
-    graph is recorded, call the rotation once.
+    exactly, in 64-bit fixed point. The frequencies are put on the current GPU when the rotation is made (if
+    the program has used a GPU by then) and on others at the first use there, which waits for that GPU: before a graph
+    is recorded, not in it.
     """
 
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, layout="half", scaling=None, factor=1.0,
@@ -61,20 +62,26 @@ class Rotary:
         f, m = (ctypes.c_double * (self.rotary_dim // 2))(), ctypes.c_double()
         C.check(C.lib().cuvsCertexRotaryFrequencies(ctypes.byref(self._params), f, ctypes.byref(m)))
         self.frequencies, self.magnitude = torch.tensor(list(f), dtype=torch.float64), m.value  # radians per position
+        if torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing():
+            self._on(torch.cuda.current_device())
 
-    def _handle(self, like):
-        """The frequencies on the GPU of a tensor (kept from the first use there on), as the extension's capsule."""
-        _require(isinstance(like, torch.Tensor) and like.is_cuda, "rotated tensors must be GPU tensors")
-        device = like.get_device()
+    def _on(self, device):
+        """The frequencies on a GPU, as the extension's capsule (made at the first use, or with the rotation)."""
         h = self._handles.get(device)
         if h is None:
             with self._lock:
                 h = self._handles.get(device)
                 if h is None:
                     out = ctypes.c_size_t()
-                    C.check(C.lib().cuvsCertexRotaryCreate(C.stream_resources(), ctypes.byref(self._params), ctypes.byref(out)))
+                    with torch.cuda.device(device):
+                        C.check(C.lib().cuvsCertexRotaryCreate(C.stream_resources(), ctypes.byref(self._params),
+                                                               ctypes.byref(out)))
                     h = self._handles[device] = C.operators().own(out.value)
         return h
+
+    def _handle(self, like):
+        _require(isinstance(like, torch.Tensor) and like.is_cuda, "rotated tensors must be GPU tensors")
+        return self._on(like.get_device())
 
     def __call__(self, x, positions, transpose=False, out=None):
         """x (tokens, heads, head_dim) or (batch, tokens, heads, head_dim), rotated by positions (tokens,) or (batch,
