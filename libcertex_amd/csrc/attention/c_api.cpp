@@ -314,7 +314,7 @@ auto select_args_of(DLManagedTensor* scores_, DLManagedTensor* values_, DLManage
           "the query heads must be a multiple of the value heads");
   EXPECTS(vdim >= 1 && vdim <= ops::kMaxHeadDim,
           "head dimensions must be between 1 and " + std::to_string(ops::kMaxHeadDim));
-  EXPECTS(scores->shape[0] * scores->shape[1] < (int64_t(1) << 24), "at most 2^24 - 1 queries over all heads");
+  EXPECTS(scores->shape[0] * scores->shape[1] <= (int64_t(1) << 23), "at most 2^23 queries over all heads");
   EXPECTS(scores->shape[2] < (int64_t(1) << 31), "fewer than 2^31 selected rows a query");
   a.heads    = int32_t(scores->shape[0]);
   a.kv_heads = int32_t(kv_heads);
