@@ -121,7 +121,7 @@ CUVS_EXPORT cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
  * out: dense [n_sequences, heads, vdim]; lse (or NULL): dense float32 [n_sequences, heads], the
  * logarithm of the softmax's denominator. Positions whose page the table does not hold do not count; a row
  * without positions gives zeros, and lse -inf. Slots at and past a sequence's length are not used,
- * whatever they hold. workspace: a dense uint8 vector of at least the bytes that
+ * whatever they hold. An infinite value that counts makes its column of out infinite or NaN. workspace: a dense uint8 vector of at least the bytes that
  * cuvsCertexPagedAttentionWorkspace reports for the same tensors (NULL if 0), in use until the
  * queued work is done.
  */
@@ -151,7 +151,7 @@ CUVS_EXPORT cuvsError_t cuvsCertexPagedAttentionWorkspace(DLManagedTensor* q,
  * [kv_heads, n, vdim], or with page_table (dense int32 [n], one sequence) the pages
  * [n_pages, page_size, kv_heads, vdim]; vdim at most 256; out: dense [heads, queries, vdim]; lse (or NULL):
  * dense float32 [heads, queries]. An id outside the values (as -1) and a score of -inf do not count;
- * a row of none gives zeros, and lse -inf. workspace: as for cuvsCertexPagedAttention.
+ * a row of none gives zeros, and lse -inf. Infinite values and workspace: as for cuvsCertexPagedAttention.
  */
 CUVS_EXPORT cuvsError_t cuvsCertexSelectedAttention(cuvsResources_t res,
                                                     DLManagedTensor* scores,

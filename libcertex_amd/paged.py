@@ -107,7 +107,8 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
     them, if given); query head h reads key head h // (n_heads / n_kv_heads). scale defaults to head_dim ** -0.5.
 
     A sequence of length 0 gives zeros. Lengths past the table's pages are cut to them, positions whose page the
-    table does not hold do not count, and slots past a length are never used, whatever they hold. With
+    table does not hold do not count, and slots past a length are never used, whatever they hold; an
+    infinite value that counts makes its column of the output infinite or NaN. With
     return_lse also the logarithm of the softmax's denominator (float32, -inf for an empty row), which
     joins the outputs of two calls over different positions. A cache holds head dimensions up to 256 and
     pages of a multiple of 8 positions."""
@@ -121,5 +122,6 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     page_size, n_kv_heads, value_dim). Query head h reads value head h // (n_heads / n_kv_heads).
 
     Ids outside the values (-1 marks a missing neighbour) and scores of -inf do not count; a row of none gives zeros.
+    An infinite value that counts makes its column of the output infinite or NaN.
     With return_lse also the logarithm of the softmax's denominator (float32, -inf for an empty row)."""
     return C.operators().select(scores, ids, values, scale, page_table, return_lse)

@@ -317,6 +317,24 @@ def test_attend_nan_is_seen(gpu):
     assert out[0].isnan().all() and not out[1].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_value_is_seen(gpu, dtype):
+    """An infinity among the values in use shows in its column, and in no other column, head or sequence."""
+    kp, vp, table, *_ = paged([50, 50], 16, 2, 64, 64, dtype, seed=15)
+    vp[int(table[0, 1]), 3, 1, 5] = float("inf")
+    finite = certex.paged_attention(rand(2, 4, 64, dtype=dtype), kp, vp, table, ints([50, 50])).isfinite()
+    assert not finite[0, 2:, 5].any() and finite.sum() == finite.numel() - 2
+
+    # few queries a head gather rows; many, over values larger than a die's cache, go by ranges
+    for queries, n, k in ((2, 500, 70), (64, 40_000, 2050)):
+        values = rand(2, n, 64, dtype=dtype)
+        values[1, 11, 5] = float("inf")
+        ids = torch.randint(12, n, (4, queries, k), device="cuda")
+        ids[2, 1, 9] = ids[3, 0, 0] = 11
+        finite = certex.selected_attention(rand(4, queries, k), ids, values, 0.3).isfinite()
+        assert not finite[2, 1, 5] and not finite[3, 0, 5] and finite.sum() == finite.numel() - 2
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_attend_unaligned_queries(gpu, dtype):
     """Queries that are a slice of a projection (any alignment), pools with gaps between heads."""
