@@ -464,14 +464,19 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
           }
         }
       } else {
-        // the weights enter as value and remainder: rounded once, to 8 or 11 bits, they would cost as much as the
-        // output's own rounding, and the matrix cores wait for memory
-        u32x4 hi, lo;
+        // the weights enter with all 24 bits, as three elements of 8 or 11 bits each: the value, its remainder, and what that
+        // leaves. The matrix cores wait for memory, so the third costs little (two and three, us: 64 sequences up to 8,192 157.5
+        // and 158.5, one of 131,072 89 and 89; 32 query heads on one key head 112 and 115).
+        u32x4 part[3];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const T even = T(p[2 * w]), odd = T(p[2 * w + 1]);
-          hi[w]       = pack2<T>(p[2 * w], p[2 * w + 1]);
-          lo[w]       = pack2<T>(p[2 * w] - float(even), p[2 * w + 1] - float(odd));
+          float even = p[2 * w], odd = p[2 * w + 1];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            part[i][w] = pack2<T>(even, odd);
+            even -= float(T(even));
+            odd -= float(T(odd));
+          }
         }
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) {
@@ -482,8 +487,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
             for (int w = 0; w < 4; ++w) {
               vt[w] = __builtin_amdgcn_perm(v[2 * w + 1][n][e / 2], v[2 * w][n][e / 2], e % 2 == 0 ? 0x05040100u : 0x07060302u);
             }
-            o[n * kCols + e] = mfma(T{}, vt, hi, o[n * kCols + e]);
-            o[n * kCols + e] = mfma(T{}, vt, lo, o[n * kCols + e]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) { o[n * kCols + e] = mfma(T{}, vt, part[i], o[n * kCols + e]); }
           }
         }
       }
