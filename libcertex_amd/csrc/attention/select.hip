@@ -1,5 +1,7 @@
 // Attention over a selected top k: the scores are given (a key cache returns them with the ids), so
-// no key is read again. out = sum_j p_j v[id_j] / sum_j p_j, p_j = 2^(x_j - m), x_j = scale log2(e) s_j.
+// no key is read again. out = sum_j p_j v[id_j] / sum_j p_j, p_j = 2^(scale log2(e) (s_j - m)), m the largest score
+// (the smallest, where scale < 0). The scores are subtracted before they are scaled: what is rounded is their distance
+// from m, however far from 0 they are, and scores of the type's lowest value among themselves stay at distance 0.
 //
 // What bounds it: gathers of value rows (256 bytes of 128 bfloat16 columns), one multiplication per element read.
 // A wave takes 64 ids at a time: each lane the weight and the row of one; then 16 bytes of a row per lane, as many
@@ -15,6 +17,8 @@
 #include "elements.hpp"
 
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 
 namespace certex_amd::attention {
 namespace {
@@ -30,11 +34,44 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
+/** What scores are read with. */
+struct score_scale {
+  float sign;    // of the scale: scores times this are the larger the more they weigh
+  float scale;   // its magnitude
+  float scale2;  // that times log2(e)
+};
+
+score_scale scale_of(float scale)
+{
+  const double s = std::abs(double(scale));
+  return {scale < 0.0f ? -1.0f : 1.0f, float(s), float(std::min(s * M_LOG2E, double(FLT_MAX)))};
+}
+
+/** The weight of a score relative to the finite score `top`, both signed; -inf counts nothing, NaN stays. */
+__device__ __forceinline__ float weight_of(score_scale const& s, float score, float top)
+{
+  const float d = score - top;
+  // a distance past the largest float: that much, so that a scale of 0 or near it has its say
+  return score == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((d < -FLT_MAX ? -FLT_MAX : d) * s.scale2);
+}
+
+/** What sums taken relative to the score `part` count relative to `whole` >= part. Where nothing was counted both are
+ *  -inf, and the sums are 0, or NaN of NaN scores: they pass as they are. */
+__device__ __forceinline__ float factor_of(score_scale const& s, float part, float whole)
+{
+  return whole == -INFINITY ? 1.0f : weight_of(s, part, whole);
+}
+
+__device__ __forceinline__ float lse_of(score_scale const& s, float top, float sum)
+{
+  return sum == 0.0f ? -INFINITY : __builtin_fmaf(top, s.scale, __builtin_log2f(sum) / kLog2e);
+}
+
 struct select_plan {
   int32_t splits;   // of a query's ids
   int64_t per;      // ids of a split, a multiple of kStep
   int64_t work;     // queries x splits
-  float scale2;     // scale log2(e)
+  score_scale scale;
   float* part_out;  // [work][vdim]
   float* part_max;  // [work]
   float* part_sum;
@@ -105,7 +142,7 @@ __device__ __forceinline__ void finish(select_args const& a, select_plan const& 
   float f[kWaves], sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    f[w] = factor_of(s_max[w], m);
+    f[w] = factor_of(plan.scale, s_max[w], m);
     sum += f[w] * s_sum[w];
   }
   for (int i = tid; i < a.vdim; i += kThreads) {
@@ -123,7 +160,7 @@ __device__ __forceinline__ void finish(select_args const& a, select_plan const& 
       plan.part_max[work] = m;
       plan.part_sum[work] = sum;
     } else if (a.lse != nullptr) {
-      a.lse[row] = sum == 0.0f ? -INFINITY : (m + __builtin_log2f(sum)) / kLog2e;
+      a.lse[row] = lse_of(plan.scale, m, sum);
     }
   }
 }
@@ -158,18 +195,18 @@ __global__ __launch_bounds__(kThreads) void select_kernel(select_args a, select_
     if (j < end) {
       const float raw = s[j];
       at              = row_of(a, a.ids[row * a.k + j]);
-      if (at >= 0 && raw != -INFINITY) { x = raw * plan.scale2; }
+      if (at >= 0 && raw != -INFINITY) { x = raw * plan.scale.sign; }
     }
     const float high  = lanes::max<64>(x);
     const float grown = fmaxf(top, high);
     if (grown > top) {
-      const float keep = __builtin_amdgcn_exp2f(top - grown);
+      const float keep = weight_of(plan.scale, top, grown);
       total *= keep;
 #pragma unroll
       for (int i = 0; i < E; ++i) { acc[i] *= keep; }
       top = grown;
     }
-    const float p       = __builtin_amdgcn_exp2f(x - (top == -INFINITY ? 0.0f : top));
+    const float p       = weight_of(plan.scale, x, top == -INFINITY ? 0.0f : top);
     const uint64_t some = __ballot(p != 0.0f);  // NaN too
     if (some == 0) { continue; }
     total += p;
@@ -220,7 +257,7 @@ struct phase_plan {
   int32_t ranges;
   int64_t rows;     // queries of all heads
   float per_n;      // ranges / n
-  float scale2;
+  score_scale scale;
   uint2* list;      // [rows][k]: row offset, weight
   int32_t* starts;  // [rows][ranges + 1]
   float* part;      // [ranges][rows][vdim]
@@ -257,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(select_args a, phase_pla
       const int64_t to = row_of(a, id[i]);
       at[i]            = uint32_t(to);
       range[i]         = min(uint32_t(float(max(id[i], int64_t(0))) * plan.per_n), uint32_t(plan.ranges - 1));
-      x[i]             = to >= 0 && x[i] != -INFINITY ? x[i] * plan.scale2 : -INFINITY;
+      x[i]             = to >= 0 && x[i] != -INFINITY ? x[i] * plan.scale.sign : -INFINITY;
     }
   };
 
@@ -267,11 +304,11 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(select_args a, phase_pla
     float grown = top;
 #pragma unroll
     for (int i = 0; i < kBlock; ++i) { grown = fmaxf(grown, x[i]); }
-    total *= factor_of(top, grown);
+    total *= factor_of(plan.scale, top, grown);
     top = grown;
 #pragma unroll
     for (int i = 0; i < kBlock; ++i) {
-      total += __builtin_amdgcn_exp2f(x[i] - (top == -INFINITY ? 0.0f : top));
+      total += weight_of(plan.scale, x[i], top == -INFINITY ? 0.0f : top);
       if (x[i] != -INFINITY) { atomicAdd(&s_count[wave][range[i]], 1); }
     }
   }
@@ -280,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(select_args a, phase_pla
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) { high = fmaxf(high, s_part[0][w]); }
-  total = lanes::sum<64>(factor_of(top, high) * total);
+  total = lanes::sum<64>(factor_of(plan.scale, top, high) * total);
   if (lane == 0) { s_part[1][wave] = total; }
   // a wave's counters become where its ids of each range begin
   int32_t before = 0, all = 0;
@@ -301,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(select_args a, phase_pla
   total               = (s_part[1][0] + s_part[1][1]) + (s_part[1][2] + s_part[1][3]);
   const float per_sum = 1.0f / total;
   const float from    = high == -INFINITY ? 0.0f : high;
-  if (tid == 0 && a.lse != nullptr) { a.lse[row] = total == 0.0f ? -INFINITY : (high + __builtin_log2f(total)) / kLog2e; }
+  if (tid == 0 && a.lse != nullptr) { a.lse[row] = lse_of(plan.scale, high, total); }
   uint2* list = plan.list + row * a.k;
   for (int64_t j0 = begin; j0 < end; j0 += 64 * kBlock) {
     if (end - begin > 64 * kBlock) { take(j0); }
@@ -318,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(select_args a, phase_pla
       const uint32_t rank = __builtin_amdgcn_mbcnt_hi(uint32_t(same >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(same), 0u));
       if (in) {
         const int32_t to = s_count[wave][range[i]] + int32_t(rank);
-        const float p    = __builtin_amdgcn_exp2f(x[i] - from) * per_sum;
+        const float p    = weight_of(plan.scale, x[i], from) * per_sum;
         list[to]         = make_uint2(at[i], __builtin_bit_cast(uint32_t, p));
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -414,12 +451,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(select_args a, select_pl
     float sum = 0.0f, out = 0.0f;
 #pragma unroll 8
     for (int w = 0; w < plan.splits; ++w) {
-      const float f = factor_of(plan.part_max[w0 + w], m);
+      const float f = factor_of(plan.scale, plan.part_max[w0 + w], m);
       sum += f * plan.part_sum[w0 + w];
       out += f * plan.part_out[(w0 + w) * a.vdim + i];
     }
     static_cast<T*>(a.out)[row * a.vdim + i] = T(sum == 0.0f ? 0.0f : out / sum);
-    if (i == 0 && a.lse != nullptr) { a.lse[row] = sum == 0.0f ? -INFINITY : (m + __builtin_log2f(sum)) / kLog2e; }
+    if (i == 0 && a.lse != nullptr) { a.lse[row] = lse_of(plan.scale, m, sum); }
   }
 }
 
@@ -457,7 +494,7 @@ auto plan_of(select_args const& a) -> select_plan
   p.splits             = int32_t((steps + each - 1) / each);
   p.per                = each * kStep;
   p.work               = rows * p.splits;
-  p.scale2             = a.scale * kLog2e;
+  p.scale              = scale_of(a.scale);
   return p;
 }
 
@@ -480,7 +517,7 @@ void select(elem type, select_args const& a, hipStream_t stream)
     p.ranges = ranges;
     p.rows   = a.heads * a.queries;
     p.per_n  = float(ranges) / float(a.n);
-    p.scale2 = a.scale * kLog2e;
+    p.scale  = scale_of(a.scale);
     p.list   = static_cast<uint2*>(a.workspace);
     p.starts = reinterpret_cast<int32_t*>(p.list + p.rows * a.k);
     p.part   = reinterpret_cast<float*>(p.starts + p.rows * (ranges + 1));

@@ -49,3 +49,57 @@ def test_attend_weights_are_whole(gpu, dtype):
     bound = 16 * U * spread + (ref.UNIT[dtype] + 16 * U) * want.abs() + ref.UNIT[dtype] * torch.finfo(dtype).tiny
     assert (want.abs() < spread / 1000).all()  # the output's own rounding hides nothing
     assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
+
+
+# few queries a head gather rows; many, over values larger than a die's cache, go by ranges
+ROUTES = [(2, 500, 300, 4), (64, 40_000, 2050, 128)]
+
+
+@pytest.mark.parametrize("queries, n, k, width", ROUTES)
+@pytest.mark.parametrize("offset", [0.0, 200.0, 5000.0, 1e6, -1e6])
+def test_selected_scores_far_from_zero(gpu, queries, n, k, width, offset):
+    """Scores are exact inputs, so that an offset that all of them share rounds nothing: what is rounded is their distances,
+    of up to D = 12 in powers of 2, three times (3 u D ln 2 = 25 u), besides 3 u of the exponential and the weight; each
+    of the two sums of k terms takes 4 sqrt(k) u."""
+    heads, kv, scale = 4, 2, 0.25
+    g = torch.Generator(device="cuda").manual_seed(3)
+    spread = torch.randint(0, 8 * 33, (heads, queries, k), generator=g, device="cuda") / 8.0  # scale * 33 * log2(e) < 12
+    scores, ids = spread + offset, torch.randint(0, n, (heads, queries, k), generator=g, device="cuda")
+    assert torch.equal(scores.double() - offset, spread.double())
+    values = torch.randn((kv, n, width), generator=g, device="cuda")
+    out, lse = certex.selected_attention(scores, ids, values, scale, return_lse=True)
+    host = values.double().cpu()
+    for h in range(heads):
+        for i in range(0, queries, 7):
+            w = torch.softmax(scale * scores[h, i].double().cpu(), 0)
+            rows = host[h // 2, ids[h, i].cpu()]
+            size = (w @ rows.abs()).norm()
+            e = (28 + 8 * k**0.5) * U
+            assert float((out[h, i].double().cpu() - w @ rows).norm() / size) <= e
+            want = torch.logsumexp(scale * scores[h, i].double().cpu(), 0)
+            assert abs(float(lse[h, i].double().cpu() - want)) <= e + 4 * U * abs(float(want))
+
+
+@pytest.mark.parametrize("queries, n, k, width", ROUTES)
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.0])
+def test_selected_lowest_scores(gpu, queries, n, k, width, scale):
+    """Scores of float32's lowest value, which masks are made of: they weigh nothing next to others, and alike where a row
+    holds no other, whose scaled scores are as finite; with a scale of 0 all weigh alike."""
+    low = torch.finfo(torch.float32).min if scale >= 0 else torch.finfo(torch.float32).max
+    g = torch.Generator(device="cuda").manual_seed(4)
+    scores = torch.randn((4, queries, k), generator=g, device="cuda")
+    ids = torch.randint(0, n, (4, queries, k), generator=g, device="cuda")
+    scores[:2] = low
+    scores[2:, :, k // 3 :] = low
+    scores[3, 1, 7] = -low  # as far from the others as scores can be
+    values = torch.randn((2, n, width), generator=g, device="cuda")
+    out, lse = certex.selected_attention(scores, ids, values, scale, return_lse=True)
+    host = values.double().cpu()
+    for h in range(4):
+        for i in {0, 1, queries - 1}:
+            s = scale * scores[h, i].double().cpu()
+            w, rows = torch.softmax(s, 0), host[h // 2, ids[h, i].cpu()]
+            e = (28 + 8 * k**0.5) * U
+            assert float((out[h, i].double().cpu() - w @ rows).norm() / (w @ rows.abs()).norm()) <= e
+            want = torch.logsumexp(s, 0)
+            assert abs(float(lse[h, i].double().cpu() - want)) <= e + 4 * U * abs(float(want))
