@@ -80,8 +80,7 @@ struct attend_plan {
   int32_t shares;       // of a table's tiles, at most
   int32_t halve;        // half as many shares where each of those has this many tiles or more (0: never)
   bool one_die;         // the tables of a share run on one die
-  float scale2;         // scale log2(e), and what that is rounded by
-  float scale2_rest;
+  float scale2;         // scale log2(e)
   float* part_out;      // [tables][2 shares][kRows][vdim]
   float* part_max;      // [tables][2 shares][kRows]
   float* part_sum;
@@ -412,7 +411,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       for (int j = 0; j < kGrp; ++j) { x[j] = s[j / 4][j % 4] * plan.scale2; }
       const int t      = (group + g) * kGrp;
       const bool whole = have && t >= sp.begin && t + kGrp <= sp.end;
-      if (!__all(whole)) {
+      const bool masked = !__all(whole);
+      if (masked) {
 #pragma unroll
         for (int j = 0; j < kGrp; ++j) {
           const bool in = have && t + j >= sp.begin && t + j < sp.end;
@@ -442,11 +442,13 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       float p[kGrp];
 #pragma unroll
       for (int j = 0; j < kGrp; ++j) {
-        // float32: the exponent is rounded once, after the subtraction, and the scale's own rounding is made up for
-        p[j] = __builtin_amdgcn_exp2f(
-          G::kWide && x[j] != -INFINITY
-            ? __builtin_fmaf(s[j / 4][j % 4], plan.scale2, __builtin_fmaf(s[j / 4][j % 4], plan.scale2_rest, -base))
-            : x[j] - base);
+        // the exponent is rounded once, after the subtraction, at the size of its distance from the maximum (the scale's own
+        // rounding stretches that distance by 2^-24 of itself)
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], plan.scale2, -base));
+      }
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < kGrp; ++j) { p[j] = x[j] == -INFINITY ? 0.0f : p[j]; }
       }
 #pragma unroll
       for (int j = 0; j < kGrp; j += 4) { total += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]); }
@@ -689,8 +691,7 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.row_tiles  = row_tiles_of(a);
     plan.group      = a.heads / a.kv_heads;
     plan.tables     = a.kv_heads * plan.row_tiles;
-    plan.scale2      = float(double(a.scale) * M_LOG2E);
-    plan.scale2_rest = float(double(a.scale) * M_LOG2E - double(plan.scale2));
+    plan.scale2     = float(double(a.scale) * M_LOG2E);
     plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
     // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and
     // fewer streams are read faster: 64 sequences up to 8,192 168 -> 159 us, one of 131,072 91.6 -> 89.6 us.

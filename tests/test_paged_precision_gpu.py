@@ -26,6 +26,29 @@ def cancelling(weights, width, dtype, seed):
     return v
 
 
+def check_cancelled(out, w, v, dtype, units):
+    """|out - sum w v| <= units u sum w |v|, and the output's rounding: half a unit in its last place."""
+    want, spread = (w[..., None] * v).sum(2), (w[..., None] * v.abs()).sum(2)
+    bound = units * U * spread + (ref.UNIT[dtype] + units * U) * want.abs() + ref.UNIT[dtype] * torch.finfo(dtype).tiny
+    assert (want.abs() < spread / 1000).all()  # that hides nothing
+    assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
+
+
+def attend_scores(s, v, dtype, scale, base=0.0):
+    """paged_attention over exact scores base + s (rows, heads, n) and values v (rows, heads, n, d); float64."""
+    b, h, n, d = v.shape
+    kp, vp = torch.zeros((b, 8, h, d), dtype=dtype), torch.zeros((b, 8, h, d), dtype=dtype)
+    kp[:, :n, :, 0], kp[:, :n, :, 1] = s.transpose(1, 2).to(dtype), base
+    vp[:, :n] = v.transpose(1, 2).to(dtype)
+    q = torch.zeros((b, h, d), dtype=dtype)
+    q[..., :2] = 1.0
+    assert torch.equal(kp[:, :n, :, 0].double(), s.transpose(1, 2).double()) and (kp[:, :n, :, 1] == base).all()
+    assert torch.equal(vp[:, :n].double(), v.transpose(1, 2))
+    table = torch.arange(b, dtype=torch.int32).view(b, 1)
+    return certex.paged_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), torch.full((b,), n, device="cuda"),
+                                  scale=scale).double().cpu()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attend_weights_are_whole(gpu, dtype):
     """The softmax's weights enter the product with the values as float32 has them. Scores are exact, |scale score| <= 1:
@@ -36,19 +59,21 @@ def test_attend_weights_are_whole(gpu, dtype):
     s = torch.randint(-128, 129, (b, h, n), generator=g) / 128.0
     w = torch.softmax(s.double(), -1)
     v = cancelling(w.reshape(b * h, n), d, dtype, 2).reshape(b, h, n, d)
-    kp, vp = torch.zeros((b, 8, h, d), dtype=dtype), torch.zeros((b, 8, h, d), dtype=dtype)
-    kp[:, :n, :, 0] = s.transpose(1, 2).to(dtype)
-    vp[:, :n] = v.transpose(1, 2).to(dtype)
-    q = torch.zeros((b, h, d), dtype=dtype)
-    q[..., 0] = 1.0
-    assert torch.equal(kp[:, :n, :, 0].double(), s.transpose(1, 2).double()) and torch.equal(vp[:, :n].double(), v.transpose(1, 2))
-    table = torch.arange(b, dtype=torch.int32).view(b, 1)
-    out = certex.paged_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(),
-                                 torch.full((b,), n, device="cuda"), scale=1.0).double().cpu()
-    want, spread = (w[..., None] * v).sum(2), (w[..., None] * v.abs()).sum(2)
-    bound = 16 * U * spread + (ref.UNIT[dtype] + 16 * U) * want.abs() + ref.UNIT[dtype] * torch.finfo(dtype).tiny
-    assert (want.abs() < spread / 1000).all()  # the output's own rounding hides nothing
-    assert ((out - want).abs() <= bound).all(), float(((out - want).abs() / bound).max())
+    check_cancelled(attend_scores(s, v, dtype, 1.0), w, v, dtype, 16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("base", [0, 344 - 8, 2752, 32768])
+def test_attend_scores_far_from_zero(gpu, dtype, base):
+    """A score's exponent is rounded after the maximum has left it. Scores are exact and differ by up to D = 6.5 in powers
+    of 2: the subtraction's rounding and the scale's take u D ln 2 each, 9 u; 3 u are the exponential's and the weight's, 8 u
+    the sums'. (At a score of 344.85 or 2758.8, a scale of 0.75 times log2(e) is half a unit in the last place off.)"""
+    b, h, d, n = 32, 4, 64, 4
+    g = torch.Generator().manual_seed(5)
+    s = 4 + torch.randint(0, 48, (b, h, n), generator=g) / 8.0
+    w = torch.softmax(0.75 * s.double(), -1)
+    v = cancelling(w.reshape(b * h, n), d, dtype, 6).reshape(b, h, n, d)
+    check_cancelled(attend_scores(s, v, dtype, 0.75, base), w, v, dtype, 20)
 
 
 # few queries a head gather rows; many, over values larger than a die's cache, go by ranges
