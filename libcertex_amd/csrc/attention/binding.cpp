@@ -157,8 +157,19 @@ auto ints(Tensor const& t, const char* what, bool narrow = false) -> Tensor
   return t.is_contiguous() ? t : t.contiguous();
 }
 
+/** The kernels read and write values alone: a tensor that carries a tangent of forward-mode differentiation is refused,
+ *  or the result would pass for a constant. */
+void no_tangent(std::initializer_list<Tensor const*> tensors)
+{
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) { return; }
+  for (Tensor const* t : tensors) {
+    EXPECTS(t == nullptr || !t->_fw_grad(0).defined(), "this operator has no forward-mode derivative");
+  }
+}
+
 void no_gradient(std::initializer_list<Tensor const*> tensors)
 {
+  no_tangent(tensors);
   if (!at::GradMode::is_enabled()) { return; }
   for (Tensor const* t : tensors) {
     EXPECTS(t == nullptr || !t->requires_grad(), "this operator has no gradient: call it under torch.no_grad()");
@@ -184,6 +195,7 @@ using rotary_ptr = c10::intrusive_ptr<rotary>;
 
 auto turned(Tensor const& x_, Tensor const& positions_, rotary_ptr const& r, bool transpose, maybe const& out) -> Tensor
 {
+  no_tangent({&x_, out ? &*out : nullptr});
   const Tensor x = read(x_, "x", int(x_.dim())), positions = ints(positions_, "positions");
   EXPECTS(positions.sizes() == x.sizes().slice(0, x.dim() - 2),
           "positions must have shape " + shape_of(x.sizes().slice(0, x.dim() - 2)) + ", one entry per token");
