@@ -176,6 +176,13 @@ void no_gradient(std::initializer_list<Tensor const*> tensors)
   }
 }
 
+/** Tells autograd that a call has written t through its address: a backward pass that saved t before raises, as after
+ *  torch's in-place operators. (Tensors of inference mode are saved by none and have no version.) */
+void wrote(Tensor const& t)
+{
+  if (!t.is_inference()) { t.unsafeGetTensorImpl()->bump_version(); }
+}
+
 /** Workspace of a call (none where it needs none). */
 auto workspace(int64_t bytes, Tensor const& like) -> maybe
 {
@@ -209,6 +216,7 @@ auto turned(Tensor const& x_, Tensor const& positions_, rotary_ptr const& r, boo
   }
   view xv(x), pv(positions), yv(y);
   check(cuvsCertexRotate(resources(), r->handle, &xv, &pv, &yv, transpose));
+  if (out) { wrote(y); }
   return y;
 }
 
@@ -379,6 +387,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n)
     {
       unlocked u;
       check(cuvsCertexAppendPages(resources(), r ? r->handle : 0, &kv, &vv, &kp, &vp, &tv, &pv, &sv, &qv, &ov));
+      wrote(k_pages);
+      wrote(v_pages);
     }
     if (!out) { Py_RETURN_NONE; }
     return wrap(*out);

@@ -59,3 +59,36 @@ def test_tangents_are_refused(gpu):
         with pytest.raises(RuntimeError):
             y.backward(dual(x))
     assert (pool == 0).all()
+
+
+def test_written_tensors_change_version(gpu):
+    """A backward pass whose saved tensor the calls have written over since raises, as torch's in-place operators make it."""
+    rope = certex.Rotary(64)
+    pool, table, p = cache()
+    w, x, buf = torch.ones((), device="cuda", requires_grad=True), rand(5, 2, 64), rand(5, 2, 64, seed=1)
+    y = w * buf
+    rope(x, p, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = w * buf
+    rope(buf, p, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    k_pages, v_pages = pool.clone(), pool.clone()
+    for saved in (k_pages, v_pages, k_pages.transpose(1, 2), v_pages[1:2]):  # a view shares its tensor's version
+        y = w * saved
+        certex.append_pages(x, x, k_pages, v_pages, table, p)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    # what is only read is not: these backward passes run
+    before = [t._version for t in (x, k_pages, v_pages, buf)]
+    certex.paged_attention(x, k_pages, v_pages, table, p)
+    rope(x, p)
+    certex.append_pages(x, x, pool.clone(), pool.clone(), table, p, rotary=rope, q=buf)
+    assert before == [t._version for t in (x, k_pages, v_pages, buf)]
+    with torch.inference_mode():  # tensors without a version are written as ever
+        held, pages = x.clone(), pool.clone()
+        assert torch.equal(rope(held, p, out=held), rope(x, p))
+        certex.append_pages(x, x, pages, pages.clone(), table, p)
+    certex.append_pages(x, x, pages, pages.clone(), table, p)
+    assert pages.is_inference()
