@@ -351,6 +351,8 @@ PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n)
               std::to_string(dim) + ")");
     const bool differentiated = x.requires_grad() && at::GradMode::is_enabled();
     EXPECTS(!differentiated || !out, "a rotation that is differentiated takes no out");
+    EXPECTS(!out || !out->requires_grad() || !at::GradMode::is_enabled(),
+            "out must not require a gradient: call the rotation without it, or under torch.no_grad()");
     Tensor y;
     {
       unlocked u;

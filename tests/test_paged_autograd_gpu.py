@@ -92,3 +92,18 @@ def test_written_tensors_change_version(gpu):
         certex.append_pages(x, x, pages, pages.clone(), table, p)
     certex.append_pages(x, x, pages, pages.clone(), table, p)
     assert pages.is_inference()
+
+
+def test_out_that_requires_a_gradient_is_refused(gpu):
+    """Neither a leaf nor a result of the graph is overwritten behind autograd's back."""
+    rope = certex.Rotary(64)
+    x, p = rand(5, 2, 64), torch.arange(5, device="cuda")
+    leaf = rand(5, 2, 64, seed=1).requires_grad_()
+    before = leaf.detach().clone()
+    for out in (leaf, leaf * 2.0, leaf[:]):
+        with pytest.raises(ValueError, match="out must not require a gradient"):
+            rope(x, p, out=out)
+    assert torch.equal(leaf, before)
+    with torch.no_grad():  # as torch's own in-place operators go
+        rope(x, p, out=leaf)
+    assert torch.equal(leaf.detach(), rope(x, p)) and leaf._version == 1
