@@ -10,7 +10,8 @@
  * allocate nothing and read nothing back, so that a stream capture records them.
  *
  * "Rows": a tensor whose last dimension is dense and whose other dimensions have any strides.
- * "Dense": row major without gaps. Elements are float32, float16 or bfloat16, the same for all
+ * "Dense": row major without gaps. What a call writes must share no memory with what it reads, nor within itself, unless
+ * its description says so. Elements are float32, float16 or bfloat16, the same for all
  * row tensors of a call; "integers" are int32 or int64. Sums, maxima and the rotation are computed in
  * float32 or more.
  */
@@ -77,8 +78,8 @@ CUVS_EXPORT cuvsError_t cuvsCertexRotaryFrequencies(cuvsCertexRotaryParams_t par
 /**
  * y = x with the first rotary_dim elements of every head rotated: pair (a, b) of position p and
  * frequency f becomes magnitude * (a cos pf - b sin pf, a sin pf + b cos pf).
- * x and y: rows [tokens, heads, dim] or [batch, tokens, heads, dim]; y may be x itself. positions:
- * dense integers [tokens] or [batch, tokens], of any sign and size. With `transpose` the matrix of
+ * x and y: rows [tokens, heads, dim] or [batch, tokens, heads, dim]; y may be x itself (the same address and
+ * strides), and else shares no memory with it. positions: dense integers [tokens] or [batch, tokens], of any sign and size. With `transpose` the matrix of
  * the rotation is transposed (the negative angle, the same magnitude): x is then the gradient
  * of y, and y the gradient of x.
  */
@@ -96,7 +97,8 @@ CUVS_EXPORT cuvsError_t cuvsCertexRotate(cuvsResources_t res,
  * k: rows [tokens, kv_heads, dim]; v: rows [tokens, kv_heads, vdim]; k_pages: rows [n_pages,
  * page_size, kv_heads, dim]; v_pages: the same with vdim; page_table: dense int32 [n_sequences, n]; positions:
  * dense integers [tokens]; sequences: the same, or NULL: token t belongs to sequence t. With q
- * (rows [tokens, heads, dim], or NULL) the same launch rotates the tokens' queries into q_out.
+ * (rows [tokens, heads, dim], or NULL) the same launch rotates the tokens' queries into q_out, which may be
+ * q itself and else shares no memory with q, k, v or the pages. The slots that are written must not lie in k, v or q.
  * A token of a negative position or sequence (padding), or whose page the table does not hold
  * (an entry outside [0, n_pages)), is not written. Two tokens of one position: either is kept.
  */

@@ -5,6 +5,7 @@
 
 #include "../certex_state.hpp"
 #include "attention.hpp"
+#include "overlap.hpp"
 
 #include <cmath>
 #include <exception>
@@ -138,13 +139,43 @@ auto rows(tensor t, ops::elem* type, bool first) -> tensor
   return t;
 }
 
-/** A row tensor that is written: no two of its rows may share memory through a zero stride. */
+struct dimensions {
+  ops::dimension d[kMaxDims];
+  explicit dimensions(tensor const& t)
+  {
+    for (int i = 0; i < t.ndim; ++i) { d[i] = {t.shape[i], t.stride[i]}; }
+  }
+};
+
+/** A row tensor that is written: no two of its elements may be one in memory. */
 auto written(tensor t) -> tensor
 {
+  if (t.size() == 0) { return t; }
   for (int i = 0; i < t.ndim; ++i) {
-    EXPECTS(t.stride[i] > 0 || t.size() == 0, std::string(t.name) + " is written and must not be broadcast");
+    EXPECTS(t.stride[i] > 0, std::string(t.name) + " is written and must not be broadcast");
   }
+  EXPECTS(!ops::shares_itself(dimensions(t).d, t.ndim),
+          std::string(t.name) + " is written and none of its elements may share memory");
   return t;
+}
+
+/** That b, which is written, shares no memory with a of the same element type, which is read or written by others. */
+void expects_apart(tensor const& a, tensor const& b)
+{
+  if (a.size() == 0 || b.size() == 0) { return; }
+  const int64_t distance = (static_cast<char const*>(b.p) - static_cast<char const*>(a.p)) / (b.type.bits / 8);
+  EXPECTS(!ops::shares(dimensions(a).d, a.ndim, dimensions(b).d, b.ndim, distance),
+          std::string(a.name) + " and " + b.name + " must not share memory in part");
+}
+
+/** The same, or that b is a, element for element. */
+void expects_same_or_apart(tensor const& a, tensor const& b)
+{
+  if (a.p == b.p && a.ndim == b.ndim && std::equal(a.shape, a.shape + a.ndim, b.shape) &&
+      std::equal(a.stride, a.stride + a.ndim, b.stride)) {
+    return;
+  }
+  expects_apart(a, b);
 }
 
 auto integers(DLManagedTensor* m, const char* name) -> tensor
@@ -426,6 +457,7 @@ cuvsError_t cuvsCertexRotate(cuvsResources_t res,
     EXPECTS(h.device == r.device(), "the rotary handle is on another device than the resources");
     EXPECTS(x.shape[1 + o] < (1 << 30) && x.shape[2 + o] < (1 << 30), "x is too large");
     if (x.size() == 0) { return; }
+    expects_same_or_apart(x, y);
     ops::turn_args a;
     a.frequencies = h.frequencies.as<uint64_t>();
     a.magnitude   = h.magnitude;
@@ -529,6 +561,8 @@ cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
       EXPECTS(q.ndim == 3 && q.shape[0] == tokens && q.shape[2] == k.shape[2], "q must have the tokens and head dimension of k");
       expects_shape(qo, {q.shape[0], q.shape[1], q.shape[2]});
       expects_device(r, q, qo);
+      expects_same_or_apart(q, qo);
+      for (tensor const* t : {&k, &v, &kp, &vp}) { expects_apart(*t, qo); }
       add(q, qo, rotated, false);
     }
     if (a.jobs == 0) { return; }

@@ -85,7 +85,7 @@ class Rotary:
 
     def __call__(self, x, positions, transpose=False, out=None):
         """x (tokens, heads, head_dim) or (batch, tokens, heads, head_dim), rotated by positions (tokens,) or (batch,
-        tokens): a tensor of its own, or `out` (which may be x). transpose: by the negative angle. Differentiable
+        tokens): a tensor of its own, or `out` (which may be x, and else shares no memory with it). transpose: by the negative angle. Differentiable
         in x (without out)."""
         return C.operators().rotate(self._handle(x), self.head_dim, x, positions, transpose, out)
 
