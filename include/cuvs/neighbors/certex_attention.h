@@ -100,7 +100,8 @@ CUVS_EXPORT cuvsError_t cuvsCertexRotate(cuvsResources_t res,
  * (rows [tokens, heads, dim], or NULL) the same launch rotates the tokens' queries into q_out, which may be
  * q itself and else shares no memory with q, k, v or the pages. The slots that are written must not lie in k, v or q.
  * A token of a negative position or sequence (padding), or whose page the table does not hold
- * (an entry outside [0, n_pages)), is not written. Two tokens of one position: either is kept.
+ * (an entry outside [0, n_pages)), is not written. The tokens of one call are to have positions of their own: a slot
+ * that several name ends with elements of any of them mixed.
  */
 CUVS_EXPORT cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
                                               cuvsCertexRotary_t rotary,

@@ -96,7 +96,8 @@ def append_pages(k, v, k_pages, v_pages, page_table, positions, sequences=None, 
     head_dim) the same launch rotates the queries, which are returned (else None).
 
     A token with a negative position or sequence is padding and is not written; neither is one whose page the
-    table does not hold (an entry outside the pool, such as -1). Positions of one call are to be distinct."""
+    table does not hold (an entry outside the pool, such as -1). The tokens of one call are to have positions of their own: a slot that
+    several name ends with elements of any of them mixed."""
     return C.operators().append(None if rotary is None else rotary._handle(k), 0 if rotary is None else rotary.head_dim, k, v,
                                 k_pages, v_pages, page_table, positions, sequences, q)
 
