@@ -207,13 +207,14 @@ __global__ __launch_bounds__(kThreads) void select_kernel(select_args a, select_
       top = grown;
     }
     const float p       = weight_of(plan.scale, x, top == -INFINITY ? 0.0f : top);
-    const uint64_t some = __ballot(p != 0.0f);  // NaN too
+    const bool counts   = x != -INFINITY;  // however little it weighs
+    const uint64_t some = __ballot(counts);
     if (some == 0) { continue; }
     total += p;
-    // what weighs nothing reads the row of an id that does: its own may hold anything
+    // what does not count reads the row of an id that does: its own may hold anything
     const int64_t other = __shfl(at, __builtin_ctzll(some));
     s_p[wave][lane]     = p;
-    s_at[wave][lane]    = p != 0.0f ? at : other;
+    s_at[wave][lane]    = counts ? at : other;
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
 #pragma unroll

@@ -128,3 +128,20 @@ def test_selected_lowest_scores(gpu, queries, n, k, width, scale):
             assert float((out[h, i].double().cpu() - w @ rows).norm() / (w @ rows.abs()).norm()) <= e
             want = torch.logsumexp(s, 0)
             assert abs(float(lse[h, i].double().cpu() - want)) <= e + 4 * U * abs(float(want))
+
+
+@pytest.mark.parametrize("queries, n, k, width", ROUTES)
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("last", [False, True])
+def test_selected_value_of_a_vanishing_weight(gpu, queries, n, k, width, value, last):
+    """A selected value that is not finite shows in its column even where its weight is too small for float32, whichever
+    way the ids are taken; a score of -inf keeps it out."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    values, scores = torch.randn((2, n, width), generator=g, device="cuda"), torch.randn((4, queries, k), generator=g, device="cuda")
+    ids = torch.randint(1, n, (4, queries, k), generator=g, device="cuda")
+    values[0, 0, 2] = value
+    j = k - 1 if last else 0
+    ids[0, 0, j], ids[1, 1, j] = 0, 0
+    scores[0, 0, j], scores[1, 1, j] = -1e5, float("-inf")
+    finite = certex.selected_attention(scores, ids, values, 1.0).isfinite()
+    assert not finite[0, 0, 2] and finite.sum() == finite.numel() - 1
