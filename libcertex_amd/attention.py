@@ -171,9 +171,15 @@ class KeyCache:
 
     def attend(self, q, values, k=None, scale=None, page_table=None, batch=None):
         """Sparse attention: softmax over the exact top k of every query, times the values of those keys. q as in
-        topk; values (n_kv_heads, n, value_dim) in key order, or with page_table the pages of this sequence (see
-        selected_attention); scale defaults to head_dim ** -0.5. Returns (n_heads, m, value_dim) or (n_heads, value_dim)
-        in the values' type."""
+        topk; values (n_kv_heads, n, value_dim) in key order, n at least the cache's size, or with page_table the pages of
+        this sequence (see selected_attention); scale defaults to head_dim ** -0.5. Returns (n_heads, m, value_dim) or
+        (n_heads, value_dim) in the values' type."""
+        paged = page_table is not None
+        tensors = all(isinstance(t, torch.Tensor) for t in ((values, page_table) if paged else (values,)))
+        if tensors and values.ndim == (4 if paged else 3):  # else selected_attention says what is wrong
+            heads, held = (values.shape[2], page_table.numel() * values.shape[1]) if paged else values.shape[:2]
+            _require(heads == self.n_kv_heads, f"values must have the cache's {self.n_kv_heads} heads, not {heads}")
+            _require(held >= self.size, f"values must hold the cache's {self.size} keys, not {held}")
         scores, ids = self.topk(q, k, batch)
         return selected_attention(scores, ids, values, self.head_dim**-0.5 if scale is None else scale, page_table)
 
