@@ -7,6 +7,7 @@ on equal scores, the lower key id first.
 
 import torch
 
+from . import _capi as C
 from .index import Index, _require
 from .paged import selected_attention
 
@@ -180,6 +181,8 @@ class KeyCache:
             heads, held = (values.shape[2], page_table.numel() * values.shape[1]) if paged else values.shape[:2]
             _require(heads == self.n_kv_heads, f"values must have the cache's {self.n_kv_heads} heads, not {heads}")
             _require(held >= self.size, f"values must hold the cache's {self.size} keys, not {held}")
+        if isinstance(q, torch.Tensor):
+            C.operators().undifferentiated(q)  # the search would drop its gradient without a word
         scores, ids = self.topk(q, k, batch)
         return selected_attention(scores, ids, values, self.head_dim**-0.5 if scale is None else scale, page_table)
 

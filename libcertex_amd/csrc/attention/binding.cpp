@@ -488,6 +488,16 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n)
   });
 }
 
+/** (tensor): refuses one that is differentiated, for callers whose first step is not of this extension. */
+PyObject* undifferentiated(PyObject*, PyObject* t)
+{
+  return guarded([&] {
+    no_gradient({&tensor(t, "the tensor")});
+    Py_INCREF(Py_None);
+    return Py_None;
+  });
+}
+
 template <typename F>
 constexpr PyCFunction fast(F f)
 {
@@ -502,6 +512,7 @@ PyMethodDef methods[] = {{"init", fast(init), METH_FASTCALL, "(CertexError, torc
                          {"attend", fast(attend), METH_FASTCALL,
                           "(q, k_pages, v_pages, page_table, lengths, scale, window, return_lse)"},
                          {"select", fast(select), METH_FASTCALL, "(scores, ids, values, scale, page_table, return_lse)"},
+                         {"undifferentiated", undifferentiated, METH_O, "(tensor): refuses one that is differentiated"},
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_attention", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,4 +1,4 @@
-"""KeyCache.attend takes the values of its own keys: of its heads, and of every key."""
+"""KeyCache.attend takes the values of its own keys: of its heads, and of every key. It has no gradient, and says so."""
 
 import pytest
 import torch
@@ -34,3 +34,21 @@ def test_values_of_other_keys_are_refused(gpu):
     missing = table.clone()
     missing[2] = -1  # a page that is gone does not count, as ever
     assert cache.attend(q, pages, page_table=missing).isfinite().all()
+
+
+def test_differentiated_queries_are_refused(gpu):
+    """A gradient or a tangent of the queries would be lost in the search: an error, as for the values."""
+    import torch.autograd.forward_ad as fwd
+
+    keys, q, values = (torch.randn(s, device="cuda") for s in ((2, 50, 64), (4, 3, 64), (2, 50, 32)))
+    cache = certex.KeyCache(2, 64, k=20).append(keys)
+    q.requires_grad_()
+    for call in (lambda: cache.attend(q, values), lambda: cache.attend(q.detach(), values.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+    with torch.no_grad():
+        want = cache.attend(q, values)
+    q = q.detach()
+    assert torch.equal(cache.attend(q, values), want) and torch.equal(cache.attend(q.cpu().numpy(), values), want)
+    with fwd.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        cache.attend(fwd.make_dual(q, torch.ones_like(q)), values)
