@@ -409,13 +409,14 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       float x[kGrp];
 #pragma unroll
       for (int j = 0; j < kGrp; ++j) { x[j] = s[j / 4][j % 4] * plan.scale2; }
-      const int t      = (group + g) * kGrp;
-      const bool whole = have && t >= sp.begin && t + kGrp <= sp.end;
+      const uint32_t t = uint32_t(group + g) * kGrp;  // past the end it may pass 2^31
+      const uint32_t t_begin = uint32_t(sp.begin), t_end = uint32_t(sp.end);
+      const bool whole  = have && t >= t_begin && t + kGrp <= t_end;
       const bool masked = !__all(whole);
       if (masked) {
 #pragma unroll
         for (int j = 0; j < kGrp; ++j) {
-          const bool in = have && t + j >= sp.begin && t + j < sp.end;
+          const bool in = have && t + j >= t_begin && t + j < t_end;
           x[j]          = in ? x[j] : -INFINITY;
 #pragma unroll
           for (int n = 0; n < kBlocks; ++n) {
