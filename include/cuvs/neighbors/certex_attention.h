@@ -63,7 +63,7 @@ typedef struct cuvsCertexRotaryParams* cuvsCertexRotaryParams_t;
 CUVS_EXPORT cuvsError_t cuvsCertexRotaryParamsCreate(cuvsCertexRotaryParams_t* params);
 CUVS_EXPORT cuvsError_t cuvsCertexRotaryParamsDestroy(cuvsCertexRotaryParams_t params);
 
-/** A rotation: its frequencies in the memory of one device. */
+/** A rotation: its frequencies in the memory of one device. A recorded graph reads them there: destroy it after the graph. */
 typedef uintptr_t cuvsCertexRotary_t;
 CUVS_EXPORT cuvsError_t cuvsCertexRotaryCreate(cuvsResources_t res,
                                                cuvsCertexRotaryParams_t params,
@@ -124,9 +124,9 @@ CUVS_EXPORT cuvsError_t cuvsCertexAppendPages(cuvsResources_t res,
  * out: dense [n_sequences, heads, vdim]; lse (or NULL): dense float32 [n_sequences, heads], the
  * logarithm of the softmax's denominator. Positions whose page the table does not hold do not count; a row
  * without positions gives zeros, and lse -inf. Slots at and past a sequence's length are not used,
- * whatever they hold. An infinite value that counts makes its column of out infinite or NaN. workspace: a dense uint8 vector of at least the bytes that
- * cuvsCertexPagedAttentionWorkspace reports for the same tensors (NULL if 0), in use until the
- * queued work is done.
+ * whatever they hold. An infinite value that counts, however little it weighs, makes its column of out infinite or NaN.
+ * workspace: a dense uint8 vector of at least the bytes that cuvsCertexPagedAttentionWorkspace reports
+ * for the same tensors (NULL if 0), in use until the queued work is done.
  */
 CUVS_EXPORT cuvsError_t cuvsCertexPagedAttention(cuvsResources_t res,
                                                  DLManagedTensor* q,

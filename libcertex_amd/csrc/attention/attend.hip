@@ -11,12 +11,12 @@
 // - a wave takes 32 positions (float32: 16); S^T = K Q^T has the positions as rows and up to 16 query heads
 //   as columns, so that K rows go from memory to the operand registers as they lie (16 bytes per lane);
 // - the rows of the two 16-position products are permuted such that a lane's 8 results are the 8
-//   consecutive positions that it holds as k-slots of O^T = V^T P^T: the weights never move;
+//   consecutive positions that it holds as k-slots of O^T = V^T P^T: the weights never move (16-bit types take them
+//   whole, as three elements, and so this product three times);
 // - V^T is formed in registers: a lane loads 8 positions x 8 columns (16 bytes of a row each, whole rows
 //   per 16 lanes) and swaps halfwords (v_perm), 32 instructions per 32 x 128 values (float32: as it lies);
 // - m, the sum and the scaling are per query head, that is per lane.
 // The loads of the next keys and of this tile's values are in flight during both products.
-//
 //
 // Work is dealt on the device, from the lengths: the tiles of all sequences, one after the other, in
 // equal shares, each share to one workgroup per key head. So any mix of lengths fills the chip and the
@@ -27,7 +27,8 @@
 // Measured (8 key heads of 128 bfloat16, 32 query heads; reading alone reaches 6.4 TB/s): 64 sequences up
 // to 8,192, 0.94 GB of keys and values: 158 us with the 6 us of the join, 5.9 TB/s; one sequence of
 // 131,072, 0.54 GB: 88 us, 6.1 TB/s; four of up to 131,072: 6.3 TB/s. Heads of 64: 5.4 TB/s where a slot holds
-// all heads (128 bytes of a line pair each), 6.2 with the heads first. More workgroups or waves per
+// all heads (128 bytes of a line pair each), 6.2 with the heads first; of 256 6.2, and 5.8 in float32; of 160, and of 192
+// with values of 128, which run as 256, 4.4. More workgroups or waves per
 // compute unit read slower (three: 193 us for the 64 sequences): the memory prefers fewer streams.
 #include "../kernels/lanes.hpp"
 #include "attention.hpp"

@@ -8,9 +8,10 @@
 // angle costs the sines less than their own rounding.
 //
 // What bounds it: every element is read and written once. A thread takes one vector of a row over several heads of a token,
-// so that sines are computed once for up to 8 heads. Measured: 131,072 tokens x 8 heads of 128 bfloat16, 0.54 GB: 84 us
-// a pass, 6.4 TB/s (a copy of 2 GiB: 4.9); prompts of 15,443 tokens appended with their queries, 190 MB: 35 us,
-// 5.4 TB/s; 64 queries of a step 4.6 us, their append 5.3 us: launch and three dependent loads.
+// so that sines are computed once for up to 8 heads. Measured, the kernel alone: 131,072 tokens x 8 heads of 128 bfloat16,
+// 0.54 GB: 82 us, 6.5 TB/s (with fresh outputs in turn 96 us a pass, where torch's clone of as much takes 99); prompts of
+// 15,443 tokens appended with their queries, 190 MB: 33 us, 5.7 TB/s; 64 queries of a step 4.8 us, their append 5.2 us:
+// launch and three dependent loads.
 #include "attention.hpp"
 #include "elements.hpp"
 

@@ -9,7 +9,10 @@ A paged cache is two pools, keys (n_pages, page_size, n_kv_heads, head_dim) and 
 dimension), and a page table (n_sequences, n) of int32: position p of sequence s is slot p % page_size of
 page table[s, p // page_size]. The program that schedules the sequences owns the pools, the table and the lengths;
 the pools may be views of any strides with a dense last dimension. The calls run on torch's current
-stream, read nothing back to the host and allocate from torch, so a graph capture records them.
+stream, read nothing back to the host and allocate from torch, so a graph capture records them. As for an Index their tensors
+are on the current GPU (torch.cuda.device chooses it); tensors of another one are an error. Only the rotation has a
+gradient; tensors that ask for another, or carry a tangent of forward-mode differentiation, are refused. What a call
+writes in place (out, k_pages, v_pages) changes its version, so that a backward pass that saved it before raises.
 """
 
 import ctypes
@@ -39,7 +42,7 @@ class Rotary:
     0.1 ln(factor) + 1 unless given. Any position goes: its product with the frequency (a double) is reduced to a turn
     exactly, in 64-bit fixed point. The frequencies are put on the current GPU when the rotation is made (if
     the program has used a GPU by then) and on others at the first use there, which waits for that GPU: before a graph
-    is recorded, not in it.
+    is recorded, not in it. A graph that rotates reads them there: keep the rotation as long as the graph.
     """
 
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, layout="half", scaling=None, factor=1.0,
@@ -109,7 +112,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
 
     A sequence of length 0 gives zeros. Lengths past the table's pages are cut to them, positions whose page the
     table does not hold do not count, and slots past a length are never used, whatever they hold; an
-    infinite value that counts makes its column of the output infinite or NaN. With
+    infinite value that counts, however little it weighs, makes its column of the output infinite or NaN. With
     return_lse also the logarithm of the softmax's denominator (float32, -inf for an empty row), which
     joins the outputs of two calls over different positions. A cache holds head dimensions up to 256 and
     pages of a multiple of 8 positions."""
@@ -123,6 +126,6 @@ def selected_attention(scores, ids, values, scale, page_table=None, return_lse=F
     page_size, n_kv_heads, value_dim). Query head h reads value head h // (n_heads / n_kv_heads).
 
     Ids outside the values (-1 marks a missing neighbour) and scores of -inf do not count; a row of none gives zeros.
-    An infinite value that counts makes its column of the output infinite or NaN.
+    An infinite value that counts, however little it weighs, makes its column of the output infinite or NaN.
     With return_lse also the logarithm of the softmax's denominator (float32, -inf for an empty row)."""
     return C.operators().select(scores, ids, values, scale, page_table, return_lse)
