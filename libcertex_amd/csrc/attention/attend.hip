@@ -1,8 +1,8 @@
 // Attention of one new token of every sequence over its pages of keys and values.
 //
-// out = sum_t p_t v_t / sum_t p_t with p_t = 2^(x_t - m), x_t = scale log2(e) q.k_t, over the positions t
+// out = sum_t p_t v_t / sum_t p_t with p_t = 2^(scale log2(e) (x_t - m)), x_t = q.k_t, over the positions t
 // of [max(0, len - window), len). One pass over the positions keeps a reference m, the sum and the
-// output in float32, and scales the last two where m grows.
+// output in float32, and scales the last two where m grows. A negative scale turns q's sign.
 //
 // What bounds it: every key and value is read once and used by the heads / kv_heads query heads that share
 // it, a few operations per byte, so the rate at which memory is read. The kernel keeps the two products
@@ -44,7 +44,6 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kRows    = 16;   // query heads of a product
 constexpr int kUnits   = 256;  // compute units
 constexpr int kMaxShares = 2 * kUnits;
-constexpr float kLog2e = 1.44269504088896340736f;
 
 using f32x4  = __attribute__((ext_vector_type(4))) float;
 using u32x4  = __attribute__((ext_vector_type(4))) uint32_t;
@@ -81,7 +80,8 @@ struct attend_plan {
   int32_t shares;       // of a table's tiles, at most
   int32_t halve;        // half as many shares where each of those has this many tiles or more (0: never)
   bool one_die;         // the tables of a share run on one die
-  float scale2;         // scale log2(e)
+  score_scale scale;
+  float slack;          // kSlack in scores
   float* part_out;      // [tables][2 shares][kRows][vdim]
   float* part_max;      // [tables][2 shares][kRows]
   float* part_sum;
@@ -182,12 +182,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
   return w;
 }
 
-/** The weights' reference may lag the largest exponent by this much before the sums are rescaled, and weights are
- *  multiplied by 2^kLift: float16 weights reach 2^15 and keep their precision down to 2^-28 of the largest. */
+/** The weights' reference may lag the largest exponent by this much (twice as much where large scores round it) before the
+ *  sums are rescaled, and weights are multiplied by 2^kLift: float16 weights reach 2^15 and keep their precision down to
+ *  2^-27 of the largest. */
 template <typename T>
 constexpr float kSlack = 8.0f;
 template <>
-constexpr float kSlack<f16_t> = 2.0f;
+constexpr float kSlack<f16_t> = 1.0f;
 template <typename T>
 constexpr float kLift = 0.0f;
 template <>
@@ -260,6 +261,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
   const int dim = FULL ? D : a.dim, vdim = FULL ? D : a.vdim;
   const int kv = table % a.kv_heads, row0 = table / a.kv_heads * kRows;
   const int rows = min(kRows, plan.group - row0), h0 = kv * plan.group + row0;
+  const uint32_t flip = plan.scale.sign < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;  // of a word of q
   const T* k_head = static_cast<const T*>(a.k) + kv * a.k_head;
   const T* v_head = static_cast<const T*>(a.v) + kv * a.v_head;
 
@@ -339,7 +341,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       const int dim0 = (c * 4 + g) * kPiece;
       const int skip = FIT == fit::part ? dim0 - min(dim0, key_off) : 0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) { q[c][w] = r < rows ? q[c][w] & counted<T>(skip, w) : 0u; }
+      for (int w = 0; w < 4; ++w) { q[c][w] = r < rows ? (q[c][w] & counted<T>(skip, w)) ^ flip : 0u; }
     }
     f32x4 o[kOut];
 #pragma unroll
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       // weights: lane group g holds the positions t + 0..kGrp - 1 of query r
       float x[kGrp];
 #pragma unroll
-      for (int j = 0; j < kGrp; ++j) { x[j] = s[j / 4][j % 4] * plan.scale2; }
+      for (int j = 0; j < kGrp; ++j) { x[j] = s[j / 4][j % 4]; }
       const uint32_t t = uint32_t(group + g) * kGrp;  // past the end it may pass 2^31
       const uint32_t t_begin = uint32_t(sp.begin), t_end = uint32_t(sp.end);
       const bool whole  = have && t >= t_begin && t + kGrp <= t_end;
@@ -433,20 +435,20 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         const auto larger = [](float u, float w) { return fmaxf(u, w); };
         high              = lanes::fold16(lanes::fold32(high, larger), larger);
         const float grown = fmaxf(top, high);
-        const float keep  = grown == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - grown);
+        const float keep  = grown == -INFINITY ? 0.0f : weight_of(plan.scale, top, grown);
         total *= keep;
 #pragma unroll
         for (int i = 0; i < kOut; ++i) { o[i] *= keep; }
         top   = grown;
-        limit = grown + kSlack<T>;
-        base  = grown == -INFINITY ? 0.0f : grown - kLift<T>;
+        limit = grown + plan.slack;
+        // with a scale of 0 all weigh alike, wherever the scores are
+        base = grown == -INFINITY || plan.scale.scale2 == 0.0f ? 0.0f : grown;
       }
       float p[kGrp];
 #pragma unroll
       for (int j = 0; j < kGrp; ++j) {
-        // the exponent is rounded once, after the subtraction, at the size of its distance from the maximum (the scale's own
-        // rounding stretches that distance by 2^-24 of itself)
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], plan.scale2, -base));
+        // what is rounded is the distance from the reference
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - base, plan.scale.scale2, kLift<T>));
       }
       if (masked) {
 #pragma unroll
@@ -541,7 +543,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
       float sum = 0.0f, acc = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = factor_of(s_max[w][row], m);
+        const float f = factor_of(plan.scale, s_max[w][row], m);
         sum += f * s_sum[w][row];
         acc += f * s_out[w][row][col];
       }
@@ -549,7 +551,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
         const int64_t at = out0 + row;
         if (col < vdim) { static_cast<T*>(a.out)[at * vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum); }
         if (col == 0 && a.lse != nullptr) {
-          a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
+          a.lse[at] = lse_of(plan.scale, m, sum, kLift<T>);
         }
       } else {
         if (col < vdim) { plan.part_out[(slot * kRows + row) * vdim + col] = acc; }
@@ -611,7 +613,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(attend_args a, attend_pla
   __syncthreads();
   float sum = 0.0f;
   for (int i = tid; i < n; i += THREADS) {
-    s_factor[i] = factor_of(s_factor[i], m);
+    s_factor[i] = factor_of(plan.scale, s_factor[i], m);
     sum += s_factor[i] * plan.part_sum[slot(i)];
   }
   sum = lanes::sum<64>(sum);
@@ -641,7 +643,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(attend_args a, attend_pla
     }
   }
   if (tid == 0 && a.lse != nullptr) {
-    a.lse[at] = sum == 0.0f ? -INFINITY : (m - kLift<T> + __builtin_log2f(sum)) / kLog2e;
+    a.lse[at] = lse_of(plan.scale, m, sum, kLift<T>);
   }
 }
 
@@ -693,7 +695,8 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.row_tiles  = row_tiles_of(a);
     plan.group      = a.heads / a.kv_heads;
     plan.tables     = a.kv_heads * plan.row_tiles;
-    plan.scale2     = float(double(a.scale) * M_LOG2E);
+    plan.scale      = scale_of(a.scale);
+    plan.slack      = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
     plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
     // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and
     // fewer streams are read faster: 64 sequences up to 8,192 168 -> 159 us, one of 131,072 91.6 -> 89.6 us.

@@ -1,8 +1,12 @@
-// Elements of the attention operators' tensors: float32, float16 and bfloat16, computed in float32.
+// Elements of the attention operators' tensors (float32, float16 and bfloat16, computed in float32), and the weights of a
+// softmax.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
 #include <cstdint>
 
 namespace certex_amd::attention {
@@ -52,11 +56,44 @@ __device__ __forceinline__ void store(T* p, pack<T, N> const& v)
   *reinterpret_cast<pack<T, N>*>(p) = v;
 }
 
-/** What sums taken relative to the maximum `part` count relative to `whole` >= part (both in powers of 2). Where nothing
- *  was counted both are -inf, and the sums are 0, or NaN of NaN scores: they pass as they are. */
-__device__ __forceinline__ float factor_of(float part, float whole)
+constexpr float kLog2e = 1.44269504088896340736f;
+
+/**
+ * The scale of a softmax's scores: weights are 2^(scale2 (score - top)). Scores are subtracted before they are scaled: what
+ * is rounded is their distance from the largest one, however far from 0 they are, and that one weighs 1. They are signed
+ * by the scale's sign, so that the largest weighs most.
+ */
+struct score_scale {
+  float sign;    // of the scale
+  float scale;   // its magnitude
+  float scale2;  // that times log2(e)
+};
+
+inline score_scale scale_of(float scale)
 {
-  return whole == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(part - whole);
+  const double s = std::abs(double(scale));
+  return {scale < 0.0f ? -1.0f : 1.0f, float(s), float(std::min(s * M_LOG2E, double(FLT_MAX)))};
+}
+
+/** The weight of a score relative to the finite score `top`; -inf counts nothing, NaN stays. */
+__device__ __forceinline__ float weight_of(score_scale const& s, float score, float top)
+{
+  const float d = score - top;
+  // a distance past the largest float: that much, so that a scale of 0 or near it has its say
+  return score == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((d < -FLT_MAX ? -FLT_MAX : d) * s.scale2);
+}
+
+/** What sums taken relative to the score `part` count relative to `whole` >= part. Where nothing was counted both are
+ *  -inf, and the sums are 0, or NaN of NaN scores: they pass as they are. */
+__device__ __forceinline__ float factor_of(score_scale const& s, float part, float whole)
+{
+  return whole == -INFINITY ? 1.0f : weight_of(s, part, whole);
+}
+
+/** The logarithm of a sum of weights relative to `top`, 2^lift times themselves. */
+__device__ __forceinline__ float lse_of(score_scale const& s, float top, float sum, float lift = 0.0f)
+{
+  return sum == 0.0f ? -INFINITY : __builtin_fmaf(top, s.scale, (__builtin_log2f(sum) - lift) / kLog2e);
 }
 
 }  // namespace certex_amd::attention

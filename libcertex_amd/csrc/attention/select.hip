@@ -17,8 +17,6 @@
 #include "elements.hpp"
 
 #include <algorithm>
-#include <cfloat>
-#include <cmath>
 
 namespace certex_amd::attention {
 namespace {
@@ -30,42 +28,8 @@ constexpr int kStep    = kIds * kWaves;   // of a workgroup's
 // Workgroups that fill the chip: fewer queries than this split their ids. Measured, 32 heads, k = 2,048, with 1, 256,
 // 1,024 and 4,096: one query a head 35, 10.8, 10.9 and 10.8 us; 8 queries 50, 50, 29 and 31; 32 queries 81 (1,024), 88 (4,096).
 constexpr int kFill    = 1024;
-constexpr float kLog2e = 1.44269504088896340736f;
 
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
-
-/** What scores are read with. */
-struct score_scale {
-  float sign;    // of the scale: scores times this are the larger the more they weigh
-  float scale;   // its magnitude
-  float scale2;  // that times log2(e)
-};
-
-score_scale scale_of(float scale)
-{
-  const double s = std::abs(double(scale));
-  return {scale < 0.0f ? -1.0f : 1.0f, float(s), float(std::min(s * M_LOG2E, double(FLT_MAX)))};
-}
-
-/** The weight of a score relative to the finite score `top`, both signed; -inf counts nothing, NaN stays. */
-__device__ __forceinline__ float weight_of(score_scale const& s, float score, float top)
-{
-  const float d = score - top;
-  // a distance past the largest float: that much, so that a scale of 0 or near it has its say
-  return score == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((d < -FLT_MAX ? -FLT_MAX : d) * s.scale2);
-}
-
-/** What sums taken relative to the score `part` count relative to `whole` >= part. Where nothing was counted both are
- *  -inf, and the sums are 0, or NaN of NaN scores: they pass as they are. */
-__device__ __forceinline__ float factor_of(score_scale const& s, float part, float whole)
-{
-  return whole == -INFINITY ? 1.0f : weight_of(s, part, whole);
-}
-
-__device__ __forceinline__ float lse_of(score_scale const& s, float top, float sum)
-{
-  return sum == 0.0f ? -INFINITY : __builtin_fmaf(top, s.scale, __builtin_log2f(sum) / kLog2e);
-}
 
 struct select_plan {
   int32_t splits;   // of a query's ids

@@ -1,11 +1,14 @@
 """How precise the attention operators are inside, where the rounding of their outputs does not hide it: values that
 cancel, scores far from 0. Bounds are in units u = 2^-24, half a unit in the last place of float32."""
 
+import math
+
 import pytest
 import torch
 
 import libcertex_amd as certex
 from tests import paged_reference as ref
+from tests.test_paged_gpu import paged
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -66,7 +69,7 @@ def test_attend_weights_are_whole(gpu, dtype):
 @pytest.mark.parametrize("base", [0, 344 - 8, 2752, 32768])
 def test_attend_scores_far_from_zero(gpu, dtype, base):
     """A score's exponent is rounded after the maximum has left it. Scores are exact and differ by up to D = 6.5 in powers
-    of 2: the subtraction's rounding and the scale's take u D ln 2 each, 9 u; 3 u are the exponential's and the weight's, 8 u
+    of 2: the scale's rounding and their product's take u D ln 2 each, 9 u; 3 u are the exponential's and the weight's, 8 u
     the sums'. (At a score of 344.85 or 2758.8, a scale of 0.75 times log2(e) is half a unit in the last place off.)"""
     b, h, d, n = 32, 4, 64, 4
     g = torch.Generator().manual_seed(5)
@@ -145,3 +148,41 @@ def test_selected_value_of_a_vanishing_weight(gpu, queries, n, k, width, value, 
     scores[0, 0, j], scores[1, 1, j] = -1e5, float("-inf")
     finite = certex.selected_attention(scores, ids, values, 1.0).isfinite()
     assert not finite[0, 0, 2] and finite.sum() == finite.numel() - 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("factor", [1.0, 100.0, 10_000.0])
+@pytest.mark.parametrize("scale", [0.125, -0.125, 1.0, 0.0])
+def test_attend_huge_scores(gpu, dtype, factor, scale):
+    """Scores up to 4e10, far past where float32 has a fraction: alike, they weigh alike; next to the largest the others
+    weigh nothing. A share and several, one wave's positions and all waves'."""
+    lens, d, heads, kv, page = [3, 200, 9000], 64, 4, 2, 16
+    kp, vp, table, _, values = paged(lens, page, kv, d, d, dtype, seed=31)
+    kp[:] = -60_000.0
+    q = torch.full((3, heads, d), factor, dtype=dtype, device="cuda")
+    q[:, 1] = -factor
+    out, lse = certex.paged_attention(q, kp, vp, table, torch.tensor(lens, device="cuda"), scale=scale, return_lse=True)
+    low = float(torch.tensor(-60_000.0, dtype=dtype))
+    for s, n in enumerate(lens):
+        v = values[s].double().cpu()
+        for h in range(heads):
+            mean, spread = v[:, h // 2].mean(0), v[:, h // 2].abs().mean(0)
+            score = scale * float(q[s, h, 0]) * low * d
+            ref.assert_attended(out[s, h][None], mean[None], spread[None], torch.zeros(1), n, 1)
+            want = score + math.log(n)
+            assert abs(float(lse[s, h]) - want) <= 80 * U * (1 + abs(want))  # of 64 products and the logarithm's scale
+    # one key less far down, or, where the sign is the other one's, all others
+    kp[int(table[2, 70]), 5] = -40_000.0
+    out = certex.paged_attention(q, kp, vp, table, torch.tensor(lens, device="cuda"), scale=scale)
+    v = values[2].double().cpu()
+    for h in range(heads):
+        sign = scale * float(q[2, h, 0])
+        if sign == 0:
+            want, spread = v[:, h // 2].mean(0), v[:, h // 2].abs().mean(0)
+        elif sign > 0:
+            want = v[70 * page + 5, h // 2]
+            spread = want.abs()
+        else:
+            rest = torch.cat([v[: 70 * page + 5, h // 2], v[70 * page + 6 :, h // 2]])
+            want, spread = rest.mean(0), rest.abs().mean(0)
+        ref.assert_attended(out[2, h][None], want[None], spread[None], torch.zeros(1), lens[2], 1)
