@@ -8,9 +8,9 @@
 // rows at once as 64 lanes hold, 16 loads in flight. The running maximum is per wave. Workgroups of few
 // queries split a query's ids, and a second launch joins the parts.
 //
-// Measured (32 query heads, 8 value heads of 131,072 rows of 128 bfloat16, k = 2,048): one query a head, 17 MB: 8.4 us
-// and 3.2 us of the join; 16 queries a head 44 us, 268 MB of gathers at 6.1 TB/s; 64 queries a head, taken by
-// ranges of rows, 115 us a pass where 1.07 GB of gathers as they come take 154: ids sorted in 25 us, rows gathered in 91
+// Measured (32 query heads, 8 value heads of 131,072 rows of 128 bfloat16, k = 2,048): one query a head, 17 MB: 8.2 us
+// and 2.4 us of the join; 16 queries a head 44 us, 268 MB of gathers at 6.1 TB/s; 64 queries a head, taken by
+// ranges of rows, 116 us a pass where 1.07 GB of gathers as they come take 154: ids sorted in 25 us, rows gathered in 91
 // (11.8 TB/s, 72% of them from the dies' caches; values that fit there are gathered at 18 TB/s), parts added in 5.
 #include "../kernels/lanes.hpp"
 #include "attention.hpp"
