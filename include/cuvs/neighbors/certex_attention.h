@@ -1,7 +1,7 @@
 /*
  * C API of the attention operators next to the key cache: rotation by position, appending keys and
- * values to a paged cache, attention of one new token over it, and attention over the top k that
- * a search of the cache returned.
+ * values to a paged cache, attention of one new token or of prompts over it, attention over the top k that
+ * a search of the cache returned, and a paged cache of 4-bit elements.
  *
  * They have no counterpart in the reference, whose attention support ends at the ids and scores of
  * the top k (certex/attention.py:84-106). As in certex.h every call returns CUVS_SUCCESS or CUVS_ERROR with
@@ -145,6 +145,61 @@ CUVS_EXPORT cuvsError_t cuvsCertexPagedAttentionWorkspace(DLManagedTensor* q,
                                                           DLManagedTensor* page_table,
                                                           int64_t window,
                                                           int64_t* bytes);
+
+/**
+ * cuvsCertexPagedAttention whose scores are bent before the softmax: y = cap tanh(scale <q, k> / cap) (cap 0: scale <q, k>),
+ * then y - slopes[h] |p - t| (slopes NULL: y) with p = length - 1 the position of the new token and t that of the key.
+ * cap: at least 0; slopes: dense float32 [heads], finite. The workspace is that of cuvsCertexPagedAttention.
+ */
+CUVS_EXPORT cuvsError_t cuvsCertexPagedAttentionShaped(cuvsResources_t res,
+                                                       DLManagedTensor* q,
+                                                       DLManagedTensor* k_pages,
+                                                       DLManagedTensor* v_pages,
+                                                       DLManagedTensor* page_table,
+                                                       DLManagedTensor* lengths,
+                                                       float scale,
+                                                       float cap,
+                                                       DLManagedTensor* slopes,
+                                                       int64_t window,
+                                                       DLManagedTensor* workspace,
+                                                       DLManagedTensor* out,
+                                                       DLManagedTensor* lse);
+
+/**
+ * Attention of the new tokens of every sequence over its pages: sequence s has the tokens [first[s], first[s + 1]) of q, which
+ * are its last ones: the i-th of n is at position p = lengths[s] - n + i, and its key is in the pages. It sees the
+ * positions t < lengths[s] with t <= p or t < prefix[s], and with p - t < window (0: any distance). Scores as for
+ * cuvsCertexPagedAttentionShaped, key and value head h / (heads / kv_heads).
+ * q: rows [tokens, heads, dim]; pages and page_table [n_sequences, n] as for cuvsCertexPagedAttention, the pages of a sequence of
+ * at most 2^31 - 64 positions; lengths: dense integers [n_sequences], cut to the table's pages; first: dense integers
+ * [n_sequences + 1] that do not decrease; prefix (or NULL): dense integers [n_sequences]; out: dense [tokens, heads, vdim];
+ * lse (or NULL): dense float32 [tokens, heads]. Tokens that see no position (before position 0: more tokens than the
+ * length), and tokens of no sequence, give zeros, and lse -inf. Missing pages, slots past a length and infinite values as for
+ * cuvsCertexPagedAttention, except that a value shows in the rows that see it and in no other. The weights of 16-bit types are rounded to the type before they meet the values.
+ * workspace: a dense uint8 vector of at least the bytes that cuvsCertexPromptAttentionWorkspace reports for the same tensors
+ * (NULL if 0), in use until the queued work is done.
+ */
+CUVS_EXPORT cuvsError_t cuvsCertexPromptAttention(cuvsResources_t res,
+                                                  DLManagedTensor* q,
+                                                  DLManagedTensor* k_pages,
+                                                  DLManagedTensor* v_pages,
+                                                  DLManagedTensor* page_table,
+                                                  DLManagedTensor* lengths,
+                                                  DLManagedTensor* first,
+                                                  DLManagedTensor* prefix,
+                                                  float scale,
+                                                  float cap,
+                                                  DLManagedTensor* slopes,
+                                                  int64_t window,
+                                                  DLManagedTensor* workspace,
+                                                  DLManagedTensor* out,
+                                                  DLManagedTensor* lse);
+CUVS_EXPORT cuvsError_t cuvsCertexPromptAttentionWorkspace(DLManagedTensor* q,
+                                                           DLManagedTensor* k_pages,
+                                                           DLManagedTensor* v_pages,
+                                                           DLManagedTensor* page_table,
+                                                           int64_t window,
+                                                           int64_t* bytes);
 
 /**
  * Attention over a selected top k: out[h, i] = sum_j w_j values[id_j] with w the softmax of

@@ -210,6 +210,9 @@ def lib():
                     "cuvsCertexAppendPages": [st, st] + [vp] * 9,
                     "cuvsCertexPagedAttentionWorkspace": [vp, vp, vp, vp, i64, P(i64)],
                     "cuvsCertexPagedAttention": [st] + [vp] * 5 + [ctypes.c_float, i64] + [vp] * 3,
+                    "cuvsCertexPagedAttentionShaped": [st] + [vp] * 5 + [ctypes.c_float] * 2 + [vp, i64] + [vp] * 3,
+                    "cuvsCertexPromptAttentionWorkspace": [vp, vp, vp, vp, i64, P(i64)],
+                    "cuvsCertexPromptAttention": [st] + [vp] * 7 + [ctypes.c_float] * 2 + [vp, i64] + [vp] * 3,
                     "cuvsCertexSelectedAttentionWorkspace": [vp, vp, vp, P(i64)],
                     "cuvsCertexSelectedAttention": [st] + [vp] * 4 + [ctypes.c_float] + [vp] * 3,
                 }

@@ -31,6 +31,9 @@ SOURCES = [
     "attention/rotate.hip",
     "attention/attend.hip",
     "attention/select.hip",
+    "attention/prompt_f32.hip",
+    "attention/prompt_f16.hip",
+    "attention/prompt_bf16.hip",
     "attention/c_api.cpp",
     "device_memory.cpp",
     "certex.cpp",

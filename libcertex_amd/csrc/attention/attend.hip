@@ -30,40 +30,12 @@
 // all heads (128 bytes of a line pair each), 6.2 with the heads first; of 256 6.2, and 5.8 in float32; of 160, and of 192
 // with values of 128, which run as 256, 4.4. More workgroups or waves per
 // compute unit read slower (three: 193 us for the 64 sequences): the memory prefers fewer streams.
-#include "../kernels/lanes.hpp"
-#include "attention.hpp"
-#include "elements.hpp"
-
-#include <algorithm>
+#include "scores.hpp"
+#include "shares.hpp"
+#include "tiles.hpp"
 
 namespace certex_amd::attention {
 namespace {
-
-constexpr int kWaves   = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kRows    = 16;   // query heads of a product
-constexpr int kUnits   = 256;  // compute units
-constexpr int kMaxShares = 2 * kUnits;
-
-using f32x4  = __attribute__((ext_vector_type(4))) float;
-using u32x4  = __attribute__((ext_vector_type(4))) uint32_t;
-using u32x2  = __attribute__((ext_vector_type(2))) uint32_t;
-using f16x8  = __attribute__((ext_vector_type(8))) _Float16;
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
-
-/** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less
- *  than 1, so n m / 2^(29 + s) exceeds n / d by less than 1 / d. */
-struct divisor {
-  uint32_t m, shift, d;
-  explicit divisor(uint32_t by) : d(by)
-  {
-    uint32_t s = 0;
-    while ((uint64_t(1) << s) < by) { ++s; }
-    shift = 29 + s;
-    m     = uint32_t(((uint64_t(1) << shift) + by - 1) / by);
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> shift); }
-};
 
 /** Positions of a lane group in a step: its rows of the 16-position products (two of 16 bits, one of float32). */
 template <typename T>
@@ -71,57 +43,6 @@ constexpr int kGroup = sizeof(T) == 4 ? 4 : 8;
 /** Positions of a workgroup's step: a tile. */
 template <typename T>
 constexpr int kTile = 4 * kGroup<T> * kWaves;
-
-struct attend_plan {
-  divisor page_groups;  // lane groups' positions per page
-  int32_t row_tiles;    // products of 16 query heads per key head
-  int32_t group;        // query heads per key head
-  int32_t tables;       // key heads x row_tiles: table t is key head t % kv_heads, product t / kv_heads
-  int32_t shares;       // of a table's tiles, at most
-  int32_t halve;        // half as many shares where each of those has this many tiles or more (0: never)
-  bool one_die;         // the tables of a share run on one die
-  score_scale scale;
-  float slack;          // kSlack in scores
-  float* part_out;      // [tables][2 shares][kRows][vdim]
-  float* part_max;      // [tables][2 shares][kRows]
-  float* part_sum;
-};
-
-/** Positions [begin, end) of a sequence, and its tiles of TILE from begin rounded down to 8. */
-struct span {
-  int32_t begin, end, tiles;
-};
-
-template <int TILE>
-__device__ __forceinline__ span span_of(attend_args const& a, int64_t b)
-{
-  int64_t end = a.lengths[b];
-  end         = end < 0 ? 0 : min(end, int64_t(a.pages.width) * a.pages.page);
-  if (a.pages.n_pages == 0) { end = 0; }
-  const int64_t begin = a.window > 0 && end > a.window ? end - a.window : 0;
-  return {int32_t(begin), int32_t(end), int32_t((end - (begin & ~int64_t(7)) + TILE - 1) / TILE)};
-}
-
-/** The shares of a table: share w takes the tiles [w tiles / n, (w + 1) tiles / n) of all sequences'. */
-struct shares {
-  int64_t tiles, n;
-  __device__ __forceinline__ int64_t first(int64_t w) const { return w * tiles / n; }
-  __device__ __forceinline__ int64_t of(int64_t tile) const { return ((tile + 1) * n - 1) / tiles; }
-};
-
-__device__ __forceinline__ shares split(attend_plan const& p, int64_t tiles)
-{
-  const int64_t half = p.shares / 2;
-  return {tiles, p.halve > 0 && half > 0 && tiles >= half * p.halve ? half : min(int64_t(p.shares), tiles)};
-}
-
-template <int TILE>
-__device__ __forceinline__ shares shares_of(attend_args const& a, attend_plan const& p)
-{
-  int64_t mine = 0;
-  for (int64_t b = threadIdx.x % 64; b < a.pages.sequences; b += 64) { mine += span_of<TILE>(a, b).tiles; }
-  return split(p, lanes::sum<64>(mine));
-}
 
 /** The elements of a lane's piece: 16 bytes of a row at any alignment of the elements (the memory takes
  *  misaligned vector loads); TINY rows are shorter than a piece and read element by element. */
@@ -164,24 +85,6 @@ struct geometry {
   using value = std::conditional_t<kCols * sizeof(T) == 16, u32x4, u32x2>;
 };
 
-__device__ __forceinline__ f32x4 mfma(f16_t, u32x4 a, u32x4 b, f32x4 c)
-{
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mfma(bf16_t, u32x4 a, u32x4 b, f32x4 c)
-{
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-  const T v[2] = {T(lo), T(hi)};
-  uint32_t w;
-  __builtin_memcpy(&w, v, 4);
-  return w;
-}
-
 /** The weights' reference may lag the largest exponent by this much (twice as much where large scores round it) before the
  *  sums are rescaled, and weights are multiplied by 2^kLift: float16 weights reach 2^15 and keep their precision down to
  *  2^-27 of the largest. */
@@ -209,7 +112,7 @@ __device__ __forceinline__ uint32_t counted(int skip, int w)
   return skip > 2 * w + 1 ? 0u : skip > 2 * w ? 0xffff0000u : 0xffffffffu;
 }
 
-template <typename T, int D, fit FIT>
+template <typename T, int D, fit FIT, bool BENT>
 __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(attend_args a, attend_plan plan)
 {
   constexpr bool TINY    = FIT == fit::tiny;
@@ -261,6 +164,9 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
   const int dim = FULL ? D : a.dim, vdim = FULL ? D : a.vdim;
   const int kv = table % a.kv_heads, row0 = table / a.kv_heads * kRows;
   const int rows = min(kRows, plan.group - row0), h0 = kv * plan.group + row0;
+  // bent scores take the scale with its sign before the softmax, which then has a scale of 1
+  const float slope   = BENT && a.shape.slopes != nullptr ? a.shape.slopes[h0 + min(r, rows - 1)] : 0.0f;
+  const float per_cap = BENT && a.shape.cap != 0.0f ? a.scale / a.shape.cap : 0.0f;
   const uint32_t flip = plan.scale.sign < 0.0f ? (sizeof(T) == 4 ? 0x80000000u : 0x80008000u) : 0u;  // of a word of q
   const T* k_head = static_cast<const T*>(a.k) + kv * a.k_head;
   const T* v_head = static_cast<const T*>(a.v) + kv * a.v_head;
@@ -413,6 +319,12 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
 #pragma unroll
       for (int j = 0; j < kGrp; ++j) { x[j] = s[j / 4][j % 4]; }
       const uint32_t t = uint32_t(group + g) * kGrp;  // past the end it may pass 2^31
+      if constexpr (BENT) {
+#pragma unroll
+        for (int j = 0; j < kGrp; ++j) {
+          x[j] = bent(x[j], a.scale, per_cap, a.shape.cap, slope, float(uint32_t(sp.end) - 1u - (t + j)));
+        }
+      }
       const uint32_t t_begin = uint32_t(sp.begin), t_end = uint32_t(sp.end);
       const bool whole  = have && t >= t_begin && t + kGrp <= t_end;
       const bool masked = !__all(whole);
@@ -565,97 +477,6 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void attend_kernel(atte
   }
 }
 
-/**
- * One workgroup per sequence and query head: joins the partials of a sequence that shares cut. Their
- * factors first, in LDS; then a thread per column and part of the partials.
- */
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void join_kernel(attend_args a, attend_plan plan)
-{
-  constexpr int kTiles = kTile<T>;
-  __shared__ float s_factor[kMaxShares];
-  __shared__ float s_out[THREADS];
-  __shared__ float s_part[THREADS / 64];
-  const int h = blockIdx.x, tid = threadIdx.x;
-  const int64_t b = blockIdx.y;
-  const int kv = h / plan.group, in_group = h - kv * plan.group;
-  const int table = in_group / kRows * a.kv_heads + kv, row = in_group % kRows;
-  const int tiles = span_of<kTiles>(a, b).tiles;
-  int64_t before = 0, all = 0;
-  for (int64_t i = tid % 64; i < a.pages.sequences; i += 64) {
-    const int n = span_of<kTiles>(a, i).tiles;
-    before += i < b ? n : 0;
-    all += n;
-  }
-  before = lanes::sum<64>(before);
-  all    = lanes::sum<64>(all);
-  if (tiles == 0) { return; }
-  const shares sh = split(plan, all);
-  const int64_t w0 = sh.of(before), w1 = sh.of(before + tiles - 1);
-  if (w0 == w1) { return; }
-  const int n = int(w1 - w0) + 1;
-  // the later shares begin inside the sequence: their first slot
-  const int64_t slot0 = 2 * w0 + (sh.first(w0) == before ? 0 : 1);
-  const auto slot     = [&](int i) {
-    return (int64_t(table) * plan.shares * 2 + (i == 0 ? slot0 : 2 * (w0 + i))) * kRows + row;
-  };
-
-  float m = -INFINITY;
-  for (int i = tid; i < n; i += THREADS) {
-    s_factor[i] = plan.part_max[slot(i)];
-    m           = fmaxf(m, s_factor[i]);
-  }
-  m = lanes::max<64>(m);
-  if (tid % 64 == 0) { s_part[tid / 64] = m; }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) { m = fmaxf(m, s_part[w]); }
-  __syncthreads();
-  float sum = 0.0f;
-  for (int i = tid; i < n; i += THREADS) {
-    s_factor[i] = factor_of(plan.scale, s_factor[i], m);
-    sum += s_factor[i] * plan.part_sum[slot(i)];
-  }
-  sum = lanes::sum<64>(sum);
-  if (tid % 64 == 0) { s_part[tid / 64] = sum; }
-  __syncthreads();
-  sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) { sum += s_part[w]; }
-
-  const int64_t at = b * a.heads + h;
-  const int cols = min(THREADS, a.vdim <= 64 ? 64 : a.vdim <= 128 ? 128 : 256);
-  const int part = tid / cols, parts = THREADS / cols;
-  for (int col0 = 0; col0 < a.vdim; col0 += cols) {  // more than once only with one part
-    const int col = col0 + tid % cols;
-    float acc     = 0.0f;
-    if (col < a.vdim) {
-#pragma unroll 8
-      for (int i = part; i < n; i += parts) { acc = __builtin_fmaf(s_factor[i], plan.part_out[slot(i) * a.vdim + col], acc); }
-    }
-    if (parts > 1) {
-      s_out[tid] = acc;
-      __syncthreads();
-    }
-    if (part == 0 && col < a.vdim) {
-      for (int i = 1; i < parts; ++i) { acc += s_out[i * cols + tid]; }
-      static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
-    }
-  }
-  if (tid == 0 && a.lse != nullptr) {
-    a.lse[at] = lse_of(plan.scale, m, sum, kLift<T>);
-  }
-}
-
-int row_tiles_of(attend_args const& a) { return (a.heads / a.kv_heads + kRows - 1) / kRows; }
-
-/** Most positions of a sequence, from begin rounded down to 8. */
-int64_t longest_of(attend_args const& a)
-{
-  const int64_t most = int64_t(a.pages.width) * a.pages.page;
-  return a.window > 0 && a.window < most ? std::min(most, a.window + 7) : most;
-}
-
 /** Whether tables read the same cache lines, so that one die's cache should serve them: several products of
  *  query heads of a key head, or rows of heads that begin within a line. Measured, over all dies and on one: 32
  *  query heads of one key head 147 and 114 us, heads of 80 145 and 131 us; of 128 168 and 174 us. */
@@ -695,7 +516,8 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.row_tiles  = row_tiles_of(a);
     plan.group      = a.heads / a.kv_heads;
     plan.tables     = a.kv_heads * plan.row_tiles;
-    plan.scale      = scale_of(a.scale);
+    plan.scale      = scale_of(a.shape.any() ? 1.0f : a.scale);
+    plan.lift       = kLift<T>;
     plan.slack      = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
     plan.shares     = shares_for(a, kTile<T>, kPerUnit<T, D>);
     // Long shares of 16-bit heads of 128 keep the memory busy with one workgroup per compute unit, and
@@ -709,14 +531,18 @@ void attend(elem type, attend_args const& a, hipStream_t stream)
     plan.part_sum   = plan.part_max + slots;
     plan.one_die        = shares_lines(a, sizeof(T)) && plan.shares >= 8;
     const int blocks    = (plan.one_die ? (plan.shares + 7) / 8 * 8 : plan.shares) * plan.tables;
-    attend_kernel<T, D, decltype(how)::value><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a, plan);
+    if (a.shape.any()) {
+      attend_kernel<T, D, decltype(how)::value, true><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a, plan);
+    } else {
+      attend_kernel<T, D, decltype(how)::value, false><<<dim3(uint32_t(blocks)), kThreads, 0, stream>>>(a, plan);
+    }
     if (longest_of(a) > kTile<T>) {
       const dim3 grid(uint32_t(a.heads), uint32_t(a.pages.sequences));
       // a few partials per sequence, or many (64 sequences: 13 us with 512 threads, 6 with 128)
       if (plan.shares <= 8 * a.pages.sequences) {
-        join_kernel<T, 128><<<grid, 128, 0, stream>>>(a, plan);
+        join_kernel<T, 128, kTile<T>><<<grid, 128, 0, stream>>>(a, plan);
       } else {
-        join_kernel<T, 512><<<grid, 512, 0, stream>>>(a, plan);
+        join_kernel<T, 512, kTile<T>><<<grid, 512, 0, stream>>>(a, plan);
       }
     }
   };

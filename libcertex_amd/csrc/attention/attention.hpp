@@ -4,6 +4,8 @@
 // none allocates or synchronises.
 #pragma once
 
+#include "scores.hpp"
+
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -79,11 +81,50 @@ struct attend_args {
   int_vector lengths;
   int32_t heads = 0, kv_heads = 0, dim = 0, vdim = 0;
   float scale    = 0;
+  score_shape shape;
   int64_t window = 0;  // the last `window` positions only; 0: all
   void* out      = nullptr;  // [sequences, heads, vdim] dense
   float* lse     = nullptr;  // [sequences, heads] dense, or NULL
   void* workspace = nullptr;
 };
+
+struct prompt_args {
+  const void* q = nullptr;  // [tokens, heads, dim]
+  int64_t q_token = 0, q_head = 0;
+  const void* k = nullptr;
+  int64_t k_page = 0, k_slot = 0, k_head = 0;
+  const void* v = nullptr;
+  int64_t v_page = 0, v_slot = 0, v_head = 0;
+  page_map pages;
+  int_vector lengths;
+  int_vector first;   // [sequences + 1]: sequence s has the tokens [first[s], first[s + 1]), its last ones
+  int_vector prefix;  // [sequences], or none: positions that every token sees
+  int64_t tokens = 0;
+  int32_t heads = 0, kv_heads = 0, dim = 0, vdim = 0;
+  float scale = 0;
+  score_shape shape;
+  int64_t window = 0;
+  void* out      = nullptr;  // [tokens, heads, vdim] dense
+  float* lse     = nullptr;  // [tokens, heads] dense, or NULL
+  void* workspace = nullptr;
+};
+
+// a source for each element type
+size_t prompt_workspace_f32(prompt_args const& args);
+size_t prompt_workspace_f16(prompt_args const& args);
+size_t prompt_workspace_bf16(prompt_args const& args);
+void prompt_f32(prompt_args const& args, hipStream_t stream);
+void prompt_f16(prompt_args const& args, hipStream_t stream);
+void prompt_bf16(prompt_args const& args, hipStream_t stream);
+
+inline size_t prompt_workspace(elem type, prompt_args const& args)
+{
+  return type == elem::f32 ? prompt_workspace_f32(args) : type == elem::f16 ? prompt_workspace_f16(args) : prompt_workspace_bf16(args);
+}
+inline void prompt(elem type, prompt_args const& args, hipStream_t stream)
+{
+  type == elem::f32 ? prompt_f32(args, stream) : type == elem::f16 ? prompt_f16(args, stream) : prompt_bf16(args, stream);
+}
 
 /** Largest head dimension of keys and of values. */
 constexpr int kMaxHeadDim = 256;

@@ -409,10 +409,35 @@ auto with_lse(Tensor const& out, maybe const& lse) -> PyObject*
   return t;
 }
 
-/** (q, k_pages, v_pages, page_table, lengths, scale or None, window or None, return_lse) */
+/** What shapes the scores of an attention: the scale (or None for dim ** -0.5), the window, the cap and the slopes (or None). */
+struct score_options {
+  double scale   = 0;
+  int64_t window = 0;
+  double cap     = 0;
+  maybe slopes;
+  score_options(PyObject* scale_, PyObject* window_, PyObject* cap_, PyObject* slopes_, int64_t dim)
+  {
+    scale  = scale_ != Py_None ? PyFloat_AsDouble(scale_) : 1.0 / std::sqrt(double(dim));
+    window = window_ != Py_None ? PyLong_AsLongLong(window_) : 0;
+    cap    = cap_ != Py_None ? PyFloat_AsDouble(cap_) : 0.0;
+    if (PyErr_Occurred()) { throw python_error{}; }
+    EXPECTS(window_ == Py_None || window >= 1, "the window must be at least 1, not " + std::to_string(window));
+    EXPECTS(cap_ == Py_None || (std::isfinite(cap) && float(cap) > 0.0f && std::isfinite(float(cap))),
+            "the cap must be positive and finite, not " + std::to_string(cap));
+    if (slopes_ != Py_None) {
+      Tensor const& s = tensor(slopes_, "slopes");
+      EXPECTS(s.is_cuda() && s.layout() == at::kStrided && s.scalar_type() == at::kFloat,
+              "slopes must be a float32 GPU tensor");
+      no_gradient({&s});
+      slopes = s.is_contiguous() ? s : s.contiguous();
+    }
+  }
+};
+
+/** (q, k_pages, v_pages, page_table, lengths, scale or None, window or None, return_lse, cap or None, slopes or None) */
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-  if (!counted(n, 8)) { return nullptr; }
+  if (!counted(n, 10)) { return nullptr; }
   return guarded([&] {
     const Tensor q        = read(tensor(a[0], "q"), "q", 3);
     Tensor const& k_pages = rows(tensor(a[1], "k_pages"), "k_pages", 4, &q);
@@ -420,10 +445,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
     no_gradient({&q, &k_pages, &v_pages});
     const Tensor table   = ints(tensor(a[3], "page_table"), "page_table", true);
     const Tensor lengths = ints(tensor(a[4], "lengths"), "lengths");
-    const double scale   = a[5] != Py_None ? PyFloat_AsDouble(a[5]) : 1.0 / std::sqrt(double(q.size(2)));
-    const int64_t window = a[6] != Py_None ? PyLong_AsLongLong(a[6]) : 0;
-    if (PyErr_Occurred()) { throw python_error{}; }
-    EXPECTS(a[6] == Py_None || window >= 1, "the window must be at least 1, not " + std::to_string(window));
+    const score_options how(a[5], a[6], a[8], a[9], q.size(2));
     const bool want = PyObject_IsTrue(a[7]) == 1;
     Tensor out;
     maybe lse;
@@ -431,12 +453,47 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n)
       unlocked u;
       out = at::empty({q.size(0), q.size(1), v_pages.size(3)}, q.options());
       if (want) { lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)); }
-      view qv(q), kv(k_pages), vv(v_pages), tv(table), lv(lengths), ov(out), ev(lse);
+      view qv(q), kv(k_pages), vv(v_pages), tv(table), lv(lengths), ov(out), ev(lse), sv(how.slopes);
       int64_t bytes = 0;
-      check(cuvsCertexPagedAttentionWorkspace(&qv, &kv, &vv, &tv, window, &bytes));
+      check(cuvsCertexPagedAttentionWorkspace(&qv, &kv, &vv, &tv, how.window, &bytes));
       const maybe work = workspace(bytes, q);
       view wv(work);
-      check(cuvsCertexPagedAttention(resources(), &qv, &kv, &vv, &tv, &lv, float(scale), window, &wv, &ov, &ev));
+      check(cuvsCertexPagedAttentionShaped(resources(), &qv, &kv, &vv, &tv, &lv, float(how.scale), float(how.cap), &sv,
+                                           how.window, &wv, &ov, &ev));
+    }
+    return with_lse(out, lse);
+  });
+}
+
+/** (q, k_pages, v_pages, page_table, lengths, first, scale or None, window or None, prefix or None, cap or None, slopes or None,
+ *  return_lse) */
+PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+  if (!counted(n, 12)) { return nullptr; }
+  return guarded([&] {
+    const Tensor q        = read(tensor(a[0], "q"), "q", 3);
+    Tensor const& k_pages = rows(tensor(a[1], "k_pages"), "k_pages", 4, &q);
+    Tensor const& v_pages = rows(tensor(a[2], "v_pages"), "v_pages", 4, &q);
+    no_gradient({&q, &k_pages, &v_pages});
+    const Tensor table   = ints(tensor(a[3], "page_table"), "page_table", true);
+    const Tensor lengths = ints(tensor(a[4], "lengths"), "lengths"), first = ints(tensor(a[5], "first"), "first");
+    const score_options how(a[6], a[7], a[9], a[10], q.size(2));
+    maybe prefix = maybe_tensor(a[8], "prefix");
+    if (prefix) { prefix = ints(*prefix, "prefix"); }
+    const bool want = PyObject_IsTrue(a[11]) == 1;
+    Tensor out;
+    maybe lse;
+    {
+      unlocked u;
+      out = at::empty({q.size(0), q.size(1), v_pages.size(3)}, q.options());
+      if (want) { lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)); }
+      view qv(q), kv(k_pages), vv(v_pages), tv(table), lv(lengths), fv(first), pv(prefix), ov(out), ev(lse), sv(how.slopes);
+      int64_t bytes = 0;
+      check(cuvsCertexPromptAttentionWorkspace(&qv, &kv, &vv, &tv, how.window, &bytes));
+      const maybe work = workspace(bytes, q);
+      view wv(work);
+      check(cuvsCertexPromptAttention(resources(), &qv, &kv, &vv, &tv, &lv, &fv, &pv, float(how.scale), float(how.cap), &sv,
+                                      how.window, &wv, &ov, &ev));
     }
     return with_lse(out, lse);
   });
@@ -510,7 +567,9 @@ PyMethodDef methods[] = {{"init", fast(init), METH_FASTCALL, "(CertexError, torc
                          {"append", fast(append), METH_FASTCALL,
                           "(capsule, head_dim, k, v, k_pages, v_pages, page_table, positions, sequences, q)"},
                          {"attend", fast(attend), METH_FASTCALL,
-                          "(q, k_pages, v_pages, page_table, lengths, scale, window, return_lse)"},
+                          "(q, k_pages, v_pages, page_table, lengths, scale, window, return_lse, cap, slopes)"},
+                         {"prompt", fast(prompt), METH_FASTCALL,
+                          "(q, k_pages, v_pages, page_table, lengths, first, scale, window, prefix, cap, slopes, return_lse)"},
                          {"select", fast(select), METH_FASTCALL, "(scores, ids, values, scale, page_table, return_lse)"},
                          {"undifferentiated", undifferentiated, METH_O, "(tensor): refuses one that is differentiated"},
                          {nullptr, nullptr, 0, nullptr}};

@@ -271,10 +271,11 @@ auto frequencies_of(cuvsCertexRotaryParams const& p, double* magnitude) -> std::
   return f;
 }
 
-/** Queries, pages and table of an attention call, checked against each other. */
-auto attend_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v_, DLManagedTensor* table_,
-                    int64_t window, ops::elem* type, tensor* q, tensor* k, tensor* v, tensor* table)
-  -> ops::attend_args
+/** Queries, pages and table of an attention call, checked against each other. With `prompts` the queries are tokens of
+ *  any of the table's sequences, else one of each. */
+template <typename Args>
+auto paged_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v_, DLManagedTensor* table_,
+                   int64_t window, bool prompts, ops::elem* type, tensor* q, tensor* k, tensor* v, tensor* table) -> Args
 {
   *q     = rows(tensor_of(q_, "q"), type, true);
   *k     = rows(tensor_of(k_, "k_pages"), type, false);
@@ -283,26 +284,25 @@ auto attend_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v
   expects_ndim(*q, 3);
   expects_ndim(*k, 4);
   expects_ndim(*v, 4);
-  ops::attend_args a;
+  Args a;
   a.heads    = int32_t(q->shape[1]);
   a.kv_heads = int32_t(k->shape[2]);
   a.dim      = int32_t(q->shape[2]);
   a.vdim     = int32_t(v->shape[3]);
   EXPECTS(q->shape[1] >= 1 && q->shape[1] <= 65535 && k->shape[2] >= 1 && q->shape[1] % k->shape[2] == 0,
           "the query heads must be a multiple of the key heads (and at most 65535)");
-  EXPECTS(q->shape[0] <= 65535, "at most 65535 sequences");
   EXPECTS(a.dim >= 1 && k->shape[3] == a.dim, "q and k_pages must have the same head dimension");
   EXPECTS(q->shape[2] <= ops::kMaxHeadDim && v->shape[3] >= 1 && v->shape[3] <= ops::kMaxHeadDim,
           "head dimensions must be between 1 and " + std::to_string(ops::kMaxHeadDim));
   expects_shape(*v, {k->shape[0], k->shape[1], k->shape[2], v->shape[3]});
   expects_ndim(*table, 2);
-  EXPECTS(table->shape[0] == q->shape[0], "page_table must have one row per sequence");
+  EXPECTS(prompts || table->shape[0] == q->shape[0], "page_table must have one row per sequence");
+  EXPECTS(table->shape[0] <= 65535, "at most 65535 sequences");
   EXPECTS(k->shape[1] % ops::kPageUnit == 0 && k->shape[1] >= ops::kPageUnit,
           "the page size must be a multiple of " + std::to_string(ops::kPageUnit));
   EXPECTS(window >= 0, "the window must not be negative");
-  a.pages  = page_map_of(*table, q->shape[0], *k);
+  a.pages  = page_map_of(*table, table->shape[0], *k);
   a.q      = q->p;
-  a.q_seq  = q->stride[0];
   a.q_head = q->stride[1];
   a.k      = k->p;
   a.k_page = k->stride[0];
@@ -314,6 +314,47 @@ auto attend_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v
   a.v_head = v->stride[2];
   a.window = window;
   return a;
+}
+
+auto attend_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v_, DLManagedTensor* table_,
+                    int64_t window, ops::elem* type, tensor* q, tensor* k, tensor* v, tensor* table)
+  -> ops::attend_args
+{
+  auto a  = paged_args_of<ops::attend_args>(q_, k_, v_, table_, window, false, type, q, k, v, table);
+  a.q_seq = q->stride[0];
+  return a;
+}
+
+auto prompt_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v_, DLManagedTensor* table_,
+                    int64_t window, ops::elem* type, tensor* q, tensor* k, tensor* v, tensor* table)
+  -> ops::prompt_args
+{
+  auto a    = paged_args_of<ops::prompt_args>(q_, k_, v_, table_, window, true, type, q, k, v, table);
+  a.q_token = q->stride[0];
+  a.tokens  = q->shape[0];
+  const int64_t group = a.heads / a.kv_heads;
+  // rows of a key head, and blocks of 256 threads that a launch may have
+  EXPECTS(a.tokens < (int64_t(1) << 29) && a.tokens * group < (int64_t(1) << 29) &&
+            (a.tokens * group / 128 + table->shape[0]) * a.kv_heads < (int64_t(1) << 23),
+          "too many tokens in one call");
+  EXPECTS(int64_t(a.pages.width) * a.pages.page <= (int64_t(1) << 31) - 64, "a sequence's pages hold at most 2^31 - 64 positions");
+  return a;
+}
+
+/** The bent scores' parameters: a cap of 0 and no slopes leave the scores as they are. */
+auto shape_of(cuvs::resources const& r, float cap, DLManagedTensor* slopes, int64_t heads) -> ops::score_shape
+{
+  EXPECTS(std::isfinite(cap) && cap >= 0.0f, "the cap must be finite and not negative");
+  ops::score_shape s;
+  s.cap = cap;
+  if (slopes != nullptr) {
+    const tensor t = dense(tensor_of(slopes, "slopes"));
+    EXPECTS(t.is(kDLFloat, 32), "slopes must be float32");
+    expects_shape(t, {heads});
+    expects_device(r, t);
+    s.slopes = static_cast<const float*>(t.p);
+  }
+  return s;
 }
 
 auto select_args_of(DLManagedTensor* scores_, DLManagedTensor* values_, DLManagedTensor* table_, ops::elem* type,
@@ -587,17 +628,19 @@ cuvsError_t cuvsCertexPagedAttentionWorkspace(DLManagedTensor* q_,
   });
 }
 
-cuvsError_t cuvsCertexPagedAttention(cuvsResources_t res,
-                                     DLManagedTensor* q_,
-                                     DLManagedTensor* k_pages_,
-                                     DLManagedTensor* v_pages_,
-                                     DLManagedTensor* page_table_,
-                                     DLManagedTensor* lengths_,
-                                     float scale,
-                                     int64_t window,
-                                     DLManagedTensor* workspace_,
-                                     DLManagedTensor* out_,
-                                     DLManagedTensor* lse_)
+cuvsError_t cuvsCertexPagedAttentionShaped(cuvsResources_t res,
+                                           DLManagedTensor* q_,
+                                           DLManagedTensor* k_pages_,
+                                           DLManagedTensor* v_pages_,
+                                           DLManagedTensor* page_table_,
+                                           DLManagedTensor* lengths_,
+                                           float scale,
+                                           float cap,
+                                           DLManagedTensor* slopes_,
+                                           int64_t window,
+                                           DLManagedTensor* workspace_,
+                                           DLManagedTensor* out_,
+                                           DLManagedTensor* lse_)
 {
   return translate([=] {
     auto& r = res_of(res);
@@ -610,13 +653,95 @@ cuvsError_t cuvsCertexPagedAttention(cuvsResources_t res,
     expects_shape(out, {q.shape[0], q.shape[1], v.shape[3]});
     expects_device(r, q, k, v, table, lengths, out);
     EXPECTS(std::isfinite(scale), "the scale must be finite");
+    const auto shape = shape_of(r, cap, slopes_, q.shape[1]);
     a.lse = lse_of(r, lse_, q.shape[0], q.shape[1]);
     if (q.shape[0] == 0) { return; }
     a.lengths   = int_vector_of(lengths);
     a.scale     = scale;
+    a.shape     = shape;
     a.out       = out.p;
     a.workspace = workspace_of(r, workspace_, ops::attend_workspace(type, a));
     ops::attend(type, a, stream_of(r));
+    check_launch();
+  });
+}
+
+cuvsError_t cuvsCertexPagedAttention(cuvsResources_t res,
+                                     DLManagedTensor* q_,
+                                     DLManagedTensor* k_pages_,
+                                     DLManagedTensor* v_pages_,
+                                     DLManagedTensor* page_table_,
+                                     DLManagedTensor* lengths_,
+                                     float scale,
+                                     int64_t window,
+                                     DLManagedTensor* workspace_,
+                                     DLManagedTensor* out_,
+                                     DLManagedTensor* lse_)
+{
+  return cuvsCertexPagedAttentionShaped(res, q_, k_pages_, v_pages_, page_table_, lengths_, scale, 0.0f, nullptr, window,
+                                        workspace_, out_, lse_);
+}
+
+cuvsError_t cuvsCertexPromptAttentionWorkspace(DLManagedTensor* q_,
+                                               DLManagedTensor* k_pages_,
+                                               DLManagedTensor* v_pages_,
+                                               DLManagedTensor* page_table_,
+                                               int64_t window,
+                                               int64_t* bytes)
+{
+  return translate([=] {
+    EXPECTS(bytes != nullptr, "NULL argument");
+    ops::elem type{};
+    tensor q, k, v, table;
+    const auto a = prompt_args_of(q_, k_pages_, v_pages_, page_table_, window, &type, &q, &k, &v, &table);
+    *bytes       = int64_t(ops::prompt_workspace(type, a));
+  });
+}
+
+cuvsError_t cuvsCertexPromptAttention(cuvsResources_t res,
+                                      DLManagedTensor* q_,
+                                      DLManagedTensor* k_pages_,
+                                      DLManagedTensor* v_pages_,
+                                      DLManagedTensor* page_table_,
+                                      DLManagedTensor* lengths_,
+                                      DLManagedTensor* first_,
+                                      DLManagedTensor* prefix_,
+                                      float scale,
+                                      float cap,
+                                      DLManagedTensor* slopes_,
+                                      int64_t window,
+                                      DLManagedTensor* workspace_,
+                                      DLManagedTensor* out_,
+                                      DLManagedTensor* lse_)
+{
+  return translate([=] {
+    auto& r = res_of(res);
+    ops::elem type{};
+    tensor q, k, v, table;
+    auto a = prompt_args_of(q_, k_pages_, v_pages_, page_table_, window, &type, &q, &k, &v, &table);
+    const int64_t sequences = table.shape[0];
+    const tensor lengths = integers(lengths_, "lengths"), first = integers(first_, "first");
+    expects_shape(lengths, {sequences});
+    expects_shape(first, {sequences + 1});
+    const tensor out = dense(rows(tensor_of(out_, "out"), &type, false));
+    expects_shape(out, {q.shape[0], q.shape[1], v.shape[3]});
+    expects_device(r, q, k, v, table, lengths, first, out);
+    EXPECTS(std::isfinite(scale), "the scale must be finite");
+    if (prefix_ != nullptr) {
+      const tensor prefix = integers(prefix_, "prefix");
+      expects_shape(prefix, {sequences});
+      expects_device(r, prefix);
+      a.prefix = int_vector_of(prefix);
+    }
+    a.shape = shape_of(r, cap, slopes_, q.shape[1]);
+    a.lse   = lse_of(r, lse_, q.shape[0], q.shape[1]);
+    if (q.shape[0] == 0) { return; }
+    a.lengths   = int_vector_of(lengths);
+    a.first     = int_vector_of(first);
+    a.scale     = scale;
+    a.out       = out.p;
+    a.workspace = workspace_of(r, workspace_, ops::prompt_workspace(type, a));
+    ops::prompt(type, a, stream_of(r));
     check_launch();
   });
 }

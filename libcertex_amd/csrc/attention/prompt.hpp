@@ -1,0 +1,629 @@
+// Attention of the new tokens of every sequence over its pages of keys and values: prompts, and pieces of prompts.
+//
+// Row (i, h) of a sequence with n new tokens and `length` positions in the cache is its query at position
+// p = length - n + i of query head h. It sees the positions t < length with t <= p or t < prefix, and p - t < window:
+// out = sum_t w_t v_t / sum_t w_t, w_t = 2^(log2(e) (y_t - m)), y_t the score scale q.k_t or its bent form. One pass over
+// the positions keeps a reference m per row, the sum and the output in float32.
+//
+// What bounds it: two products of 2 dim operations per row and position it sees, and about five vector
+// operations per score, of which the exponential takes a quarter of the vector rate. The rows of a key head are taken
+// together: the tokens' query heads that share it, 128 rows a workgroup, 32 a wave. So K and V pass from memory to
+// LDS once per 128 rows, and each wave reads them from there.
+// - S^T = K Q^T in products of 32 positions x 32 rows: a row is a lane's column, so that the reference, the sum and the
+//   scaling are per lane; the products begin at -m, so that they end as distances from the reference.
+// - The rows of S^T that a lane holds are the positions that it feeds to O^T = V^T P^T: the weights never move.
+//   V is turned on its way into LDS, in the order of positions of these rows.
+// - Weights are rounded to the element type for the second product (bfloat16 2^-9, float16 2^-12 at most, relative); their
+//   sum is not. The output is rounded as much again, and weights with twice the bits would cost half as many products more.
+// - Tiles of positions are in two buffers: the next one's loads are in flight during the products.
+//
+// Work is dealt without reading the lengths back: the host launches as many tiles of rows as there may be, the
+// kernel finds the sequence of each. The last rows of a prompt see most and go first. Where tiles are too few to
+// fill the chip their positions are split over workgroups, which leave partials (m, sum, output) for join_kernel.
+#pragma once
+
+#include "../kernels/lanes.hpp"
+#include "attention.hpp"
+#include "elements.hpp"
+#include "tiles.hpp"
+
+#include <algorithm>
+#include <climits>
+
+namespace certex_amd::attention {
+namespace {
+
+constexpr int kWaves   = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kRows    = 32 * kWaves;  // of a tile
+constexpr int kUnits   = 256;          // compute units
+constexpr int kMaxSplits = 64;
+/** Fewest tiles of positions of a split. */
+constexpr int kLeast = 4;
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+
+struct prompt_plan {
+  divisor page_groups;  // groups of 8 positions per page
+  divisor group;        // query heads per key head
+  int32_t tiles;        // of rows, at most, over all sequences
+  int32_t splits;       // of a tile's positions, at most
+  score_scale scale;
+  float slack;          // kSlack in scores
+  float* part_out;      // [tiles][kv_heads][splits][kRows][vdim]
+  float* part_max;      // [tiles][kv_heads][splits][kRows]
+  float* part_sum;
+};
+
+/** A tile of rows: its sequence, the first of its rows there, and what those see. */
+struct row_tile {
+  int32_t sequence;
+  int32_t row0, rows;   // rows of the sequence (token major): the tile's first, and all
+  int64_t token0;       // of the sequence
+  int32_t past;         // position of the sequence's first token
+  int32_t length;
+  int32_t prefix;
+  int32_t begin, tiles; // positions from begin on, in tiles of TILE
+};
+
+__device__ __forceinline__ int64_t clamped(int64_t x, int64_t hi) { return x < 0 ? 0 : x > hi ? hi : x; }
+
+/**
+ * Tile `index`: sequence s has the indexes from floor(first[s] group / kRows) + s on, of which the first
+ * ceil(rows / kRows) are its tiles; the next sequence's begin behind them. False where there is none.
+ */
+template <int TILE>
+__device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan const& plan, int64_t index, row_tile* out)
+{
+  if (a.pages.sequences == 0) { return false; }  // first has one entry, the lengths none
+  const int lane        = threadIdx.x % 64;
+  const int64_t group   = plan.group.d;
+  const auto token      = [&](int64_t s) { return clamped(a.first[s], a.tokens); };
+  // the last sequence that begins at or before the index, 64 at a time
+  int64_t lo = 0, n = a.pages.sequences;
+  while (n > 0) {
+    const int64_t step = (n + 63) / 64, s = lo + lane * step;
+    const bool before  = s < lo + n && token(s) * group / kRows + s <= index;
+    const int count    = __builtin_popcountll(__ballot(before));
+    if (count == 0) { return false; }
+    lo += (count - 1) * step;
+    n = step == 1 ? 0 : min(step, a.pages.sequences - lo);
+  }
+  const int64_t t0 = token(lo), t1 = token(lo + 1);
+  const int64_t at = index - (t0 * group / kRows + lo);
+  const int64_t rows = (t1 - t0) * group;
+  if (at < 0 || at * kRows >= rows) { return false; }  // at < 0: first does not rise
+  const int64_t most = int64_t(a.pages.width) * a.pages.page;
+  int64_t length     = a.pages.n_pages > 0 ? clamped(a.lengths[lo], most) : 0;
+  const int64_t past = length - (t1 - t0);
+  const int64_t prefix = a.prefix.p != nullptr ? clamped(a.prefix[lo], length) : 0;
+  // the positions that any row sees
+  const int row0   = int(at * kRows);
+  const int64_t i0 = plan.group(uint32_t(row0)), i1 = plan.group(uint32_t(min(rows, int64_t(row0) + kRows) - 1));
+  const int64_t end   = max(min(past + i1 + 1, length), prefix);
+  const int64_t begin = a.window > 0 ? max(int64_t(0), past + i0 + 1 - a.window) & ~int64_t(7) : 0;
+  *out = {int32_t(lo),     row0,           int32_t(rows), t0, int32_t(past), int32_t(length), int32_t(prefix),
+          int32_t(begin), int32_t(end > begin ? (end - begin + TILE - 1) / TILE : 0)};
+  return true;
+}
+
+/** The splits of a tile. */
+__device__ __forceinline__ int splits_of(prompt_plan const& plan, int tiles)
+{
+  return max(1, min(plan.splits, tiles / kLeast));
+}
+
+__device__ __forceinline__ f32x16 mfma32(f16_t, u32x4 a, u32x4 b, f32x16 c)
+{
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(bf16_t, u32x4 a, u32x4 b, f32x16 c)
+{
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(float, u32x4 a, u32x4 b, f32x16 c)
+{
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, uint32_t(a[i])),
+                                             __builtin_bit_cast(float, uint32_t(b[i])), c, 0, 0, 0);
+  }
+  return c;
+}
+
+/** N elements as words. */
+template <typename T, int N>
+struct words {
+  uint32_t w[N * sizeof(T) / 4];
+};
+
+/** Elements [off, off + N) of a row of n; what is past its end is 0. */
+template <bool FULL, int N, typename T>
+__device__ __forceinline__ words<T, N> row_piece(const T* row, int off, int n)
+{
+  words<T, N> v{};
+  if (FULL || off + N <= n) {
+    __builtin_memcpy(&v, __builtin_assume_aligned(row + off, sizeof(T)), sizeof(v));
+  } else if (off < n) {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) { e[i] = off + i < n ? row[off + i] : T(0.0f); }
+    __builtin_memcpy(&v, e, sizeof(v));
+  }
+  return v;
+}
+
+/** The elements of a word that are infinite or NaN, as 0; whether there are any. */
+template <typename T>
+__device__ __forceinline__ bool drop_unbounded(uint32_t& w)
+{
+  if constexpr (sizeof(T) == 4) {
+    if ((w & 0x7f800000u) != 0x7f800000u) { return false; }
+    w = 0;
+    return true;
+  }
+  constexpr uint32_t kExponent = std::is_same_v<T, f16_t> ? 0x7c00u : 0x7f80u;
+  bool any = false;
+  if ((w & kExponent) == kExponent) {
+    w &= 0xffff0000u;
+    any = true;
+  }
+  if ((w >> 16 & kExponent) == kExponent) {
+    w &= 0x0000ffffu;
+    any = true;
+  }
+  return any;
+}
+
+/** The weights' reference may lag the largest exponent by this much, and weights are multiplied by 2^kLift: float16 weights
+ *  reach 2^15 and keep their precision down to 2^-27 of the largest. */
+template <typename T>
+constexpr float kSlack = 8.0f;
+template <>
+constexpr float kSlack<f16_t> = 1.0f;
+template <typename T>
+constexpr float kLift = 0.0f;
+template <>
+constexpr float kLift<f16_t> = 13.0f;
+
+/** Positions of a tile: 128 bytes of a turned row. */
+template <typename T>
+constexpr int kTile = 128 / sizeof(T);
+
+/** Workgroups per compute unit, by registers and LDS. */
+template <typename T, int D>
+constexpr int kPerUnit = sizeof(T) == 2 && D <= 128 ? 2 : 1;
+
+constexpr int power_of_two(int n) { return n <= 1 ? 1 : 2 * power_of_two((n + 1) / 2); }
+
+template <typename T, int D, bool FULL, bool BENT>
+__global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prompt_args a, prompt_plan plan)
+{
+  constexpr bool WIDE   = sizeof(T) == 4;
+  constexpr int TILE    = kTile<T>;
+  constexpr int kPiece  = 16 / sizeof(T);       // elements of 16 bytes
+  constexpr int kChunks = D / (2 * kPiece);     // products along a row, of a piece per half wave
+  constexpr int kBlocks = TILE / 32;            // products along the positions
+  constexpr int kCols   = D / 32;               // products along the columns of V
+  constexpr int kGroups = TILE / 8;             // groups of 8 positions, which lie in one page
+  constexpr int kRowBytes = D * sizeof(T) + 16; // of a key row in LDS: rows begin in other banks
+  // threads of a key row, rows at a time
+  constexpr int kPieces = D / kPiece, kAcross = power_of_two(kPieces), kDown = kThreads / kAcross, kPasses = TILE / kDown;
+  // columns of a thread in V's turn, the positions of its slot
+  constexpr int kTurn = std::max(power_of_two(D / 32), 2), kSlot = kPiece;
+  __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TILE * kRowBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][D * 128];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
+  const int column = lane % 32, half = lane / 32;
+
+  const int kv        = blockIdx.x % a.kv_heads;
+  const int rest      = blockIdx.x / a.kv_heads;
+  const int split     = rest % plan.splits;
+  const int64_t index = plan.tiles - 1 - rest / plan.splits;
+
+  // rows of no sequence
+  {
+    const int64_t t0 = clamped(a.first[0], a.tokens), t1 = clamped(a.first[a.pages.sequences], a.tokens);
+    for (int64_t i = blockIdx.x; i < t0 + a.tokens - max(t0, t1); i += gridDim.x) {
+      const int64_t token = i < t0 ? i : max(t0, t1) + i - t0;
+      T* out              = static_cast<T*>(a.out) + token * a.heads * a.vdim;
+      for (int j = tid; j < a.heads * a.vdim; j += kThreads) { out[j] = T(0.0f); }
+      if (a.lse != nullptr) {
+        for (int j = tid; j < a.heads; j += kThreads) { a.lse[token * a.heads + j] = -INFINITY; }
+      }
+    }
+  }
+  row_tile rt;
+  if (!find_tile<TILE>(a, plan, index, &rt)) { return; }
+  const int splits = splits_of(plan, rt.tiles);
+  if (split >= splits) { return; }
+  const int tile0 = int(int64_t(split) * rt.tiles / splits), tile1 = int(int64_t(split + 1) * rt.tiles / splits);
+
+  // this lane's row: its token and head, and the positions [lo, hi) that it sees
+  const int row     = rt.row0 + wave * 32 + column;
+  const bool exists = row < rt.rows;
+  const uint32_t i  = plan.group(uint32_t(exists ? row : rt.row0));
+  const int head    = kv * int(plan.group.d) + (exists ? row : rt.row0) - int(i * plan.group.d);
+  const int p       = rt.past + int(i);
+  const int hi      = exists ? max(min(p + 1, rt.length), rt.prefix) : 0;
+  const int lo      = a.window > 0 ? int(max(int64_t(0), int64_t(p) + 1 - a.window)) : 0;
+  const int dim = FULL ? D : a.dim, vdim = FULL ? D : a.vdim;
+
+  u32x4 q[kChunks];
+  {
+    const T* from       = static_cast<const T*>(a.q) + (rt.token0 + i) * a.q_token + head * a.q_head;
+    const uint32_t flip = plan.scale.sign < 0.0f ? (WIDE ? 0x80000000u : 0x80008000u) : 0u;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const auto v = row_piece<FULL, kPiece>(from, (c * 2 + half) * kPiece, dim);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) { q[c][w] = exists ? v.w[w] ^ flip : 0u; }
+    }
+  }
+  const float slope   = BENT && a.shape.slopes != nullptr ? a.shape.slopes[head] : 0.0f;
+  const float per_cap = BENT && a.shape.cap != 0.0f ? a.scale / a.shape.cap : 0.0f;
+
+  // the pages of a tile's groups: lane l has group l % kGroups
+  struct places {
+    int32_t page, slot;
+    uint32_t there;  // bit per group: the sequence has its page
+  };
+  const int32_t* table = a.pages.table + int64_t(rt.sequence) * a.pages.width;
+  const int final      = max(0, rt.length - 1) / 8;
+  const auto look_up   = [&](int tile) {
+    const int g = min(rt.begin / 8 + tile * kGroups + lane % kGroups, final);
+    const int e = int(plan.page_groups(uint32_t(g)));
+    const int32_t page = table[e];
+    const bool there   = uint32_t(page) < uint32_t(a.pages.n_pages);
+    return places{there ? page : 0, (g - e * int(plan.page_groups.d)) * 8,
+                  uint32_t(__ballot(there)) & ((1u << kGroups) - 1u)};
+  };
+  const auto address = [&](const T* base, int64_t page_stride, int64_t slot_stride, places const& at, int g) {
+    const int page = __builtin_amdgcn_readlane(at.page, g), slot = __builtin_amdgcn_readlane(at.slot, g);
+    return base + page * page_stride + slot * slot_stride;
+  };
+  const T* k_head = static_cast<const T*>(a.k) + kv * a.k_head;
+  const T* v_head = static_cast<const T*>(a.v) + kv * a.v_head;
+  const int k_piece = tid % kAcross;
+  const int v_col   = column * kTurn;
+
+  words<T, kPiece> k_next[kPasses];
+  words<T, kTurn> v_next[kSlot];
+  const auto load_tile = [&](places const& at) {
+#pragma unroll
+    for (int n = 0; n < kPasses; ++n) {
+      // a wave's rows of a pass are in one group
+      const int first = n * kDown + wave * (kDown / kWaves), r = n * kDown + tid / kAcross;
+      const T* from   = address(k_head, a.k_page, a.k_slot, at, first / 8) + int64_t(r % 8) * a.k_slot;
+      if (kPieces == kAcross || k_piece < kPieces) { k_next[n] = row_piece<FULL, kPiece>(from, k_piece * kPiece, dim); }
+    }
+#pragma unroll
+    for (int j = 0; j < kSlot; ++j) {
+      const int g   = WIDE ? wave : 2 * wave + j / 4;
+      const T* from = address(v_head, a.v_page, a.v_slot, at, g) + int64_t(4 * half + j % 4) * a.v_slot;
+      if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from, v_col, vdim); }
+    }
+  };
+  /** Into LDS: keys as they lie, V turned. At an edge values that no row sees are 0 and unbounded ones are left out; true
+   *  if there are any. */
+  const auto store_tile = [&](int buffer, int tile, places const& at, bool edge) {
+    bool unbounded = false;
+    if (edge) {
+#pragma unroll
+      for (int j = 0; j < kSlot; ++j) {
+        const int g    = WIDE ? wave : 2 * wave + j / 4;
+        const bool use = (at.there >> g & 1u) != 0 && rt.begin + tile * TILE + g * 8 + 4 * half + j % 4 < rt.length;
+#pragma unroll
+        for (uint32_t& w : v_next[j].w) {
+          if (!use) { w = 0; }
+          unbounded |= drop_unbounded<T>(w);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kPasses; ++n) {
+      const int r = n * kDown + tid / kAcross;
+      if (kPieces == kAcross || k_piece < kPieces) {
+        *reinterpret_cast<u32x4*>(&s_k[buffer][r * kRowBytes + k_piece * 16]) = __builtin_bit_cast(u32x4, k_next[n]);
+      }
+    }
+    if (D % (32 * kTurn) == 0 || v_col < D) {
+#pragma unroll
+      for (int e = 0; e < kTurn; ++e) {
+        u32x4 t;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (WIDE) {
+            t[w] = v_next[w].w[e];
+          } else {
+            t[w] = __builtin_amdgcn_perm(v_next[2 * w + 1].w[e / 2], v_next[2 * w].w[e / 2],
+                                         e % 2 == 0 ? 0x05040100u : 0x07060302u);
+          }
+        }
+        const int col = v_col + e, slot = (2 * wave + half) ^ ((col / 4 + 2 * (col % 4)) % 8);
+        *reinterpret_cast<u32x4*>(&s_v[buffer][col * 128 + slot * 16]) = t;
+      }
+    }
+    return unbounded;
+  };
+  // whether some row does not see all of a tile
+  const int first_hi = max(min(rt.past + int(plan.group(uint32_t(rt.row0))) + 1, rt.length), rt.prefix);
+  const int last_row = min(rt.row0 + kRows, rt.rows) - 1;
+  const int last_lo =
+    a.window > 0 ? int(max(int64_t(0), int64_t(rt.past) + plan.group(uint32_t(last_row)) + 1 - a.window)) : 0;
+  const auto at_edge = [&](int tile, places const& at) {
+    const int t = rt.begin + tile * TILE;
+    return at.there != (1u << kGroups) - 1u || t < last_lo || t + TILE > first_hi;
+  };
+
+  f32x16 o[kCols];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n) { o[n] = f32x16{}; }
+  float base = 0.0f, limit = -INFINITY, total = 0.0f;
+
+  if (tile0 < tile1) {
+    places here = look_up(tile0), next = tile0 + 1 < tile1 ? look_up(tile0 + 1) : here;
+    load_tile(here);
+    bool edge      = at_edge(tile0, here);
+    bool unbounded = store_tile(0, tile0, here, edge);
+    unbounded      = edge ? __syncthreads_or(unbounded) != 0 : (__syncthreads(), false);
+    for (int tile = tile0; tile < tile1; ++tile) {
+      const int buffer = (tile - tile0) % 2;
+      const bool more  = tile + 1 < tile1;
+      places ahead     = next;
+      if (more) {
+        load_tile(next);
+        if (tile + 2 < tile1) { ahead = look_up(tile + 2); }
+      }
+      const int t0    = rt.begin + tile * TILE;
+      const bool some = t0 < hi && t0 + TILE > lo;
+      if (__any(some)) {
+        f32x16 s[kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) { s[b][e] = BENT ? 0.0f : -base; }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const u32x4 k = *reinterpret_cast<const u32x4*>(&s_k[buffer][(b * 32 + column) * kRowBytes + (c * 2 + half) * 16]);
+            s[b]          = mfma32(T{}, k, q[c], s[b]);
+          }
+        }
+        if constexpr (BENT) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int t = t0 + b * 32 + 8 * (e / 4) + 4 * half + e % 4;
+              s[b][e]     = bent(s[b][e], a.scale, per_cap, a.shape.cap, slope, __builtin_fabsf(float(p - t))) - base;
+            }
+          }
+        }
+        const bool masked = edge && !(here.there == (1u << kGroups) - 1u && __all(!exists || (t0 >= lo && t0 + TILE <= hi)));
+        if (masked) {
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int t   = t0 + b * 32 + 8 * (e / 4) + 4 * half + e % 4;
+              const bool in = t >= lo && t < hi && (here.there >> (b * 4 + e / 4) & 1u) != 0;
+              s[b][e]       = in ? s[b][e] : -INFINITY;
+            }
+          }
+        }
+        float high = s[0][0];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) { high = fmaxf(high, s[b][e]); }
+        }
+        if (__any(high > limit)) {
+          high = lanes::fold32(high, [](float u, float w) { return fmaxf(u, w); });
+          // relative to base: where something was counted before, base itself is 0
+          const float up = limit == -INFINITY ? high : fmaxf(high, 0.0f);
+          const bool set = up > -INFINITY;
+          // with a scale of 0 all weigh alike, wherever the scores are
+          const float grown = !set || plan.scale.scale2 == 0.0f ? base : base + up;
+          const float moved = grown - base;
+          const float keep  = limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-moved * plan.scale.scale2);
+          total *= keep;
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) { o[n] *= keep; }
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { s[b][e] -= moved; }
+          }
+          base  = grown;
+          limit = set ? (plan.scale.scale2 == 0.0f ? INFINITY : plan.slack) : limit;
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], plan.scale.scale2, kLift<T>));
+            s[b][e]       = masked && s[b][e] == -INFINITY ? 0.0f : w;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) { total += (s[b][e] + s[b][e + 1]) + (s[b][e + 2] + s[b][e + 3]); }
+        }
+        constexpr int kSteps = TILE / (2 * kSlot);  // products along the positions, of a slot per half wave
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (WIDE) {
+              w[e] = __builtin_bit_cast(uint32_t, float(s[0][4 * m + e]));
+            } else {
+              w[e] = pack2<T>(s[m / 2][8 * (m % 2) + 2 * e], s[m / 2][8 * (m % 2) + 2 * e + 1]);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) {
+            const int col = n * 32 + column, slot = (2 * m + half) ^ ((col / 4 + 2 * (col % 4)) % 8);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(&s_v[buffer][col * 128 + slot * 16]);
+            o[n]          = mfma32(T{}, v, w, o[n]);
+          }
+        }
+        if (unbounded) {
+          // values that are infinite or NaN show in the rows that see them, and in no other: each by itself
+          for (int j = 0; j < TILE; ++j) {
+            const int t = t0 + j, g = j / 8;
+            if (t >= rt.length || (here.there >> g & 1u) == 0) { continue; }
+            const T* from = address(v_head, a.v_page, a.v_slot, here, g) + int64_t(j % 8) * a.v_slot;
+            const bool in = t >= lo && t < hi;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int col = n * 32 + 8 * (e / 4) + 4 * half + e % 4;
+                const float v = in && col < vdim ? float(from[col]) : 0.0f;
+                o[n][e] += __builtin_fabsf(v) < INFINITY ? 0.0f : v;
+              }
+            }
+          }
+        }
+      }
+      if (more) {
+        edge      = at_edge(tile + 1, next);
+        unbounded = store_tile(1 - buffer, tile + 1, next, edge);
+        unbounded = edge ? __syncthreads_or(unbounded) != 0 : (__syncthreads(), false);
+      }
+      here = next;
+      next = ahead;
+    }
+  }
+
+  total = lanes::fold32(total, [](float u, float w) { return u + w; });
+  if (!exists) { return; }
+  const bool counted = limit != -INFINITY;
+  if (splits == 1) {
+    const int64_t at  = (rt.token0 + i) * a.heads + head;
+    const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+    T* out            = static_cast<T*>(a.out) + at * vdim;
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int col = n * 32 + 8 * (e / 4) + 4 * half + e % 4;
+        if (col < vdim) { out[col] = T(total == 0.0f ? 0.0f : o[n][e] * scale); }
+      }
+    }
+    if (half == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, base, total, kLift<T>); }
+  } else {
+    const int64_t at = ((index * a.kv_heads + kv) * plan.splits + split) * kRows + wave * 32 + column;
+#pragma unroll
+    for (int n = 0; n < kCols; ++n) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int col = n * 32 + 8 * (e / 4) + 4 * half + e % 4;
+        if (col < vdim) { plan.part_out[at * vdim + col] = o[n][e]; }
+      }
+    }
+    if (half == 0) {
+      plan.part_max[at] = counted ? base : -INFINITY;
+      plan.part_sum[at] = total;
+    }
+  }
+}
+
+/** 8 rows of a tile that was split, 32 threads each: joins their partials in order of position. */
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(prompt_args a, prompt_plan plan)
+{
+  const int kv        = blockIdx.x % a.kv_heads;
+  const int64_t index = blockIdx.x / a.kv_heads;
+  row_tile rt;
+  if (!find_tile<kTile<T>>(a, plan, index, &rt)) { return; }
+  const int n = splits_of(plan, rt.tiles);
+  const int r = blockIdx.y * (kThreads / 32) + threadIdx.x / 32, row = rt.row0 + r;
+  if (n == 1 || row >= rt.rows) { return; }
+  const uint32_t i   = plan.group(uint32_t(row));
+  const int64_t at   = (rt.token0 + i) * a.heads + kv * int(plan.group.d) + row - int(i * plan.group.d);
+  const int64_t part = (index * a.kv_heads + kv) * plan.splits * kRows + r;
+  float m = -INFINITY;
+  for (int s = 0; s < n; ++s) { m = fmaxf(m, plan.part_max[part + s * kRows]); }
+  float sum = 0.0f;
+  for (int s = 0; s < n; ++s) {
+    sum += factor_of(plan.scale, plan.part_max[part + s * kRows], m) * plan.part_sum[part + s * kRows];
+  }
+  for (int col = threadIdx.x % 32; col < a.vdim; col += 32) {
+    float acc = 0.0f;
+    for (int s = 0; s < n; ++s) {
+      const int64_t slot = part + s * kRows;
+      acc = __builtin_fmaf(factor_of(plan.scale, plan.part_max[slot], m), plan.part_out[slot * a.vdim + col], acc);
+    }
+    static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
+  }
+  if (threadIdx.x % 32 == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, m, sum, kLift<T>); }
+}
+
+int64_t tiles_of(prompt_args const& a) { return a.tokens * (a.heads / a.kv_heads) / kRows + a.pages.sequences; }
+
+/** Splits of a tile's positions: as many workgroups as the chip holds where the tiles alone are fewer. */
+int splits_for(prompt_args const& a, int tile, int per_unit)
+{
+  const int64_t most   = int64_t(a.pages.width) * a.pages.page;
+  const int64_t seen   = a.window > 0 ? std::min(most, a.window + kRows) : most;
+  const int64_t blocks = std::max<int64_t>(1, tiles_of(a) * a.kv_heads);
+  const int64_t wanted = (int64_t(kUnits) * per_unit + blocks - 1) / blocks;
+  return int(std::max<int64_t>(1, std::min({wanted, int64_t(kMaxSplits), seen / tile / kLeast})));
+}
+
+template <typename T>
+size_t workspace_for(prompt_args const& a)
+{
+  // the most splits that any variant takes
+  const int splits = std::max(splits_for(a, kTile<T>, 1), splits_for(a, kTile<T>, 2));
+  return splits == 1 ? 0 : sizeof(float) * size_t(tiles_of(a)) * a.kv_heads * splits * kRows * (a.vdim + 2);
+}
+
+template <typename T>
+void launch(prompt_args const& a, hipStream_t stream)
+{
+  const auto launched = [&](auto bucket, auto full) {
+    constexpr int D = decltype(bucket)::value;
+    prompt_plan plan{divisor(uint32_t(a.pages.page / 8)), divisor(uint32_t(a.heads / a.kv_heads))};
+    plan.tiles  = int32_t(tiles_of(a));
+    plan.splits = splits_for(a, kTile<T>, kPerUnit<T, D>);
+    plan.scale  = scale_of(a.shape.any() ? 1.0f : a.scale);
+    plan.slack  = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
+    const int64_t slots = int64_t(plan.tiles) * a.kv_heads * plan.splits * kRows;
+    plan.part_out       = static_cast<float*>(a.workspace);
+    plan.part_max       = plan.part_out + slots * a.vdim;
+    plan.part_sum       = plan.part_max + slots;
+    const dim3 grid(uint32_t(plan.tiles) * a.kv_heads * plan.splits);
+    if (a.shape.any()) {
+      prompt_kernel<T, D, decltype(full)::value, true><<<grid, kThreads, 0, stream>>>(a, plan);
+    } else {
+      prompt_kernel<T, D, decltype(full)::value, false><<<grid, kThreads, 0, stream>>>(a, plan);
+    }
+    if (plan.splits > 1) {
+      join_kernel<T><<<dim3(uint32_t(plan.tiles) * a.kv_heads, kRows * 32 / kThreads), kThreads, 0, stream>>>(a, plan);
+    }
+  };
+  const auto bucket = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    a.dim == D && a.vdim == D ? launched(d, std::true_type{}) : launched(d, std::false_type{});
+  };
+  const int dim = std::max(a.dim, a.vdim);
+  if (dim <= 64) {
+    bucket(std::integral_constant<int, 64>{});
+  } else if (dim <= 96) {
+    bucket(std::integral_constant<int, 96>{});
+  } else if (dim <= 128) {
+    bucket(std::integral_constant<int, 128>{});
+  } else {
+    bucket(std::integral_constant<int, 256>{});
+  }
+}
+
+}  // namespace
+}  // namespace certex_amd::attention

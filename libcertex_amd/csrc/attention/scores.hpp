@@ -1,0 +1,38 @@
+// Scores that are bent before the softmax: capped by a tanh, leaning on distance.
+#pragma once
+
+#include "elements.hpp"
+
+namespace certex_amd::attention {
+
+/** y = cap tanh(scale x / cap) - slopes[head] * |p - t| for the query's position p and the key's t. */
+struct score_shape {
+  float cap           = 0;        // 0: scale x as it is
+  const float* slopes = nullptr;  // [heads], or NULL: none
+  [[nodiscard]] bool any() const { return cap != 0.0f || slopes != nullptr; }
+};
+
+/**
+ * tanh(u) within 2 units in the last place, NaN where u is. Up to 0.6 in size the fifth convergent of its
+ * continued fraction, u (945 + 105 u^2 + u^4) / (945 + 420 u^2 + 15 u^4), which is off by u^10 / (945 * 10395) of it, 6e-10;
+ * beyond (e - 1) / (e + 1) with e = 2^(2 log2(e) |u|), where e - 1 loses no more than one bit. One reciprocal for both.
+ */
+__device__ __forceinline__ float tanh_of(float u)
+{
+  const float a = __builtin_fabsf(u);
+  const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * kLog2e));
+  const float s = u * u;
+  const bool small = a < 0.6f;
+  const float over = small ? a * __builtin_fmaf(s, s + 105.0f, 945.0f) : e - 1.0f;
+  const float under = small ? __builtin_fmaf(s, __builtin_fmaf(s, 15.0f, 420.0f), 945.0f) : e + 1.0f;
+  return __builtin_copysignf(over * __builtin_amdgcn_rcpf(under), u);
+}
+
+/** The bent score of a product x; per_cap = scale / cap. */
+__device__ __forceinline__ float bent(float x, float scale, float per_cap, float cap, float slope, float distance)
+{
+  const float y = cap != 0.0f ? cap * tanh_of(x * per_cap) : x * scale;
+  return __builtin_fmaf(-slope, distance, y);
+}
+
+}  // namespace certex_amd::attention

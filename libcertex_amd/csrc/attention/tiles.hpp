@@ -1,0 +1,46 @@
+// What the attention kernels share: vectors of words, products on the matrix cores, quotients.
+#pragma once
+
+#include "elements.hpp"
+
+namespace certex_amd::attention {
+
+using f32x4  = __attribute__((ext_vector_type(4))) float;
+using u32x4  = __attribute__((ext_vector_type(4))) uint32_t;
+using u32x2  = __attribute__((ext_vector_type(2))) uint32_t;
+using f16x8  = __attribute__((ext_vector_type(8))) _Float16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+
+/** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less
+ *  than 1, so n m / 2^(29 + s) exceeds n / d by less than 1 / d. */
+struct divisor {
+  uint32_t m, shift, d;
+  explicit divisor(uint32_t by) : d(by)
+  {
+    uint32_t s = 0;
+    while ((uint64_t(1) << s) < by) { ++s; }
+    shift = 29 + s;
+    m     = uint32_t(((uint64_t(1) << shift) + by - 1) / by);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n) * m) >> shift); }
+};
+
+__device__ __forceinline__ f32x4 mfma(f16_t, u32x4 a, u32x4 b, f32x4 c)
+{
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(bf16_t, u32x4 a, u32x4 b, f32x4 c)
+{
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+  const T v[2] = {T(lo), T(hi)};
+  uint32_t w;
+  __builtin_memcpy(&w, v, 4);
+  return w;
+}
+
+}  // namespace certex_amd::attention

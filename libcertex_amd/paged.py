@@ -1,7 +1,7 @@
 """Attention operators next to the key cache, over the C API (include/cuvs/neighbors/certex_attention.h).
 
 Rotary turns queries and keys by their positions; append_pages writes keys (turned on the way) and values
-into a paged cache; paged_attention is the attention of one new token of every sequence over its pages;
+into a paged cache; paged_attention is the attention of one new token of every sequence over its pages, prompt_attention that of many;
 selected_attention is the attention over the top k that KeyCache.topk returned. The reference has
 no counterpart: its attention support ends at the ids and scores (certex/attention.py:84-106).
 
@@ -105,10 +105,14 @@ def append_pages(k, v, k_pages, v_pages, page_table, positions, sequences=None, 
                                 k_pages, v_pages, page_table, positions, sequences, q)
 
 
-def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window=None, return_lse=False):
+def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window=None, return_lse=False, cap=None,
+                    slopes=None):
     """Attention of one new token of every sequence over its pages: q (n_sequences, n_heads, head_dim) gives
     (n_sequences, n_heads, value_dim), softmax(scale q k) v over the positions below lengths[s] (the last `window` of
     them, if given); query head h reads key head h // (n_heads / n_kv_heads). scale defaults to head_dim ** -0.5.
+
+    With a cap the scores are cap * tanh(scale q k / cap); with slopes (float32 (n_heads,), finite) a score loses slopes[h] times the
+    distance of its key from the new token, after the cap.
 
     A sequence of length 0 gives zeros. Lengths past the table's pages are cut to them, positions whose page the
     table does not hold do not count, and slots past a length are never used, whatever they hold; an
@@ -116,7 +120,24 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, scale=None, window
     return_lse also the logarithm of the softmax's denominator (float32, -inf for an empty row), which
     joins the outputs of two calls over different positions. A cache holds head dimensions up to 256 and
     pages of a multiple of 8 positions."""
-    return C.operators().attend(q, k_pages, v_pages, page_table, lengths, scale, window, return_lse)
+    return C.operators().attend(q, k_pages, v_pages, page_table, lengths, scale, window, return_lse, cap, slopes)
+
+
+def prompt_attention(q, k_pages, v_pages, page_table, lengths, first, scale=None, window=None, prefix=None, cap=None,
+                     slopes=None, return_lse=False):
+    """Attention of the new tokens of every sequence over its pages, where append_pages has put their keys and values: q
+    (tokens, n_heads, head_dim) gives (tokens, n_heads, value_dim). Sequence s has the tokens q[first[s] : first[s + 1]] (first:
+    (n_sequences + 1,), not decreasing), which are the last of its lengths[s] positions: a whole prompt, a piece of one
+    behind what the cache holds, or one new token.
+
+    A token at position p sees the positions t <= p of its sequence, and with prefix (n_sequences,) those below
+    prefix[s] too; with a window only those less than `window` before it (t > p - window). Scores, cap and slopes as in
+    paged_attention, slopes times |p - t|. Weights of 16-bit types are rounded to the type before they meet the values.
+
+    Tokens that see nothing (more tokens than the length has positions) and tokens of no sequence give zeros. Lengths, missing
+    pages, unused slots, return_lse and the cache's sizes as in paged_attention; an infinite value shows in the rows that see it."""
+    return C.operators().prompt(q, k_pages, v_pages, page_table, lengths, first, scale, window, prefix, cap, slopes,
+                                return_lse)
 
 
 def selected_attention(scores, ids, values, scale, page_table=None, return_lse=False):
