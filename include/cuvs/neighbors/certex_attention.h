@@ -202,6 +202,66 @@ CUVS_EXPORT cuvsError_t cuvsCertexPromptAttentionWorkspace(DLManagedTensor* q,
                                                            int64_t* bytes);
 
 /**
+ * A paged cache of 4-bit elements: dense uint8 [n_pages, kv_heads, page_size / 8, record], aligned to 16 bytes, whose last
+ * extent is what cuvsCertexPackedRecord reports; page_size is a multiple of 8. A record holds 8 positions of a head. Every
+ * 64 consecutive elements x of a key or value (the last ones of a head fewer) share a float16 offset o, the nearest to their minimum,
+ * and a float16 scale s, the nearest to the float32 quotient (maximum - o) / 15, both cut to float16's finite range; an
+ * element is held as the code round((x - o) / s) (half to even; cut to 0..15; 0 where s is 0) and stands for o + s code. NaN makes
+ * its 64 elements NaN. How codes, scales and offsets lie in a record is up to the library; records can be copied
+ * and pages exchanged as bytes.
+ */
+CUVS_EXPORT cuvsError_t cuvsCertexPackedRecord(int64_t dim, int64_t vdim, int64_t* bytes);
+
+/**
+ * cuvsCertexAppendPages into such pages: keys (rotated on the way unless `rotary` is 0, and rounded to their type) and values
+ * as above. k: rows [tokens, kv_heads, dim]; v: rows [tokens, kv_heads, vdim]; dim and vdim at most 256. Padding,
+ * missing pages and repeated positions as there.
+ */
+CUVS_EXPORT cuvsError_t cuvsCertexPackPages(cuvsResources_t res,
+                                            cuvsCertexRotary_t rotary,
+                                            DLManagedTensor* k,
+                                            DLManagedTensor* v,
+                                            DLManagedTensor* pages,
+                                            DLManagedTensor* page_table,
+                                            DLManagedTensor* positions,
+                                            DLManagedTensor* sequences);
+
+/** What the pages hold at positions[t] of sequence sequences[t] (NULL: t), rounded to the type of k and v (rows, written);
+ *  zeros where a position or sequence is out of range or the table does not hold the page. */
+CUVS_EXPORT cuvsError_t cuvsCertexUnpackPages(cuvsResources_t res,
+                                              DLManagedTensor* pages,
+                                              DLManagedTensor* page_table,
+                                              DLManagedTensor* positions,
+                                              DLManagedTensor* sequences,
+                                              DLManagedTensor* k,
+                                              DLManagedTensor* v);
+
+/**
+ * cuvsCertexPagedAttentionShaped over such pages, of heads of vdim elements of values. q: rows [n_sequences, heads, dim] of any element
+ * type, which is also that of out, dense [n_sequences, heads, vdim]. The workspace is that of
+ * cuvsCertexPackedAttentionWorkspace.
+ */
+CUVS_EXPORT cuvsError_t cuvsCertexPackedAttention(cuvsResources_t res,
+                                                  DLManagedTensor* q,
+                                                  DLManagedTensor* pages,
+                                                  int64_t vdim,
+                                                  DLManagedTensor* page_table,
+                                                  DLManagedTensor* lengths,
+                                                  float scale,
+                                                  float cap,
+                                                  DLManagedTensor* slopes,
+                                                  int64_t window,
+                                                  DLManagedTensor* workspace,
+                                                  DLManagedTensor* out,
+                                                  DLManagedTensor* lse);
+CUVS_EXPORT cuvsError_t cuvsCertexPackedAttentionWorkspace(DLManagedTensor* q,
+                                                           DLManagedTensor* pages,
+                                                           int64_t vdim,
+                                                           DLManagedTensor* page_table,
+                                                           int64_t window,
+                                                           int64_t* bytes);
+
+/**
  * Attention over a selected top k: out[h, i] = sum_j w_j values[id_j] with w the softmax of
  * scale * scores[h, i, j] over j, value head h / (heads / kv_heads); scores and ids as
  * cuvsCertexSearchWithLabelsMapped returns them for a key cache.

@@ -213,6 +213,11 @@ def lib():
                     "cuvsCertexPagedAttentionShaped": [st] + [vp] * 5 + [ctypes.c_float] * 2 + [vp, i64] + [vp] * 3,
                     "cuvsCertexPromptAttentionWorkspace": [vp, vp, vp, vp, i64, P(i64)],
                     "cuvsCertexPromptAttention": [st] + [vp] * 7 + [ctypes.c_float] * 2 + [vp, i64] + [vp] * 3,
+                    "cuvsCertexPackedRecord": [i64, i64, P(i64)],
+                    "cuvsCertexPackPages": [st, st] + [vp] * 6,
+                    "cuvsCertexUnpackPages": [st] + [vp] * 6,
+                    "cuvsCertexPackedAttentionWorkspace": [vp, vp, i64, vp, i64, P(i64)],
+                    "cuvsCertexPackedAttention": [st, vp, vp, i64, vp, vp] + [ctypes.c_float] * 2 + [vp, i64] + [vp] * 3,
                     "cuvsCertexSelectedAttentionWorkspace": [vp, vp, vp, P(i64)],
                     "cuvsCertexSelectedAttention": [st] + [vp] * 4 + [ctypes.c_float] + [vp] * 3,
                 }

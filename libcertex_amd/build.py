@@ -31,6 +31,8 @@ SOURCES = [
     "attention/rotate.hip",
     "attention/attend.hip",
     "attention/select.hip",
+    "attention/pack.hip",
+    "attention/packed.hip",
     "attention/prompt_f32.hip",
     "attention/prompt_f16.hip",
     "attention/prompt_bf16.hip",

@@ -485,16 +485,6 @@ bool shares_lines(attend_args const& a, int bytes)
   return row_tiles_of(a) > 1 || (a.kv_heads > 1 && (a.k_head * bytes % 128 != 0 || a.v_head * bytes % 128 != 0));
 }
 
-/** Shares of a table: one workgroup per place on the chip over all tables, two rounds where that would leave places
- *  empty; no more than there can be tiles. */
-int shares_for(attend_args const& a, int tile, int per_unit)
-{
-  const int64_t places = int64_t(kUnits) * per_unit, tables = int64_t(a.kv_heads) * row_tiles_of(a);
-  int64_t n = std::max<int64_t>(1, places / tables);
-  if (n * tables * 4 < places * 3) { n = (2 * places + tables - 1) / tables; }
-  return int(std::min({n, int64_t(kMaxShares), std::max<int64_t>(1, a.pages.sequences * ((longest_of(a) + tile - 1) / tile))}));
-}
-
 }  // namespace
 
 size_t attend_workspace(elem type, attend_args const& a)

@@ -126,6 +126,75 @@ inline void prompt(elem type, prompt_args const& args, hipStream_t stream)
   type == elem::f32 ? prompt_f32(args, stream) : type == elem::f16 ? prompt_f16(args, stream) : prompt_bf16(args, stream);
 }
 
+/** Dimensions that a packed row of dim elements takes: its chunks of 32. */
+#ifdef __HIPCC__
+__host__ __device__
+#endif
+constexpr int packed_chunks(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : dim <= 128 ? 4 : dim <= 192 ? 6 : 8; }
+
+/**
+ * 4-bit pages, [n_pages][kv_heads][page / 8] records of 8 positions of a head. Every group of 64 elements of a key or value
+ * has a scale s and an offset o (float16); an element is o + s code. A record holds, for C chunks of 32 dimensions and
+ * G = (C + 1) / 2 groups, of the key and then of the value:
+ * - the codes, 128 C bytes. Keys: 16 C bytes a position, word (g C + c) the dimensions [32 c + 8 g, + 8), of which the i-th
+ *   is nibble i / 2 + 4 (i % 2). Values: 64 dimensions are 16 x 2 x 8 bytes, (l, j, position) the dimensions 4 l + 2 j in the
+ *   low nibble and 4 l + 2 j + 1 in the high one; 32 dimensions at the end are 16 x 8 bytes, (l, position) 2 l and 2 l + 1;
+ * - 32 G bytes: of each group the scales of the 8 positions, then their offsets.
+ */
+struct packed_pages {
+  uint8_t* p       = nullptr;
+  int32_t kv_heads = 0, dim = 0, vdim = 0;
+  page_map map;
+  static constexpr int kGroup = 64;
+#ifdef __HIPCC__
+  __host__ __device__
+#endif
+  static constexpr int
+  half_bytes(int dim)
+  {
+    return 128 * packed_chunks(dim) + 32 * ((packed_chunks(dim) + 1) / 2);
+  }
+#ifdef __HIPCC__
+  __host__ __device__
+#endif
+  [[nodiscard]] int record() const
+  {
+    return half_bytes(dim) + half_bytes(vdim);
+  }
+};
+
+/** One side (keys or values) of tokens that are packed into pages, or read from them. */
+struct pack_side {
+  const void* src = nullptr;  // packed from
+  void* dst       = nullptr;  // read into
+  int64_t token = 0, head = 0;
+};
+
+struct pack_args {
+  packed_pages pages;
+  pack_side k, v;
+  const uint64_t* frequencies = nullptr;  // as turn_args; none: keys as they are
+  float magnitude             = 1.0f;
+  bool interleaved            = false;
+  int32_t rotary              = 0;
+  int_vector positions;
+  int_vector sequences;  // none: token t belongs to sequence t
+  int64_t tokens = 0;
+  int32_t heads_per_wave = 0;  // set by the launcher
+};
+
+void pack_pages(elem type, pack_args args, hipStream_t stream);
+void unpack_pages(elem type, pack_args args, hipStream_t stream);
+
+/** attend_args whose keys and values are packed: k, v and their strides are not used. */
+struct packed_args {
+  attend_args a;
+  packed_pages pages;
+};
+
+size_t packed_workspace(packed_args const& args);
+void packed_attend(elem type, packed_args const& args, hipStream_t stream);
+
 /** Largest head dimension of keys and of values. */
 constexpr int kMaxHeadDim = 256;
 /** Positions per page are a multiple of this. */

@@ -499,6 +499,102 @@ PyObject* prompt(PyObject*, PyObject* const* a, Py_ssize_t n)
   });
 }
 
+/** 4-bit pages. */
+auto packed(PyObject* o) -> Tensor const&
+{
+  Tensor const& t = tensor(o, "pages");
+  EXPECTS(t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kByte && t.dim() == 4 && t.is_contiguous(),
+          "pages must be a contiguous uint8 GPU tensor of 4 dimensions");
+  return t;
+}
+
+/** (capsule or None, head_dim, value_dim, k, v, pages, page_table, positions, sequences) */
+PyObject* pack(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+  if (!counted(n, 9)) { return nullptr; }
+  return guarded([&]() -> PyObject* {
+    const rotary_ptr r     = a[0] != Py_None ? rotary_of(a[0]) : rotary_ptr();
+    const int64_t dim      = PyLong_AsLongLong(a[1]), vdim = PyLong_AsLongLong(a[2]);
+    const Tensor k         = read(tensor(a[3], "k"), "k", 3);
+    const Tensor v         = read(tensor(a[4], "v"), "v", 3, &k);
+    Tensor const& pages    = packed(a[5]);
+    const Tensor table     = ints(tensor(a[6], "page_table"), "page_table", true);
+    const Tensor positions = ints(tensor(a[7], "positions"), "positions");
+    maybe sequences        = maybe_tensor(a[8], "sequences");
+    if (sequences) { sequences = ints(*sequences, "sequences"); }
+    no_gradient({&k, &v});
+    EXPECTS(k.size(2) == dim && v.size(2) == vdim, "these pages are of heads of " + std::to_string(dim) + " and values of " +
+                                                     std::to_string(vdim) + ", not " + std::to_string(k.size(2)) + " and " +
+                                                     std::to_string(v.size(2)));
+    view kv(k), vv(v), gv(pages), tv(table), pv(positions), sv(sequences);
+    {
+      unlocked u;
+      check(cuvsCertexPackPages(resources(), r ? r->handle : 0, &kv, &vv, &gv, &tv, &pv, &sv));
+      wrote(pages);
+    }
+    Py_RETURN_NONE;
+  });
+}
+
+/** (head_dim, value_dim, pages, page_table, positions, sequences, a tensor of the outputs' type) */
+PyObject* unpack(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+  if (!counted(n, 7)) { return nullptr; }
+  return guarded([&] {
+    const int64_t dim      = PyLong_AsLongLong(a[0]), vdim = PyLong_AsLongLong(a[1]);
+    Tensor const& pages    = packed(a[2]);
+    const Tensor table     = ints(tensor(a[3], "page_table"), "page_table", true);
+    const Tensor positions = ints(tensor(a[4], "positions"), "positions");
+    EXPECTS(positions.dim() == 1, "positions must have 1 dimension, not shape " + shape_of(positions.sizes()));
+    maybe sequences = maybe_tensor(a[5], "sequences");
+    if (sequences) { sequences = ints(*sequences, "sequences"); }
+    const auto type = tensor(a[6], "dtype").scalar_type();
+    EXPECTS(type == at::kFloat || type == at::kHalf || type == at::kBFloat16,
+            "dtype must be float32, float16 or bfloat16, not " + name_of(type));
+    Tensor k, v;
+    {
+      unlocked u;
+      k = at::empty({positions.size(0), pages.size(1), dim}, pages.options().dtype(type));
+      v = at::empty({positions.size(0), pages.size(1), vdim}, pages.options().dtype(type));
+      view gv(pages), tv(table), pv(positions), sv(sequences), kv(k), vv(v);
+      check(cuvsCertexUnpackPages(resources(), &gv, &tv, &pv, &sv, &kv, &vv));
+    }
+    return with_lse(k, v);
+  });
+}
+
+/** (head_dim, value_dim, q, pages, page_table, lengths, scale or None, window or None, cap or None, slopes or None, return_lse) */
+PyObject* attend_packed(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+  if (!counted(n, 11)) { return nullptr; }
+  return guarded([&] {
+    const int64_t dim   = PyLong_AsLongLong(a[0]), vdim = PyLong_AsLongLong(a[1]);
+    const Tensor q      = read(tensor(a[2], "q"), "q", 3);
+    Tensor const& pages = packed(a[3]);
+    no_gradient({&q});
+    EXPECTS(q.size(2) == dim, "these pages are of heads of " + std::to_string(dim) + ", not " + std::to_string(q.size(2)));
+    const Tensor table   = ints(tensor(a[4], "page_table"), "page_table", true);
+    const Tensor lengths = ints(tensor(a[5], "lengths"), "lengths");
+    const score_options how(a[6], a[7], a[8], a[9], dim);
+    const bool want = PyObject_IsTrue(a[10]) == 1;
+    Tensor out;
+    maybe lse;
+    {
+      unlocked u;
+      out = at::empty({q.size(0), q.size(1), vdim}, q.options());
+      if (want) { lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat)); }
+      view qv(q), gv(pages), tv(table), lv(lengths), ov(out), ev(lse), sv(how.slopes);
+      int64_t bytes = 0;
+      check(cuvsCertexPackedAttentionWorkspace(&qv, &gv, vdim, &tv, how.window, &bytes));
+      const maybe work = workspace(bytes, q);
+      view wv(work);
+      check(cuvsCertexPackedAttention(resources(), &qv, &gv, vdim, &tv, &lv, float(how.scale), float(how.cap), &sv, how.window,
+                                      &wv, &ov, &ev));
+    }
+    return with_lse(out, lse);
+  });
+}
+
 /** (scores, ids, values, scale, page_table or None, return_lse) */
 PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
@@ -570,6 +666,12 @@ PyMethodDef methods[] = {{"init", fast(init), METH_FASTCALL, "(CertexError, torc
                           "(q, k_pages, v_pages, page_table, lengths, scale, window, return_lse, cap, slopes)"},
                          {"prompt", fast(prompt), METH_FASTCALL,
                           "(q, k_pages, v_pages, page_table, lengths, first, scale, window, prefix, cap, slopes, return_lse)"},
+                         {"pack", fast(pack), METH_FASTCALL,
+                          "(capsule, head_dim, value_dim, k, v, pages, page_table, positions, sequences)"},
+                         {"unpack", fast(unpack), METH_FASTCALL,
+                          "(head_dim, value_dim, pages, page_table, positions, sequences, like)"},
+                         {"attend_packed", fast(attend_packed), METH_FASTCALL,
+                          "(head_dim, value_dim, q, pages, page_table, lengths, scale, window, cap, slopes, return_lse)"},
                          {"select", fast(select), METH_FASTCALL, "(scores, ids, values, scale, page_table, return_lse)"},
                          {"undifferentiated", undifferentiated, METH_O, "(tensor): refuses one that is differentiated"},
                          {nullptr, nullptr, 0, nullptr}};

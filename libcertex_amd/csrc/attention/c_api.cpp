@@ -357,6 +357,58 @@ auto shape_of(cuvs::resources const& r, float cap, DLManagedTensor* slopes, int6
   return s;
 }
 
+/** 4-bit pages of heads of dim and vdim elements, and the table over them. */
+auto packed_pages_of(DLManagedTensor* pages_, DLManagedTensor* table_, int64_t dim, int64_t vdim, tensor* pages, tensor* table)
+  -> ops::packed_pages
+{
+  *pages = dense(tensor_of(pages_, "pages"));
+  *table = dense(tensor_of(table_, "page_table"));
+  expects_ndim(*pages, 4);
+  expects_ndim(*table, 2);
+  EXPECTS(pages->is(kDLUInt, 8), "pages must be uint8");
+  EXPECTS(dim >= 1 && dim <= ops::kMaxHeadDim && vdim >= 1 && vdim <= ops::kMaxHeadDim,
+          "head dimensions must be between 1 and " + std::to_string(ops::kMaxHeadDim));
+  EXPECTS(pages->shape[1] >= 1 && pages->shape[1] <= 65535, "pages must have between 1 and 65535 heads");
+  EXPECTS(pages->shape[2] >= 1 && pages->shape[2] < (int64_t(1) << 28), "pages must hold a multiple of 8 positions");
+  EXPECTS(reinterpret_cast<uintptr_t>(pages->p) % 16 == 0, "pages must be aligned to 16 bytes");
+  EXPECTS(table->shape[0] <= 65535, "at most 65535 sequences");
+  ops::packed_pages p;
+  p.p        = static_cast<uint8_t*>(pages->p);
+  p.kv_heads = int32_t(pages->shape[1]);
+  p.dim      = int32_t(dim);
+  p.vdim     = int32_t(vdim);
+  EXPECTS(pages->shape[3] == p.record(), "pages of heads of these dimensions have records of " + std::to_string(p.record()) +
+                                           " bytes, not " + std::to_string(pages->shape[3]));
+  tensor slots   = *pages;  // as the pages of other types are described: positions in their second extent
+  slots.shape[1] = pages->shape[2] * 8;
+  p.map          = page_map_of(*table, table->shape[0], slots);
+  return p;
+}
+
+auto packed_args_of(DLManagedTensor* q_, DLManagedTensor* pages_, int64_t vdim, DLManagedTensor* table_, int64_t window,
+                    ops::elem* type, tensor* q, tensor* pages, tensor* table) -> ops::packed_args
+{
+  *q = rows(tensor_of(q_, "q"), type, true);
+  expects_ndim(*q, 3);
+  ops::packed_args args;
+  args.pages = packed_pages_of(pages_, table_, q->shape[2], vdim, pages, table);
+  auto& a    = args.a;
+  EXPECTS(q->shape[1] >= 1 && q->shape[1] <= 65535 && q->shape[1] % args.pages.kv_heads == 0,
+          "the query heads must be a multiple of the key heads (and at most 65535)");
+  EXPECTS(table->shape[0] == q->shape[0], "page_table must have one row per sequence");
+  EXPECTS(window >= 0, "the window must not be negative");
+  a.heads    = int32_t(q->shape[1]);
+  a.kv_heads = args.pages.kv_heads;
+  a.dim      = int32_t(q->shape[2]);
+  a.vdim     = int32_t(vdim);
+  a.pages    = args.pages.map;
+  a.q        = q->p;
+  a.q_seq    = q->stride[0];
+  a.q_head   = q->stride[1];
+  a.window   = window;
+  return args;
+}
+
 auto select_args_of(DLManagedTensor* scores_, DLManagedTensor* values_, DLManagedTensor* table_, ops::elem* type,
                     tensor* scores, tensor* values, tensor* table) -> ops::select_args
 {
@@ -742,6 +794,165 @@ cuvsError_t cuvsCertexPromptAttention(cuvsResources_t res,
     a.out       = out.p;
     a.workspace = workspace_of(r, workspace_, ops::prompt_workspace(type, a));
     ops::prompt(type, a, stream_of(r));
+    check_launch();
+  });
+}
+
+cuvsError_t cuvsCertexPackedRecord(int64_t dim, int64_t vdim, int64_t* bytes)
+{
+  return translate([=] {
+    EXPECTS(bytes != nullptr, "NULL argument");
+    EXPECTS(dim >= 1 && dim <= ops::kMaxHeadDim && vdim >= 1 && vdim <= ops::kMaxHeadDim,
+            "head dimensions must be between 1 and " + std::to_string(ops::kMaxHeadDim));
+    ops::packed_pages p;
+    p.dim  = int32_t(dim);
+    p.vdim = int32_t(vdim);
+    *bytes = p.record();
+  });
+}
+
+cuvsError_t cuvsCertexPackPages(cuvsResources_t res,
+                                cuvsCertexRotary_t rotary_,
+                                DLManagedTensor* k_,
+                                DLManagedTensor* v_,
+                                DLManagedTensor* pages_,
+                                DLManagedTensor* page_table_,
+                                DLManagedTensor* positions_,
+                                DLManagedTensor* sequences_)
+{
+  return translate([=] {
+    auto& r = res_of(res);
+    auto* h = rotary_ != 0 ? &rotary_of(rotary_) : nullptr;
+    ops::elem type{};
+    const tensor k = rows(tensor_of(k_, "k"), &type, true), v = rows(tensor_of(v_, "v"), &type, false);
+    expects_ndim(k, 3);
+    expects_ndim(v, 3);
+    tensor pages, table;
+    ops::pack_args a;
+    a.pages             = packed_pages_of(pages_, page_table_, k.shape[2], v.shape[2], &pages, &table);
+    const int64_t tokens = k.shape[0];
+    EXPECTS(k.shape[1] == a.pages.kv_heads, "k must have the heads of the pages");
+    EXPECTS(v.shape[0] == tokens && v.shape[1] == k.shape[1], "v must have the tokens and heads of k");
+    a.tokens = tokens;
+    const tensor positions = integers(positions_, "positions");
+    expects_shape(positions, {tokens});
+    a.positions = int_vector_of(positions);
+    expects_device(r, k, v, pages, table, positions);
+    if (sequences_ != nullptr) {
+      const tensor s = integers(sequences_, "sequences");
+      expects_shape(s, {tokens});
+      expects_device(r, s);
+      a.sequences = int_vector_of(s);
+    } else {
+      EXPECTS(table.shape[0] >= tokens, "without sequences, page_table must have one row per token");
+    }
+    if (h != nullptr) {
+      EXPECTS(h->rotary_dim <= k.shape[2], "the rotation is wider than the heads");
+      EXPECTS(h->device == r.device(), "the rotary handle is on another device than the resources");
+      a.frequencies = h->frequencies.as<uint64_t>();
+      a.magnitude   = h->magnitude;
+      a.interleaved = h->interleaved;
+      a.rotary      = h->rotary_dim;
+    }
+    if (tokens == 0 || pages.size() == 0) { return; }
+    a.k = {k.p, nullptr, k.stride[0], k.stride[1]};
+    a.v = {v.p, nullptr, v.stride[0], v.stride[1]};
+    ops::pack_pages(type, a, stream_of(r));
+    check_launch();
+  });
+}
+
+cuvsError_t cuvsCertexUnpackPages(cuvsResources_t res,
+                                  DLManagedTensor* pages_,
+                                  DLManagedTensor* page_table_,
+                                  DLManagedTensor* positions_,
+                                  DLManagedTensor* sequences_,
+                                  DLManagedTensor* k_,
+                                  DLManagedTensor* v_)
+{
+  return translate([=] {
+    auto& r = res_of(res);
+    ops::elem type{};
+    const tensor k = written(rows(tensor_of(k_, "k"), &type, true)), v = written(rows(tensor_of(v_, "v"), &type, false));
+    expects_ndim(k, 3);
+    expects_ndim(v, 3);
+    tensor pages, table;
+    ops::pack_args a;
+    a.pages             = packed_pages_of(pages_, page_table_, k.shape[2], v.shape[2], &pages, &table);
+    const int64_t tokens = k.shape[0];
+    EXPECTS(k.shape[1] == a.pages.kv_heads, "k must have the heads of the pages");
+    EXPECTS(v.shape[0] == tokens && v.shape[1] == k.shape[1], "v must have the tokens and heads of k");
+    a.tokens = tokens;
+    const tensor positions = integers(positions_, "positions");
+    expects_shape(positions, {tokens});
+    a.positions = int_vector_of(positions);
+    expects_device(r, k, v, pages, table, positions);
+    expects_apart(k, v);
+    if (sequences_ != nullptr) {
+      const tensor s = integers(sequences_, "sequences");
+      expects_shape(s, {tokens});
+      expects_device(r, s);
+      a.sequences = int_vector_of(s);
+    } else {
+      EXPECTS(table.shape[0] >= tokens, "without sequences, page_table must have one row per token");
+    }
+    if (tokens == 0) { return; }
+    a.k = {nullptr, k.p, k.stride[0], k.stride[1]};
+    a.v = {nullptr, v.p, v.stride[0], v.stride[1]};
+    ops::unpack_pages(type, a, stream_of(r));
+    check_launch();
+  });
+}
+
+cuvsError_t cuvsCertexPackedAttentionWorkspace(DLManagedTensor* q_,
+                                               DLManagedTensor* pages_,
+                                               int64_t vdim,
+                                               DLManagedTensor* page_table_,
+                                               int64_t window,
+                                               int64_t* bytes)
+{
+  return translate([=] {
+    EXPECTS(bytes != nullptr, "NULL argument");
+    ops::elem type{};
+    tensor q, pages, table;
+    *bytes = int64_t(ops::packed_workspace(packed_args_of(q_, pages_, vdim, page_table_, window, &type, &q, &pages, &table)));
+  });
+}
+
+cuvsError_t cuvsCertexPackedAttention(cuvsResources_t res,
+                                      DLManagedTensor* q_,
+                                      DLManagedTensor* pages_,
+                                      int64_t vdim,
+                                      DLManagedTensor* page_table_,
+                                      DLManagedTensor* lengths_,
+                                      float scale,
+                                      float cap,
+                                      DLManagedTensor* slopes_,
+                                      int64_t window,
+                                      DLManagedTensor* workspace_,
+                                      DLManagedTensor* out_,
+                                      DLManagedTensor* lse_)
+{
+  return translate([=] {
+    auto& r = res_of(res);
+    ops::elem type{};
+    tensor q, pages, table;
+    auto args            = packed_args_of(q_, pages_, vdim, page_table_, window, &type, &q, &pages, &table);
+    auto& a              = args.a;
+    const tensor lengths = integers(lengths_, "lengths");
+    expects_shape(lengths, {q.shape[0]});
+    const tensor out = dense(rows(tensor_of(out_, "out"), &type, false));
+    expects_shape(out, {q.shape[0], q.shape[1], vdim});
+    expects_device(r, q, pages, table, lengths, out);
+    EXPECTS(std::isfinite(scale), "the scale must be finite");
+    a.shape = shape_of(r, cap, slopes_, q.shape[1]);
+    a.lse   = lse_of(r, lse_, q.shape[0], q.shape[1]);
+    if (q.shape[0] == 0) { return; }
+    a.lengths   = int_vector_of(lengths);
+    a.scale     = scale;
+    a.out       = out.p;
+    a.workspace = workspace_of(r, workspace_, ops::packed_workspace(args));
+    ops::packed_attend(type, args, stream_of(r));
     check_launch();
   });
 }

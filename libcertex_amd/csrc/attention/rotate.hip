@@ -14,6 +14,7 @@
 // launch and three dependent loads.
 #include "attention.hpp"
 #include "elements.hpp"
+#include "turn.hpp"
 
 #include <algorithm>
 #include <numeric>
@@ -24,15 +25,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBatch   = 4;
-
-/** x in the element type, rounded from its float32 value: the compiler would round some float16 results once from the
- *  exact sum of products (v_fma_mixlo_f16) and others twice, so that the vector's width showed in the bits. */
-template <typename T>
-__device__ __forceinline__ T narrowed(float x)
-{
-  if constexpr (std::is_same_v<T, f16_t>) { asm("" : "+v"(x)); }
-  return T(x);
-}
 
 /**
  * One thread: one vector of V elements of a row (of both halves in the half layout), over
@@ -116,14 +108,9 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
   if (turned) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      const uint32_t turns = uint32_t((uint64_t(p) * a.frequencies[pair + i]) >> 32);
-      float sine, cosine;
-      sincospif(float(int32_t(turns & ~255u)) * 0x1p-31f, &sine, &cosine);
-      const float rest = float(turns & 255u) * float(M_PI * 0x1p-31);
-      s[i]             = __builtin_fmaf(cosine, rest, sine);
-      c[i]             = __builtin_fmaf(sine, -rest, cosine);
-      c[i] *= a.magnitude;
-      s[i] *= a.transpose ? -a.magnitude : a.magnitude;
+      const sines at = sines_of(p, a.frequencies[pair + i]);
+      c[i]           = at.c * a.magnitude;
+      s[i]           = at.s * (a.transpose ? -a.magnitude : a.magnitude);
     }
   }
   const auto put = [](T* p, pack<T, V> const& v) {
@@ -144,8 +131,8 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(turn_args a)
           T& u          = kAdjacent ? x[i].e[2 * j] : x[i].e[j];
           T& w          = kAdjacent ? x[i].e[2 * j + 1] : y[i].e[j];
           const float f = float(u), g = float(w);
-          u = narrowed<T>(__builtin_fmaf(f, c[j], -(g * s[j])));
-          w = narrowed<T>(__builtin_fmaf(f, s[j], g * c[j]));
+          u = turned_first<T>(f, g, c[j], s[j]);
+          w = turned_second<T>(f, g, c[j], s[j]);
         }
         if constexpr (!kAdjacent) { put(row + second, y[i]); }
       }

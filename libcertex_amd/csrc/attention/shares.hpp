@@ -160,5 +160,15 @@ int64_t longest_of(attend_args const& a)
   return a.window > 0 && a.window < most ? std::min(most, a.window + 7) : most;
 }
 
+/** Shares of a table: one workgroup per place on the chip over all tables, two rounds where that would leave places
+ *  empty; no more than there can be tiles. */
+int shares_for(attend_args const& a, int tile, int per_unit)
+{
+  const int64_t places = int64_t(kUnits) * per_unit, tables = int64_t(a.kv_heads) * row_tiles_of(a);
+  int64_t n = std::max<int64_t>(1, places / tables);
+  if (n * tables * 4 < places * 3) { n = (2 * places + tables - 1) / tables; }
+  return int(std::min({n, int64_t(kMaxShares), std::max<int64_t>(1, a.pages.sequences * ((longest_of(a) + tile - 1) / tile))}));
+}
+
 }  // namespace
 }  // namespace certex_amd::attention

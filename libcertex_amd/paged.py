@@ -2,7 +2,7 @@
 
 Rotary turns queries and keys by their positions; append_pages writes keys (turned on the way) and values
 into a paged cache; paged_attention is the attention of one new token of every sequence over its pages, prompt_attention that of many;
-selected_attention is the attention over the top k that KeyCache.topk returned. The reference has
+selected_attention is the attention over the top k that KeyCache.topk returned. PackedPages is a paged cache of 4-bit elements. The reference has
 no counterpart: its attention support ends at the ids and scores (certex/attention.py:84-106).
 
 A paged cache is two pools, keys (n_pages, page_size, n_kv_heads, head_dim) and values (the same with their own
@@ -138,6 +138,62 @@ def prompt_attention(q, k_pages, v_pages, page_table, lengths, first, scale=None
     pages, unused slots, return_lse and the cache's sizes as in paged_attention; an infinite value shows in the rows that see it."""
     return C.operators().prompt(q, k_pages, v_pages, page_table, lengths, first, scale, window, prefix, cap, slopes,
                                 return_lse)
+
+
+class PackedPages:
+    """A paged cache of 4-bit keys and values, in 9/32 of what 16-bit pages take (heads of 64, 128, 192 and 256 elements;
+    others are padded to 64, 96, 128, 192 or 256).
+
+        pages = certex.PackedPages(n_pages, page_size=64, n_kv_heads=8, head_dim=128)
+        pages.append(k, v, table, positions, sequences, rotary=rope)
+        out = pages.attend(q, table, lengths)
+
+    Of every 64 consecutive elements x of a key or value (the last ones of a head fewer): an offset o, the float16 nearest to their
+    minimum, a scale s, the float16 nearest to the float32 quotient (maximum - o) / 15, and codes round((x - o) / s) in
+    0..15 (half to even; all 0 where s is 0), which stand for o + s code. o and s are cut to float16's finite range; NaN makes its 64 elements
+    NaN. Page tables, positions and lengths are those of append_pages and paged_attention, pages of a multiple of 8 positions.
+
+    `data` holds the pages, uint8 (n_pages, n_kv_heads, page_size / 8, record): pages can be copied in it, as
+    data[new] = data[old], and a program may bring its own memory of that shape (contiguous, aligned to 16 bytes)."""
+
+    def __init__(self, n_pages, page_size, n_kv_heads, head_dim, value_dim=None, data=None):
+        self.page_size, self.n_kv_heads, self.head_dim = int(page_size), int(n_kv_heads), int(head_dim)
+        self.value_dim = self.head_dim if value_dim is None else int(value_dim)
+        _require(int(n_pages) >= 0 and self.n_kv_heads >= 1, "n_pages must not be negative and n_kv_heads positive")
+        _require(self.page_size >= 8 and self.page_size % 8 == 0,
+                 f"the page size must be a multiple of 8, not {self.page_size}")
+        record = ctypes.c_int64()
+        C.check(C.lib().cuvsCertexPackedRecord(self.head_dim, self.value_dim, ctypes.byref(record)))
+        shape = (int(n_pages), self.n_kv_heads, self.page_size // 8, record.value)
+        if data is None:
+            data = torch.zeros(shape, dtype=torch.uint8, device="cuda")
+        _require(isinstance(data, torch.Tensor) and data.is_cuda and data.dtype == torch.uint8 and data.is_contiguous()
+                 and tuple(data.shape) == shape, f"data must be a contiguous uint8 GPU tensor of shape {shape}")
+        self.data = data
+
+    def append(self, k, v, page_table, positions, sequences=None, rotary=None):
+        """As append_pages: token t's keys k[t] (n_kv_heads, head_dim), turned by `rotary` and rounded to their type, and values
+        v[t] to position positions[t] of sequence sequences[t] (default: t), in 4 bits."""
+        C.operators().pack(None if rotary is None else self._turn(rotary, k), self.head_dim, self.value_dim, k, v, self.data,
+                           page_table, positions, sequences)
+
+    def _turn(self, rotary, k):
+        _require(rotary.head_dim == self.head_dim,
+                 f"this rotation is of heads of {rotary.head_dim}, not {self.head_dim}")
+        return rotary._handle(k)
+
+    def read(self, page_table, positions, sequences=None, dtype=torch.bfloat16):
+        """The keys (tokens, n_kv_heads, head_dim) and values that the pages hold at positions[t] of sequence sequences[t] (default:
+        t), rounded to dtype; zeros where the table does not hold the page."""
+        _require(isinstance(dtype, torch.dtype), f"dtype must be a torch.dtype, not {dtype!r}")
+        return C.operators().unpack(self.head_dim, self.value_dim, self.data, page_table, positions, sequences,
+                                    torch.empty(0, dtype=dtype))
+
+    def attend(self, q, page_table, lengths, scale=None, window=None, return_lse=False, cap=None, slopes=None):
+        """As paged_attention: q (n_sequences, n_heads, head_dim) of any element type gives (n_sequences, n_heads, value_dim)
+        of the same."""
+        return C.operators().attend_packed(self.head_dim, self.value_dim, q, self.data, page_table, lengths, scale, window, cap,
+                                           slopes, return_lse)
 
 
 def selected_attention(scores, ids, values, scale, page_table=None, return_lse=False):

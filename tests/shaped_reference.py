@@ -7,7 +7,8 @@ from tests.paged_reference import UNIT
 U = 2.0**-24
 
 
-def attend(q, positions, keys, values, scale, prefix=0, window=None, cap=None, slopes=None, there=None, weight=0.0):
+def attend(q, positions, keys, values, scale, prefix=0, window=None, cap=None, slopes=None, there=None, weight=0.0,
+           key_sizes=None, value_sizes=None):
     """Queries (n, heads, d) at `positions` (n,) over the keys (length, kv, d) and values of one sequence. Returns out (n, heads, dv),
     lse (n, heads) and bounds of their errors before the output is rounded.
 
@@ -15,7 +16,8 @@ def attend(q, positions, keys, values, scale, prefix=0, window=None, cap=None, s
     of d terms; 8 u (cap + slope distance + |y|) of the bent score, whose last operations round what is of that size, and
     4 u of the difference from the reference, of the exponential and of the weight, which `weight` adds to if weights are
     rounded again. An output of weights w / sum w is then off by sum w e |v| + (sum w e) |out|, and the two sums of n
-    terms add 4 (sqrt(n) + 1) u of sum w |v| each."""
+    terms add 4 (sqrt(n) + 1) u of sum w |v| each. key_sizes and value_sizes: what |k| and |v| are where those are computed as
+    sums of terms, the sizes of the terms."""
     q, keys, values = q.double().cpu(), keys.double().cpu(), values.double().cpu()
     n, heads, d = q.shape
     length, group = keys.shape[0], heads // keys.shape[1]
@@ -30,11 +32,16 @@ def attend(q, positions, keys, values, scale, prefix=0, window=None, cap=None, s
     out_room, lse_room = torch.zeros_like(out), torch.zeros_like(lse)
     if length == 0:
         return out, lse, out_room, lse_room
+    key_sizes = keys.abs() if key_sizes is None else key_sizes
+    value_sizes = values.abs() if value_sizes is None else value_sizes
     for h in range(heads):
         k, v = keys[:, h // group], values[:, h // group]
-        k, v = torch.where(seen.any(0)[:, None], k, 0.0), torch.where(seen.any(0)[:, None], v, 0.0)
+        used = seen.any(0)[:, None]
+        k, v = torch.where(used, k, 0.0), torch.where(used, v, 0.0)
+        k_size = torch.where(used, key_sizes[:, h // group], 0.0)
+        v_size = torch.where(used, value_sizes[:, h // group], 0.0)
         x = scale * (q[:, h] @ k.T)
-        size = abs(scale) * (q[:, h].abs() @ k.abs().T)
+        size = abs(scale) * (q[:, h].abs() @ k_size.T)
         y = cap * torch.tanh(x / cap) if cap else x
         lean = float(slopes[h]) * (p - t).abs() if slopes is not None else torch.zeros(1, dtype=torch.float64)
         y = y - lean
@@ -47,7 +54,7 @@ def attend(q, positions, keys, values, scale, prefix=0, window=None, cap=None, s
         out[:, h], lse[:, h] = w @ v, torch.logsumexp(y, -1)
         off = torch.where(seen, w * e, 0.0)
         sums = 4 * (length**0.5 + 1) * U
-        out_room[:, h] = off @ v.abs() + off.sum(-1, keepdim=True) * out[:, h].abs() + 2 * sums * (w @ v.abs())
+        out_room[:, h] = off @ v_size + off.sum(-1, keepdim=True) * out[:, h].abs() + 2 * sums * (w @ v_size)
         lse_room[:, h] = off.sum(-1) + sums + 8 * U * (1 + torch.where(some, lse[:, h].abs(), 0.0))
     return out, lse, out_room, lse_room
 
