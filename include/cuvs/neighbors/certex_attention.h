@@ -205,7 +205,7 @@ CUVS_EXPORT cuvsError_t cuvsCertexPromptAttentionWorkspace(DLManagedTensor* q,
  * A paged cache of 4-bit elements: dense uint8 [n_pages, kv_heads, page_size / 8, record], aligned to 16 bytes, whose last
  * extent is what cuvsCertexPackedRecord reports; page_size is a multiple of 8. A record holds 8 positions of a head. Every
  * 64 consecutive elements x of a key or value (the last ones of a head fewer) share a float16 offset o, the nearest to their minimum,
- * and a float16 scale s, the nearest to the float32 quotient (maximum - o) / 15, both cut to float16's finite range; an
+ * and a float16 scale s, the nearest to the float32 product of maximum - o and float32(1 / 15), both cut to float16's finite range; an
  * element is held as the code round((x - o) / s) (half to even; cut to 0..15; 0 where s is 0) and stands for o + s code. NaN makes
  * its 64 elements NaN. How codes, scales and offsets lie in a record is up to the library; records can be copied
  * and pages exchanged as bytes.

@@ -192,7 +192,7 @@ struct packed_args {
   packed_pages pages;
 };
 
-size_t packed_workspace(packed_args const& args);
+size_t packed_workspace(elem type, packed_args const& args);
 void packed_attend(elem type, packed_args const& args, hipStream_t stream);
 
 /** Largest head dimension of keys and of values. */

@@ -915,7 +915,8 @@ cuvsError_t cuvsCertexPackedAttentionWorkspace(DLManagedTensor* q_,
     EXPECTS(bytes != nullptr, "NULL argument");
     ops::elem type{};
     tensor q, pages, table;
-    *bytes = int64_t(ops::packed_workspace(packed_args_of(q_, pages_, vdim, page_table_, window, &type, &q, &pages, &table)));
+    const auto args = packed_args_of(q_, pages_, vdim, page_table_, window, &type, &q, &pages, &table);
+    *bytes          = int64_t(ops::packed_workspace(type, args));
   });
 }
 
@@ -951,7 +952,7 @@ cuvsError_t cuvsCertexPackedAttention(cuvsResources_t res,
     a.lengths   = int_vector_of(lengths);
     a.scale     = scale;
     a.out       = out.p;
-    a.workspace = workspace_of(r, workspace_, ops::packed_workspace(args));
+    a.workspace = workspace_of(r, workspace_, ops::packed_workspace(type, args));
     ops::packed_attend(type, args, stream_of(r));
     check_launch();
   });

@@ -1,6 +1,6 @@
 // Keys and values of new tokens into 4-bit pages, the keys turned on the way, and back from them.
 //
-// Of every 64 elements x of a head: offset o = float16(min x), scale s = float16((max x - o) / 15), and codes
+// Of every 64 elements x of a head: offset o = float16(min x), scale s = float16((max x - o) * (1 / 15 as float32)), and codes
 // c = round((x - o) / s) in 0..15, so that o + s c is x within s / 2 (and what o and s are rounded by). Which of two codes is
 // nearer is decided in 64 bits: the distance x - o is exact there, and so is its remainder x - o - s c.
 //
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(pack_args a)
     const float low = lanes::min<64>(in ? x : INFINITY), high = lanes::max<64>(in ? x : -INFINITY);
     const bool nan  = __any(x != x);
     const f16_t offset = nan ? f16_t(__builtin_nanf("")) : f16_t(fminf(fmaxf(low, -kMost), kMost));
-    const f16_t scale  = nan ? offset : f16_t(fminf(fmaxf((high - float(offset)) / 15.0f, 0.0f), kMost));
+    const f16_t scale  = nan ? offset : f16_t(fminf(fmaxf((high - float(offset)) * (1.0f / 15.0f), 0.0f), kMost));
     uint32_t code = 0;
     if (float(scale) > 0.0f) {
       const double s = double(float(scale)), distance = double(x) - double(float(offset));

@@ -37,19 +37,76 @@ struct packed_plan {
   elem type;
 };
 
-/** Workgroups per compute unit, by registers. */
-template <int C>
-constexpr int kPerUnit = C <= 4 ? 2 : 1;
-
-template <int N>
-__device__ __forceinline__ void copy_words(uint32_t* to, const uint8_t* from)
+/** Workgroups per compute unit: as many as registers and LDS hold without spilling. */
+constexpr int per_unit(int chunks, bool full, int parts)
 {
-  __builtin_memcpy(to, __builtin_assume_aligned(from, 4), 4 * N);
+  return chunks <= 2 ? 4 : chunks == 3 ? (full ? 3 : 2) : chunks == 4 ? (full && parts == 1 ? 3 : 2) : full && parts == 1 ? 2 : 1;
+}
+
+/** Bytes of a record of C chunks of dimensions on both sides: the most that a kernel's records take. */
+template <int C>
+constexpr int kRecord = 256 * C + 64 * ((C + 1) / 2);
+
+/** A wave's steps in LDS: one that is worked on, one that is on its way. */
+constexpr int kBuffers = 2;
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(4))) int32_t* constant_ints;
+
+/** A value that all lanes have, in scalar registers. */
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x)
+{
+  const uint32_t lo = uint32_t(uniform(int(x))), hi = uint32_t(uniform(int(x >> 32)));
+  return int64_t(uint64_t(hi) << 32 | lo);
+}
+template <typename T>
+__device__ __forceinline__ const T* uniform(const T* p)
+{
+  return reinterpret_cast<const T*>(uniform(int64_t(reinterpret_cast<uintptr_t>(p))));
+}
+
+/** 16 bytes a lane from base + offset to LDS byte m0 + 16 lane. In assembly, so that the compiler does not order LDS reads
+ *  against it: the copies of a step go to a buffer that its wave has read, and landed() comes before they are. */
+__device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t m0)
+{
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(uniform(base)), "s"(m0) : "m0", "memory");
+}
+
+/** Waits until at most n of this wave's copies are on their way (n as they are issued: 0, or those of one step). */
+__device__ __forceinline__ void landed(int n)
+{
+  switch (n) {
+    case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+    case 1: asm volatile("s_waitcnt vmcnt(1)" ::: "memory"); break;
+    case 2: asm volatile("s_waitcnt vmcnt(2)" ::: "memory"); break;
+    case 3: asm volatile("s_waitcnt vmcnt(3)" ::: "memory"); break;
+    case 4: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
+    case 5: asm volatile("s_waitcnt vmcnt(5)" ::: "memory"); break;
+    case 6: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
+    case 7: asm volatile("s_waitcnt vmcnt(7)" ::: "memory"); break;
+    case 8: asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); break;
+    default: asm volatile("s_waitcnt vmcnt(9)" ::: "memory"); break;  // and any larger number
+  }
+}
+
+/** N words of LDS; N and `from` are multiples of ALIGN words. */
+template <int N, int ALIGN>
+__device__ __forceinline__ void read_words(uint32_t* to, const uint8_t* from)
+{
+  __builtin_memcpy(to, __builtin_assume_aligned(from, 4 * ALIGN), 4 * N);
 }
 
 __device__ __forceinline__ float half_of(uint32_t w, int i)
 {
   return float(__builtin_bit_cast(f16x2, w)[i]);
+}
+
+/** The codes in the low 4 bits of a word's halves, less 8, as float16: 1024 + code is the number with the code in its last bits. */
+__device__ __forceinline__ uint32_t less_eight(uint32_t w)
+{
+  const f16x2 far = __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u);
+  return __builtin_bit_cast(uint32_t, far - f16x2{1032.0f, 1032.0f});
 }
 
 /** Elements [d, d + 8) of a query of dim elements, in float32. */
@@ -80,11 +137,14 @@ __device__ __forceinline__ void load_query(elem type, const void* q, int64_t at,
 
 /** C chunks of 32 dimensions; FULL: of keys and of values alike, else at most. P: elements that a query enters as. */
 template <int C, bool FULL, int P>
-__global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_args args, packed_plan pp)
+__global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(packed_args args, packed_plan pp)
 {
   constexpr int G = (C + 1) / 2;  // groups
   constexpr int D = 32 * C;
-  __shared__ float s_out[kWaves][kRows][D];
+  constexpr bool FINE = P > 1;  // float32: more of the products' low bits
+  // the waves' steps, then their outputs
+  __shared__ __attribute__((aligned(16))) uint8_t s_steps[kWaves][kBuffers][4 * kRecord<C>];
+  static_assert(sizeof(float) * kRows * D <= sizeof(s_steps[0]));
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
   attend_args const& a    = args.a;
   attend_plan const& plan = pp.at;
@@ -141,83 +201,71 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
   const bool bends     = a.shape.cap != 0.0f || a.shape.slopes != nullptr;
   const int per_page   = int(plan.page_groups.d);  // records
   const int64_t head   = int64_t(record) * per_page, page_bytes = head * a.kv_heads;
-  const uint8_t* base_ = args.pages.p + kv * head;
+  const uint8_t* pool  = args.pages.p + kv * head;
 
   span sp{};
   int t0 = 0, t1 = 0, group = 0, stop = 0, final = 0;
-  const int32_t* pages = nullptr;
-  // the record of a group's positions; the sequence has its page
+  constant_ints pages = nullptr;
+  // where a step's 4 records begin; bit per record: the sequence has its page
   struct place {
-    const uint8_t* p;
-    bool there;
+    const uint8_t* p[4];
+    uint32_t there;
   };
-  place v_at{};
-  const auto entry = [&](int group) {
-    const int at = min(group, final);
-    const int e  = int(plan.page_groups(uint32_t(at)));
+  // the records of a step follow one another if pages hold whole steps and the sequence's first step begins one
+  bool follow = false;
+  const auto entry = [&](int at, const uint8_t** p) {
+    at             = min(at, final);
+    const int e    = int(plan.page_groups(uint32_t(at)));
     const int page = pages[e];
     const bool there = uint32_t(page) < uint32_t(a.pages.n_pages);
-    return place{base_ + (there ? page : 0) * page_bytes + (at - e * per_page) * record, there};
+    *p = pool + (there ? page : 0) * page_bytes + int64_t(at - e * per_page) * record;
+    return there;
   };
-  uint32_t k[2][C], ks[G][4], ko[G][4];  // codes of two rows; scales and offsets of 8 positions
-  uint32_t v[(C + 1) / 2][4], vs[G][4], vo[G][4];
-  const auto load_keys = [&](place rows_at, place mine) {
+  const auto look_up = [&](int group) {
+    place at{};
+    if (follow) {
+      at.there = entry(group, &at.p[0]) ? 15u : 0u;
+    } else {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      copy_words<C>(k[half], rows_at.p + (half * 4 + r % 4) * 16 * k_chunks + g * 4 * k_chunks);
+      for (int i = 0; i < 4; ++i) { at.there |= uint32_t(entry(group + i, &at.p[i])) << i; }
     }
+    return at;
+  };
+  /** The copies of a step, and how many they are. */
+  const auto copy = [&](place const& at, int buffer) {
+    const uint32_t to = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr)&s_steps[wave][buffer][0]));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read there has arrived
+    int n = 0;
+    if (follow) {
+      for (int from = 0; from < 4 * record; from += 1024, ++n) {
+        if (from + lane * 16 < 4 * record) { copy_to_lds(at.p[0] + from, lane * 16, to + from); }
+      }
+    } else {
 #pragma unroll
-    for (int n = 0; n < G; ++n) {
-      if (FULL || n < k_groups) {
-        copy_words<4>(ks[n], mine.p + 128 * k_chunks + n * 32);
-        copy_words<4>(ko[n], mine.p + 128 * k_chunks + n * 32 + 16);
+      for (int i = 0; i < 4; ++i) {
+        for (int from = 0; from < record; from += 1024, ++n) {
+          if (from + lane * 16 < record) { copy_to_lds(at.p[i] + from, lane * 16, to + i * record + from); }
+        }
       }
     }
+    return n;
   };
-  const auto load_values = [&](place mine) {
-    const uint8_t* at = mine.p + k_bytes;
-#pragma unroll
-    for (int u = 0; u < (C + 1) / 2; ++u) {
-      if (2 * u + 1 < C && (FULL || 2 * u + 1 < v_chunks)) {
-        copy_words<4>(v[u], at + u * 256 + r * 16);
-      } else if (FULL || 2 * u < v_chunks) {
-        copy_words<2>(v[u], at + u * 256 + r * 8);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < G; ++n) {
-      if (FULL || n < v_groups) {
-        copy_words<4>(vs[n], at + 128 * v_chunks + n * 32);
-        copy_words<4>(vo[n], at + 128 * v_chunks + n * 32 + 16);
-      }
-    }
-  };
-  // unused words are 0 from the start
-#pragma unroll
-  for (int n = 0; n < G; ++n) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) { ks[n][w] = ko[n][w] = vs[n][w] = vo[n][w] = 0; }
-  }
-#pragma unroll
-  for (int u = 0; u < (C + 1) / 2; ++u) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) { v[u][w] = 0; }
-  }
-  place k_next{}, v_next{};
-  // the share's tiles of sequence b (or of the next that has any): their range, and the first step's loads
+  place here{}, next_at{};
+  // the share's tiles of sequence b (or of the next that has any): their range, and the first step's copies
   const auto begin = [&] {
     for (sp = span_of<kTile>(a, b); sp.tiles == 0; sp = span_of<kTile>(a, b)) { ++b; }
-    t0    = int(tile - before);
-    t1    = int(min(int64_t(sp.tiles), t0 + last - tile));
-    pages = a.pages.table + b * a.pages.width;
-    final = (sp.end - 1) / 8;
-    group = sp.begin / 8 + (t0 * kWaves + wave) * 4;
-    stop  = min(sp.begin / 8 + t1 * kWaves * 4, final + 1);
+    sp     = {uniform(sp.begin), uniform(sp.end), uniform(sp.tiles)};
+    t0     = uniform(int(tile - before));
+    t1     = uniform(int(min(int64_t(sp.tiles), t0 + last - tile)));
+    pages  = (constant_ints)uniform(a.pages.table + b * a.pages.width);
+    final  = (sp.end - 1) / 8;
+    group  = sp.begin / 8 + (t0 * kWaves + wave) * 4;
+    stop   = min(sp.begin / 8 + t1 * kWaves * 4, final + 1);
+    follow = per_page % 4 == 0 && sp.begin / 8 % 4 == 0;
     if (group < stop) {
-      k_next = entry(group + r / 4);
-      v_next = entry(group + g);
-      load_keys(k_next, v_next);
-      load_values(v_next);
+      here = look_up(group);
+      copy(here, 0);
+      if (group + kWaves * 4 < stop) { next_at = look_up(group + kWaves * 4); }
     }
   };
 
@@ -250,9 +298,9 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          // codes of the odd words are 16 times themselves
+          // codes that are 16 times themselves
           float lo = e[c][2 * w], hi = e[c][2 * w + 1];
-          if (w % 2 == 1) { lo *= 0.0625f, hi *= 0.0625f; }
+          if (!FINE && w % 2 == 1) { lo *= 0.0625f, hi *= 0.0625f; }
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             q[c][i][w] = pack2<f16_t>(lo, hi);
@@ -263,8 +311,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
       }
       const auto plus = [](float u, float w) { return u + w; };
 #pragma unroll
-      for (int n = 0; n < G; ++n) { q_sum[n] = lanes::fold16(lanes::fold32(q_sum[n], plus), plus) * 0x1p-24f; }
-      exponent += 24;
+      for (int n = 0; n < G; ++n) { q_sum[n] = lanes::fold16(lanes::fold32(q_sum[n], plus), plus) * (FINE ? 1.0f : 0x1p-24f); }
+      exponent += FINE ? 0 : 24;
     }
     f32x4 o[C][2];   // tiles of 16 columns: chunk c of V's units, even and odd dimensions of a pair
     float shift[G];  // sum of p times the offsets, of this lane's positions
@@ -277,41 +325,65 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
     int lift          = kRoom + 23;
     float scale_limit = __builtin_amdgcn_ldexpf(1.0f, kRoom - lift);
 
+    int buffer = 0;
     while (group < stop) {
       const int next = group + kWaves * 4;
-      const bool have = v_next.there;
+      const uint32_t there = here.there;
+      int coming = 0;
+      if (next < stop) {
+        coming = copy(next_at, 1 - buffer);
+        here   = next_at;
+        if (next + kWaves * 4 < stop) { next_at = look_up(next + kWaves * 4); }
+      }
+      landed(coming);
+      const bool have       = (there >> g & 1u) != 0;
+      const uint8_t* rows_  = &s_steps[wave][buffer][r / 4 * record];  // of the product's row
+      const uint8_t* mine   = &s_steps[wave][buffer][g * record];      // of the positions that this lane weighs
+      const uint8_t* values = mine + k_bytes;
       f32x4 s[2][G];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int n = 0; n < G; ++n) { s[half][n] = f32x4{0, 0, 0, 0}; }
-      }
+        uint32_t k[C];
+        read_words<C, C == 4 || C == 8 ? 4 : C % 2 == 0 ? 2 : 1>(
+          k, FULL ? rows_ + (half * 4 + r % 4) * 16 * C + g * 4 * C : rows_ + (half * 4 + r % 4) * 16 * k_chunks + g * 4 * k_chunks);
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
+        for (int c = 0; c < C; ++c) {
+          const uint32_t w = k[c], up = w >> 8;
+          u32x4 codes{w & 0x000f000fu, w & 0x00f000f0u, up & 0x000f000fu, up & 0x00f000f0u};
+          if (FINE) { codes = {less_eight(w), less_eight(w >> 4), less_eight(up), less_eight(w >> 12)}; }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t w = k[half][c], up = w >> 8;
-          const u32x4 codes{w & 0x000f000fu, w & 0x00f000f0u, up & 0x000f000fu, up & 0x00f000f0u};
-#pragma unroll
-          for (int i = 0; i < P; ++i) { s[half][c / 2] = mfma(f16_t{}, codes, q[c][i], s[half][c / 2]); }
+          for (int i = P - 1; i >= 0; --i) { s[half][c / 2] = mfma(f16_t{}, codes, q[c][i], s[half][c / 2]); }
         }
       }
       float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = 0.0f;
+      for (int j = 0; j < 8; ++j) { x[j] = 0.0f; }
 #pragma unroll
-        for (int n = 0; n < G; ++n) {
-          x[j] = __builtin_fmaf(half_of(ks[n][j / 2], j % 2), s[j / 4][n][j % 4],
-                                __builtin_fmaf(half_of(ko[n][j / 2], j % 2), q_sum[n], x[j]));
+      for (int n = 0; n < G; ++n) {
+        if (!FULL && n >= k_groups) { break; }
+        uint32_t scales[4], offsets[4];
+        read_words<4, 4>(scales, mine + 128 * k_chunks + n * 32);
+        read_words<4, 4>(offsets, mine + 128 * k_chunks + n * 32 + 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float scale = half_of(scales[j / 2], j % 2), sum = s[j / 4][n][j % 4];
+          x[j] = __builtin_fmaf(scale, FINE ? __builtin_fmaf(8.0f, q_sum[n], sum) : sum,
+                                __builtin_fmaf(half_of(offsets[j / 2], j % 2), q_sum[n], x[j]));
         }
-        x[j] = __builtin_amdgcn_ldexpf(x[j], exponent);
       }
-      // the next step's keys
-      if (next < stop) {
-        k_next = entry(next + r / 4);
-        v_next = entry(next + g);
-        load_keys(k_next, v_next);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { x[j] = __builtin_amdgcn_ldexpf(x[j], exponent); }
+      uint32_t vs[G][4], vo[G][4];
+#pragma unroll
+      for (int n = 0; n < G; ++n) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) { vs[n][w] = vo[n][w] = 0; }
+        if (FULL || n < v_groups) {
+          read_words<4, 4>(vs[n], values + 128 * v_chunks + n * 32);
+          read_words<4, 4>(vo[n], values + 128 * v_chunks + n * 32 + 16);
+        }
       }
       const uint32_t t = uint32_t(group + g) * 8;  // past the end it may pass 2^31
       const uint32_t t_begin = uint32_t(sp.begin), t_end = uint32_t(sp.end);
@@ -381,43 +453,62 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
       for (int j = 0; j < 8; j += 4) { total += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]); }
 #pragma unroll
       for (int n = 0; n < G; ++n) {
+        if (!FULL && n >= v_groups) { break; }
         // p s of the group in the order of the codes' words (0, 2), (1, 3), (4, 6), (5, 7), as two elements each
         u32x4 part[2];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int j = w / 2 * 4 + w % 2;
-          float lo = p[j] * half_of(vs[n][j / 2], j % 2), hi = p[j + 2] * half_of(vs[n][j / 2 + 1], j % 2);
-          const auto whole = __builtin_amdgcn_cvt_pkrtz(lo, hi);
-          lo -= float(whole[0]);
-          hi -= float(whole[1]);
-          part[0][w] = __builtin_bit_cast(uint32_t, whole);
+          float lo = __builtin_fmaf(p[j], half_of(vs[n][j / 2], j % 2), 0.0f);
+          float hi = __builtin_fmaf(p[j + 2], half_of(vs[n][j / 2 + 1], j % 2), 0.0f);
+          // offsets of codes that are less 8
+          if (FINE) { shift[n] = __builtin_fmaf(8.0f, hi, __builtin_fmaf(8.0f, lo, shift[n])); }
+          shift[n] = __builtin_fmaf(p[j], half_of(vo[n][j / 2], j % 2), shift[n]);
+          shift[n] = __builtin_fmaf(p[j + 2], half_of(vo[n][j / 2 + 1], j % 2), shift[n]);
+          const f16x2 near{f16_t(lo), f16_t(hi)};
+          lo         = __builtin_fmaf(float(near[0]), -1.0f, lo);
+          hi         = __builtin_fmaf(float(near[1]), -1.0f, hi);
+          part[0][w] = __builtin_bit_cast(uint32_t, near);
           part[1][w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { shift[n] = __builtin_fmaf(p[j], half_of(vo[n][j / 2], j % 2), shift[n]); }
+        uint32_t v[4] = {0, 0, 0, 0};
+        const bool pair = 2 * n + 1 < C && (FULL || 2 * n + 1 < v_chunks);  // a unit of 64 dimensions, else of 32
+        if (pair) {
+          read_words<4, 4>(v, values + n * 256 + r * 16);
+        } else {
+          read_words<2, 2>(v, values + n * 256 + r * 8);
+        }
 #pragma unroll
         for (int c = 2 * n; c < 2 * n + 2 && c < C; ++c) {
-          const uint32_t w0 = v[n][c % 2 * 2], w1 = v[n][c % 2 * 2 + 1], up0 = w0 >> 8, up1 = w1 >> 8;
-          const u32x4 even{w0 & 0x000f000fu, up0 & 0x000f000fu, w1 & 0x000f000fu, up1 & 0x000f000fu};
-          const u32x4 odd{w0 & 0x00f000f0u, up0 & 0x00f000f0u, w1 & 0x00f000f0u, up1 & 0x00f000f0u};
+          const uint32_t w0 = v[c % 2 * 2], w1 = v[c % 2 * 2 + 1], up0 = w0 >> 8, up1 = w1 >> 8;
+          u32x4 even{w0 & 0x000f000fu, up0 & 0x000f000fu, w1 & 0x000f000fu, up1 & 0x000f000fu};
+          u32x4 odd{w0 & 0x00f000f0u, up0 & 0x00f000f0u, w1 & 0x00f000f0u, up1 & 0x00f000f0u};
+          if (FINE) {
+            even = {less_eight(w0), less_eight(up0), less_eight(w1), less_eight(up1)};
+            odd  = {less_eight(w0 >> 4), less_eight(w0 >> 12), less_eight(w1 >> 4), less_eight(w1 >> 12)};
+            const f32x4 zero{0, 0, 0, 0};
+            o[c][0] += mfma(f16_t{}, even, part[0], mfma(f16_t{}, even, part[1], zero));
+            o[c][1] += mfma(f16_t{}, odd, part[0], mfma(f16_t{}, odd, part[1], zero));
+          } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            o[c][0] = mfma(f16_t{}, even, part[i], o[c][0]);
-            o[c][1] = mfma(f16_t{}, odd, part[i], o[c][1]);
+            for (int i = 1; i >= 0; --i) {
+              o[c][0] = mfma(f16_t{}, even, part[i], o[c][0]);
+              o[c][1] = mfma(f16_t{}, odd, part[i], o[c][1]);
+            }
           }
         }
       }
-      if (next < stop) { load_values(v_next); }
-      group = next;
+      group  = next;
+      buffer = 1 - buffer;
     }
 
-    // join the waves, while the next sequence's first loads are in flight
+    // join the waves; their outputs take the place of their steps
     const auto plus = [](float u, float w) { return u + w; };
     total = __builtin_amdgcn_ldexpf(lanes::fold16(lanes::fold32(total, plus), plus), -lift);
 #pragma unroll
     for (int n = 0; n < G; ++n) { shift[n] = __builtin_amdgcn_ldexpf(lanes::fold16(lanes::fold32(shift[n], plus), plus), -lift); }
-    __syncthreads();
     if (r < rows) {
+      float* out = reinterpret_cast<float*>(&s_steps[wave][0][0]);
       if (g == 0) {
         s_max[wave][r] = top;
         s_sum[wave][r] = total;
@@ -432,7 +523,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
           for (int i = 0; i < 4; ++i) {
             const int row = g * 4 + i, col = unit * 64 + (pair ? row * 4 + c % 2 * 2 : row * 2) + e;
             if ((pair || c % 2 == 0) && col < vdim) {
-              s_out[wave][r][col] = __builtin_amdgcn_ldexpf(o[c][e][i], 24 - 4 * e - lift) + shift[unit];
+              out[r * D + col] = __builtin_amdgcn_ldexpf(o[c][e][i], (FINE ? 0 : 24 - 4 * e) - lift) + shift[unit];
             }
           }
         }
@@ -446,7 +537,6 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
       before += sp.tiles;
       ++b;
     }
-    if (more) { begin(); }
     __syncthreads();
     const int64_t slot = (int64_t(table) * plan.shares + share) * 2 + (first ? 0 : 1);
     for (int at = tid; at < rows * vdim; at += kThreads) {
@@ -459,7 +549,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
       for (int w = 0; w < kWaves; ++w) {
         const float f = factor_of(plan.scale, s_max[w][row], m);
         sum += f * s_sum[w][row];
-        acc += f * s_out[w][row][col];
+        acc += f * reinterpret_cast<const float*>(&s_steps[w][0][0])[row * D + col];
       }
       if (done) {
         put((out0 + row) * vdim + col, sum == 0.0f ? 0.0f : acc / sum);
@@ -473,21 +563,24 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<C>)) void packed_kernel(packed_
       }
     }
     if (!more) { break; }
+    __syncthreads();
+    begin();
   }
 }
 
-int per_unit_of(packed_args const& args)
+int per_unit_of(elem type, attend_args const& a)
 {
-  return packed_chunks(std::max(args.a.dim, args.a.vdim)) <= 4 ? kPerUnit<4> : kPerUnit<8>;
+  const int chunks = packed_chunks(std::max(a.dim, a.vdim));
+  return per_unit(chunks, a.dim == 32 * chunks && a.vdim == 32 * chunks, type == elem::f32 ? 3 : 1);
 }
 
 }  // namespace
 
-size_t packed_workspace(packed_args const& args)
+size_t packed_workspace(elem type, packed_args const& args)
 {
   attend_args const& a = args.a;
   if (longest_of(a) <= kTile) { return 0; }  // nothing to cut
-  const size_t slots = size_t(2) * a.kv_heads * row_tiles_of(a) * shares_for(a, kTile, per_unit_of(args));
+  const size_t slots = size_t(2) * a.kv_heads * row_tiles_of(a) * shares_for(a, kTile, per_unit_of(type, a));
   return sizeof(float) * slots * kRows * (a.vdim + 2);
 }
 
@@ -504,7 +597,7 @@ void packed_attend(elem type, packed_args const& args, hipStream_t stream)
     plan.scale          = scale_of(a.shape.any() ? 1.0f : a.scale);
     plan.lift           = 0.0f;
     plan.slack          = float(std::min(double(kSlack) / double(plan.scale.scale2), double(FLT_MAX)));
-    plan.shares         = shares_for(a, kTile, kPerUnit<C>);
+    plan.shares         = shares_for(a, kTile, per_unit_of(type, a));
     plan.halve          = 0;
     const int64_t slots = int64_t(2) * plan.tables * plan.shares * kRows;
     plan.part_out       = static_cast<float*>(a.workspace);

@@ -149,7 +149,7 @@ class PackedPages:
         out = pages.attend(q, table, lengths)
 
     Of every 64 consecutive elements x of a key or value (the last ones of a head fewer): an offset o, the float16 nearest to their
-    minimum, a scale s, the float16 nearest to the float32 quotient (maximum - o) / 15, and codes round((x - o) / s) in
+    minimum, a scale s, the float16 nearest to the float32 product (maximum - o) * float32(1 / 15), and codes round((x - o) / s) in
     0..15 (half to even; all 0 where s is 0), which stand for o + s code. o and s are cut to float16's finite range; NaN makes its 64 elements
     NaN. Page tables, positions and lengths are those of append_pages and paged_attention, pages of a multiple of 8 positions.
 

@@ -2,7 +2,7 @@
 
 import torch
 
-GROUP, MOST = 64, 65504.0
+GROUP, MOST, FIFTEENTH = 64, 65504.0, torch.tensor(1 / 15, dtype=torch.float32)
 
 
 def quantise(x):
@@ -12,7 +12,7 @@ def quantise(x):
     for at in range(0, x.shape[-1], GROUP):
         part = x[..., at : at + GROUP]
         low = part.float().amin(-1, keepdim=True).clamp(-MOST, MOST).half()
-        step = ((part.float().amax(-1, keepdim=True) - low.float()) / 15).clamp(0, MOST).half()
+        step = ((part.float().amax(-1, keepdim=True) - low.float()) * FIFTEENTH).clamp(0, MOST).half()
         o, s = low.double(), step.double()
         c = torch.where(s > 0, ((part.double() - o) / torch.where(s > 0, s, 1.0)).round().clamp(0, 15), 0.0)
         nan = part.isnan().any(-1, keepdim=True)
