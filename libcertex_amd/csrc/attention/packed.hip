@@ -53,19 +53,6 @@ constexpr int kBuffers = 2;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(4))) int32_t* constant_ints;
 
-/** A value that all lanes have, in scalar registers. */
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x)
-{
-  const uint32_t lo = uint32_t(uniform(int(x))), hi = uint32_t(uniform(int(x >> 32)));
-  return int64_t(uint64_t(hi) << 32 | lo);
-}
-template <typename T>
-__device__ __forceinline__ const T* uniform(const T* p)
-{
-  return reinterpret_cast<const T*>(uniform(int64_t(reinterpret_cast<uintptr_t>(p))));
-}
-
 /** 16 bytes a lane from base + offset to LDS byte m0 + 16 lane. In assembly, so that the compiler does not order LDS reads
  *  against it: the copies of a step go to a buffer that its wave has read, and landed() comes before they are. */
 __device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t m0)

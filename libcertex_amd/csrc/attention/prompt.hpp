@@ -48,6 +48,7 @@ struct prompt_plan {
   divisor group;        // query heads per key head
   int32_t tiles;        // of rows, at most, over all sequences
   int32_t splits;       // of a tile's positions, at most
+  bool near;            // rows of a tile are within 2^30 elements
   score_scale scale;
   float slack;          // kSlack in scores
   float* part_out;      // [tiles][kv_heads][splits][kRows][vdim]
@@ -102,8 +103,9 @@ __device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan cons
   const int64_t i0 = plan.group(uint32_t(row0)), i1 = plan.group(uint32_t(min(rows, int64_t(row0) + kRows) - 1));
   const int64_t end   = max(min(past + i1 + 1, length), prefix);
   const int64_t begin = a.window > 0 ? max(int64_t(0), past + i0 + 1 - a.window) & ~int64_t(7) : 0;
-  *out = {int32_t(lo),     row0,           int32_t(rows), t0, int32_t(past), int32_t(length), int32_t(prefix),
-          int32_t(begin), int32_t(end > begin ? (end - begin + TILE - 1) / TILE : 0)};
+  *out = {uniform(int(lo)),     uniform(row0),        uniform(int(rows)),   uniform(t0),
+          uniform(int(past)),   uniform(int(length)), uniform(int(prefix)), uniform(int(begin)),
+          uniform(int(end > begin ? (end - begin + TILE - 1) / TILE : 0))};
   return true;
 }
 
@@ -137,17 +139,17 @@ struct words {
   uint32_t w[N * sizeof(T) / 4];
 };
 
-/** Elements [off, off + N) of a row of n; what is past its end is 0. */
+/** Elements [off, off + N) of a row of n, which are at from[at]; what is past its end is 0. */
 template <bool FULL, int N, typename T>
-__device__ __forceinline__ words<T, N> row_piece(const T* row, int off, int n)
+__device__ __forceinline__ words<T, N> row_piece(const T* from, uint32_t at, int off, int n)
 {
   words<T, N> v{};
   if (FULL || off + N <= n) {
-    __builtin_memcpy(&v, __builtin_assume_aligned(row + off, sizeof(T)), sizeof(v));
+    __builtin_memcpy(&v, __builtin_assume_aligned(from + at, sizeof(T)), sizeof(v));
   } else if (off < n) {
     T e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) { e[i] = off + i < n ? row[off + i] : T(0.0f); }
+    for (int i = 0; i < N; ++i) { e[i] = off + i < n ? from[at + i] : T(0.0f); }
     __builtin_memcpy(&v, e, sizeof(v));
   }
   return v;
@@ -192,7 +194,7 @@ constexpr int kTile = 128 / sizeof(T);
 
 /** Workgroups per compute unit, by registers and LDS. */
 template <typename T, int D>
-constexpr int kPerUnit = sizeof(T) == 2 && D <= 128 ? 2 : 1;
+constexpr int kPerUnit = D <= 128 ? 2 : 1;
 
 constexpr int power_of_two(int n) { return n <= 1 ? 1 : 2 * power_of_two((n + 1) / 2); }
 
@@ -255,7 +257,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     const uint32_t flip = plan.scale.sign < 0.0f ? (WIDE ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const auto v = row_piece<FULL, kPiece>(from, (c * 2 + half) * kPiece, dim);
+      const uint32_t off = (c * 2 + half) * kPiece;
+      const auto v       = row_piece<FULL, kPiece>(from, off, off, dim);
 #pragma unroll
       for (int w = 0; w < 4; ++w) { q[c][w] = exists ? v.w[w] ^ flip : 0u; }
     }
@@ -289,19 +292,41 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 
   words<T, kPiece> k_next[kPasses];
   words<T, kTurn> v_next[kSlot];
+  // tiles that lie in one page each, with rows near each other: one place, and 32-bit offsets of the lanes
+  const bool in_page     = plan.near && plan.page_groups.d % kGroups == 0 && rt.begin % TILE == 0;
+  const uint32_t k_lane  = uint32_t(tid / kAcross) * uint32_t(a.k_slot) + k_piece * kPiece;
+  const uint32_t v_lane  = (4 * half) * uint32_t(a.v_slot) + v_col;
   const auto load_tile = [&](places const& at) {
+    if (in_page) {
+      const int page = uniform(at.page), slot = uniform(at.slot);
+      const T* k_from = k_head + page * a.k_page + slot * a.k_slot;
+      const T* v_from = v_head + page * a.v_page + (slot + wave * (2 * kSlot)) * a.v_slot;
+#pragma unroll
+      for (int n = 0; n < kPasses; ++n) {
+        if (kPieces == kAcross || k_piece < kPieces) {
+          k_next[n] = row_piece<FULL, kPiece>(k_from + n * kDown * a.k_slot, k_lane, k_piece * kPiece, dim);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kSlot; ++j) {
+        if (D % (32 * kTurn) == 0 || v_col < D) {
+          v_next[j] = row_piece<FULL, kTurn>(v_from + (j / 4 * 8 + j % 4) * a.v_slot, v_lane, v_col, vdim);
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < kPasses; ++n) {
       // a wave's rows of a pass are in one group
       const int first = n * kDown + wave * (kDown / kWaves), r = n * kDown + tid / kAcross;
       const T* from   = address(k_head, a.k_page, a.k_slot, at, first / 8) + int64_t(r % 8) * a.k_slot;
-      if (kPieces == kAcross || k_piece < kPieces) { k_next[n] = row_piece<FULL, kPiece>(from, k_piece * kPiece, dim); }
+      if (kPieces == kAcross || k_piece < kPieces) { k_next[n] = row_piece<FULL, kPiece>(from, k_piece * kPiece, k_piece * kPiece, dim); }
     }
 #pragma unroll
     for (int j = 0; j < kSlot; ++j) {
       const int g   = WIDE ? wave : 2 * wave + j / 4;
       const T* from = address(v_head, a.v_page, a.v_slot, at, g) + int64_t(4 * half + j % 4) * a.v_slot;
-      if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from, v_col, vdim); }
+      if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from, v_col, v_col, vdim); }
     }
   };
   /** Into LDS: keys as they lie, V turned. At an edge values that no row sees are 0 and unbounded ones are left out; true
@@ -393,12 +418,40 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           }
         }
         if constexpr (BENT) {
+          // less base, which is the last operation's other term
+          const float ahead_of = float(p - t0 - 4 * half);
+          if (a.shape.cap != 0.0f) {
+            const float whole = a.shape.cap - base, twice = -2.0f * a.shape.cap;
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
+            for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int t = t0 + b * 32 + 8 * (e / 4) + 4 * half + e % 4;
-              s[b][e]     = bent(s[b][e], a.scale, per_cap, a.shape.cap, slope, __builtin_fabsf(float(p - t))) - base;
+              for (int e = 0; e < 16; ++e) {
+                if constexpr (WIDE) {
+                  s[b][e] = __builtin_fmaf(a.shape.cap, tanh_of(s[b][e] * per_cap), -base);
+                } else {
+                  // cap (1 - 2 / (e^(2u) + 1)): off by 2^-23 cap, which the rounded weights hide
+                  const float e2u = __builtin_amdgcn_exp2f(s[b][e] * (per_cap * (2.0f * kLog2e)));
+                  s[b][e]         = __builtin_fmaf(twice, __builtin_amdgcn_rcpf(e2u + 1.0f), whole);
+                }
+              }
+            }
+            if (a.shape.slopes != nullptr) {
+#pragma unroll
+              for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  s[b][e] = __builtin_fmaf(-slope, __builtin_fabsf(ahead_of - float(b * 32 + 8 * (e / 4) + e % 4)), s[b][e]);
+                }
+              }
+            }
+          } else {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float lean = __builtin_fabsf(ahead_of - float(b * 32 + 8 * (e / 4) + e % 4));
+                s[b][e]          = __builtin_fmaf(s[b][e], a.scale, __builtin_fmaf(-slope, lean, -base));
+              }
             }
           }
         }
@@ -440,12 +493,19 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           base  = grown;
           limit = set ? (plan.scale.scale2 == 0.0f ? INFINITY : plan.slack) : limit;
         }
+        if (masked && plan.scale.scale2 == 0.0f) {  // -inf times 0
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { s[b][e] = s[b][e] == -INFINITY ? -INFINITY : s[b][e] * 0.0f; }
+          }
+        }
+        const float scale2 = masked && plan.scale.scale2 == 0.0f ? 1.0f : plan.scale.scale2;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], plan.scale.scale2, kLift<T>));
-            s[b][e]       = masked && s[b][e] == -INFINITY ? 0.0f : w;
+            s[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], scale2, kLift<T>));
           }
         }
 #pragma unroll
@@ -593,6 +653,7 @@ void launch(prompt_args const& a, hipStream_t stream)
     prompt_plan plan{divisor(uint32_t(a.pages.page / 8)), divisor(uint32_t(a.heads / a.kv_heads))};
     plan.tiles  = int32_t(tiles_of(a));
     plan.splits = splits_for(a, kTile<T>, kPerUnit<T, D>);
+    plan.near   = std::max(a.k_slot, a.v_slot) < (int64_t(1) << 30) / kTile<T>;
     plan.scale  = scale_of(a.shape.any() ? 1.0f : a.scale);
     plan.slack  = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
     const int64_t slots = int64_t(plan.tiles) * a.kv_heads * plan.splits * kRows;

@@ -11,6 +11,19 @@ using u32x2  = __attribute__((ext_vector_type(2))) uint32_t;
 using f16x8  = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
+/** A value that all lanes have, in scalar registers. */
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x)
+{
+  const uint32_t lo = uint32_t(uniform(int(x))), hi = uint32_t(uniform(int(x >> 32)));
+  return int64_t(uint64_t(hi) << 32 | lo);
+}
+template <typename T>
+__device__ __forceinline__ const T* uniform(const T* p)
+{
+  return reinterpret_cast<const T*>(uniform(int64_t(reinterpret_cast<uintptr_t>(p))));
+}
+
 /** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less
  *  than 1, so n m / 2^(29 + s) exceeds n / d by less than 1 / d. */
 struct divisor {
@@ -37,10 +50,9 @@ __device__ __forceinline__ f32x4 mfma(bf16_t, u32x4 a, u32x4 b, f32x4 c)
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 {
-  const T v[2] = {T(lo), T(hi)};
-  uint32_t w;
-  __builtin_memcpy(&w, v, 4);
-  return w;
+  using two = __attribute__((ext_vector_type(2))) T;
+  using f32x2 = __attribute__((ext_vector_type(2))) float;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), two));
 }
 
 }  // namespace certex_amd::attention
