@@ -50,15 +50,7 @@ constexpr int kRecord = 256 * C + 64 * ((C + 1) / 2);
 /** A wave's steps in LDS: one that is worked on, one that is on its way. */
 constexpr int kBuffers = 2;
 
-typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(4))) int32_t* constant_ints;
-
-/** 16 bytes a lane from base + offset to LDS byte m0 + 16 lane. In assembly, so that the compiler does not order LDS reads
- *  against it: the copies of a step go to a buffer that its wave has read, and landed() comes before they are. */
-__device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t m0)
-{
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(uniform(base)), "s"(m0) : "m0", "memory");
-}
 
 /** Waits until at most n of this wave's copies are on their way (n as they are issued: 0, or those of one step). */
 __device__ __forceinline__ void landed(int n)
@@ -220,7 +212,7 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
   };
   /** The copies of a step, and how many they are. */
   const auto copy = [&](place const& at, int buffer) {
-    const uint32_t to = uint32_t(reinterpret_cast<uintptr_t>((lds_ptr)&s_steps[wave][buffer][0]));
+    const uint32_t to = lds_address(&s_steps[wave][buffer][0]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read there has arrived
     int n = 0;
     if (follow) {

@@ -48,7 +48,6 @@ struct prompt_plan {
   divisor group;        // query heads per key head
   int32_t tiles;        // of rows, at most, over all sequences
   int32_t splits;       // of a tile's positions, at most
-  bool near;            // rows of a tile are within 2^30 elements
   score_scale scale;
   float slack;          // kSlack in scores
   float* part_out;      // [tiles][kv_heads][splits][kRows][vdim]
@@ -139,17 +138,17 @@ struct words {
   uint32_t w[N * sizeof(T) / 4];
 };
 
-/** Elements [off, off + N) of a row of n, which are at from[at]; what is past its end is 0. */
+/** Elements [off, off + N) of a row of n, which begin at `from`; what is past its end is 0. */
 template <bool FULL, int N, typename T>
-__device__ __forceinline__ words<T, N> row_piece(const T* from, uint32_t at, int off, int n)
+__device__ __forceinline__ words<T, N> row_piece(const T* from, int off, int n)
 {
   words<T, N> v{};
   if (FULL || off + N <= n) {
-    __builtin_memcpy(&v, __builtin_assume_aligned(from + at, sizeof(T)), sizeof(v));
+    __builtin_memcpy(&v, __builtin_assume_aligned(from, sizeof(T)), sizeof(v));
   } else if (off < n) {
     T e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) { e[i] = off + i < n ? from[at + i] : T(0.0f); }
+    for (int i = 0; i < N; ++i) { e[i] = off + i < n ? from[i] : T(0.0f); }
     __builtin_memcpy(&v, e, sizeof(v));
   }
   return v;
@@ -208,9 +207,11 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   constexpr int kBlocks = TILE / 32;            // products along the positions
   constexpr int kCols   = D / 32;               // products along the columns of V
   constexpr int kGroups = TILE / 8;             // groups of 8 positions, which lie in one page
-  constexpr int kRowBytes = D * sizeof(T) + 16; // of a key row in LDS: rows begin in other banks
   // threads of a key row, rows at a time
   constexpr int kPieces = D / kPiece, kAcross = power_of_two(kPieces), kDown = kThreads / kAcross, kPasses = TILE / kDown;
+  // Key rows in LDS. FULL: copied there as the lanes are, 16 bytes each; a row's pieces are exchanged by its number, so that
+  // 8 rows' same pieces are in 8 places. Else stored from registers, 16 bytes apart.
+  constexpr int kRowBytes = FULL ? kAcross * 16 : D * sizeof(T) + 16;
   // columns of a thread in V's turn, the positions of its slot
   constexpr int kTurn = std::max(power_of_two(D / 32), 2), kSlot = kPiece;
   __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TILE * kRowBytes];
@@ -257,8 +258,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     const uint32_t flip = plan.scale.sign < 0.0f ? (WIDE ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const uint32_t off = (c * 2 + half) * kPiece;
-      const auto v       = row_piece<FULL, kPiece>(from, off, off, dim);
+      const int off = (c * 2 + half) * kPiece;
+      const auto v  = row_piece<FULL, kPiece>(from + off, off, dim);
 #pragma unroll
       for (int w = 0; w < 4; ++w) { q[c][w] = exists ? v.w[w] ^ flip : 0u; }
     }
@@ -266,67 +267,59 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   const float slope   = BENT && a.shape.slopes != nullptr ? a.shape.slopes[head] : 0.0f;
   const float per_cap = BENT && a.shape.cap != 0.0f ? a.scale / a.shape.cap : 0.0f;
 
-  // the pages of a tile's groups: lane l has group l % kGroups
+  // where the groups of a tile begin in the pools: lane l has group l % kGroups
   struct places {
-    int32_t page, slot;
+    const T *k, *v;
     uint32_t there;  // bit per group: the sequence has its page
   };
+  const T* k_head      = static_cast<const T*>(a.k) + kv * a.k_head;
+  const T* v_head      = static_cast<const T*>(a.v) + kv * a.v_head;
   const int32_t* table = a.pages.table + int64_t(rt.sequence) * a.pages.width;
   const int final      = max(0, rt.length - 1) / 8;
   const auto look_up   = [&](int tile) {
     const int g = min(rt.begin / 8 + tile * kGroups + lane % kGroups, final);
     const int e = int(plan.page_groups(uint32_t(g)));
-    const int32_t page = table[e];
-    const bool there   = uint32_t(page) < uint32_t(a.pages.n_pages);
-    return places{there ? page : 0, (g - e * int(plan.page_groups.d)) * 8,
+    const int32_t found = table[e];
+    const bool there    = uint32_t(found) < uint32_t(a.pages.n_pages);
+    const int64_t page = there ? found : 0, slot = (g - e * int(plan.page_groups.d)) * 8;
+    return places{k_head + page * a.k_page + slot * a.k_slot, v_head + page * a.v_page + slot * a.v_slot,
                   uint32_t(__ballot(there)) & ((1u << kGroups) - 1u)};
   };
-  const auto address = [&](const T* base, int64_t page_stride, int64_t slot_stride, places const& at, int g) {
-    const int page = __builtin_amdgcn_readlane(at.page, g), slot = __builtin_amdgcn_readlane(at.slot, g);
-    return base + page * page_stride + slot * slot_stride;
+  const auto of_group = [](const T* p, int g) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readlane(int(at), g), hi = __builtin_amdgcn_readlane(int(at >> 32), g);
+    return reinterpret_cast<const T*>(uint64_t(hi) << 32 | lo);
   };
-  const T* k_head = static_cast<const T*>(a.k) + kv * a.k_head;
-  const T* v_head = static_cast<const T*>(a.v) + kv * a.v_head;
   const int k_piece = tid % kAcross;
   const int v_col   = column * kTurn;
+  // rows of a thread within a group
+  constexpr int kStep  = std::min(8, kDown);
+  // (rows of a thread are 8 apart, or 4: then the second is exchanged otherwise)
+  const int64_t k_lane = int64_t(tid / kAcross % kStep) * a.k_slot;
+  const auto piece_of  = [&](int n) { return FULL ? k_piece ^ ((n * kDown + tid / kAcross) % 8) : k_piece; };
+  const int64_t v_lane = 4 * half * a.v_slot + v_col;
 
-  words<T, kPiece> k_next[kPasses];
+  words<T, kPiece> k_next[FULL ? 1 : kPasses];
   words<T, kTurn> v_next[kSlot];
-  // tiles that lie in one page each, with rows near each other: one place, and 32-bit offsets of the lanes
-  const bool in_page     = plan.near && plan.page_groups.d % kGroups == 0 && rt.begin % TILE == 0;
-  const uint32_t k_lane  = uint32_t(tid / kAcross) * uint32_t(a.k_slot) + k_piece * kPiece;
-  const uint32_t v_lane  = (4 * half) * uint32_t(a.v_slot) + v_col;
-  const auto load_tile = [&](places const& at) {
-    if (in_page) {
-      const int page = uniform(at.page), slot = uniform(at.slot);
-      const T* k_from = k_head + page * a.k_page + slot * a.k_slot;
-      const T* v_from = v_head + page * a.v_page + (slot + wave * (2 * kSlot)) * a.v_slot;
-#pragma unroll
-      for (int n = 0; n < kPasses; ++n) {
-        if (kPieces == kAcross || k_piece < kPieces) {
-          k_next[n] = row_piece<FULL, kPiece>(k_from + n * kDown * a.k_slot, k_lane, k_piece * kPiece, dim);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kSlot; ++j) {
-        if (D % (32 * kTurn) == 0 || v_col < D) {
-          v_next[j] = row_piece<FULL, kTurn>(v_from + (j / 4 * 8 + j % 4) * a.v_slot, v_lane, v_col, vdim);
-        }
-      }
-      return;
-    }
+  const auto load_tile = [&](places const& at, int buffer) {
 #pragma unroll
     for (int n = 0; n < kPasses; ++n) {
       // a wave's rows of a pass are in one group
-      const int first = n * kDown + wave * (kDown / kWaves), r = n * kDown + tid / kAcross;
-      const T* from   = address(k_head, a.k_page, a.k_slot, at, first / 8) + int64_t(r % 8) * a.k_slot;
-      if (kPieces == kAcross || k_piece < kPieces) { k_next[n] = row_piece<FULL, kPiece>(from, k_piece * kPiece, k_piece * kPiece, dim); }
+      const int first = n * kDown + wave * (kDown / kWaves);
+      const T* from   = of_group(at.k, first / 8) + int64_t(n * kDown % 8) * a.k_slot;
+      const int piece = piece_of(n);
+      if (kPieces == kAcross || piece < kPieces) {
+        if constexpr (FULL) {
+          copy_to_lds(from + k_lane + piece * kPiece, lds_address(&s_k[buffer][first * kRowBytes]));
+        } else {
+          k_next[n] = row_piece<FULL, kPiece>(from + k_lane + piece * kPiece, piece * kPiece, dim);
+        }
+      }
     }
 #pragma unroll
     for (int j = 0; j < kSlot; ++j) {
-      const int g   = WIDE ? wave : 2 * wave + j / 4;
-      const T* from = address(v_head, a.v_page, a.v_slot, at, g) + int64_t(4 * half + j % 4) * a.v_slot;
-      if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from, v_col, v_col, vdim); }
+      const T* from = of_group(at.v, WIDE ? wave : 2 * wave + j / 4) + int64_t(j % 4) * a.v_slot;
+      if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from + v_lane, v_col, vdim); }
     }
   };
   /** Into LDS: keys as they lie, V turned. At an edge values that no row sees are 0 and unbounded ones are left out; true
@@ -345,11 +338,13 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         }
       }
     }
+    if constexpr (!FULL) {
 #pragma unroll
-    for (int n = 0; n < kPasses; ++n) {
-      const int r = n * kDown + tid / kAcross;
-      if (kPieces == kAcross || k_piece < kPieces) {
-        *reinterpret_cast<u32x4*>(&s_k[buffer][r * kRowBytes + k_piece * 16]) = __builtin_bit_cast(u32x4, k_next[n]);
+      for (int n = 0; n < kPasses; ++n) {
+        const int r = n * kDown + tid / kAcross;
+        if (kPieces == kAcross || k_piece < kPieces) {
+          *reinterpret_cast<u32x4*>(&s_k[buffer][r * kRowBytes + k_piece * 16]) = __builtin_bit_cast(u32x4, k_next[n]);
+        }
       }
     }
     if (D % (32 * kTurn) == 0 || v_col < D) {
@@ -369,6 +364,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         *reinterpret_cast<u32x4*>(&s_v[buffer][col * 128 + slot * 16]) = t;
       }
     }
+    if constexpr (FULL) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }  // the keys' copies
     return unbounded;
   };
   // whether some row does not see all of a tile
@@ -388,7 +384,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 
   if (tile0 < tile1) {
     places here = look_up(tile0), next = tile0 + 1 < tile1 ? look_up(tile0 + 1) : here;
-    load_tile(here);
+    load_tile(here, 0);
     bool edge      = at_edge(tile0, here);
     bool unbounded = store_tile(0, tile0, here, edge);
     unbounded      = edge ? __syncthreads_or(unbounded) != 0 : (__syncthreads(), false);
@@ -397,7 +393,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
       const bool more  = tile + 1 < tile1;
       places ahead     = next;
       if (more) {
-        load_tile(next);
+        load_tile(next, 1 - buffer);
         if (tile + 2 < tile1) { ahead = look_up(tile + 2); }
       }
       const int t0    = rt.begin + tile * TILE;
@@ -413,7 +409,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(&s_k[buffer][(b * 32 + column) * kRowBytes + (c * 2 + half) * 16]);
+            const int piece = FULL ? (c * 2 + half) ^ (column % 8) : c * 2 + half;
+            const u32x4 k   = *reinterpret_cast<const u32x4*>(&s_k[buffer][(b * 32 + column) * kRowBytes + piece * 16]);
             s[b]          = mfma32(T{}, k, q[c], s[b]);
           }
         }
@@ -537,7 +534,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           for (int j = 0; j < TILE; ++j) {
             const int t = t0 + j, g = j / 8;
             if (t >= rt.length || (here.there >> g & 1u) == 0) { continue; }
-            const T* from = address(v_head, a.v_page, a.v_slot, here, g) + int64_t(j % 8) * a.v_slot;
+            const T* from = of_group(here.v, g) + int64_t(j % 8) * a.v_slot;
             const bool in = t >= lo && t < hi;
 #pragma unroll
             for (int n = 0; n < kCols; ++n) {
@@ -653,7 +650,6 @@ void launch(prompt_args const& a, hipStream_t stream)
     prompt_plan plan{divisor(uint32_t(a.pages.page / 8)), divisor(uint32_t(a.heads / a.kv_heads))};
     plan.tiles  = int32_t(tiles_of(a));
     plan.splits = splits_for(a, kTile<T>, kPerUnit<T, D>);
-    plan.near   = std::max(a.k_slot, a.v_slot) < (int64_t(1) << 30) / kTile<T>;
     plan.scale  = scale_of(a.shape.any() ? 1.0f : a.scale);
     plan.slack  = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
     const int64_t slots = int64_t(plan.tiles) * a.kv_heads * plan.splits * kRows;
@@ -670,9 +666,12 @@ void launch(prompt_args const& a, hipStream_t stream)
       join_kernel<T><<<dim3(uint32_t(plan.tiles) * a.kv_heads, kRows * 32 / kThreads), kThreads, 0, stream>>>(a, plan);
     }
   };
+  // key rows at multiples of 16 bytes are copied to LDS as they lie
+  const bool aligned = reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && (a.k_page * sizeof(T)) % 16 == 0 &&
+                       (a.k_slot * sizeof(T)) % 16 == 0 && (a.k_head * sizeof(T)) % 16 == 0;
   const auto bucket = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    a.dim == D && a.vdim == D ? launched(d, std::true_type{}) : launched(d, std::false_type{});
+    a.dim == D && a.vdim == D && aligned ? launched(d, std::true_type{}) : launched(d, std::false_type{});
   };
   const int dim = std::max(a.dim, a.vdim);
   if (dim <= 64) {

@@ -24,6 +24,26 @@ __device__ __forceinline__ const T* uniform(const T* p)
   return reinterpret_cast<const T*>(uniform(int64_t(reinterpret_cast<uintptr_t>(p))));
 }
 
+/** The LDS byte address of p. */
+__device__ __forceinline__ uint32_t lds_address(const void* p)
+{
+  return uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(const_cast<void*>(p))));
+}
+
+/** 16 bytes a lane from base + offset to LDS byte m0 + 16 lane. In assembly, so that the compiler does not order LDS reads
+ *  against it: the kernels see to it that what is copied over has been read, and wait for vmcnt before they read the copy.
+ *  (It is among the loads that the compiler's own waits pass over in order: those can only wait longer.) */
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t m0)
+{
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
+               "s"(uniform(static_cast<const char*>(base))), "s"(m0)
+               : "m0", "memory");
+}
+__device__ __forceinline__ void copy_to_lds(const void* from, uint32_t m0)
+{
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(m0) : "m0", "memory");
+}
+
 /** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less
  *  than 1, so n m / 2^(29 + s) exceeds n / d by less than 1 / d. */
 struct divisor {
