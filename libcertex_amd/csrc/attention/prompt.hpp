@@ -405,14 +405,23 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 #pragma unroll
           for (int e = 0; e < 16; ++e) { s[b][e] = BENT ? 0.0f : -base; }
         }
+        // operands are read one product ahead, and no further: registers are what is short
+        const auto key_at = [&](int c, int b) {
+          const int piece = FULL ? (c * 2 + half) ^ (column % 8) : c * 2 + half;
+          return *reinterpret_cast<const u32x4*>(&s_k[buffer][(b * 32 + column) * kRowBytes + piece * 16]);
+        };
+        u32x4 k[2][kBlocks];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) { k[0][b] = key_at(0, b); }
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) {
-            const int piece = FULL ? (c * 2 + half) ^ (column % 8) : c * 2 + half;
-            const u32x4 k   = *reinterpret_cast<const u32x4*>(&s_k[buffer][(b * 32 + column) * kRowBytes + piece * 16]);
-            s[b]          = mfma32(T{}, k, q[c], s[b]);
+            if (c + 1 < kChunks) { k[(c + 1) % 2][b] = key_at(c + 1, b); }
           }
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) { s[b] = mfma32(T{}, k[c % 2][b], q[c], s[b]); }
+          __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (BENT) {
           // less base, which is the last operation's other term
@@ -511,6 +520,13 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           for (int e = 0; e < 16; e += 4) { total += (s[b][e] + s[b][e + 1]) + (s[b][e + 2] + s[b][e + 3]); }
         }
         constexpr int kSteps = TILE / (2 * kSlot);  // products along the positions, of a slot per half wave
+        const auto value_at  = [&](int m, int n) {
+          const int col = n * 32 + column, slot = (2 * m + half) ^ ((col / 4 + 2 * (col % 4)) % 8);
+          return *reinterpret_cast<const u32x4*>(&s_v[buffer][col * 128 + slot * 16]);
+        };
+        u32x4 v[2][kCols];
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) { v[0][n] = value_at(0, n); }
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
           u32x4 w;
@@ -524,10 +540,11 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           }
 #pragma unroll
           for (int n = 0; n < kCols; ++n) {
-            const int col = n * 32 + column, slot = (2 * m + half) ^ ((col / 4 + 2 * (col % 4)) % 8);
-            const u32x4 v = *reinterpret_cast<const u32x4*>(&s_v[buffer][col * 128 + slot * 16]);
-            o[n]          = mfma32(T{}, v, w, o[n]);
+            if (m + 1 < kSteps) { v[(m + 1) % 2][n] = value_at(m + 1, n); }
           }
+#pragma unroll
+          for (int n = 0; n < kCols; ++n) { o[n] = mfma32(T{}, v[m % 2][n], w, o[n]); }
+          __builtin_amdgcn_sched_barrier(0);
         }
         if (unbounded) {
           // values that are infinite or NaN show in the rows that see them, and in no other: each by itself
