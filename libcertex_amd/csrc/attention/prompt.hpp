@@ -393,8 +393,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
       const bool more  = tile + 1 < tile1;
       places ahead     = next;
       if (more) {
-        load_tile(next, 1 - buffer);
         if (tile + 2 < tile1) { ahead = look_up(tile + 2); }
+        load_tile(next, 1 - buffer);
       }
       const int t0    = rt.begin + tile * TILE;
       const bool some = t0 < hi && t0 + TILE > lo;
