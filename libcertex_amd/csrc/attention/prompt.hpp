@@ -48,6 +48,7 @@ struct prompt_plan {
   divisor group;        // query heads per key head
   int32_t tiles;        // of rows, at most, over all sequences
   int32_t splits;       // of a tile's positions, at most
+  bool near;            // strides of pages and of 8 slots fit 32 bits
   score_scale scale;
   float slack;          // kSlack in scores
   float* part_out;      // [tiles][kv_heads][splits][kRows][vdim]
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 
   // where the groups of a tile begin in the pools: lane l has group l % kGroups
   struct places {
-    const T *k, *v;
+    int64_t k, v;    // elements behind the head's first
     uint32_t there;  // bit per group: the sequence has its page
   };
   const T* k_head      = static_cast<const T*>(a.k) + kv * a.k_head;
@@ -281,14 +282,21 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     const int e = int(plan.page_groups(uint32_t(g)));
     const int32_t found = table[e];
     const bool there    = uint32_t(found) < uint32_t(a.pages.n_pages);
-    const int64_t page = there ? found : 0, slot = (g - e * int(plan.page_groups.d)) * 8;
-    return places{k_head + page * a.k_page + slot * a.k_slot, v_head + page * a.v_page + slot * a.v_slot,
-                  uint32_t(__ballot(there)) & ((1u << kGroups) - 1u)};
+    const uint32_t page = there ? found : 0, group = g - e * int(plan.page_groups.d);
+    places at;
+    if (plan.near) {
+      at.k = int64_t(uint64_t(page) * uint32_t(a.k_page) + uint64_t(group) * uint32_t(8 * a.k_slot));
+      at.v = int64_t(uint64_t(page) * uint32_t(a.v_page) + uint64_t(group) * uint32_t(8 * a.v_slot));
+    } else {
+      at.k = int64_t(page) * a.k_page + int64_t(group) * 8 * a.k_slot;
+      at.v = int64_t(page) * a.v_page + int64_t(group) * 8 * a.v_slot;
+    }
+    at.there = uint32_t(__ballot(there)) & ((1u << kGroups) - 1u);
+    return at;
   };
-  const auto of_group = [](const T* p, int g) {
-    const uint64_t at = reinterpret_cast<uintptr_t>(p);
+  const auto of_group = [](int64_t at, int g) {
     const uint32_t lo = __builtin_amdgcn_readlane(int(at), g), hi = __builtin_amdgcn_readlane(int(at >> 32), g);
-    return reinterpret_cast<const T*>(uint64_t(hi) << 32 | lo);
+    return int64_t(uint64_t(hi) << 32 | lo);
   };
   const int k_piece = tid % kAcross;
   const int v_col   = column * kTurn;
@@ -306,7 +314,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     for (int n = 0; n < kPasses; ++n) {
       // a wave's rows of a pass are in one group
       const int first = n * kDown + wave * (kDown / kWaves);
-      const T* from   = of_group(at.k, first / 8) + int64_t(n * kDown % 8) * a.k_slot;
+      const T* from   = k_head + of_group(at.k, first / 8) + int64_t(n * kDown % 8) * a.k_slot;
       const int piece = piece_of(n);
       if (kPieces == kAcross || piece < kPieces) {
         if constexpr (FULL) {
@@ -318,7 +326,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     }
 #pragma unroll
     for (int j = 0; j < kSlot; ++j) {
-      const T* from = of_group(at.v, WIDE ? wave : 2 * wave + j / 4) + int64_t(j % 4) * a.v_slot;
+      const T* from = v_head + of_group(at.v, WIDE ? wave : 2 * wave + j / 4) + int64_t(j % 4) * a.v_slot;
       if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from + v_lane, v_col, vdim); }
     }
   };
@@ -551,7 +559,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           for (int j = 0; j < TILE; ++j) {
             const int t = t0 + j, g = j / 8;
             if (t >= rt.length || (here.there >> g & 1u) == 0) { continue; }
-            const T* from = of_group(here.v, g) + int64_t(j % 8) * a.v_slot;
+            const T* from = v_head + of_group(here.v, g) + int64_t(j % 8) * a.v_slot;
             const bool in = t >= lo && t < hi;
 #pragma unroll
             for (int n = 0; n < kCols; ++n) {
@@ -667,6 +675,7 @@ void launch(prompt_args const& a, hipStream_t stream)
     prompt_plan plan{divisor(uint32_t(a.pages.page / 8)), divisor(uint32_t(a.heads / a.kv_heads))};
     plan.tiles  = int32_t(tiles_of(a));
     plan.splits = splits_for(a, kTile<T>, kPerUnit<T, D>);
+    plan.near   = std::max({a.k_page, a.v_page, 8 * a.k_slot, 8 * a.v_slot}) < (int64_t(1) << 32);
     plan.scale  = scale_of(a.shape.any() ? 1.0f : a.scale);
     plan.slack  = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
     const int64_t slots = int64_t(plan.tiles) * a.kv_heads * plan.splits * kRows;
