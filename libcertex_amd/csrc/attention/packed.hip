@@ -14,7 +14,11 @@
 // offsets are one piece of memory.
 // - Queries enter as float16, scaled by a power of two that brings a row's largest to [2^13, 2^14): 16-bit types whole
 //   (what is 2^-28 of the largest loses bits, none that float32 sums would keep), float32 as three elements of 11 bits.
-// - p_t s_t enters as two elements of 11 bits each, p's reference being kept such that the largest is below 2^15.
+// - p_t s_t enters as the nearest float16 where queries (and outputs) are of 16 bits, 2^-11 of it off at most, which
+//   is what float16 outputs are rounded by and an eighth of bfloat16's; as two elements of 11 bits for float32. p's reference is
+//   kept such that the largest is below 2^15. Their sum is not rounded.
+// - Products of subnormal numbers keep fewer of their low bits beside large sums, so that float32 takes other
+//   codes: less 8, as normal numbers (two operations more each), whose sums stay small; and joins steps outside the products.
 // Work is dealt as in attend.hip (shares.hpp).
 #include "scores.hpp"
 #include "shares.hpp"
@@ -26,6 +30,7 @@ namespace {
 constexpr int kTile = 32 * kWaves;  // positions of a workgroup's step
 
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
+using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
 
 /** The reference may lag the largest exponent by this much. */
 constexpr float kSlack = 1.0f;
@@ -389,14 +394,14 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
       float high = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) { high = fmaxf(high, x[j]); }
-      // the largest of the scales
-      f16x2 most = __builtin_bit_cast(f16x2, vs[0][0]);
+      // the largest of the scales, which are not negative: as whole numbers (NaN is the largest, and no steeper than any)
+      u16x2 most = __builtin_bit_cast(u16x2, vs[0][0]);
 #pragma unroll
       for (int n = 0; n < G; ++n) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) { most = __builtin_elementwise_max(most, __builtin_bit_cast(f16x2, vs[n][w])); }
+        for (int w = n == 0 ? 1 : 0; w < 4; ++w) { most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, vs[n][w])); }
       }
-      const float steep = fmaxf(float(most[0]), float(most[1]));
+      const float steep = fmaxf(half_of(__builtin_bit_cast(uint32_t, most), 0), half_of(__builtin_bit_cast(uint32_t, most), 1));
       if (__any(high > limit || steep >= scale_limit)) {
         const auto larger = [](float u, float w) { return fmaxf(u, w); };
         high              = lanes::fold16(lanes::fold32(high, larger), larger);
@@ -420,21 +425,24 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
         base = grown == -INFINITY || plan.scale.scale2 == 0.0f ? 0.0f : grown;
       }
       float p[8];
+      if (masked && plan.scale.scale2 == 0.0f) {  // what is masked is no number times 0
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - base, plan.scale.scale2, float(lift)));
-      }
-      if (masked) {
+        for (int j = 0; j < 8; ++j) {
+          p[j] = x[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - base, 0.0f, float(lift)));
+        }
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { p[j] = x[j] == -INFINITY ? 0.0f : p[j]; }
+        for (int j = 0; j < 8; ++j) {
+          p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j] - base, plan.scale.scale2, float(lift)));
+        }
       }
 #pragma unroll
       for (int j = 0; j < 8; j += 4) { total += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]); }
 #pragma unroll
       for (int n = 0; n < G; ++n) {
         if (!FULL && n >= v_groups) { break; }
-        // p s of the group in the order of the codes' words (0, 2), (1, 3), (4, 6), (5, 7), as two elements each
-        u32x4 part[2];
+        // p s of the group in the order of the codes' words (0, 2), (1, 3), (4, 6), (5, 7): the nearest, and what it leaves
+        u32x4 part[FINE ? 2 : 1];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int j = w / 2 * 4 + w % 2;
@@ -444,11 +452,12 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
           if (FINE) { shift[n] = __builtin_fmaf(8.0f, hi, __builtin_fmaf(8.0f, lo, shift[n])); }
           shift[n] = __builtin_fmaf(p[j], half_of(vo[n][j / 2], j % 2), shift[n]);
           shift[n] = __builtin_fmaf(p[j + 2], half_of(vo[n][j / 2 + 1], j % 2), shift[n]);
-          const f16x2 near{f16_t(lo), f16_t(hi)};
-          lo         = __builtin_fmaf(float(near[0]), -1.0f, lo);
-          hi         = __builtin_fmaf(float(near[1]), -1.0f, hi);
-          part[0][w] = __builtin_bit_cast(uint32_t, near);
-          part[1][w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+          part[0][w] = pack2<f16_t>(lo, hi);
+          if (FINE) {
+            lo         = __builtin_fmaf(half_of(part[0][w], 0), -1.0f, lo);
+            hi         = __builtin_fmaf(half_of(part[0][w], 1), -1.0f, hi);
+            part[1][w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+          }
         }
         uint32_t v[4] = {0, 0, 0, 0};
         const bool pair = 2 * n + 1 < C && (FULL || 2 * n + 1 < v_chunks);  // a unit of 64 dimensions, else of 32
@@ -469,11 +478,8 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
             o[c][0] += mfma(f16_t{}, even, part[0], mfma(f16_t{}, even, part[1], zero));
             o[c][1] += mfma(f16_t{}, odd, part[0], mfma(f16_t{}, odd, part[1], zero));
           } else {
-#pragma unroll
-            for (int i = 1; i >= 0; --i) {
-              o[c][0] = mfma(f16_t{}, even, part[i], o[c][0]);
-              o[c][1] = mfma(f16_t{}, odd, part[i], o[c][1]);
-            }
+            o[c][0] = mfma(f16_t{}, even, part[0], o[c][0]);
+            o[c][1] = mfma(f16_t{}, odd, part[0], o[c][1]);
           }
         }
       }

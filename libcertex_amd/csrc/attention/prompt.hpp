@@ -13,7 +13,7 @@
 //   scaling are per lane; the products begin at -m, so that they end as distances from the reference.
 // - The rows of S^T that a lane holds are the positions that it feeds to O^T = V^T P^T: the weights never move.
 //   V is turned on its way into LDS, in the order of positions of these rows.
-// - Weights are rounded to the element type for the second product (bfloat16 2^-9, float16 2^-12 at most, relative); their
+// - Weights are rounded to the element type for the second product (bfloat16 2^-8, float16 2^-11 of them at most); their
 //   sum is not. The output is rounded as much again, and weights with twice the bits would cost half as many products more.
 // - Tiles of positions are in two buffers: the next one's loads are in flight during the products.
 //

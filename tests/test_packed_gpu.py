@@ -11,10 +11,14 @@ from tests.test_prompt_gpu import slopes_of
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
-# weights and scales meet the codes as two float16 elements, each cut after 11 bits, and their product is rounded once
-WEIGHT = 2.0**-21 + 2.0**-24
 DIMS = [(128, 128), (64, 64), (96, 96), (192, 192), (256, 256), (80, 72), (192, 128), (64, 256), (256, 40), (33, 17), (130, 66),
         (1, 1), (255, 200), (97, 160), (8, 129)]
+
+
+def weight_unit(dtype):
+    """Weights times scales meet the codes rounded to float16, or as two such elements for float32, the second cut; their product is
+    rounded once before."""
+    return (2.0**-21 if dtype == torch.float32 else 2.0**-11) + 2.0**-24
 
 
 def packed(lens, page, kv, d, dv, dtype, seed=0, spare=2, fill=0xff, capacity=None):
@@ -136,7 +140,7 @@ def check_attend(lens, heads, kv, d, dv, page, dtype, seed=0, loud=1.0, scale=No
     for s, n in enumerate(lens):
         (keys, key_sizes), (values, value_sizes) = (pack.stored(x[at : at + n]) for x in (k, v))
         at += n
-        want = ref.attend(q[s : s + 1], torch.tensor([n - 1]), keys, values, d**-0.5 if scale is None else scale, weight=WEIGHT,
+        want = ref.attend(q[s : s + 1], torch.tensor([n - 1]), keys, values, d**-0.5 if scale is None else scale, weight=weight_unit(dtype),
                           key_sizes=key_sizes, value_sizes=value_sizes, **how)
         ref.check(out[s : s + 1], lse[s : s + 1], want)
     assert torch.equal(out, pages.attend(q, table, ints(lens, torch.int64), scale=scale, **how))
@@ -207,7 +211,7 @@ def test_attend_value_sizes(gpu, dtype, size):
         q = rand(1, 8, d, dtype=dtype, seed=2, scale=loud)
         scale = d**-0.5 / loud
         out, lse = pages.attend(q, table, ints([n]), scale=scale, return_lse=True)
-        ref.check(out, lse, ref.attend(q, torch.tensor([n - 1]), keys, values, scale, weight=WEIGHT, key_sizes=key_sizes,
+        ref.check(out, lse, ref.attend(q, torch.tensor([n - 1]), keys, values, scale, weight=weight_unit(dtype), key_sizes=key_sizes,
                                        value_sizes=value_sizes))
 
 
@@ -233,7 +237,7 @@ def test_attend_lengths_and_holes(gpu):
     for s, there in ((1, None), (2, torch.arange(64) // page != 1)):
         (keys, key_sizes), (values, value_sizes) = (pack.stored(x[64 * s : 64 * s + 64]) for x in (k, v))
         ref.check(out[s : s + 1], lse[s : s + 1],
-                  ref.attend(q[s : s + 1], torch.tensor([63]), keys, values, 64**-0.5, weight=WEIGHT, key_sizes=key_sizes,
+                  ref.attend(q[s : s + 1], torch.tensor([63]), keys, values, 64**-0.5, weight=weight_unit(dtype), key_sizes=key_sizes,
                              value_sizes=value_sizes, there=there))
 
 
@@ -277,7 +281,7 @@ def test_offsets_past_32_bits(gpu):
     out = pages.attend(q, table, ints([n, n]))
     for s in range(2):
         (keys, key_sizes), (values, value_sizes) = (pack.stored(x[s * n : s * n + n]) for x in (k, v))
-        ref.check(out[s : s + 1], None, ref.attend(q[s : s + 1], torch.tensor([n - 1]), keys, values, d**-0.5, weight=WEIGHT,
+        ref.check(out[s : s + 1], None, ref.attend(q[s : s + 1], torch.tensor([n - 1]), keys, values, d**-0.5, weight=weight_unit(torch.bfloat16),
                                                   key_sizes=key_sizes, value_sizes=value_sizes))
 
 
