@@ -235,9 +235,14 @@ constexpr int kPerUnit = D <= 64 ? 3 : D <= 128 ? 2 : 1;
 
 constexpr int power_of_two(int n) { return n <= 1 ? 1 : 2 * power_of_two((n + 1) / 2); }
 
-template <typename T, int D, bool FULL, bool BENT>
+/** Rows of D elements; of whole pieces, the keys at multiples of 16 bytes; of any length and alignment. */
+enum class fit : int { full, whole, ragged };
+
+template <typename T, int D, fit FIT, bool BENT>
 __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prompt_args a, prompt_plan plan)
 {
+  constexpr bool FULL   = FIT == fit::full;
+  constexpr bool COPIED = FIT != fit::ragged;   // keys go to LDS as they lie
   constexpr bool WIDE   = sizeof(T) == 4;
   constexpr int TILE    = kTile<T>;
   constexpr int kPiece  = 16 / sizeof(T);       // elements of 16 bytes
@@ -247,9 +252,9 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   constexpr int kGroups = TILE / 8;             // groups of 8 positions, which lie in one page
   // threads of a key row, rows at a time
   constexpr int kPieces = D / kPiece, kAcross = power_of_two(kPieces), kDown = kThreads / kAcross, kPasses = TILE / kDown;
-  // Key rows in LDS. FULL: copied there as the lanes are, 16 bytes each; a row's pieces are exchanged by its number, so that
-  // 8 rows' same pieces are in 8 places. Else stored from registers, 16 bytes apart.
-  constexpr int kRowBytes = FULL ? kAcross * 16 : D * sizeof(T) + 16;
+  // Key rows in LDS. Copied there as the lanes are, 16 bytes each; a row's pieces are exchanged by its number, so that 8
+  // rows' same pieces are in 8 places. Else stored from registers, 16 bytes apart.
+  constexpr int kRowBytes = COPIED ? kAcross * 16 : D * sizeof(T) + 16;
   // columns of a thread in V's turn, the positions of its slot
   constexpr int kTurn = std::max(power_of_two(D / 32), 2), kSlot = kPiece;
   __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TILE * kRowBytes];
@@ -341,11 +346,13 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   constexpr int kStep  = std::min(8, kDown);
   // (rows of a thread are 8 apart, or 4: then the second is exchanged otherwise)
   const int64_t k_lane = int64_t(tid / kAcross % kStep) * a.k_slot;
-  const auto piece_of  = [&](int n) { return FULL ? k_piece ^ ((n * kDown + tid / kAcross) % 8) : k_piece; };
+  const auto piece_of  = [&](int n) { return COPIED ? k_piece ^ ((n * kDown + tid / kAcross) % 8) : k_piece; };
   const int64_t v_lane = 4 * half * a.v_slot + v_col;
 
-  words<T, kPiece> k_next[FULL ? 1 : kPasses];
+  words<T, kPiece> k_next[COPIED ? 1 : kPasses];
   words<T, kTurn> v_next[kSlot];
+  // whether this thread turns columns of V (whole ones, or some that the row has not)
+  const bool turns = (FULL && D % (32 * kTurn) == 0) || v_col < (COPIED ? vdim : D);
   const auto load_tile = [&](places const& at, int buffer) {
 #pragma unroll
     for (int n = 0; n < kPasses; ++n) {
@@ -353,25 +360,25 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
       const int first = n * kDown + wave * (kDown / kWaves);
       const T* from   = k_head + of_group(at.k, first / 8) + int64_t(n * kDown % 8) * a.k_slot;
       const int piece = piece_of(n);
-      if (kPieces == kAcross || piece < kPieces) {
-        if constexpr (FULL) {
+      if ((FULL && kPieces == kAcross) || piece < (COPIED ? dim / kPiece : kPieces)) {
+        if constexpr (COPIED) {
           copy_to_lds(from + k_lane + piece * kPiece, lds_address(&s_k[buffer][first * kRowBytes]));
         } else {
-          k_next[n] = row_piece<FULL, kPiece>(from + k_lane + piece * kPiece, piece * kPiece, dim);
+          k_next[n] = row_piece<false, kPiece>(from + k_lane + piece * kPiece, piece * kPiece, dim);
         }
       }
     }
 #pragma unroll
     for (int j = 0; j < kSlot; ++j) {
       const T* from = v_head + of_group(at.v, WIDE ? wave : 2 * wave + j / 4) + int64_t(j % 4) * a.v_slot;
-      if (D % (32 * kTurn) == 0 || v_col < D) { v_next[j] = row_piece<FULL, kTurn>(from + v_lane, v_col, vdim); }
+      if (turns) { v_next[j] = row_piece<COPIED, kTurn>(from + v_lane, v_col, vdim); }
     }
   };
   /** Into LDS: keys as they lie, V turned. At an edge values that no row sees are 0 and unbounded ones are left out; true
    *  if there are any. */
   const auto store_tile = [&](int buffer, int tile, places const& at, bool edge) {
     bool unbounded = false;
-    if (edge) {
+    if (edge && turns) {
 #pragma unroll
       for (int j = 0; j < kSlot; ++j) {
         const int g    = WIDE ? wave : 2 * wave + j / 4;
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         }
       }
     }
-    if constexpr (!FULL) {
+    if constexpr (!COPIED) {
 #pragma unroll
       for (int n = 0; n < kPasses; ++n) {
         const int r = n * kDown + tid / kAcross;
@@ -392,7 +399,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         }
       }
     }
-    if (D % (32 * kTurn) == 0 || v_col < D) {
+    if (turns) {
 #pragma unroll
       for (int e = 0; e < kTurn; ++e) {
         u32x4 t;
@@ -409,7 +416,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         *reinterpret_cast<u32x4*>(&s_v[buffer][col * 128 + slot * 16]) = t;
       }
     }
-    if constexpr (FULL) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }  // the keys' copies
+    if constexpr (COPIED) { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }  // the keys' copies
     return unbounded;
   };
   // whether some row does not see all of a tile
@@ -427,6 +434,11 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   for (int n = 0; n < kCols; ++n) { o[n] = f32x16{}; }
   float base = 0.0f, limit = -INFINITY, total = 0.0f;
 
+  if constexpr (FIT == fit::whole) {
+    // pieces that no row has, which meet the query's 0
+    for (int at = tid * 16; at < int(sizeof(s_k)); at += kThreads * 16) { *reinterpret_cast<u32x4*>(&s_k[0][0] + at) = u32x4{}; }
+    __syncthreads();
+  }
   if (tile0 < tile1) {
     places here = look_up(tile0), next = tile0 + 1 < tile1 ? look_up(tile0 + 1) : here;
     load_tile(here, 0);
@@ -450,24 +462,21 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 #pragma unroll
           for (int e = 0; e < 16; ++e) { s[b][e] = BENT ? 0.0f : -base; }
         }
-        // operands are read one product ahead, and no further: registers are what is short
+        // operands are read four products ahead, and no further: registers are what is short
         const auto key_at = [&](int c, int b) {
-          const int piece = FULL ? (c * 2 + half) ^ (column % 8) : c * 2 + half;
+          const int piece = COPIED ? (c * 2 + half) ^ (column % 8) : c * 2 + half;
           return *reinterpret_cast<const u32x4*>(&s_k[buffer][(b * 32 + column) * kRowBytes + piece * 16]);
         };
-        u32x4 k[2][kBlocks];
+        constexpr int kAhead = 4;
+        u32x4 k[kAhead];
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) { k[0][b] = key_at(0, b); }
+        for (int i = 0; i < kAhead; ++i) { k[i] = key_at(i / kBlocks, i % kBlocks); }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-            if (c + 1 < kChunks) { k[(c + 1) % 2][b] = key_at(c + 1, b); }
-          }
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) { s[b] = mfma32(T{}, k[c % 2][b], q[c], s[b]); }
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < kChunks * kBlocks; ++i) {
+          s[i % kBlocks] = mfma32(T{}, k[i % kAhead], q[i / kBlocks], s[i % kBlocks]);
+          if (i + kAhead < kChunks * kBlocks) { k[i % kAhead] = key_at((i + kAhead) / kBlocks, i % kBlocks); }
+          if (i % kAhead == kAhead - 1) { __builtin_amdgcn_sched_barrier(0); }
         }
         __builtin_amdgcn_s_setprio(0);
         if constexpr (BENT) {
@@ -571,9 +580,9 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           const int col = n * 32 + column, slot = (2 * m + half) ^ ((col / 4 + 2 * (col % 4)) % 8);
           return *reinterpret_cast<const u32x4*>(&s_v[buffer][col * 128 + slot * 16]);
         };
-        u32x4 v[2][kCols];
+        u32x4 v[kAhead];
 #pragma unroll
-        for (int n = 0; n < kCols; ++n) { v[0][n] = value_at(0, n); }
+        for (int i = 0; i < kAhead; ++i) { v[i] = value_at(i / kCols, i % kCols); }
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
           u32x4 w;
@@ -587,10 +596,10 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           }
 #pragma unroll
           for (int n = 0; n < kCols; ++n) {
-            if (m + 1 < kSteps) { v[(m + 1) % 2][n] = value_at(m + 1, n); }
+            const int i = m * kCols + n;
+            o[n]        = mfma32(T{}, v[i % kAhead], w, o[n]);
+            if (i + kAhead < kSteps * kCols) { v[i % kAhead] = value_at((i + kAhead) / kCols, (i + kAhead) % kCols); }
           }
-#pragma unroll
-          for (int n = 0; n < kCols; ++n) { o[n] = mfma32(T{}, v[m % 2][n], w, o[n]); }
           __builtin_amdgcn_sched_barrier(0);
         }
         if (unbounded) {
@@ -715,7 +724,7 @@ size_t workspace_for(prompt_args const& a)
 template <typename T>
 void launch(prompt_args const& a, hipStream_t stream)
 {
-  const auto launched = [&](auto bucket, auto full) {
+  const auto launched = [&](auto bucket, auto how) {
     constexpr int D = decltype(bucket)::value;
     prompt_plan plan{divisor(uint32_t(a.pages.page / 8)), divisor(uint32_t(a.heads / a.kv_heads))};
     plan.tiles  = int32_t(tiles_of(a));
@@ -729,20 +738,26 @@ void launch(prompt_args const& a, hipStream_t stream)
     plan.part_sum       = plan.part_max + slots;
     const dim3 grid(uint32_t(plan.tiles) * a.kv_heads * plan.splits);
     if (a.shape.any()) {
-      prompt_kernel<T, D, decltype(full)::value, true><<<grid, kThreads, 0, stream>>>(a, plan);
+      prompt_kernel<T, D, decltype(how)::value, true><<<grid, kThreads, 0, stream>>>(a, plan);
     } else {
-      prompt_kernel<T, D, decltype(full)::value, false><<<grid, kThreads, 0, stream>>>(a, plan);
+      prompt_kernel<T, D, decltype(how)::value, false><<<grid, kThreads, 0, stream>>>(a, plan);
     }
     if (plan.splits > 1) {
       join_kernel<T><<<dim3(uint32_t(plan.tiles) * a.kv_heads, kRows / kJoinRows), kThreads, 0, stream>>>(a, plan);
     }
   };
-  // key rows at multiples of 16 bytes are copied to LDS as they lie
-  const bool aligned = reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && (a.k_page * sizeof(T)) % 16 == 0 &&
-                       (a.k_slot * sizeof(T)) % 16 == 0 && (a.k_head * sizeof(T)) % 16 == 0;
+  const auto aligned = [](int64_t elements) { return elements * sizeof(T) % 16 == 0; };
+  const bool whole   = reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && aligned(a.k_page) && aligned(a.k_slot) &&
+                     aligned(a.k_head) && aligned(a.dim) && a.vdim % 8 == 0;
   const auto bucket = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    a.dim == D && a.vdim == D && aligned ? launched(d, std::true_type{}) : launched(d, std::false_type{});
+    if (whole && a.dim == D && a.vdim == D) {
+      launched(d, std::integral_constant<fit, fit::full>{});
+    } else if (whole) {
+      launched(d, std::integral_constant<fit, fit::whole>{});
+    } else {
+      launched(d, std::integral_constant<fit, fit::ragged>{});
+    }
   };
   const int dim = std::max(a.dim, a.vdim);
   if (dim <= 64) {
