@@ -342,9 +342,11 @@ auto prompt_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v
 }
 
 /** The bent scores' parameters: a cap of 0 and no slopes leave the scores as they are. */
-auto shape_of(cuvs::resources const& r, float cap, DLManagedTensor* slopes, int64_t heads) -> ops::score_shape
+auto shape_of(cuvs::resources const& r, float scale, float cap, DLManagedTensor* slopes, int64_t heads) -> ops::score_shape
 {
+  EXPECTS(std::isfinite(scale), "the scale must be finite");
   EXPECTS(std::isfinite(cap) && cap >= 0.0f, "the cap must be finite and not negative");
+  EXPECTS(cap == 0.0f || std::abs(scale / cap) < 1e37f, "the cap is too small for the scale");
   ops::score_shape s;
   s.cap = cap;
   if (slopes != nullptr) {
@@ -705,7 +707,7 @@ cuvsError_t cuvsCertexPagedAttentionShaped(cuvsResources_t res,
     expects_shape(out, {q.shape[0], q.shape[1], v.shape[3]});
     expects_device(r, q, k, v, table, lengths, out);
     EXPECTS(std::isfinite(scale), "the scale must be finite");
-    const auto shape = shape_of(r, cap, slopes_, q.shape[1]);
+    const auto shape = shape_of(r, scale, cap, slopes_, q.shape[1]);
     a.lse = lse_of(r, lse_, q.shape[0], q.shape[1]);
     if (q.shape[0] == 0) { return; }
     a.lengths   = int_vector_of(lengths);
@@ -785,7 +787,7 @@ cuvsError_t cuvsCertexPromptAttention(cuvsResources_t res,
       expects_device(r, prefix);
       a.prefix = int_vector_of(prefix);
     }
-    a.shape = shape_of(r, cap, slopes_, q.shape[1]);
+    a.shape = shape_of(r, scale, cap, slopes_, q.shape[1]);
     a.lse   = lse_of(r, lse_, q.shape[0], q.shape[1]);
     if (q.shape[0] == 0) { return; }
     a.lengths   = int_vector_of(lengths);
@@ -946,7 +948,7 @@ cuvsError_t cuvsCertexPackedAttention(cuvsResources_t res,
     expects_shape(out, {q.shape[0], q.shape[1], vdim});
     expects_device(r, q, pages, table, lengths, out);
     EXPECTS(std::isfinite(scale), "the scale must be finite");
-    a.shape = shape_of(r, cap, slopes_, q.shape[1]);
+    a.shape = shape_of(r, scale, cap, slopes_, q.shape[1]);
     a.lse   = lse_of(r, lse_, q.shape[0], q.shape[1]);
     if (q.shape[0] == 0) { return; }
     a.lengths   = int_vector_of(lengths);

@@ -701,7 +701,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(prompt_args a, prompt_pl
   }
 }
 
-int64_t tiles_of(prompt_args const& a) { return a.tokens * (a.heads / a.kv_heads) / kRows + a.pages.sequences; }
+/** Tiles of rows over all sequences, at most; one where there is no sequence, for the tokens' zeros. */
+int64_t tiles_of(prompt_args const& a)
+{
+  return std::max<int64_t>(1, a.tokens * (a.heads / a.kv_heads) / kRows + a.pages.sequences);
+}
 
 /** Splits of a tile's positions: as many workgroups as the chip holds where the tiles alone are fewer. */
 int splits_for(prompt_args const& a, int tile, int per_unit)
