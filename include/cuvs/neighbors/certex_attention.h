@@ -149,7 +149,7 @@ CUVS_EXPORT cuvsError_t cuvsCertexPagedAttentionWorkspace(DLManagedTensor* q,
 /**
  * cuvsCertexPagedAttention whose scores are bent before the softmax: y = cap tanh(scale <q, k> / cap) (cap 0: scale <q, k>),
  * then y - slopes[h] |p - t| (slopes NULL: y) with p = length - 1 the position of the new token and t that of the key.
- * cap: at least 0; slopes: dense float32 [heads], finite. The workspace is that of cuvsCertexPagedAttention.
+ * cap: at least 0, at most 10^30; slopes: dense float32 [heads], finite. The workspace is that of cuvsCertexPagedAttention.
  */
 CUVS_EXPORT cuvsError_t cuvsCertexPagedAttentionShaped(cuvsResources_t res,
                                                        DLManagedTensor* q,

@@ -7,6 +7,7 @@
 #include "attention.hpp"
 #include "overlap.hpp"
 
+#include <cfloat>
 #include <cmath>
 #include <exception>
 #include <string>
@@ -347,6 +348,8 @@ auto shape_of(cuvs::resources const& r, float scale, float cap, DLManagedTensor*
   EXPECTS(std::isfinite(scale), "the scale must be finite");
   EXPECTS(std::isfinite(cap) && cap >= 0.0f, "the cap must be finite and not negative");
   EXPECTS(cap == 0.0f || std::abs(scale / cap) < 1e37f, "the cap is too small for the scale");
+  // scores are taken as fractions of it, which float32 has to hold
+  EXPECTS(cap <= 1e30f && (cap == 0.0f || scale == 0.0f || std::abs(scale / cap) >= FLT_MIN), "the cap is too large");
   ops::score_shape s;
   s.cap = cap;
   if (slopes != nullptr) {

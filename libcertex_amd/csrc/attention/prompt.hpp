@@ -225,6 +225,10 @@ constexpr float kLift = 0.0f;
 template <>
 constexpr float kLift<f16_t> = 13.0f;
 
+/** Up to this cap 16-bit rows take cap tanh(u) as cap (1 - 2 / (e^(2u) + 1)), 5 operations for tanh_of's 14: it is off by
+ *  some 2^-22 cap however small u is, here a 32nd of what rounding the weights to float16 is. Beyond, and in float32, tanh_of. */
+constexpr float kShortCap = 64.0f;
+
 /** Positions of a tile: 128 bytes of a turned row. */
 template <typename T>
 constexpr int kTile = 128 / sizeof(T);
@@ -483,18 +487,21 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
           // less base, which is the last operation's other term
           const float ahead_of = float(p - t0 - 4 * half);
           if (a.shape.cap != 0.0f) {
-            const float whole = a.shape.cap - base, twice = -2.0f * a.shape.cap;
+            if (!WIDE && a.shape.cap <= kShortCap) {
+              const float whole = a.shape.cap - base, twice = -2.0f * a.shape.cap;
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
+              for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if constexpr (WIDE) {
-                  s[b][e] = __builtin_fmaf(a.shape.cap, tanh_of(s[b][e] * per_cap), -base);
-                } else {
-                  // cap (1 - 2 / (e^(2u) + 1)): off by 2^-23 cap, which the rounded weights hide
+                for (int e = 0; e < 16; ++e) {
                   const float e2u = __builtin_amdgcn_exp2f(s[b][e] * (per_cap * (2.0f * kLog2e)));
                   s[b][e]         = __builtin_fmaf(twice, __builtin_amdgcn_rcpf(e2u + 1.0f), whole);
                 }
+              }
+            } else {
+#pragma unroll
+              for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { s[b][e] = __builtin_fmaf(a.shape.cap, tanh_of(s[b][e] * per_cap), -base); }
               }
             }
             if (a.shape.slopes != nullptr) {

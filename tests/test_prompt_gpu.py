@@ -86,6 +86,25 @@ def test_prompt_bent(gpu, dtype, cap, lean, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [65.0, 3e4, 1e6, 1e30])
+def test_prompt_large_cap(gpu, dtype, cap):
+    """A cap far beyond the scores leaves them: cap tanh(y / cap) is y within 5 units in the last place, with the y^3 / (3 cap^2)
+    by which it is less."""
+    lens, q = [200, 90], rand(60, 4, 64, dtype=dtype, seed=61)
+    kp, vp, table, keys, values = paged(lens, 16, 2, 64, 64, dtype, seed=60)
+    out, lse = certex.prompt_attention(q, kp, vp, table, ints(lens), ints([0, 20, 60]), cap=cap, return_lse=True)
+    for s, rows in enumerate([slice(0, 20), slice(20, 60)]):
+        n = rows.stop - rows.start
+        scores = q[rows].double().cpu().abs().norm(dim=-1).max() * keys[s].double().cpu().norm(dim=-1).max() / 8
+        bend = float(scores) ** 3 / (3 * cap**2) + 5 * 2.0**-24 * float(scores)
+        want = ref.attend(q[rows], torch.arange(lens[s] - n, lens[s]), keys[s], values[s], 0.125, weight=weight_unit(dtype) + bend)
+        if cap < 100:  # where the bend shows, the definition's own
+            exact = ref.attend(q[rows], torch.arange(lens[s] - n, lens[s]), keys[s], values[s], 0.125, cap=cap)
+            want = (*exact[:2], *want[2:])
+        ref.check(out[rows], lse[rows], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("news, pasts", [([16], [20_000]), ([1, 1, 1, 2], [9_000, 50, 0, 3_000]), ([300], [2_000]),
                                          ([3] * 20, [100 * i for i in range(20)])])
 def test_prompt_long(gpu, dtype, news, pasts):
@@ -285,6 +304,7 @@ def test_refusals(gpu):
         (dict(first=ints([0, 10])), "first must have shape"), (dict(lens=ints([64])), "lengths must have shape"),
         (dict(prefix=ints([1])), "prefix must have shape"), (dict(cap=0.0), "positive"), (dict(cap=-1.0), "positive"),
         (dict(cap=float("nan")), "positive"), (dict(cap=float("inf")), "positive"), (dict(cap=1e-60), "positive"),
+        (dict(cap=1e31), "too large"), (dict(cap=1e10, scale=1e-30), "too large"),
         (dict(window=0), "at least 1"),
         (dict(slopes=slopes[:3]), "slopes must have shape"), (dict(slopes=slopes.half()), "float32"),
         (dict(slopes=slopes.cpu()), "GPU"), (dict(scale=float("inf")), "finite"),
