@@ -30,6 +30,9 @@
 // all heads (128 bytes of a line pair each), 6.2 with the heads first; of 256 6.2, and 5.8 in float32; of 160, and of 192
 // with values of 128, which run as 256, 4.4. More workgroups or waves per
 // compute unit read slower (three: 193 us for the 64 sequences): the memory prefers fewer streams.
+//
+// Bent scores (BENT) are taken between the products, some 20 operations each in the shade of the reads: the 64
+// sequences with a cap 159 us; three of up to 3,001 float16 positions of heads of 64 with slopes 7.1 us and 5 for the join.
 #include "scores.hpp"
 #include "shares.hpp"
 #include "tiles.hpp"

@@ -145,7 +145,6 @@ struct packed_pages {
   uint8_t* p       = nullptr;
   int32_t kv_heads = 0, dim = 0, vdim = 0;
   page_map map;
-  static constexpr int kGroup = 64;
 #ifdef __HIPCC__
   __host__ __device__
 #endif

@@ -20,6 +20,13 @@
 // Work is dealt without reading the lengths back: the host launches as many tiles of rows as there may be, the
 // kernel finds the sequence of each. The last rows of a prompt see most and go first. Where tiles are too few to
 // fill the chip their positions are split over workgroups, which leave partials (m, sum, output) for join_kernel.
+//
+// Measured (bfloat16, 32 heads on 8 of 128; products alone reach 1,227 TFLOP/s): a prompt of 8,192 tokens 658 to 770 us,
+// 715 to 835 TFLOP/s; 512 capped tokens behind 65,536 positions 855 to 970 with 14 for the join, 570 to 645: the scores' vector operations are in
+// the products' way. Seven prompts of up to 2,000 tokens, 16 leaning heads of 64 of float16, 114 to 140 us. Single precision (products alone: 154
+// TFLOP/s) 4,000 tokens of 12 heads of 128 on 4, 535 us, 92 TFLOP/s. The same in bfloat16 by head size: 128 116 us, 192 200, 256 290; rows of odd
+// sizes, which no copy into LDS takes, 111 270 us. Values loaded only after the first products: 1,009 us where 831 was then; pages
+// looked up by branches within the loads: 966.
 #pragma once
 
 #include "../kernels/lanes.hpp"
@@ -28,7 +35,7 @@
 #include "tiles.hpp"
 
 #include <algorithm>
-#include <climits>
+#include <cfloat>
 
 namespace certex_amd::attention {
 namespace {
@@ -176,13 +183,30 @@ struct words {
   uint32_t w[N * sizeof(T) / 4];
 };
 
-/** Elements [off, off + N) of a row of n, which begin at `from`; what is past its end is 0. */
+/** Elements [off, off + N) of a row of n, which begin at `from`; what is past its end is 0: the last piece is read so that it
+ *  ends with the row, and moved. (Element by element a prompt of 4,000 tokens, heads of 111 bfloat16, took 353 us.) */
 template <bool FULL, int N, typename T>
 __device__ __forceinline__ words<T, N> row_piece(const T* from, int off, int n)
 {
+  constexpr int W = N * sizeof(T) / 4;
   words<T, N> v{};
-  if (FULL || off + N <= n) {
+  if (FULL) {
     __builtin_memcpy(&v, __builtin_assume_aligned(from, sizeof(T)), sizeof(v));
+  } else if (n >= N) {
+    const int past = max(0, off + N - n);
+    __builtin_memcpy(&v, __builtin_assume_aligned(from - past, sizeof(T)), sizeof(v));
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) { v.w[i] = __builtin_amdgcn_alignbyte(i + 1 < W ? v.w[i + 1] : 0u, v.w[i], 2 * (past & 1)); }
+    }
+    const int by = past * int(sizeof(T)) / 4;
+#pragma unroll
+    for (int step = 1; step < W; step *= 2) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) { v.w[i] = (by & step) != 0 ? (i + step < W ? v.w[i + step] : 0u) : v.w[i]; }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) { v.w[i] = by < W ? v.w[i] : 0u; }
   } else if (off < n) {
     T e[N];
 #pragma unroll
@@ -237,6 +261,11 @@ constexpr int kTile = 128 / sizeof(T);
 template <typename T, int D>
 constexpr int kPerUnit = D <= 64 ? 3 : D <= 128 ? 2 : 1;
 
+/** Columns of V of a workgroup: half of 256, though both halves take the scores. Queries and all outputs leave no registers for
+ *  the rest: 4,000 tokens, 12 heads on 4 of 256, took 377 us in bfloat16 and 3,580 in float32, where halves take 288 and 1,700. */
+template <typename T, int D>
+constexpr int kColumns = D > 192 ? D / 2 : D;
+
 constexpr int power_of_two(int n) { return n <= 1 ? 1 : 2 * power_of_two((n + 1) / 2); }
 
 /** Rows of D elements; of whole pieces, the keys at multiples of 16 bytes; of any length and alignment. */
@@ -252,7 +281,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   constexpr int kPiece  = 16 / sizeof(T);       // elements of 16 bytes
   constexpr int kChunks = D / (2 * kPiece);     // products along a row, of a piece per half wave
   constexpr int kBlocks = TILE / 32;            // products along the positions
-  constexpr int kCols   = D / 32;               // products along the columns of V
+  constexpr int VD      = kColumns<T, D>;
+  constexpr int kCols   = VD / 32;              // products along the columns of V
   constexpr int kGroups = TILE / 8;             // groups of 8 positions, which lie in one page
   // threads of a key row, rows at a time
   constexpr int kPieces = D / kPiece, kAcross = power_of_two(kPieces), kDown = kThreads / kAcross, kPasses = TILE / kDown;
@@ -260,9 +290,9 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   // rows' same pieces are in 8 places. Else stored from registers, 16 bytes apart.
   constexpr int kRowBytes = COPIED ? kAcross * 16 : D * sizeof(T) + 16;
   // columns of a thread in V's turn, the positions of its slot
-  constexpr int kTurn = std::max(power_of_two(D / 32), 2), kSlot = kPiece;
+  constexpr int kTurn = std::max(power_of_two(VD / 32), 2), kSlot = kPiece;
   __shared__ __attribute__((aligned(16))) uint8_t s_k[2][TILE * kRowBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][D * 128];
+  __shared__ __attribute__((aligned(16))) uint8_t s_v[2][VD * 128];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
   const int column = lane % 32, half = lane / 32;
 
@@ -297,7 +327,8 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   const int p       = rt.past + int(i);
   const int hi      = exists ? max(min(p + 1, rt.length), rt.prefix) : 0;
   const int lo      = a.window > 0 ? int(max(int64_t(0), int64_t(p) + 1 - a.window)) : 0;
-  const int dim = FULL ? D : a.dim, vdim = FULL ? D : a.vdim;
+  const int first_col = VD < D ? blockIdx.y * VD : 0;
+  const int dim = FULL ? D : a.dim, vdim = FULL ? VD : min(VD, a.vdim - first_col);
 
   u32x4 q[kChunks];
   {
@@ -320,7 +351,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     uint32_t there;  // bit per group: the sequence has its page
   };
   const T* k_head      = static_cast<const T*>(a.k) + kv * a.k_head;
-  const T* v_head      = static_cast<const T*>(a.v) + kv * a.v_head;
+  const T* v_head      = static_cast<const T*>(a.v) + kv * a.v_head + first_col;
   const int32_t* table = a.pages.table + int64_t(rt.sequence) * a.pages.width;
   const int final      = max(0, rt.length - 1) / 8;
   const auto look_up   = [&](int tile) {
@@ -356,7 +387,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   words<T, kPiece> k_next[COPIED ? 1 : kPasses];
   words<T, kTurn> v_next[kSlot];
   // whether this thread turns columns of V (whole ones, or some that the row has not)
-  const bool turns = (FULL && D % (32 * kTurn) == 0) || v_col < (COPIED ? vdim : D);
+  const bool turns = (FULL && VD % (32 * kTurn) == 0) || v_col < (COPIED ? vdim : VD);
   const auto load_tile = [&](places const& at, int buffer) {
 #pragma unroll
     for (int n = 0; n < kPasses; ++n) {
@@ -644,7 +675,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   if (splits == 1) {
     const int64_t at  = (rt.token0 + i) * a.heads + head;
     const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-    T* out            = static_cast<T*>(a.out) + at * vdim;
+    T* out            = static_cast<T*>(a.out) + at * a.vdim + first_col;
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
 #pragma unroll
@@ -653,7 +684,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         if (col < vdim) { out[col] = T(total == 0.0f ? 0.0f : o[n][e] * scale); }
       }
     }
-    if (half == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, base, total, kLift<T>); }
+    if (half == 0 && first_col == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, base, total, kLift<T>); }
   } else {
     const int64_t at = ((index * a.kv_heads + kv) * plan.splits + split) * kRows + wave * 32 + column;
 #pragma unroll
@@ -661,16 +692,17 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int col = n * 32 + 8 * (e / 4) + 4 * half + e % 4;
-        if (col < vdim) { plan.part_out[at * vdim + col] = o[n][e]; }
+        if (col < vdim) { plan.part_out[at * a.vdim + first_col + col] = o[n][e]; }
       }
     }
-    if (half == 0) {
+    if (half == 0 && first_col == 0) {
       plan.part_max[at] = counted ? base : -INFINITY;
       plan.part_sum[at] = total;
     }
   }
 }
 
+/** Rows of a workgroup that joins: fewer, so that there are more. (32 rows: 24 us where 18 was.) */
 constexpr int kJoinRows = 8;
 
 /** Rows of a tile that was split, 32 threads each: joins their partials in order of position. */
@@ -747,7 +779,7 @@ void launch(prompt_args const& a, hipStream_t stream)
     plan.part_out       = static_cast<float*>(a.workspace);
     plan.part_max       = plan.part_out + slots * a.vdim;
     plan.part_sum       = plan.part_max + slots;
-    const dim3 grid(uint32_t(plan.tiles) * a.kv_heads * plan.splits);
+    const dim3 grid(uint32_t(plan.tiles) * a.kv_heads * plan.splits, (a.vdim + kColumns<T, D> - 1) / kColumns<T, D>);
     if (a.shape.any()) {
       prompt_kernel<T, D, decltype(how)::value, true><<<grid, kThreads, 0, stream>>>(a, plan);
     } else {
@@ -777,6 +809,8 @@ void launch(prompt_args const& a, hipStream_t stream)
     bucket(std::integral_constant<int, 96>{});
   } else if (dim <= 128) {
     bucket(std::integral_constant<int, 128>{});
+  } else if (dim <= 192) {
+    bucket(std::integral_constant<int, 192>{});
   } else {
     bucket(std::integral_constant<int, 256>{});
   }

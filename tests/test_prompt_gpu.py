@@ -113,6 +113,14 @@ def test_prompt_long(gpu, dtype, news, pasts):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d, dv", [(256, 256), (256, 130), (40, 129 + 64), (201, 255), (160, 160), (161, 63), (9, 256)])
+def test_prompt_wide_heads(gpu, dtype, d, dv):
+    """Columns that two workgroups share, whole and split over positions, with logarithms of their own once."""
+    check_prompt([20, 3], [1_500, 40], 4, 2, d, dv, 16, dtype, seed=62)
+    check_prompt([200, 130, 1], [0, 9, 0], 3, 1, d, dv, 24, dtype, prefix=[50, 0, 0], cap=30.0, slopes=slopes_of(3), seed=63)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_prompt_extreme_scores(gpu, dtype):
     """Scores in the hundreds (one weight takes all), of a scale of 0 (all equal) and of a negative one."""
     for how in (dict(loud=30.0), dict(scale=0.0), dict(scale=-0.3), dict(scale=-0.3, cap=20.0, loud=4.0), dict(scale=0.0, cap=20.0)):
