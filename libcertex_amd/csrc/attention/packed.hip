@@ -22,8 +22,8 @@
 // Work is dealt as in attend.hip (shares.hpp). A wave copies its next step to LDS while it works on one, by itself: what it
 // copies it alone reads, so that steps need no barrier.
 //
-// Measured (8 key heads of 128, 32 query heads): 64 sequences up to 8,192 of bfloat16 queries, 0.26 GB of records: 61 us and 6
-// for the join, 4.3 TB/s;
+// Measured (8 key heads of 128, 32 query heads): 64 sequences up to 8,192 of bfloat16 queries, 0.26 GB of records: 57 to 61 us
+// and 6 for the join, 4.3 to 4.6 TB/s;
 // one sequence of 131,072, float32 queries, 0.15 GB: 53 us and 6, 7e-7 off (subnormal codes: 2e-6 to 5e-6); 77 positions
 // 8.6 us, launch and five dependent loads.
 #include "scores.hpp"

@@ -22,11 +22,12 @@
 // fill the chip their positions are split over workgroups, which leave partials (m, sum, output) for join_kernel.
 //
 // Measured (bfloat16, 32 heads on 8 of 128; products alone reach 1,227 TFLOP/s): a prompt of 8,192 tokens 658 to 683 us,
-// 805 to 835 TFLOP/s (one at a time, traced: 754); 512 capped tokens behind 65,536 positions 855 to 885 with 14 for the join, 625 to 645: the scores' vector operations are in
-// the products' way. Seven prompts of up to 2,000 tokens, 16 leaning heads of 64 of float16, 114 to 140 us. Single precision (products alone: 154
-// TFLOP/s) 4,000 tokens of 12 heads of 128 on 4, 535 us, 92 TFLOP/s. The same in bfloat16 by head size: 128 116 us, 192 200, 256 290; rows of odd
-// sizes, which no copy into LDS takes, 111 270 us. Values loaded only after the first products: 1,009 us where 831 was then; pages
-// looked up by branches within the loads: 966.
+// 805 to 835 TFLOP/s (one at a time, traced: 754); 512 capped tokens behind 65,536 positions 855 to 885 with 14 for the join,
+// 625 to 645: the scores' vector operations are in the products' way. Seven prompts of up to 2,000 tokens, 16 leaning heads of
+// 64 of float16, 114 to 140 us. Single precision (products alone: 154 TFLOP/s) 4,000 tokens of 12 heads of 128 on 4, 535 us, 92
+// TFLOP/s. The same in bfloat16 by head size: 128 116 us, 192 200, 256 290; rows of odd sizes, which no copy into LDS takes, 111
+// 270 us. Values loaded only after the first products: 1,009 us where 831 was then; pages looked up by branches within the
+// loads: 966.
 #pragma once
 
 #include "../kernels/lanes.hpp"
