@@ -401,15 +401,24 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
       float high = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) { high = fmaxf(high, x[j]); }
-      // the largest of the scales, which are not negative: as whole numbers (NaN is the largest, and no steeper than any)
+      // the largest of the scales, which are not negative: as whole numbers, of which NaN is the largest
       u16x2 most = __builtin_bit_cast(u16x2, vs[0][0]);
 #pragma unroll
       for (int n = 0; n < G; ++n) {
 #pragma unroll
         for (int w = n == 0 ? 1 : 0; w < 4; ++w) { most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, vs[n][w])); }
       }
-      const float steep = fmaxf(half_of(__builtin_bit_cast(uint32_t, most), 0), half_of(__builtin_bit_cast(uint32_t, most), 1));
-      if (__any(high > limit || steep >= scale_limit)) {
+      const float even = half_of(__builtin_bit_cast(uint32_t, most), 0), odd = half_of(__builtin_bit_cast(uint32_t, most), 1);
+      const bool hidden = __builtin_isunordered(even, odd);  // scales below a NaN, which is no steeper than any
+      float steep       = fmaxf(even, odd);
+      if (__any(high > limit || steep >= scale_limit || hidden)) {
+        if (hidden) {
+#pragma unroll
+          for (int n = 0; n < G; ++n) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) { steep = fmaxf(steep, fmaxf(half_of(vs[n][w], 0), half_of(vs[n][w], 1))); }
+          }
+        }
         const auto larger = [](float u, float w) { return fmaxf(u, w); };
         high              = lanes::fold16(lanes::fold32(high, larger), larger);
         const float grown = fmaxf(top, high);

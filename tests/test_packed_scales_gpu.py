@@ -1,0 +1,52 @@
+"""4-bit attention where the scales of a record differ: NaN beside others, steep ones beside flat ones."""
+
+import pytest
+import torch
+
+import libcertex_amd as certex
+from tests import packed_reference as pack
+from tests import shaped_reference as ref
+from tests.test_packed_gpu import TYPES, weight_unit
+from tests.test_paged_gpu import ints, rand
+
+pytestmark = pytest.mark.gpu
+
+
+def check_columns(k, v, q, columns):
+    """One sequence of all positions of k and v (n, kv, d): the other columns of the output are NaN, these as defined."""
+    n, kv, d = k.shape
+    pages = certex.PackedPages(-(-n // 16), 16, kv, d)
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device="cuda").flip(0)[None]
+    positions = torch.arange(n, device="cuda")
+    pages.append(k, v, table, positions, sequences=torch.zeros_like(positions))
+    out, lse = pages.attend(q, table, ints([n]), return_lse=True)
+    (keys, key_sizes), (values, value_sizes) = pack.stored(k), pack.stored(v)
+    want = ref.attend(q, torch.tensor([n - 1]), keys, values[..., columns], d**-0.5, weight=weight_unit(q.dtype), key_sizes=key_sizes,
+                      value_sizes=value_sizes[..., columns])
+    ref.check(out[..., columns].contiguous(), lse, want)
+    rest = torch.ones(d, dtype=torch.bool)
+    rest[columns] = False
+    assert out[..., rest.cuda()].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("n", [1, 2, 33, 34, 65, 97, 130])
+def test_nan_beside_other_groups(gpu, dtype, d, n):
+    """NaN in 64 elements of a value makes these columns NaN and no others, also where few positions are weighed with it."""
+    for group in range(d // 64):
+        k, v, q = rand(n, 2, d, dtype=dtype), rand(n, 2, d, dtype=dtype, seed=1), rand(1, 4, d, dtype=dtype, seed=2)
+        v[n - 1, :, 64 * group + 5] = float("nan")
+        columns = torch.arange(d)[torch.arange(d) // 64 != group]
+        check_columns(k, v, q, columns)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nan, steep", [(0, 2), (1, 3), (6, 4), (12, 14), (20, 16)])
+def test_nan_hides_no_steep_scale(gpu, dtype, nan, steep):
+    """A scale a hundred and ten thousand times the others', in a record whose scales have a NaN among them."""
+    for times in (100.0, 10_000.0):
+        k, v, q = rand(40, 1, 128, dtype=dtype), rand(40, 1, 128, dtype=dtype, seed=1), rand(1, 4, 128, dtype=dtype, seed=2)
+        v[steep, :, 64:] *= times
+        v[nan, :, 3] = float("nan")
+        check_columns(k, v, q, torch.arange(64, 128))
