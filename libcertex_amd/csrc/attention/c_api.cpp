@@ -336,7 +336,7 @@ auto prompt_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v
   const int64_t group = a.heads / a.kv_heads;
   // rows of a key head, and blocks of 256 threads that a launch may have
   EXPECTS(a.tokens < (int64_t(1) << 29) && a.tokens * group < (int64_t(1) << 29) &&
-            (a.tokens * group / 128 + table->shape[0]) * a.kv_heads < (int64_t(1) << 23),
+            (a.tokens * group / 128 + std::min(a.tokens, table->shape[0])) * a.kv_heads < (int64_t(1) << 23),
           "too many tokens in one call");
   EXPECTS(int64_t(a.pages.width) * a.pages.page <= (int64_t(1) << 31) - 64, "a sequence's pages hold at most 2^31 - 64 positions");
   return a;

@@ -19,7 +19,8 @@
 //
 // Work is dealt without reading the lengths back: the host launches as many tiles of rows as there may be, the
 // kernel finds the sequence of each. The last rows of a prompt see most and go first. Where tiles are too few to
-// fill the chip their positions are split over workgroups, which leave partials (m, sum, output) for join_kernel.
+// fill the chip their positions are split over workgroups, which leave partials (m, sum, output) for join_kernel. The kernels count
+// the tiles for that: rows of a page table that have no new tokens take no part of the chip, and no workspace.
 //
 // Measured (bfloat16, 32 heads on 8 of 128; products alone reach 1,227 TFLOP/s): a prompt of 8,192 tokens 658 to 683 us,
 // 805 to 835 TFLOP/s (one at a time, traced: 754); 512 capped tokens behind 65,536 positions 855 to 885 with 14 for the join,
@@ -56,11 +57,13 @@ struct prompt_plan {
   divisor group;        // query heads per key head
   int32_t tiles;        // of rows, at most, over all sequences
   int32_t splits;       // of a tile's positions, at most
+  int32_t places;       // workgroups that the chip holds
   bool near;            // strides of pages and of 8 slots fit 32 bits
   score_scale scale;
   float slack;          // kSlack in scores
-  float* part_out;      // [tiles][kv_heads][splits][kRows][vdim]
-  float* part_max;      // [tiles][kv_heads][splits][kRows]
+  // (a split's side by side: workgroups that write within one cache line wait for each other)
+  float* part_out;      // [splits][tokens][heads][vdim]
+  float* part_max;      // [splits][tokens][heads]
   float* part_sum;
 };
 
@@ -77,29 +80,52 @@ struct row_tile {
 
 __device__ __forceinline__ int64_t clamped(int64_t x, int64_t hi) { return x < 0 ? 0 : x > hi ? hi : x; }
 
+/** Where a workgroup is in the launch: a tile's number, those that see most first; a piece of its positions, of `splits` at most. */
+struct dealt {
+  int64_t index;
+  int32_t split, splits;
+};
+
+/** That of number `place` in a call of `tiles` tiles, which fill the chip once with the splits. Of every split (WHOLE: of none). */
+template <bool WHOLE>
+__device__ __forceinline__ dealt deal(prompt_args const& a, prompt_plan const& plan, int64_t place, int tiles)
+{
+  const int64_t blocks = int64_t(max(1, tiles)) * a.kv_heads;
+  const int splits     = 2 * blocks > plan.places ? 1 : min(plan.splits, plan.places / int(blocks));
+  if (WHOLE || splits == 1) { return {place, 0, splits}; }
+  const uint32_t index = uint32_t(place) / uint32_t(splits);
+  return {int64_t(index), int32_t(uint32_t(place) - index * splits), splits};
+}
+
 /**
- * The tile that goes at place `index` of the launch, those that see most first; false where there is none. 2 to 64
- * sequences: by the number of row tiles that end no later (a tile's rows, and those of the sequence before them). More: or one: sequence s
- * has the indexes from floor(first[s] group / kRows) + s on, of which the first ceil(rows / kRows) are its tiles and the next
- * sequence's begin behind them; from the last one on.
+ * The tile at a place of the launch; false where there is none. 2 to 64
+ * sequences: by the number of row tiles that end no later (a tile's rows, and those of the sequence before them). One, or more than
+ * 64, from the last tile on; of more than 64 either each thread counts the tiles of some, or, where nothing is split and the number
+ * of tiles does not matter, sequence s has the indexes from floor(first[s] group / kRows) + min(s, first[s]) on, of which
+ * the first ceil(rows / kRows) are its tiles and the next sequence's begin behind them.
  * Measured, seven prompts of up to 2,000 tokens, 16 heads of 64: 161 us by sequence, 127 by length.
  */
-template <int TILE>
-__device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan const& plan, int64_t index, row_tile* out)
+template <int TILE, bool WHOLE>
+__device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan const& plan, int64_t place, row_tile* out, dealt* as)
 {
   const int64_t sequences = a.pages.sequences;
   if (sequences == 0) { return false; }  // first has one entry, the lengths none
   const int lane        = threadIdx.x % 64;
   const int64_t group   = plan.group.d;
   const auto token      = [&](int64_t s) { return clamped(a.first[s], a.tokens); };
+  const auto tiles_for  = [&](int64_t tokens) { return int((tokens * group + kRows - 1) / kRows); };
   const int64_t longest = a.pages.n_pages > 0 ? int64_t(a.pages.width) * a.pages.page : 0;
   int64_t lo = 0, t0, t1, length, at;
   if (sequences > 1 && sequences <= 64) {
     // this lane's sequence: `tiles` row tiles, of the costs behind + 1 to behind + tiles
     const int64_t s  = min(int64_t(lane), sequences - 1);
     const int64_t f0 = token(s), f1 = max(f0, token(s + 1)), n = clamped(a.lengths[s], longest);
-    const int tiles  = lane < sequences ? int(((f1 - f0) * group + kRows - 1) / kRows) : 0;
+    const int tiles  = lane < sequences ? tiles_for(f1 - f0) : 0;
     const int behind = int(min(max(int64_t(0), n - (f1 - f0)) * group / kRows, int64_t(1) << 28));  // beyond, all alike
+    *as              = deal<WHOLE>(a, plan, place, plan.splits > 1 ? uniform(lanes::sum<64>(tiles)) : 0);
+    as->splits       = uniform(as->splits);
+    as->split        = uniform(as->split);
+    const int64_t index = uniform(as->index);
     // the largest cost that more than `index` tiles have or exceed
     const auto reach = [&](int cost) { return lanes::sum<64>(min(max(behind + tiles - cost + 1, 0), tiles)); };
     int some = 0, none = uniform(lanes::max<64>(behind + tiles)) + 1;  // 1 and more, if any has
@@ -124,19 +150,80 @@ __device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan cons
     };
     lo = from, t0 = take(f0), t1 = take(f1), length = take(n);
     at = some - __builtin_amdgcn_readlane(behind, from) - 1;
+  } else if (sequences > 1 && plan.splits > 1) {
+    // a thread's sequences, which follow one another, and the tiles before them
+    __shared__ int s_tiles[kWaves], s_found[2];
+    const int64_t each = (sequences + kThreads - 1) / kThreads, s0 = min(sequences, threadIdx.x * each);
+    const int64_t s1   = min(sequences, s0 + each);
+    int tiles          = 0;
+    int64_t f0         = token(s0);
+#pragma unroll 4
+    for (int64_t s = s0; s < s1; ++s) {
+      const int64_t f1 = token(s + 1);
+      tiles += tiles_for(max(int64_t(0), f1 - f0));
+      f0 = f1;
+    }
+    tiles          = min(max(0, tiles), 1 << 22);  // no more unless first falls
+    const int incl = lanes::scan_incl(tiles);
+    if (lane == 63) { s_tiles[threadIdx.x / 64] = incl; }
+    __syncthreads();
+    int before = incl - tiles, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      before += w < int(threadIdx.x / 64) ? s_tiles[w] : 0;
+      all += s_tiles[w];
+    }
+    all = uniform(all);
+    *as = deal<WHOLE>(a, plan, place, all);
+    as->splits = uniform(as->splits);
+    as->split  = uniform(as->split);
+    if (as->index >= all) { return false; }
+    int left = all - 1 - int(as->index) - before;  // this thread's tile, if it has that one
+    if (left >= 0 && left < tiles) {
+      f0 = token(s0);
+      for (int64_t s = s0; s < s1; ++s) {
+        const int64_t f1 = token(s + 1);
+        const int n      = tiles_for(max(int64_t(0), f1 - f0));
+        if (left < n) {
+          s_found[0] = int(s);
+          s_found[1] = left;
+          break;
+        }
+        left -= n;
+        f0 = f1;
+      }
+    }
+    __syncthreads();
+    lo = uniform(s_found[0]);
+    t0 = token(lo), t1 = token(lo + 1);
+    at     = uniform(s_found[1]);
+    length = clamped(a.lengths[lo], longest);
+  } else if (sequences == 1) {
+    t0 = token(0), t1 = token(1);
+    const int tiles = tiles_for(max(int64_t(0), t1 - t0));
+    *as             = deal<WHOLE>(a, plan, place, tiles);
+    as->splits      = uniform(as->splits);
+    as->split       = uniform(as->split);
+    at              = tiles - 1 - uniform(as->index);
+    length          = clamped(a.lengths[0], longest);
   } else {
-    index = plan.tiles - 1 - index;
+    *as                 = {place, 0, 1};
+    const int64_t index = plan.tiles - 1 - place;
+    const auto begins   = [&](int64_t s) {
+      const int64_t f = token(s);
+      return f * group / kRows + min(s, f);
+    };
     // the last sequence that begins at or before the index, 64 at a time
     for (int64_t n = sequences; n > 0;) {
       const int64_t step = (n + 63) / 64, s = lo + lane * step;
-      const bool before  = s < lo + n && token(s) * group / kRows + s <= index;
+      const bool before  = s < lo + n && begins(s) <= index;
       const int count    = __builtin_popcountll(__ballot(before));
       if (count == 0) { return false; }
       lo += (count - 1) * step;
       n = step == 1 ? 0 : min(step, sequences - lo);
     }
     t0 = token(lo), t1 = token(lo + 1);
-    at     = index - (t0 * group / kRows + lo);
+    at     = index - begins(lo);
     length = clamped(a.lengths[lo], longest);
   }
   const int64_t rows = (t1 - t0) * group;
@@ -155,10 +242,7 @@ __device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan cons
 }
 
 /** The splits of a tile. */
-__device__ __forceinline__ int splits_of(prompt_plan const& plan, int tiles)
-{
-  return max(1, min(plan.splits, tiles / kLeast));
-}
+__device__ __forceinline__ int splits_of(dealt const& as, int tiles) { return max(1, min(as.splits, tiles / kLeast)); }
 
 __device__ __forceinline__ f32x16 mfma32(f16_t, u32x4 a, u32x4 b, f32x16 c)
 {
@@ -297,10 +381,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64;
   const int column = lane % 32, half = lane / 32;
 
-  const int kv        = blockIdx.x % a.kv_heads;
-  const int rest      = blockIdx.x / a.kv_heads;
-  const int split     = rest % plan.splits;
-  const int64_t index = rest / plan.splits;
+  const int kv = blockIdx.x % a.kv_heads;
 
   // rows of no sequence
   {
@@ -315,8 +396,9 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     }
   }
   row_tile rt;
-  if (!find_tile<TILE>(a, plan, index, &rt)) { return; }
-  const int splits = splits_of(plan, rt.tiles);
+  dealt as;
+  if (!find_tile<TILE, false>(a, plan, blockIdx.x / a.kv_heads, &rt, &as)) { return; }
+  const int splits = splits_of(as, rt.tiles), split = as.split;
   if (split >= splits) { return; }
   const int tile0 = int(int64_t(split) * rt.tiles / splits), tile1 = int(int64_t(split + 1) * rt.tiles / splits);
 
@@ -687,7 +769,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     }
     if (half == 0 && first_col == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, base, total, kLift<T>); }
   } else {
-    const int64_t at = ((index * a.kv_heads + kv) * plan.splits + split) * kRows + wave * 32 + column;
+    const int64_t at = (split * a.tokens + rt.token0 + i) * a.heads + head;
 #pragma unroll
     for (int n = 0; n < kCols; ++n) {
 #pragma unroll
@@ -704,52 +786,58 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
 }
 
 /** Rows of a workgroup that joins: fewer, so that there are more. (32 rows: 24 us where 18 was.) */
-constexpr int kJoinRows = 8;
+constexpr int kJoinRows = kThreads / 32;
 
 /** Rows of a tile that was split, 32 threads each: joins their partials in order of position. */
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(prompt_args a, prompt_plan plan)
 {
-  const int kv        = blockIdx.x % a.kv_heads;
-  const int64_t index = blockIdx.x / a.kv_heads;
+  __shared__ float s_factor[kJoinRows][kMaxSplits], s_sum[kJoinRows][kMaxSplits];
+  const int kv = blockIdx.x % a.kv_heads, r = threadIdx.x / 32, lane = threadIdx.x % 32;
   row_tile rt;
-  if (!find_tile<kTile<T>>(a, plan, index, &rt)) { return; }
-  const int n = splits_of(plan, rt.tiles);
-  if (n == 1) { return; }
-  for (int i = threadIdx.x / 32; i < kJoinRows; i += kThreads / 32) {
-    const int r = blockIdx.y * kJoinRows + i, row = rt.row0 + r;
-    if (row >= rt.rows) { return; }
-    const uint32_t token = plan.group(uint32_t(row));
-    const int64_t at     = (rt.token0 + token) * a.heads + kv * int(plan.group.d) + row - int(token * plan.group.d);
-    const int64_t part   = (index * a.kv_heads + kv) * plan.splits * kRows + r;
-    float m = -INFINITY;
-    for (int s = 0; s < n; ++s) { m = fmaxf(m, plan.part_max[part + s * kRows]); }
-    float sum = 0.0f;
-    for (int s = 0; s < n; ++s) {
-      sum += factor_of(plan.scale, plan.part_max[part + s * kRows], m) * plan.part_sum[part + s * kRows];
-    }
-    for (int col = threadIdx.x % 32; col < a.vdim; col += 32) {
-      float acc = 0.0f;
-#pragma unroll 4
-      for (int s = 0; s < n; ++s) {
-        const int64_t slot = part + s * kRows;
-        acc = __builtin_fmaf(factor_of(plan.scale, plan.part_max[slot], m), plan.part_out[slot * a.vdim + col], acc);
-      }
-      static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
-    }
-    if (threadIdx.x % 32 == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, m, sum, kLift<T>); }
+  dealt as;
+  if (!find_tile<kTile<T>, true>(a, plan, blockIdx.x / a.kv_heads, &rt, &as)) { return; }
+  const int n   = splits_of(as, rt.tiles);
+  const int row = rt.row0 + blockIdx.y * kJoinRows + r;
+  if (n == 1 || row - r >= rt.rows) { return; }
+  const uint32_t token = plan.group(uint32_t(min(row, rt.rows - 1)));
+  const int64_t at     = (rt.token0 + token) * a.heads + kv * int(plan.group.d) + min(row, rt.rows - 1) - int(token * plan.group.d);
+  const int64_t next   = a.tokens * a.heads;  // from a split's partials to those of the next
+  // a thread per split (or two) reads them, then all take them in order
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) {
+    s_factor[r][s] = plan.part_max[at + s * next];
+    s_sum[r][s]    = plan.part_sum[at + s * next];
+    m              = fmaxf(m, s_factor[r][s]);
   }
+  m = lanes::max<32>(m);
+  for (int s = lane; s < n; s += 32) { s_factor[r][s] = factor_of(plan.scale, s_factor[r][s], m); }
+  __syncthreads();
+  if (row >= rt.rows) { return; }
+  float sum = 0.0f;
+  for (int s = 0; s < n; ++s) { sum += s_factor[r][s] * s_sum[r][s]; }
+  for (int col = lane; col < a.vdim; col += 32) {
+    float acc = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) { acc = __builtin_fmaf(s_factor[r][s], plan.part_out[(at + s * next) * a.vdim + col], acc); }
+    static_cast<T*>(a.out)[at * a.vdim + col] = T(sum == 0.0f ? 0.0f : acc / sum);
+  }
+  if (lane == 0 && a.lse != nullptr) { a.lse[at] = lse_of(plan.scale, m, sum, kLift<T>); }
 }
 
-/** Tiles of rows over all sequences, at most; one where there is no sequence, for the tokens' zeros. */
+/** Tiles of rows over all sequences, at most: a last one of each that has tokens, and whole ones. One where there is none, for the
+ *  tokens' zeros. */
 int64_t tiles_of(prompt_args const& a)
 {
-  return std::max<int64_t>(1, a.tokens * (a.heads / a.kv_heads) / kRows + a.pages.sequences);
+  return std::max<int64_t>(1, a.tokens * (a.heads / a.kv_heads) / kRows + std::min(a.tokens, a.pages.sequences));
 }
 
-/** Splits of a tile's positions: as many as the chip holds at once where the tiles alone are fewer. One more, which takes a second
- *  round, costs most: bfloat16, 32 heads on 8 of 128, 1,500 tokens 78 us where 61 is now, pieces of up to 20 tokens behind up to 8,000
- *  positions of 16 sequences 76 where 50 is; only prompts whose rows see unequally much and fill 2.7 places had less, 152 for 187 us. */
+/** Splits of a tile's positions, at most: those of one sequence that has all tokens. The kernels count the tiles that there are, and
+ *  take as many splits as the chip holds at once where the tiles alone are fewer (deal). One more, which takes a second
+ *  round, costs most: bfloat16, 32 heads on 8 of 128, 1,500 tokens 78 us where 58 is now; only prompts whose rows see unequally much
+ *  and fill 2.7 places had less, 152 for 187 us. Pieces of up to 20 tokens behind up to 8,000 positions of 16 sequences, 104 us, take
+ *  115 where splits go by the tokens alone, 64 of one token behind 16,383 positions 817 and 1,074; 16 tokens behind 16,000 in a
+ *  table of 64 rows, 59, take 213 where a row counts as a tile. */
 int splits_for(prompt_args const& a, int tile, int per_unit)
 {
   const int64_t most   = int64_t(a.pages.width) * a.pages.page;
@@ -764,7 +852,7 @@ size_t workspace_for(prompt_args const& a)
 {
   // the most splits that any variant takes
   const int splits = std::max(splits_for(a, kTile<T>, 1), splits_for(a, kTile<T>, 3));
-  return splits == 1 ? 0 : sizeof(float) * size_t(tiles_of(a)) * a.kv_heads * splits * kRows * (a.vdim + 2);
+  return splits == 1 ? 0 : sizeof(float) * size_t(a.tokens) * a.heads * splits * (a.vdim + 2);
 }
 
 template <typename T>
@@ -778,18 +866,24 @@ void launch(prompt_args const& a, hipStream_t stream)
     plan.near   = std::max({a.k_page, a.v_page, 8 * a.k_slot, 8 * a.v_slot}) < (int64_t(1) << 32);
     plan.scale  = scale_of(a.shape.any() ? 1.0f : a.scale);
     plan.slack  = float(std::min(double(kSlack<T>) / double(plan.scale.scale2), double(FLT_MAX)));
-    const int64_t slots = int64_t(plan.tiles) * a.kv_heads * plan.splits * kRows;
+    plan.places         = kUnits * kPerUnit<T, D>;
+    const int64_t slots = a.tokens * a.heads * plan.splits;
     plan.part_out       = static_cast<float*>(a.workspace);
     plan.part_max       = plan.part_out + slots * a.vdim;
     plan.part_sum       = plan.part_max + slots;
-    const dim3 grid(uint32_t(plan.tiles) * a.kv_heads * plan.splits, (a.vdim + kColumns<T, D> - 1) / kColumns<T, D>);
+    // a workgroup per tile, or per split of fewer tiles, which are no more than the chip has places
+    const int64_t blocks = int64_t(plan.tiles) * a.kv_heads;
+    const dim3 grid(uint32_t(std::max(blocks, std::min<int64_t>(plan.places, blocks * plan.splits))),
+                    (a.vdim + kColumns<T, D> - 1) / kColumns<T, D>);
     if (a.shape.any()) {
       prompt_kernel<T, D, decltype(how)::value, true><<<grid, kThreads, 0, stream>>>(a, plan);
     } else {
       prompt_kernel<T, D, decltype(how)::value, false><<<grid, kThreads, 0, stream>>>(a, plan);
     }
     if (plan.splits > 1) {
-      join_kernel<T><<<dim3(uint32_t(plan.tiles) * a.kv_heads, kRows / kJoinRows), kThreads, 0, stream>>>(a, plan);
+      // tiles that are split take two places at least
+      const int64_t split = std::min<int64_t>(plan.tiles, plan.places / (2 * a.kv_heads));
+      join_kernel<T><<<dim3(uint32_t(split) * a.kv_heads, kRows / kJoinRows), kThreads, 0, stream>>>(a, plan);
     }
   };
   const auto aligned = [](int64_t elements) { return elements * sizeof(T) % 16 == 0; };

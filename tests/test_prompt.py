@@ -115,3 +115,24 @@ def test_host_tensors_are_refused():
                 dict(value_dim=300)):
         with pytest.raises(ValueError):
             certex.PackedPages(**{**dict(n_pages=2, page_size=8, n_kv_heads=2, head_dim=64), **bad})
+
+
+@pytest.mark.parametrize("tokens, heads, kv, rows, positions, most", [
+    (16, 32, 8, 64, 16_384, 20), (16, 32, 8, 256, 16_384, 20), (64, 32, 8, 64, 16_384, 40), (1_000, 8, 8, 1_000, 4_096, 40),
+    (1, 64, 8, 1_024, 131_072, 20), (8, 32, 8, 4_096, 32_768, 20), (128, 32, 32, 128, 8_192, 40), (1, 8, 8, 65_535, 32_704, 1),
+    (2_000, 32, 8, 2_000, 32_768, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_workspace_is_of_the_tokens(tokens, heads, kv, rows, positions, most, dtype, d):
+    """Few tokens in tables of many rows: MB of partials (heads of 128; in proportion to the dimension), a row for each token, head and
+    split, whatever rows the table has."""
+    pool = (4, 64, kv, d)
+    got = _prompt(q=(tokens, heads, d), k=pool, v=pool, table=(rows, positions // 64), dtype=dtype)
+    # (heads of 64 run three workgroups per compute unit, those of 128 two)
+    assert got <= most * 1e6 * max(1.0, (d + 2) / 128) * 1.5
+    assert got == _prompt(q=(tokens, heads, d), k=pool, v=pool, table=(1, positions // 64), dtype=dtype)
+
+
+def test_prompt_tables_of_any_rows():
+    """What a call may launch goes by its tokens: a table of the most rows is no reason to refuse one."""
+    assert _prompt(q=(1, 256, 64), k=(4, 16, 256, 64), v=(4, 16, 256, 64), table=(65_535, 2)) >= 0
