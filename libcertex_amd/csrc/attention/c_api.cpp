@@ -272,6 +272,13 @@ auto frequencies_of(cuvsCertexRotaryParams const& p, double* magnitude) -> std::
   return f;
 }
 
+/** The window, cut to 2^32, which holds all positions: what the kernels add to it and take from it stays far from 64 bits' ends. */
+auto window_of(int64_t window) -> int64_t
+{
+  EXPECTS(window >= 0, "the window must not be negative");
+  return std::min(window, int64_t(1) << 32);
+}
+
 /** Queries, pages and table of an attention call, checked against each other. With `prompts` the queries are tokens of
  *  any of the table's sequences, else one of each. */
 template <typename Args>
@@ -301,7 +308,7 @@ auto paged_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v_
   EXPECTS(table->shape[0] <= 65535, "at most 65535 sequences");
   EXPECTS(k->shape[1] % ops::kPageUnit == 0 && k->shape[1] >= ops::kPageUnit,
           "the page size must be a multiple of " + std::to_string(ops::kPageUnit));
-  EXPECTS(window >= 0, "the window must not be negative");
+  a.window = window_of(window);
   a.pages  = page_map_of(*table, table->shape[0], *k);
   a.q      = q->p;
   a.q_head = q->stride[1];
@@ -313,7 +320,6 @@ auto paged_args_of(DLManagedTensor* q_, DLManagedTensor* k_, DLManagedTensor* v_
   a.v_page = v->stride[0];
   a.v_slot = v->stride[1];
   a.v_head = v->stride[2];
-  a.window = window;
   return a;
 }
 
@@ -401,7 +407,6 @@ auto packed_args_of(DLManagedTensor* q_, DLManagedTensor* pages_, int64_t vdim, 
   EXPECTS(q->shape[1] >= 1 && q->shape[1] <= 65535 && q->shape[1] % args.pages.kv_heads == 0,
           "the query heads must be a multiple of the key heads (and at most 65535)");
   EXPECTS(table->shape[0] == q->shape[0], "page_table must have one row per sequence");
-  EXPECTS(window >= 0, "the window must not be negative");
   a.heads    = int32_t(q->shape[1]);
   a.kv_heads = args.pages.kv_heads;
   a.dim      = int32_t(q->shape[2]);
@@ -410,7 +415,7 @@ auto packed_args_of(DLManagedTensor* q_, DLManagedTensor* pages_, int64_t vdim, 
   a.q        = q->p;
   a.q_seq    = q->stride[0];
   a.q_head   = q->stride[1];
-  a.window   = window;
+  a.window   = window_of(window);
   return args;
 }
 

@@ -7,7 +7,7 @@ import torch
 
 import libcertex_amd as certex
 from libcertex_amd import _capi as C
-from tests.test_paged import _tensor
+from tests.test_paged import _need, _tensor
 
 
 def _prompt(q=(20, 8, 64), k=(4, 16, 2, 64), v=(4, 16, 2, 64), table=(2, 2), dtype=torch.float16, k_type=None, window=0,
@@ -136,3 +136,12 @@ def test_prompt_workspace_is_of_the_tokens(tokens, heads, kv, rows, positions, m
 def test_prompt_tables_of_any_rows():
     """What a call may launch goes by its tokens: a table of the most rows is no reason to refuse one."""
     assert _prompt(q=(1, 256, 64), k=(4, 16, 256, 64), v=(4, 16, 256, 64), table=(65_535, 2)) >= 0
+
+
+@pytest.mark.parametrize("window", [2**31, 2**32 + 1, 2**63 - 129, 2**63 - 1])
+def test_windows_past_all_positions(window):
+    """A window that holds every position is none: the same splits and shares, whatever is added to it."""
+    few = dict(q=(1, 32, 64), k=(4, 64, 8, 64), v=(4, 64, 8, 64), table=(1, 2048))
+    assert _prompt(**few, window=window) == _prompt(**few) > 0
+    assert _packed(table=(2, 2000), window=window) == _packed(table=(2, 2000)) > 0
+    assert _need(table=(2, 2000), window=window) == _need(table=(2, 2000)) > 0

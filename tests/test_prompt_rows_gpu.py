@@ -101,3 +101,18 @@ def test_workspace_is_enough(gpu):
         torch.cuda.synchronize()
         assert (work[bytes_.value :] == 0x5A).all()
         assert torch.equal(out, certex.prompt_attention(q, pool, pool, table, lens, first))
+
+
+@pytest.mark.parametrize("window", [2**31, 2**32 + 1, 2**63 - 129, 2**63 - 1])
+def test_windows_past_all_positions(gpu, window):
+    """A window that holds every position is none, also of tokens before position 0."""
+    dtype = torch.bfloat16
+    kp, vp, table, keys, values = paged([40, 600], 16, 2, 64, 64, dtype, seed=76)
+    q, lens, first = rand(250, 4, 64, dtype=dtype), ints([40, 600]), ints([0, 200, 250])
+    want = certex.prompt_attention(q, kp, vp, table, lens, first, return_lse=True)
+    for got, x in zip(certex.prompt_attention(q, kp, vp, table, lens, first, window=window, return_lse=True), want):
+        assert torch.equal(got, x)
+    ref.check(want[0][160:200], want[1][160:200], ref.attend(q[160:200], torch.arange(40), keys[0], values[0], 0.125,
+                                                             weight=weight_unit(dtype)))
+    one = q[:2].contiguous()
+    assert torch.equal(certex.paged_attention(one, kp, vp, table, lens, window=window), certex.paged_attention(one, kp, vp, table, lens))
