@@ -2,7 +2,8 @@
 //
 // Of every 64 elements x of a head: offset o = float16(min x), scale s = float16((max x - o) * (1 / 15 as float32)), and codes
 // c = round((x - o) / s) in 0..15, so that o + s c is x within s / 2 (and what o and s are rounded by). Which of two codes is
-// nearer is decided in 64 bits: the distance x - o is exact there, and so is its remainder x - o - s c.
+// nearer is decided in 64 bits: the distance x - o and what it is rounded by together are exact, and so is the rounded distance's
+// remainder x - o - s c, which only at half a step the rounding tells apart.
 //
 // What bounds it: every element is read once, and its half byte written. 16 lanes take a group, 4 elements each, and a wave the groups
 // of 4 heads, so that the group's minimum and maximum are 4 exchanges away. The 64-bit distance is taken only where an element of the
@@ -171,10 +172,13 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(pack_args a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const double distance = double(x[i]) - double(o), rest = __builtin_fma(-double(code[i]), double(s), distance);
+          const double of_o = distance - double(x[i]), lost = (double(x[i]) - (distance - of_o)) - (double(o) + of_o);
+          const double half = 0.5 * double(s);
           // half a step to either side goes to the even code
-          if (rest > 0.5 * double(s) || (rest == 0.5 * double(s) && (code[i] & 1) != 0)) {
+          const bool odd = (code[i] & 1) != 0;
+          if (rest > half || (rest == half && (lost > 0.0 || (lost == 0.0 && odd)))) {
             code[i] = min(code[i] + 1, 15);
-          } else if (rest < -0.5 * double(s) || (rest == -0.5 * double(s) && (code[i] & 1) != 0)) {
+          } else if (rest < -half || (rest == -half && (lost < 0.0 || (lost == 0.0 && odd)))) {
             code[i] = max(code[i] - 1, 0);
           }
         }

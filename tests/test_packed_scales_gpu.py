@@ -50,3 +50,23 @@ def test_nan_hides_no_steep_scale(gpu, dtype, nan, steep):
         v[steep, :, 64:] *= times
         v[nan, :, 3] = float("nan")
         check_columns(k, v, q, torch.arange(64, 128))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low, tiny, code", [
+    (-6.5, 2.0**-60, 7), (-6.5, -(2.0**-60), 6), (-6.5, 2.0**-120, 7), (-6.5, 0.0, 6), (-7.5, -(2.0**-60), 7), (-7.5, 2.0**-60, 8),
+    (-7.5, 0.0, 8), (-0.5, 2.0**-60, 1), (-14.5, -(2.0**-60), 14)])
+def test_codes_next_to_a_tie(gpu, dtype, low, tiny, code):
+    """Elements from `low` to low + 15, of scale 1: one next to 0 is past the middle of two codes by less than 64 bits hold of the
+    distance from the offset."""
+    x = torch.linspace(low, low + 15, 16).repeat(4)
+    x[20] = tiny
+    pages = certex.PackedPages(1, 8, 1, 64)
+    k = x.to(dtype).cuda()[None, None]
+    assert float(k[0, 0, 20]) == tiny
+    table, position = ints([[0]]), ints([3])
+    pages.append(k, k, table, position)
+    for side in pages.read(table, position, dtype=torch.float32):
+        want = x.clone()
+        want[20] = low + code
+        assert torch.equal(side[0, 0].cpu(), want)
