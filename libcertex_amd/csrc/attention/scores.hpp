@@ -13,9 +13,11 @@ struct score_shape {
 };
 
 /**
- * tanh(u) within 2 units in the last place, NaN where u is. Up to 0.6 in size the fifth convergent of its
- * continued fraction, u (945 + 105 u^2 + u^4) / (945 + 420 u^2 + 15 u^4), which is off by u^10 / (945 * 10395) of it, 6e-10;
- * beyond (e - 1) / (e + 1) with e = 2^(2 log2(e) |u|), where e - 1 loses no more than one bit. One reciprocal for both.
+ * tanh(u) within 3 units in the last place, NaN where u is, if the exponential and the reciprocal are within one. With s = u^2, up to
+ * 0.6 in size u - u s (315 + 14 s) / (945 + 420 s + 15 s^2), the fifth convergent of its continued fraction less u: it is off by
+ * u^10 / (945 * 10395) of it, 6e-10, and what is taken from u is 0.105 u at most, so that its roundings (7.3 halves of a unit) weigh an
+ * eighth. Beyond 1 - 2 / (e + 1) with e = 2^(2 log2(e) |u|): roundings of e weigh 2 e / (e + 1)^2, 0.36 at most, those of the
+ * quotient 0.46. One reciprocal for both.
  */
 __device__ __forceinline__ float tanh_of(float u)
 {
@@ -23,9 +25,10 @@ __device__ __forceinline__ float tanh_of(float u)
   const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * kLog2e));
   const float s = u * u;
   const bool small = a < 0.6f;
-  const float over = small ? a * __builtin_fmaf(s, s + 105.0f, 945.0f) : e - 1.0f;
+  const float over = small ? s * __builtin_fmaf(s, 14.0f, 315.0f) : 2.0f;
   const float under = small ? __builtin_fmaf(s, __builtin_fmaf(s, 15.0f, 420.0f), 945.0f) : e + 1.0f;
-  return __builtin_copysignf(over * __builtin_amdgcn_rcpf(under), u);
+  const float whole = small ? a : 1.0f;
+  return __builtin_copysignf(__builtin_fmaf(-whole, over * __builtin_amdgcn_rcpf(under), whole), u);
 }
 
 /** The bent score of a product x; per_cap = scale / cap. */
