@@ -32,10 +32,12 @@ __device__ __forceinline__ uint32_t lds_address(const void* p)
 
 /** 16 bytes a lane from base + offset to LDS byte m0 + 16 lane. In assembly, so that the compiler does not order LDS reads
  *  against it: the kernels see to it that what is copied over has been read, and wait for vmcnt before they read the copy.
- *  (It is among the loads that the compiler's own waits pass over in order: those can only wait longer.) */
+ *  (It is among the loads that the compiler's own waits pass over in order: those can only wait longer.) Nor does the compiler see
+ *  that it reads scalar registers: a vector instruction that writes one (a lane read, as where scalars are spilled) has to be 5 wait
+ *  states before, which are here. */
 __device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t m0)
 {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
                "s"(uniform(static_cast<const char*>(base))), "s"(m0)
                : "m0", "memory");
 }
