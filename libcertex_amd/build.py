@@ -57,6 +57,8 @@ COMMON = [
     "-Xclang",
     "-packed-fp32-ops",
     "-Wno-unused-command-line-argument",
+    # assembly that clobbers a reserved register leaves it undefined
+    "-Werror=inline-asm",
 ]
 
 

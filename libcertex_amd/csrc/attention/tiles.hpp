@@ -34,16 +34,15 @@ __device__ __forceinline__ uint32_t lds_address(const void* p)
  *  against it: the kernels see to it that what is copied over has been read, and wait for vmcnt before they read the copy.
  *  (It is among the loads that the compiler's own waits pass over in order: those can only wait longer.) Nor does the compiler see
  *  that it reads scalar registers: a vector instruction that writes one (a lane read, as where scalars are spilled) has to be 5 wait
- *  states before, which are here. */
+ *  states before, which are here. M0 is an operand, which the compiler writes: named as clobbered it would be undefined. */
 __device__ __forceinline__ void copy_to_lds(const void* base, uint32_t offset, uint32_t m0)
 {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
-               "s"(uniform(static_cast<const char*>(base))), "s"(m0)
-               : "m0", "memory");
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(uniform(static_cast<const char*>(base))), "{m0}"(m0)
+               : "memory");
 }
 __device__ __forceinline__ void copy_to_lds(const void* from, uint32_t m0)
 {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(m0) : "m0", "memory");
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(m0) : "memory");
 }
 
 /** n / d for n < 2^29 by a product: m = ceil(2^(29 + s) / d) with 2^s >= d exceeds 2^(29 + s) / d by less

@@ -86,16 +86,16 @@ __device__ __forceinline__ void wait_copies()
  *  as inline assembly: the compiler then neither counts it among the loads it waits for nor orders
  *  LDS reads against it (it models such copies as LDS stores of unknown address and would wait for
  *  every LDS read before each copy). The kernel orders the copies itself: a stage's copies target
- *  a buffer that no wave reads, and s_waitcnt vmcnt plus a barrier publish them. An LDS-DMA
- *  instruction needs one wait state after the write of M0. */
+ *  a buffer that no wave reads, and s_waitcnt vmcnt plus a barrier publish them. M0 is an operand, which the
+ *  compiler writes (named as clobbered it would be undefined); the copy may read it 5 wait states after a lane read wrote it. */
 template <int B>
 __device__ __forceinline__ void lds_copy(const void* g, uint32_t m0)
 {
   if constexpr (B == 16) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(m0) : "m0");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(m0));
   } else {
     static_assert(B == 4, "4 or 16 bytes per lane");
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(m0) : "m0");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(g), "{m0}"(m0));
   }
 }
 

@@ -63,3 +63,12 @@ def test_copies_to_lds_wait_for_their_address(tmp_path):
     states = wait_states(assembly)
     assert len(states) == 2 and states[0] is not None, said  # the probe does read lanes for the first copy's address
     assert all(n is None or n >= 5 for n in states), states
+
+
+def test_copies_to_lds_clobber_no_reserved_register(tmp_path):
+    """The copies' register M0 is an operand: named as clobbered, which the compiler only warns of, it would be undefined."""
+    assert "-Werror=inline-asm" in build.COMMON
+    assembly, said = compiled(tmp_path, PROBE)
+    assert assembly and "reserved register" not in said, said
+    assembly, said = compiled(tmp_path, PROBE.replace("vmcnt(0)\" ::: ", "vmcnt(0)\" ::: \"m0\", "))
+    assert assembly is None and "reserved register" in said
