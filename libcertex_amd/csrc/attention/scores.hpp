@@ -21,14 +21,18 @@ struct score_shape {
  */
 __device__ __forceinline__ float tanh_of(float u)
 {
-  const float a = __builtin_fabsf(u);
-  const float e = __builtin_amdgcn_exp2f((a > 15.0f ? 15.0f : a) * (2.0f * kLog2e));
-  const float s = u * u;
-  const bool small = a < 0.6f;
-  const float over = small ? s * __builtin_fmaf(s, 14.0f, 315.0f) : 2.0f;
-  const float under = small ? __builtin_fmaf(s, __builtin_fmaf(s, 15.0f, 420.0f), 945.0f) : e + 1.0f;
-  const float whole = small ? a : 1.0f;
-  return __builtin_copysignf(__builtin_fmaf(-whole, over * __builtin_amdgcn_rcpf(under), whole), u);
+  const float a = __builtin_fabsf(u), s = u * u;
+  const float e = __builtin_amdgcn_exp2f(a * (2.0f * kLog2e));  // infinite: 2 / (e + 1) is 0
+  // by a mask that the compiler does not look into: it makes branches of such conditions, 32 a tile in prompts' kernels, and spills
+  uint32_t small = a < 0.6f ? 0xffffffffu : 0u;
+  asm("" : "+v"(small));
+  const auto pick = [small](float x, float y) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & small) | (__builtin_bit_cast(uint32_t, y) & ~small));
+  };
+  const float over  = pick(s * __builtin_fmaf(s, 14.0f, 315.0f), 2.0f);
+  const float under = pick(__builtin_fmaf(s, __builtin_fmaf(s, 15.0f, 420.0f), 945.0f), e + 1.0f);
+  const float whole = pick(u, __builtin_copysignf(1.0f, u));
+  return __builtin_fmaf(-whole, over * __builtin_amdgcn_rcpf(under), whole);
 }
 
 /** The bent score of a product x; per_cap = scale / cap. */
