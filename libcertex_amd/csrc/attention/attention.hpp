@@ -132,6 +132,10 @@ __host__ __device__
 #endif
 constexpr int packed_chunks(int dim) { return dim <= 64 ? 2 : dim <= 96 ? 3 : dim <= 128 ? 4 : dim <= 192 ? 6 : 8; }
 
+/** Words that every piece of a packed key begins at a multiple of, which is a word of each chunk: keys of `chunks` chunks, or (not
+ *  `full`) of any number up to that. */
+constexpr int packed_key_align(int chunks, bool full) { return !full ? 1 : chunks % 4 == 0 ? 4 : chunks % 2 == 0 ? 2 : 1; }
+
 /**
  * 4-bit pages, [n_pages][kv_heads][page / 8] records of 8 positions of a head. Every group of 64 elements of a key or value
  * has a scale s and an offset o (float16); an element is o + s code. A record holds, for C chunks of 32 dimensions and

@@ -81,7 +81,7 @@ __device__ __forceinline__ void landed(int n)
   }
 }
 
-/** N words of LDS; N and `from` are multiples of ALIGN words. */
+/** N words of LDS, which begin at a multiple of ALIGN words. */
 template <int N, int ALIGN>
 __device__ __forceinline__ void read_words(uint32_t* to, const uint8_t* from)
 {
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
 #pragma unroll
         for (int n = 0; n < G; ++n) { s[half][n] = f32x4{0, 0, 0, 0}; }
         uint32_t k[C];
-        read_words<C, C == 4 || C == 8 ? 4 : C % 2 == 0 ? 2 : 1>(
+        read_words<C, packed_key_align(C, FULL)>(
           k, FULL ? rows_ + (half * 4 + r % 4) * 16 * C + g * 4 * C : rows_ + (half * 4 + r % 4) * 16 * k_chunks + g * 4 * k_chunks);
 #pragma unroll
         for (int c = 0; c < C; ++c) {

@@ -1,5 +1,6 @@
 """What compiled assembly has to hold that neither the compiler nor a run shows reliably."""
 
+import os
 import re
 import subprocess
 
@@ -72,3 +73,13 @@ def test_copies_to_lds_clobber_no_reserved_register(tmp_path):
     assert assembly and "reserved register" not in said, said
     assembly, said = compiled(tmp_path, PROBE.replace("vmcnt(0)\" ::: ", "vmcnt(0)\" ::: \"m0\", "))
     assert assembly is None and "reserved register" in said
+
+
+def test_packed_keys_are_aligned_as_promised(tmp_path):
+    """csrc/attention/attention.hpp: every piece of a packed key, for all head dimensions, begins where the kernels say."""
+    exe = tmp_path / "packed_align"
+    source = os.path.join(os.path.dirname(__file__), "c", "packed_align.cpp")
+    subprocess.run([build.HIPCC, "-x", "hip", *build.COMMON, "--offload-host-only", "-I", build.CSRC, "-fvisibility=default", source,
+                    "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout
