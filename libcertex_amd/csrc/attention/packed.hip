@@ -14,9 +14,10 @@
 // offsets are one piece of memory.
 // - Queries enter as float16, scaled by a power of two that brings a row's largest to [2^13, 2^14): 16-bit types whole
 //   (what is 2^-28 of the largest loses bits, none that float32 sums would keep), float32 as three elements of 11 bits.
-// - p_t s_t enters as the nearest float16 where queries (and outputs) are of 16 bits, 2^-11 of it off at most, which
-//   is what float16 outputs are rounded by and an eighth of bfloat16's; as two elements of 11 bits for float32. p's reference is
-//   kept such that the largest is below 2^15. Their sum is not rounded.
+// - p_t s_t enters as two elements of 11 bits, the nearest float16 and what it leaves: 2^-21 of it off at most. (One element
+//   would be 2^-11 off, as much as float16 outputs are rounded; 64 sequences 68 us instead of 75.) p's reference is
+//   kept such that the largest is below 2^15. Their sum is not rounded. The elements reach down to 2^-24, so that positions and
+//   groups keep these bits while their p_t s_t are within 2^17 of the largest, and lose one with each power of 2 below.
 // - Products of subnormal numbers keep fewer of their low bits beside large sums, so that float32 takes other
 //   codes: less 8, as normal numbers (two operations more each), whose sums stay small; and joins steps outside the products.
 // Work is dealt as in attend.hip (shares.hpp). A wave copies its next step to LDS while it works on one, by itself: what it
@@ -458,7 +459,7 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
       for (int n = 0; n < G; ++n) {
         if (!FULL && n >= v_groups) { break; }
         // p s of the group in the order of the codes' words (0, 2), (1, 3), (4, 6), (5, 7): the nearest, and what it leaves
-        u32x4 part[FINE ? 2 : 1];
+        u32x4 part[2];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int j = w / 2 * 4 + w % 2;
@@ -469,11 +470,9 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
           shift[n] = __builtin_fmaf(p[j], half_of(vo[n][j / 2], j % 2), shift[n]);
           shift[n] = __builtin_fmaf(p[j + 2], half_of(vo[n][j / 2 + 1], j % 2), shift[n]);
           part[0][w] = pack2<f16_t>(lo, hi);
-          if (FINE) {
-            lo         = __builtin_fmaf(half_of(part[0][w], 0), -1.0f, lo);
-            hi         = __builtin_fmaf(half_of(part[0][w], 1), -1.0f, hi);
-            part[1][w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
-          }
+          lo         = __builtin_fmaf(half_of(part[0][w], 0), -1.0f, lo);
+          hi         = __builtin_fmaf(half_of(part[0][w], 1), -1.0f, hi);
+          part[1][w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
         }
         uint32_t v[4] = {0, 0, 0, 0};
         const bool pair = 2 * n + 1 < C && (FULL || 2 * n + 1 < v_chunks);  // a unit of 64 dimensions, else of 32
@@ -494,8 +493,8 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
             o[c][0] += mfma(f16_t{}, even, part[0], mfma(f16_t{}, even, part[1], zero));
             o[c][1] += mfma(f16_t{}, odd, part[0], mfma(f16_t{}, odd, part[1], zero));
           } else {
-            o[c][0] = mfma(f16_t{}, even, part[0], o[c][0]);
-            o[c][1] = mfma(f16_t{}, odd, part[0], o[c][1]);
+            o[c][0] = mfma(f16_t{}, even, part[0], mfma(f16_t{}, even, part[1], o[c][0]));
+            o[c][1] = mfma(f16_t{}, odd, part[0], mfma(f16_t{}, odd, part[1], o[c][1]));
           }
         }
       }

@@ -70,3 +70,23 @@ def test_codes_next_to_a_tie(gpu, dtype, low, tiny, code):
         want = x.clone()
         want[20] = low + code
         assert torch.equal(side[0, 0].cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 192, 40])
+@pytest.mark.parametrize("n", [7, 33, 120])
+def test_weights_enter_whole(gpu, dtype, d, n):
+    """Outputs of every type are as far off as float32 sums of them, however small they are beside the values: weights times scales
+    meet the codes as two elements of 11 bits, the second cut (2^-21 of them at most), after one product (2^-24). Queries of 0 and slopes:
+    the scores are nearly exact, so that little else is off, and among the outputs of many heads some are near 0."""
+    heads = 64
+    k, v = rand(n, 2, d, dtype=dtype), rand(n, 2, d, dtype=dtype, seed=1)
+    q, slopes = torch.zeros(1, heads, d, dtype=dtype, device="cuda"), torch.linspace(0.001, 0.1, heads, device="cuda")
+    pages = certex.PackedPages(-(-n // 16), 16, 2, d)
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device="cuda").flip(0)[None]
+    positions = torch.arange(n, device="cuda")
+    pages.append(k, v, table, positions, sequences=torch.zeros_like(positions))
+    out, lse = pages.attend(q, table, ints([n]), return_lse=True, slopes=slopes)
+    (keys, key_sizes), (values, value_sizes) = pack.stored(k), pack.stored(v)
+    ref.check(out, lse, ref.attend(q, torch.tensor([n - 1]), keys, values, d**-0.5, weight=2.0**-21 + 2.0**-24, key_sizes=key_sizes,
+                                   value_sizes=value_sizes, slopes=slopes))
