@@ -175,7 +175,7 @@ CUVS_EXPORT cuvsError_t cuvsCertexPagedAttentionShaped(cuvsResources_t res,
  * [n_sequences + 1] that do not decrease; prefix (or NULL): dense integers [n_sequences]; out: dense [tokens, heads, vdim];
  * lse (or NULL): dense float32 [tokens, heads]. Tokens that see no position (before position 0: more tokens than the
  * length), and tokens of no sequence, give zeros, and lse -inf. Missing pages, slots past a length and infinite values as for
- * cuvsCertexPagedAttention, except that a value shows in the rows that see it and in no other. The weights of 16-bit types are rounded to the type before they meet the values.
+ * cuvsCertexPagedAttention, except that a value shows in the rows that see it and in no other.
  * workspace: a dense uint8 vector of at least the bytes that cuvsCertexPromptAttentionWorkspace reports for the same tensors
  * (NULL if 0), in use until the queued work is done.
  */

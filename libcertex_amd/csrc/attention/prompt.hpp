@@ -13,8 +13,9 @@
 //   scaling are per lane; the products begin at -m, so that they end as distances from the reference.
 // - The rows of S^T that a lane holds are the positions that it feeds to O^T = V^T P^T: the weights never move.
 //   V is turned on its way into LDS, in the order of positions of these rows.
-// - Weights are rounded to the element type for the second product (bfloat16 2^-8, float16 2^-11 of them at most); their
-//   sum is not. The output is rounded as much again, and weights with twice the bits would cost half as many products more.
+// - Weights of 16-bit types enter the second product as two elements, the nearest and what it leaves (bfloat16 2^-16, float16
+//   2^-22 of them off at most); their sum is not rounded. One element would be 2^-8 and 2^-11 off, as much again as the output is
+//   rounded, for half as many products less: 8,192 tokens 670 us where 830 is.
 // - Tiles of positions are in two buffers: the next one's loads are in flight during the products.
 //
 // Work is dealt without reading the lengths back: the host launches as many tiles of rows as there may be, the
@@ -706,19 +707,22 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
         for (int i = 0; i < kAhead; ++i) { v[i] = value_at(i / kCols, i % kCols); }
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
-          u32x4 w;
+          u32x4 w, rest;  // the weights, and what rounding them to 16 bits leaves
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if constexpr (WIDE) {
               w[e] = __builtin_bit_cast(uint32_t, float(s[0][4 * m + e]));
             } else {
-              w[e] = pack2<T>(s[m / 2][8 * (m % 2) + 2 * e], s[m / 2][8 * (m % 2) + 2 * e + 1]);
+              const float even = s[m / 2][8 * (m % 2) + 2 * e], odd = s[m / 2][8 * (m % 2) + 2 * e + 1];
+              w[e]             = pack2<T>(even, odd);
+              rest[e]          = pack2<T>(even - lower<T>(w[e]), odd - upper<T>(w[e]));
             }
           }
 #pragma unroll
           for (int n = 0; n < kCols; ++n) {
             const int i = m * kCols + n;
             o[n]        = mfma32(T{}, v[i % kAhead], w, o[n]);
+            if constexpr (!WIDE) { o[n] = mfma32(T{}, v[i % kAhead], rest, o[n]); }
             if (i + kAhead < kSteps * kCols) { v[i % kAhead] = value_at((i + kAhead) / kCols, (i + kAhead) % kCols); }
           }
           __builtin_amdgcn_sched_barrier(0);

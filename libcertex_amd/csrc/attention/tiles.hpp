@@ -76,4 +76,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), two));
 }
 
+/** The elements of a word. */
+template <typename T>
+__device__ __forceinline__ float lower(uint32_t w)
+{
+  using two = __attribute__((ext_vector_type(2))) T;
+  return float(__builtin_bit_cast(two, w)[0]);
+}
+template <typename T>
+__device__ __forceinline__ float upper(uint32_t w)
+{
+  using two = __attribute__((ext_vector_type(2))) T;
+  return float(__builtin_bit_cast(two, w)[1]);
+}
+
 }  // namespace certex_amd::attention

@@ -132,7 +132,7 @@ def prompt_attention(q, k_pages, v_pages, page_table, lengths, first, scale=None
 
     A token at position p sees the positions t <= p of its sequence, and with prefix (n_sequences,) those below
     prefix[s] too; with a window only those less than `window` before it (t > p - window). Scores, cap and slopes as in
-    paged_attention, slopes times |p - t|. Weights of 16-bit types are rounded to the type before they meet the values.
+    paged_attention, slopes times |p - t|.
 
     Tokens that see nothing (more tokens than the length has positions) and tokens of no sequence give zeros. Lengths, missing
     pages, unused slots, return_lse and the cache's sizes as in paged_attention; an infinite value shows in the rows that see it."""

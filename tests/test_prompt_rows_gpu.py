@@ -116,3 +116,19 @@ def test_windows_past_all_positions(gpu, window):
                                                              weight=weight_unit(dtype)))
     one = q[:2].contiguous()
     assert torch.equal(certex.paged_attention(one, kp, vp, table, lens, window=window), certex.paged_attention(one, kp, vp, table, lens))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 192, 256, 40])
+@pytest.mark.parametrize("n, past", [(7, 0), (33, 0), (20, 100), (3, 1_500)])
+def test_weights_enter_whole(gpu, dtype, d, n, past):
+    """Outputs of 16-bit types are nearly as far off as float32 sums of their values, however small they are beside these: a weight is the
+    sum of two elements of the type, each the nearest, so that it is off by the square of the type's half unit (and float32's). Queries
+    of 0 and slopes: the scores are nearly exact, so that little else is off, and among the outputs of many heads some are near 0."""
+    heads = 16
+    slopes = torch.linspace(0.001, 0.1, heads, device="cuda")
+    kp, vp, table, keys, values = paged([past + n], 16, 2, d, d, dtype, seed=77)
+    q = torch.zeros(n, heads, d, dtype=dtype, device="cuda")
+    out, lse = certex.prompt_attention(q, kp, vp, table, ints([past + n]), ints([0, n]), slopes=slopes, return_lse=True)
+    weight = 0.0 if dtype == torch.float32 else weight_unit(dtype) ** 2
+    ref.check(out, lse, ref.attend(q, torch.arange(past, past + n), keys[0], values[0], d**-0.5, slopes=slopes, weight=weight))
