@@ -26,7 +26,7 @@ def capped(u, operator):
 
 
 @pytest.mark.parametrize("operator", ["paged", "prompt"])
-@pytest.mark.parametrize("lo, hi", [(1e-30, 1e-3), (1e-3, 0.3), (0.3, 0.6), (0.59, 0.61), (0.6, 1.0), (1.0, 2.0), (2.0, 9.1), (9.0, 1e30)])
+@pytest.mark.parametrize("lo, hi", [(1e-30, 1e-3), (1e-3, 0.3), (0.3, 0.6), (0.59, 0.61), (0.6, 1.0), (0.79, 0.81), (1.0, 2.0), (2.0, 9.1), (9.0, 1e30)])
 def test_tanh(gpu, operator, lo, hi):
     """3 units in the last place (derived where tanh_of is), on both sides of where its form changes and of 0."""
     g = torch.Generator(device="cuda").manual_seed(1)
@@ -44,3 +44,33 @@ def test_tanh_ends(gpu, operator):
     u = torch.tensor([0.0, 1e-38, 15.0, 1e38, -1e38, float("nan")], device="cuda")
     got = capped(u, operator)
     assert got[:5].tolist() == [0.0, float(u[1]), 1.0, 1.0, -1.0] and got[5].isnan()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("operator", ["paged", "prompt", "packed"])
+@pytest.mark.parametrize("cap", [5.0, 50.0, 64.0, 1000.0])
+def test_capped_scores(gpu, operator, dtype, cap):
+    """cap tanh(x / cap) of one position in every type, small beside the cap and not: 3 units of tanh, and a rounding of 1 / cap, of its
+    product with x (neither weighs more in tanh than in its argument) and of the product with cap, half a unit each of what may be a
+    unit of half the size: 6 units in the last place."""
+    heads = 30_000
+    key = torch.zeros(1, 8, 1, 64, device="cuda", dtype=dtype)
+    key[..., 0] = 1
+    q = torch.zeros(1, heads, 64, device="cuda", dtype=dtype)
+    q[0, :, 0] = (torch.logspace(-4, 2.5, heads, device="cuda") * torch.where(torch.arange(heads, device="cuda") % 2 == 0, 1, -1)).to(dtype)
+    how = dict(scale=1.0, cap=cap, return_lse=True)
+    if operator == "packed":
+        # elements of 0 and 1 are held exactly, as codes 0 and 15 of a scale that float16 rounds: the key is what the pages hold
+        pages = certex.PackedPages(1, 8, 1, 64)
+        pages.append(key[:, 0], key[:, 0], ints([[0]]), ints([0]))
+        x = q[0, :, 0].double() * pages.read(ints([[0]]), ints([0]), dtype=torch.float32)[0][0, 0, 0].double()
+        lse = pages.attend(q, ints([[0]]), ints([1]), **how)[1]
+    else:
+        x = q[0, :, 0].double()
+        if operator == "paged":
+            lse = certex.paged_attention(q, key, key, ints([[0]]), ints([1]), **how)[1]
+        else:
+            lse = certex.prompt_attention(q, key, key, ints([[0]]), ints([1]), ints([0, 1]), **how)[1]
+    want = cap * torch.tanh(x / cap)
+    unit = 2.0 ** (torch.frexp(want)[1] - 24).double()
+    assert float(((lse[0].double() - want).abs() / unit).max()) <= (8.0 if operator == "packed" else 6.0)  # (packed: its product's, too)
