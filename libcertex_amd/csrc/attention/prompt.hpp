@@ -21,15 +21,16 @@
 // Work is dealt without reading the lengths back: the host launches as many tiles of rows as there may be, the
 // kernel finds the sequence of each. The last rows of a prompt see most and go first. Where tiles are too few to
 // fill the chip their positions are split over workgroups, which leave partials (m, sum, output) for join_kernel. The kernels count
-// the tiles for that: rows of a page table that have no new tokens take no part of the chip, and no workspace.
+// what the tiles see for that: rows of a page table that have no new tokens take no part of the chip, and no workspace.
 //
-// Measured (bfloat16, 32 heads on 8 of 128; products alone reach 1,227 TFLOP/s): a prompt of 8,192 tokens 658 to 683 us,
-// 805 to 835 TFLOP/s (one at a time, traced: 754); 512 capped tokens behind 65,536 positions 855 to 885 with 14 for the join,
-// 625 to 645: the scores' vector operations are in the products' way. Seven prompts of up to 2,000 tokens, 16 leaning heads of
-// 64 of float16, 114 to 140 us. Single precision (products alone: 154 TFLOP/s) 4,000 tokens of 12 heads of 128 on 4, 535 us, 92
-// TFLOP/s. The same in bfloat16 by head size: 128 116 us, 192 200, 256 290; rows of odd sizes, which no copy into LDS takes, 111
-// 270 us. Values loaded only after the first products: 1,009 us where 831 was then; pages looked up by branches within the
-// loads: 966.
+// Measured (bfloat16, 32 heads on 8 of 128; products alone reach 1,227 TFLOP/s): a prompt of 8,192 tokens 815 to 840 us,
+// 655 to 675 TFLOP/s, and half as many products more for the weights (one at a time, traced: 896); the matrix units are busy 41
+// percent of the time, the vector units 43. 512 capped tokens behind 65,536 positions 1,125 to 1,140 with 12 for the join: matrix
+// units 28 percent, vector units 54. Seven prompts of up to 2,000 tokens, 16 leaning heads of
+// 64 of float16, 125 to 131 us. Single precision (products alone: 154 TFLOP/s) 4,000 tokens of 12 heads of 128 on 4, 815 us, 60
+// TFLOP/s, on 0.7 of the chip's places. The same in bfloat16 by head size: 128 148 us, 192 217, 256 318; rows of odd sizes, which no
+// copy into LDS takes, 111 466 us. With weights of one element: values loaded only after the first products 1,009 us where 831 was
+// then; pages looked up by branches within the loads 966.
 #pragma once
 
 #include "../kernels/lanes.hpp"
@@ -81,33 +82,32 @@ struct row_tile {
 
 __device__ __forceinline__ int64_t clamped(int64_t x, int64_t hi) { return x < 0 ? 0 : x > hi ? hi : x; }
 
-/** Where a workgroup is in the launch: a tile's number, those that see most first; a piece of its positions, of `splits` at most. */
-struct dealt {
-  int64_t index;
+/** A piece of a tile's positions: which, and of how many at most. */
+struct piece_of {
   int32_t split, splits;
 };
 
-/** That of number `place` in a call of `tiles` tiles, which fill the chip once with the splits. Of every split (WHOLE: of none). */
-template <bool WHOLE>
-__device__ __forceinline__ dealt deal(prompt_args const& a, prompt_plan const& plan, int64_t place, int tiles)
+/** Splits of `tiles` equal tiles per key head, which are to fill the chip once. */
+__device__ __forceinline__ int splits_alone(prompt_args const& a, prompt_plan const& plan, int tiles)
 {
   const int64_t blocks = int64_t(max(1, tiles)) * a.kv_heads;
-  const int splits     = 2 * blocks > plan.places ? 1 : min(plan.splits, plan.places / int(blocks));
-  if (WHOLE || splits == 1) { return {place, 0, splits}; }
-  const uint32_t index = uint32_t(place) / uint32_t(splits);
-  return {int64_t(index), int32_t(uint32_t(place) - index * splits), splits};
+  return 2 * blocks > plan.places ? 1 : min(plan.splits, plan.places / int(blocks));
 }
 
 /**
- * The tile at a place of the launch; false where there is none. 2 to 64
- * sequences: by the number of row tiles that end no later (a tile's rows, and those of the sequence before them). One, or more than
- * 64, from the last tile on; of more than 64 either each thread counts the tiles of some, or, where nothing is split and the number
- * of tiles does not matter, sequence s has the indexes from floor(first[s] group / kRows) + min(s, first[s]) on, of which
- * the first ceil(rows / kRows) are its tiles and the next sequence's begin behind them.
- * Measured, seven prompts of up to 2,000 tokens, 16 heads of 64: 161 us by sequence, 127 by length.
+ * The tile at a place of the launch, and its piece (WHOLE: all of it, of the tiles that are split); false where there is none.
+ * - One sequence: from the last tile on, a tile's pieces side by side.
+ * - Several, where something may be split (few tokens): pieces of equal length, of which the chip holds one each. The positions that
+ *   the tiles see are counted (a sequence's tiles as its last one); a sequence's tiles are split as often as its length is a multiple
+ *   of that share, to the nearest. (Split alike: one piece of 128 tokens behind 20,000 positions beside 63 sequences of one token and
+ *   2,000 positions, 32 heads on 8 of 128, 719 us for 224.) Up to 64 sequences a lane counts one's pieces, else a thread some.
+ * - 2 to 64, whole: those that see most first, by the number of row tiles that end no later (a tile's rows, and those of the
+ *   sequence before them). Measured, seven prompts of up to 2,000 tokens, 16 heads of 64: 161 us by sequence, 127 by length.
+ * - More, whole: from the last tile on; sequence s has the indexes from floor(first[s] group / kRows) + min(s, first[s]) on, of which
+ *   the first ceil(rows / kRows) are its tiles and the next sequence's begin behind them.
  */
 template <int TILE, bool WHOLE>
-__device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan const& plan, int64_t place, row_tile* out, dealt* as)
+__device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan const& plan, int64_t place, row_tile* out, piece_of* as)
 {
   const int64_t sequences = a.pages.sequences;
   if (sequences == 0) { return false; }  // first has one entry, the lengths none
@@ -117,16 +117,138 @@ __device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan cons
   const auto tiles_for  = [&](int64_t tokens) { return int((tokens * group + kRows - 1) / kRows); };
   const int64_t longest = a.pages.n_pages > 0 ? int64_t(a.pages.width) * a.pages.page : 0;
   int64_t lo = 0, t0, t1, length, at;
-  if (sequences > 1 && sequences <= 64) {
+  if (sequences == 1) {
+    t0 = token(0), t1 = token(1);
+    const int tiles  = tiles_for(max(int64_t(0), t1 - t0));
+    const int splits = uniform(splits_alone(a, plan, tiles));
+    const int index  = int(uint32_t(place) / uint32_t(WHOLE ? 1 : splits));
+    *as              = {uniform(int(place) - index * (WHOLE ? 1 : splits)), splits};
+    at               = tiles - 1 - uniform(index);
+    length           = clamped(a.lengths[0], longest);
+  } else if (plan.splits > 1) {
+    const auto tiles_of = [&](int f0, int f1) { return int((uint32_t(max(0, f1 - f0)) * uint32_t(group) + kRows - 1) / kRows); };
+    const auto seen_by  = [&](int length) {  // tiles of positions, by a sequence's last tile
+      return int((uint32_t(a.window > 0 ? min(int64_t(length), a.window + kRows) : length) + TILE - 1) / TILE);
+    };
+    const auto splits_for = [&](int tiles, int seen, int64_t all_work) {
+      if (seen > 0 && int64_t(tiles) * seen == all_work) { return splits_alone(a, plan, tiles); }  // as without the others
+      const float share = float(plan.places) / (float(max(all_work, int64_t(1))) * float(a.kv_heads));  // places per position
+      return min(plan.splits, max(1, int(float(seen) * share + 0.5f)));
+    };
+    constexpr int kMost = 1 << 22;  // pieces; no more unless first falls
+    // the pieces of tiles that are split go first: the others are shorter
+    bool of_split;
+    int left;  // of this lane's or thread's pieces of that kind, the place's number, if it has that one
+    const auto find = [&](int split, int split_before, int all_split, int single, int single_before, int all) {
+      of_split = place < all_split;
+      left     = int(place) - (of_split ? split_before : all_split + single_before);
+      return place < all && left >= 0 && left < (of_split ? split : single);
+    };
+    int tile, splits;
+    if (sequences <= 64) {  // a lane's sequence
+      const int64_t s  = min(int64_t(lane), sequences - 1);
+      const int f0 = int(token(s)), f1 = int(token(s + 1)), n = int(clamped(a.lengths[s], longest));
+      const int tiles = lane < sequences ? tiles_of(f0, f1) : 0, seen = seen_by(n);
+      splits              = splits_for(tiles, seen, lanes::sum<64>(int64_t(tiles) * seen));
+      const int pieces    = min(WHOLE ? tiles : tiles * splits, kMost);
+      const int split     = splits > 1 ? pieces : 0, single = splits > 1 || WHOLE ? 0 : pieces;
+      const int split_up  = lanes::scan_incl(split), single_up = lanes::scan_incl(single);
+      const int all_split = __builtin_amdgcn_readlane(split_up, 63), all = all_split + __builtin_amdgcn_readlane(single_up, 63);
+      const uint64_t mine = __ballot(find(split, split_up - split, all_split, single, single_up - single, all));
+      if (mine == 0) { return false; }
+      const int from   = __builtin_ctzll(mine);
+      const auto taken = [&](int x) { return __builtin_amdgcn_readlane(x, from); };
+      lo = from, t0 = taken(f0), t1 = taken(f1), length = taken(n);
+      splits = taken(splits), tile = taken(tiles), left = taken(left);
+    } else {
+      // A thread's sequences, which follow one another. (Loops that are not unrolled: the code is run once by each workgroup, so that
+      // fetching it is what counts. Unrolled by 4, 64 sequences of one token and 2,000 positions took 151 us for 130.)
+      __shared__ int64_t s_work[kWaves];
+      __shared__ int s_pieces[2][kWaves], s_found[7];
+      const int wave     = threadIdx.x / 64;
+      const int64_t each = (sequences + kThreads - 1) / kThreads, s0 = min(sequences, threadIdx.x * each);
+      const int64_t s1   = min(sequences, s0 + each);
+      int64_t busy       = s1;  // the first of them that has tokens
+      // f(sequence, its first token and the next one's, its length) of those that have tokens, until that is true
+      const auto each_of = [&](int64_t from, auto f) {
+        int f0 = int(token(from));
+#pragma unroll 1
+        for (int64_t s = from; s < s1; ++s) {
+          const int f1 = int(token(s + 1));
+          if (f1 > f0) {
+            busy = min(busy, s);
+            if (f(s, f0, f1, int(clamped(a.lengths[s], longest)))) { return; }
+          }
+          f0 = f1;
+        }
+      };
+      int64_t work = 0;
+      each_of(s0, [&](int64_t, int f0, int f1, int n) {
+        work += int64_t(tiles_of(f0, f1)) * seen_by(n);
+        return false;
+      });
+      work = lanes::sum<64>(work);
+      if (lane == 0) { s_work[wave] = work; }
+      __syncthreads();
+      int64_t all_work = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) { all_work += s_work[w]; }
+      int split = 0, single = 0;
+      each_of(busy, [&](int64_t, int f0, int f1, int n) {
+        const int tiles = tiles_of(f0, f1), many = splits_for(tiles, seen_by(n), all_work);
+        (many > 1 ? split : single) += WHOLE ? tiles : tiles * many;
+        return false;
+      });
+      split              = min(max(0, split), kMost);
+      single             = WHOLE ? 0 : min(max(0, single), kMost);
+      const int split_up = lanes::scan_incl(split), single_up = lanes::scan_incl(single);
+      if (lane == 63) {
+        s_pieces[0][wave] = split_up;
+        s_pieces[1][wave] = single_up;
+      }
+      __syncthreads();
+      int split_before = split_up - split, single_before = single_up - single, all_split = 0, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        split_before += w < wave ? s_pieces[0][w] : 0;
+        single_before += w < wave ? s_pieces[1][w] : 0;
+        all_split += s_pieces[0][w];
+        all += s_pieces[0][w] + s_pieces[1][w];
+      }
+      if (place >= uniform(all)) { return false; }
+      if (find(split, split_before, all_split, single, single_before, all)) {
+        each_of(busy, [&](int64_t s, int f0, int f1, int n) {
+          const int tiles = tiles_of(f0, f1), many = splits_for(tiles, seen_by(n), all_work), pieces = WHOLE ? tiles : tiles * many;
+          if ((many > 1) != of_split) { return false; }
+          if (left >= pieces) {
+            left -= pieces;
+            return false;
+          }
+          s_found[0] = int(s);
+          s_found[1] = left;
+          s_found[2] = many;
+          s_found[3] = tiles;
+          s_found[4] = f0;
+          s_found[5] = f1;
+          s_found[6] = n;
+          return true;
+        });
+      }
+      __syncthreads();
+      lo = uniform(s_found[0]), left = uniform(s_found[1]), splits = uniform(s_found[2]), tile = uniform(s_found[3]);
+      t0 = uniform(s_found[4]), t1 = uniform(s_found[5]), length = uniform(s_found[6]);
+    }
+    const int index = WHOLE ? left : int(uint32_t(left) / uint32_t(splits));
+    *as             = {WHOLE ? 0 : uniform(left - index * splits), uniform(splits)};
+    at              = tile - 1 - uniform(index);
+  } else if (sequences > 1 && sequences <= 64) {
     // this lane's sequence: `tiles` row tiles, of the costs behind + 1 to behind + tiles
     const int64_t s  = min(int64_t(lane), sequences - 1);
     const int64_t f0 = token(s), f1 = max(f0, token(s + 1)), n = clamped(a.lengths[s], longest);
     const int tiles  = lane < sequences ? tiles_for(f1 - f0) : 0;
     const int behind = int(min(max(int64_t(0), n - (f1 - f0)) * group / kRows, int64_t(1) << 28));  // beyond, all alike
-    *as              = deal<WHOLE>(a, plan, place, plan.splits > 1 ? uniform(lanes::sum<64>(tiles)) : 0);
-    as->splits       = uniform(as->splits);
-    as->split        = uniform(as->split);
-    const int64_t index = uniform(as->index);
+    *as              = {0, 1};
+    const int64_t index = place;
     // the largest cost that more than `index` tiles have or exceed
     const auto reach = [&](int cost) { return lanes::sum<64>(min(max(behind + tiles - cost + 1, 0), tiles)); };
     int some = 0, none = uniform(lanes::max<64>(behind + tiles)) + 1;  // 1 and more, if any has
@@ -151,64 +273,8 @@ __device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan cons
     };
     lo = from, t0 = take(f0), t1 = take(f1), length = take(n);
     at = some - __builtin_amdgcn_readlane(behind, from) - 1;
-  } else if (sequences > 1 && plan.splits > 1) {
-    // a thread's sequences, which follow one another, and the tiles before them
-    __shared__ int s_tiles[kWaves], s_found[2];
-    const int64_t each = (sequences + kThreads - 1) / kThreads, s0 = min(sequences, threadIdx.x * each);
-    const int64_t s1   = min(sequences, s0 + each);
-    int tiles          = 0;
-    int64_t f0         = token(s0);
-#pragma unroll 4
-    for (int64_t s = s0; s < s1; ++s) {
-      const int64_t f1 = token(s + 1);
-      tiles += tiles_for(max(int64_t(0), f1 - f0));
-      f0 = f1;
-    }
-    tiles          = min(max(0, tiles), 1 << 22);  // no more unless first falls
-    const int incl = lanes::scan_incl(tiles);
-    if (lane == 63) { s_tiles[threadIdx.x / 64] = incl; }
-    __syncthreads();
-    int before = incl - tiles, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      before += w < int(threadIdx.x / 64) ? s_tiles[w] : 0;
-      all += s_tiles[w];
-    }
-    all = uniform(all);
-    *as = deal<WHOLE>(a, plan, place, all);
-    as->splits = uniform(as->splits);
-    as->split  = uniform(as->split);
-    if (as->index >= all) { return false; }
-    int left = all - 1 - int(as->index) - before;  // this thread's tile, if it has that one
-    if (left >= 0 && left < tiles) {
-      f0 = token(s0);
-      for (int64_t s = s0; s < s1; ++s) {
-        const int64_t f1 = token(s + 1);
-        const int n      = tiles_for(max(int64_t(0), f1 - f0));
-        if (left < n) {
-          s_found[0] = int(s);
-          s_found[1] = left;
-          break;
-        }
-        left -= n;
-        f0 = f1;
-      }
-    }
-    __syncthreads();
-    lo = uniform(s_found[0]);
-    t0 = token(lo), t1 = token(lo + 1);
-    at     = uniform(s_found[1]);
-    length = clamped(a.lengths[lo], longest);
-  } else if (sequences == 1) {
-    t0 = token(0), t1 = token(1);
-    const int tiles = tiles_for(max(int64_t(0), t1 - t0));
-    *as             = deal<WHOLE>(a, plan, place, tiles);
-    as->splits      = uniform(as->splits);
-    as->split       = uniform(as->split);
-    at              = tiles - 1 - uniform(as->index);
-    length          = clamped(a.lengths[0], longest);
   } else {
-    *as                 = {place, 0, 1};
+    *as                 = {0, 1};
     const int64_t index = plan.tiles - 1 - place;
     const auto begins   = [&](int64_t s) {
       const int64_t f = token(s);
@@ -243,7 +309,7 @@ __device__ __forceinline__ bool find_tile(prompt_args const& a, prompt_plan cons
 }
 
 /** The splits of a tile. */
-__device__ __forceinline__ int splits_of(dealt const& as, int tiles) { return max(1, min(as.splits, tiles / kLeast)); }
+__device__ __forceinline__ int splits_of(piece_of const& as, int tiles) { return max(1, min(as.splits, tiles / kLeast)); }
 
 __device__ __forceinline__ f32x16 mfma32(f16_t, u32x4 a, u32x4 b, f32x16 c)
 {
@@ -393,7 +459,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
     }
   }
   row_tile rt;
-  dealt as;
+  piece_of as;
   if (!find_tile<TILE, false>(a, plan, blockIdx.x / a.kv_heads, &rt, &as)) { return; }
   const int splits = splits_of(as, rt.tiles), split = as.split;
   if (split >= splits) { return; }
@@ -461,7 +527,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
   constexpr int kStep  = std::min(8, kDown);
   // (rows of a thread are 8 apart, or 4: then the second is exchanged otherwise)
   const int64_t k_lane = int64_t(tid / kAcross % kStep) * a.k_slot;
-  const auto piece_of  = [&](int n) { return COPIED ? k_piece ^ ((n * kDown + tid / kAcross) % 8) : k_piece; };
+  const auto key_piece = [&](int n) { return COPIED ? k_piece ^ ((n * kDown + tid / kAcross) % 8) : k_piece; };
   const int64_t v_lane = 4 * half * a.v_slot + v_col;
 
   words<T, kPiece> k_next[COPIED ? 1 : kPasses];
@@ -474,7 +540,7 @@ __global__ __launch_bounds__(kThreads, (kPerUnit<T, D>)) void prompt_kernel(prom
       // a wave's rows of a pass are in one group
       const int first = n * kDown + wave * (kDown / kWaves);
       const T* from   = k_head + of_group(at.k, first / 8) + int64_t(n * kDown % 8) * a.k_slot;
-      const int piece = piece_of(n);
+      const int piece = key_piece(n);
       if ((FULL && kPieces == kAcross) || piece < (COPIED ? dim / kPiece : kPieces)) {
         if constexpr (COPIED) {
           copy_to_lds(from + k_lane + piece * kPiece, lds_address(&s_k[buffer][first * kRowBytes]));
@@ -803,7 +869,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(prompt_args a, prompt_pl
   __shared__ float s_factor[kJoinRows][kMaxSplits], s_sum[kJoinRows][kMaxSplits];
   const int kv = blockIdx.x % a.kv_heads, r = threadIdx.x / 32, lane = threadIdx.x % 32;
   row_tile rt;
-  dealt as;
+  piece_of as;
   if (!find_tile<kTile<T>, true>(a, plan, blockIdx.x / a.kv_heads, &rt, &as)) { return; }
   const int n   = splits_of(as, rt.tiles);
   const int row = rt.row0 + blockIdx.y * kJoinRows + r;
@@ -840,12 +906,12 @@ int64_t tiles_of(prompt_args const& a)
   return std::max<int64_t>(1, a.tokens * (a.heads / a.kv_heads) / kRows + std::min(a.tokens, a.pages.sequences));
 }
 
-/** Splits of a tile's positions, at most: those of one sequence that has all tokens. The kernels count the tiles that there are, and
- *  take as many splits as the chip holds at once where the tiles alone are fewer (deal). One more, which takes a second
- *  round, costs most: bfloat16, 32 heads on 8 of 128, 1,500 tokens 78 us where 58 is now; only prompts whose rows see unequally much
- *  and fill 2.7 places had less, 152 for 187 us. Pieces of up to 20 tokens behind up to 8,000 positions of 16 sequences, 104 us, take
- *  115 where splits go by the tokens alone, 64 of one token behind 16,383 positions 817 and 1,074; 16 tokens behind 16,000 in a
- *  table of 64 rows, 59, take 213 where a row counts as a tile. */
+/** Splits of a tile's positions, at most: those of one sequence that has all tokens. The kernels count what the tiles see, and take
+ *  as many splits as the chip holds at once (find_tile). One more, which takes a second
+ *  round, costs most: bfloat16, 32 heads on 8 of 128, 1,500 tokens 80 us where 65 is now. Long prompts whose rows see unequally much and
+ *  that fill some three quarters of the places would have less: 4,000 tokens, 12 heads on 4 of 128, 125 us for 148, of 111 275 for
+ *  466, float32 526 for 815. 64 sequences of one token behind 16,383 positions, 813 us, took 1,074 where splits went by the tokens
+ *  alone; 16 tokens behind 16,000 in a table of 64 rows, 60, took 213 where a row counted as a tile. */
 int splits_for(prompt_args const& a, int tile, int per_unit)
 {
   const int64_t most   = int64_t(a.pages.width) * a.pages.page;
@@ -879,18 +945,17 @@ void launch(prompt_args const& a, hipStream_t stream)
     plan.part_out       = static_cast<float*>(a.workspace);
     plan.part_max       = plan.part_out + slots * a.vdim;
     plan.part_sum       = plan.part_max + slots;
-    // a workgroup per tile, or per split of fewer tiles, which are no more than the chip has places
+    // a workgroup per piece: to the nearest, they are as many as the chip's places and the tiles at most
     const int64_t blocks = int64_t(plan.tiles) * a.kv_heads;
-    const dim3 grid(uint32_t(std::max(blocks, std::min<int64_t>(plan.places, blocks * plan.splits))),
-                    (a.vdim + kColumns<T, D> - 1) / kColumns<T, D>);
+    const dim3 grid(uint32_t(std::min(blocks * plan.splits, blocks + plan.places)), (a.vdim + kColumns<T, D> - 1) / kColumns<T, D>);
     if (a.shape.any()) {
       prompt_kernel<T, D, decltype(how)::value, true><<<grid, kThreads, 0, stream>>>(a, plan);
     } else {
       prompt_kernel<T, D, decltype(how)::value, false><<<grid, kThreads, 0, stream>>>(a, plan);
     }
     if (plan.splits > 1) {
-      // tiles that are split take two places at least
-      const int64_t split = std::min<int64_t>(plan.tiles, plan.places / (2 * a.kv_heads));
+      // tiles that are split see 1.5 places' share of the positions at least
+      const int64_t split = std::min<int64_t>(plan.tiles, plan.places * 2 / (3 * a.kv_heads) + 1);
       join_kernel<T><<<dim3(uint32_t(split) * a.kv_heads, kRows / kJoinRows), kThreads, 0, stream>>>(a, plan);
     }
   };

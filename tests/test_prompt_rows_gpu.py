@@ -132,3 +132,20 @@ def test_weights_enter_whole(gpu, dtype, d, n, past):
     out, lse = certex.prompt_attention(q, kp, vp, table, ints([past + n]), ints([0, n]), slopes=slopes, return_lse=True)
     weight = 0.0 if dtype == torch.float32 else weight_unit(dtype) ** 2
     ref.check(out, lse, ref.attend(q, torch.arange(past, past + n), keys[0], values[0], d**-0.5, slopes=slopes, weight=weight))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [8, 64, 70, 300])
+def test_prompts_beside_single_tokens(gpu, dtype, rows):
+    """A piece of a prompt behind a long cache beside single tokens of short ones: the long one alone is split. Lengths of 0 and below the
+    tokens among them, and calls of nothing else."""
+    g = torch.Generator().manual_seed(78)
+    news = [70, 1, 1, 1, 0, 1, 1, 1] + [int(torch.randint(0, 2, (1,), generator=g)) for _ in range(rows - 8)]
+    pasts = [6_000, 100, 40, 0, 9, 300, 2_000, 5] + [int(torch.randint(0, 90, (1,), generator=g)) for _ in range(rows - 8)]
+    check_prompt(news, pasts, 4, 1, 64, 64, 16, dtype, seed=79)
+    kp, vp, table, *_ = paged([200] * rows, 16, 1, 64, 64, dtype, seed=80)
+    q, first = rand(2 * rows, 4, 64, dtype=dtype), ints([2 * i for i in range(rows + 1)])
+    out, lse = certex.prompt_attention(q, kp, vp, table, ints([0] * rows), first, return_lse=True)
+    assert (out == 0).all() and (lse == float("-inf")).all()
+    out, lse = certex.prompt_attention(q, kp, vp, table, ints([1, 200] * (rows // 2)), first, return_lse=True)
+    assert (out[0::4] == 0).all() and (lse[0::4] == float("-inf")).all() and lse[1::4].isfinite().all() and lse[2::4].isfinite().all()
