@@ -2,12 +2,14 @@
 //
 // out = sum_t p_t v_t / sum_t p_t with p_t = 2^(log2(e) (x_t - m)); with scales s, offsets o and codes n per group of 64 dimensions
 //   q.k_t = sum_group s_t (sum_d q_d n_td) + o_t (sum_d q_d),    sum_t p_t v_td = sum_t (p_t s_t) n_td + sum_t p_t o_t.
-// The sums over codes go to the matrix cores as float16 products: a code n in the low bits of a halfword is the subnormal
-// float16 n 2^-24, four bits higher 16 n 2^-24, which the products take exactly. So two codes become two operands by one
-// AND (and every other one a shift), nothing is converted, and the powers of two are taken back where sums are used.
+// The sums over codes go to the matrix cores as float16 products: a code n in bits 4 to 7 of a halfword is the subnormal
+// float16 n 2^-20. So two codes become operands by an AND (and three of four a shift), nothing is converted, and the power of two is
+// taken back where sums are used.
 //
-// What bounds it: 144 bytes of a position and head of 128 (codes 128, scales and offsets 16), read once; in the kernel as it is
-// the vector operations that open the codes and weigh the scales, about 240 per 32 positions and wave.
+// What bounds it: 144 bytes of a position and head of 128 (codes 128, scales and offsets 16), read once. In the kernel as it is
+// no unit is full: for 32 positions a wave has some 420 vector instructions (float32 queries 620), which take 54 percent of the vector
+// units' time (57), the matrix units are busy 13 percent (15), memory is read at 0.64 of its rate. The 3 waves of a SIMD (2) wait 35
+// percent of theirs (30) for LDS and memory, and registers hold no more.
 //
 // The shape of the products is that of attend.hip: a wave takes 32 positions, 8 to a lane group, and holds of each product's result
 // the positions that it feeds to the next. A record holds 8 positions of a head, so that a lane group's codes, scales and
@@ -15,18 +17,19 @@
 // - Queries enter as float16, scaled by a power of two that brings a row's largest to [2^13, 2^14): 16-bit types whole
 //   (what is 2^-28 of the largest loses bits, none that float32 sums would keep), float32 as three elements of 11 bits.
 // - p_t s_t enters as two elements of 11 bits, the nearest float16 and what it leaves: 2^-21 of it off at most. (One element
-//   would be 2^-11 off, as much as float16 outputs are rounded; 64 sequences 68 us instead of 75.) p's reference is
+//   would be 2^-11 off, as much as float16 outputs are rounded; 64 sequences 57 us instead of 63.) p's reference is
 //   kept such that the largest is below 2^15. Their sum is not rounded. The elements reach down to 2^-24, so that positions and
 //   groups keep these bits while their p_t s_t are within 2^17 of the largest, and lose one with each power of 2 below.
-// - Products of subnormal numbers keep fewer of their low bits beside large sums, so that float32 takes other
+// - Products of subnormal numbers keep fewer of their low bits beside large sums, the fewer the smaller they are: codes in bits 0 to
+//   3, as n 2^-24, were 2e-6 to 5e-6 of the values off (64 sequences 63 us instead of 65). float32 takes other
 //   codes: less 8, as normal numbers (two operations more each), whose sums stay small; and joins steps outside the products.
 // Work is dealt as in attend.hip (shares.hpp). A wave copies its next step to LDS while it works on one, by itself: what it
 // copies it alone reads, so that steps need no barrier.
 //
-// Measured (8 key heads of 128, 32 query heads): 64 sequences up to 8,192 of bfloat16 queries, 0.26 GB of records: 57 to 61 us
-// and 6 for the join, 4.3 to 4.6 TB/s;
-// one sequence of 131,072, float32 queries, 0.15 GB: 53 us and 6, 7e-7 off (subnormal codes: 2e-6 to 5e-6); 77 positions
-// 8.6 us, launch and five dependent loads.
+// Measured (8 key heads of 128, 32 query heads): 64 sequences up to 8,192 of bfloat16 queries, 0.26 GB of records: 65 us
+// and 6 for the join, 4.0 TB/s; a call 73 us, capped 85, leaning 75;
+// one sequence of 131,072, float32 queries, 0.15 GB: 53 us and 6, 7e-7 off; 77 positions
+// 8.7 us, launch and five dependent loads.
 #include "scores.hpp"
 #include "shares.hpp"
 #include "tiles.hpp"
@@ -93,6 +96,10 @@ __device__ __forceinline__ float half_of(uint32_t w, int i)
 {
   return float(__builtin_bit_cast(f16x2, w)[i]);
 }
+
+/** The codes in bits 4 to 7 of a word's halves as float16 of kCode each, subnormal: no conversion. */
+constexpr float kCode = 0x1p-20f;
+__device__ __forceinline__ uint32_t opened(uint32_t w) { return w & 0x00f000f0u; }
 
 /** The codes in the low 4 bits of a word's halves, less 8, as float16: 1024 + code is the number with the code in its last bits. */
 __device__ __forceinline__ uint32_t less_eight(uint32_t w)
@@ -290,9 +297,7 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          // codes that are 16 times themselves
           float lo = e[c][2 * w], hi = e[c][2 * w + 1];
-          if (!FINE && w % 2 == 1) { lo *= 0.0625f, hi *= 0.0625f; }
 #pragma unroll
           for (int i = 0; i < P; ++i) {
             q[c][i][w] = pack2<f16_t>(lo, hi);
@@ -303,8 +308,8 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
       }
       const auto plus = [](float u, float w) { return u + w; };
 #pragma unroll
-      for (int n = 0; n < G; ++n) { q_sum[n] = lanes::fold16(lanes::fold32(q_sum[n], plus), plus) * (FINE ? 1.0f : 0x1p-24f); }
-      exponent += FINE ? 0 : 24;
+      for (int n = 0; n < G; ++n) { q_sum[n] = lanes::fold16(lanes::fold32(q_sum[n], plus), plus) * (FINE ? 1.0f : kCode); }
+      exponent += FINE ? 0 : 20;  // what kCode takes
     }
     f32x4 o[C][2];   // tiles of 16 columns: chunk c of V's units, even and odd dimensions of a pair
     float shift[G];  // sum of p times the offsets, of this lane's positions
@@ -342,9 +347,9 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
           k, FULL ? rows_ + (half * 4 + r % 4) * 16 * C + g * 4 * C : rows_ + (half * 4 + r % 4) * 16 * k_chunks + g * 4 * k_chunks);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const uint32_t w = k[c], up = w >> 8;
-          u32x4 codes{w & 0x000f000fu, w & 0x00f000f0u, up & 0x000f000fu, up & 0x00f000f0u};
-          if (FINE) { codes = {less_eight(w), less_eight(w >> 4), less_eight(up), less_eight(w >> 12)}; }
+          const uint32_t w = k[c];
+          const u32x4 codes = FINE ? u32x4{less_eight(w), less_eight(w >> 4), less_eight(w >> 8), less_eight(w >> 12)}
+                                   : u32x4{opened(w << 4), opened(w), opened(w >> 4), opened(w >> 8)};
 #pragma unroll
           for (int i = P - 1; i >= 0; --i) { s[half][c / 2] = mfma(f16_t{}, codes, q[c][i], s[half][c / 2]); }
         }
@@ -483,16 +488,16 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
         }
 #pragma unroll
         for (int c = 2 * n; c < 2 * n + 2 && c < C; ++c) {
-          const uint32_t w0 = v[c % 2 * 2], w1 = v[c % 2 * 2 + 1], up0 = w0 >> 8, up1 = w1 >> 8;
-          u32x4 even{w0 & 0x000f000fu, up0 & 0x000f000fu, w1 & 0x000f000fu, up1 & 0x000f000fu};
-          u32x4 odd{w0 & 0x00f000f0u, up0 & 0x00f000f0u, w1 & 0x00f000f0u, up1 & 0x00f000f0u};
+          const uint32_t w0 = v[c % 2 * 2], w1 = v[c % 2 * 2 + 1];
           if (FINE) {
-            even = {less_eight(w0), less_eight(up0), less_eight(w1), less_eight(up1)};
-            odd  = {less_eight(w0 >> 4), less_eight(w0 >> 12), less_eight(w1 >> 4), less_eight(w1 >> 12)};
+            const u32x4 even{less_eight(w0), less_eight(w0 >> 8), less_eight(w1), less_eight(w1 >> 8)};
+            const u32x4 odd{less_eight(w0 >> 4), less_eight(w0 >> 12), less_eight(w1 >> 4), less_eight(w1 >> 12)};
             const f32x4 zero{0, 0, 0, 0};
             o[c][0] += mfma(f16_t{}, even, part[0], mfma(f16_t{}, even, part[1], zero));
             o[c][1] += mfma(f16_t{}, odd, part[0], mfma(f16_t{}, odd, part[1], zero));
           } else {
+            const u32x4 even{opened(w0 << 4), opened(w0 >> 4), opened(w1 << 4), opened(w1 >> 4)};
+            const u32x4 odd{opened(w0), opened(w0 >> 8), opened(w1), opened(w1 >> 8)};
             o[c][0] = mfma(f16_t{}, even, part[0], mfma(f16_t{}, even, part[1], o[c][0]));
             o[c][1] = mfma(f16_t{}, odd, part[0], mfma(f16_t{}, odd, part[1], o[c][1]));
           }
@@ -523,7 +528,7 @@ __global__ __launch_bounds__(kThreads, per_unit(C, FULL, P)) void packed_kernel(
           for (int i = 0; i < 4; ++i) {
             const int row = g * 4 + i, col = unit * 64 + (pair ? row * 4 + c % 2 * 2 : row * 2) + e;
             if ((pair || c % 2 == 0) && col < vdim) {
-              out[r * D + col] = __builtin_amdgcn_ldexpf(o[c][e][i], (FINE ? 0 : 24 - 4 * e) - lift) + shift[unit];
+              out[r * D + col] = __builtin_amdgcn_ldexpf(o[c][e][i], (FINE ? 0 : 20) - lift) + shift[unit];
             }
           }
         }

@@ -90,3 +90,22 @@ def test_weights_enter_whole(gpu, dtype, d, n):
     (keys, key_sizes), (values, value_sizes) = pack.stored(k), pack.stored(v)
     ref.check(out, lse, ref.attend(q, torch.tensor([n - 1]), keys, values, d**-0.5, weight=2.0**-21 + 2.0**-24, key_sizes=key_sizes,
                                    value_sizes=value_sizes, slopes=slopes))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 96, 128, 192, 256, 80])
+def test_scores_are_float32_sums(gpu, dtype, d):
+    """Scores, which the float32 logarithms show where a sequence has one position, are off as float32 sums of their terms in any order
+    are, as random roundings: u sum |scale q k| / sqrt(d) in the mean over dimensions and 8 u of the terms' own, 4 times that at most, and
+    8 u of the logarithm itself. Products of codes as numbers of 4 bits only would keep no such sums."""
+    heads = 64
+    k, v, q = rand(1, 1, d, dtype=dtype), rand(1, 1, d, dtype=dtype, seed=1), rand(1, heads, d, dtype=dtype, seed=2)
+    pages = certex.PackedPages(1, 8, 1, d)
+    table, zero = ints([[0]]), ints([0])
+    pages.append(k, v, table, zero)
+    lse = pages.attend(q, table, ints([1]), return_lse=True)[1]
+    held, sizes = pack.stored(k)
+    want = (q[0].double().cpu() @ held[0, 0]) * d**-0.5
+    size = float((q[0].double().cpu().abs() @ sizes[0, 0]).max()) * d**-0.5
+    u = 2.0**-24
+    assert float((lse[0].double().cpu() - want).abs().max()) <= 4 * (size / d**0.5 + 8) * u + 8 * u * float(want.abs().max())
