@@ -8,7 +8,7 @@
 //
 // What bounds it: 144 bytes of a position and head of 128 (codes 128, scales and offsets 16), read once. In the kernel as it is
 // no unit is full: for 32 positions a wave has some 420 vector instructions (float32 queries 620), which take 54 percent of the vector
-// units' time (57), the matrix units are busy 13 percent (15), memory is read at 0.64 of its rate. The 3 waves of a SIMD (2) wait 35
+// units' time (57), the matrix units are busy 13 percent (15), memory is read at 0.62 of its rate. The 3 waves of a SIMD (2) wait 33
 // percent of theirs (30) for LDS and memory, and registers hold no more.
 //
 // The shape of the products is that of attend.hip: a wave takes 32 positions, 8 to a lane group, and holds of each product's result
