@@ -238,7 +238,9 @@ CUVS_EXPORT cuvsError_t cuvsCertexUnpackPages(cuvsResources_t res,
 
 /**
  * cuvsCertexPagedAttentionShaped over such pages, of heads of vdim elements of values. q: rows [n_sequences, heads, dim] of any element
- * type, which is also that of out, dense [n_sequences, heads, vdim]. The workspace is that of
+ * type, which is also that of out, dense [n_sequences, heads, vdim]. A weight is off by 2^-21 of itself at most, or by 2^-37 r
+ * of the largest weight, if that is more: r is the quotient of the largest scale of the head's values so far and the scale of these 64
+ * elements. Values that are 2^14 times smaller than others of their head keep float32's precision, 2^26 times smaller ones float16's. The workspace is that of
  * cuvsCertexPackedAttentionWorkspace.
  */
 CUVS_EXPORT cuvsError_t cuvsCertexPackedAttention(cuvsResources_t res,

@@ -18,8 +18,8 @@
 //   (what is 2^-28 of the largest loses bits, none that float32 sums would keep), float32 as three elements of 11 bits.
 // - p_t s_t enters as two elements of 11 bits, the nearest float16 and what it leaves: 2^-21 of it off at most. (One element
 //   would be 2^-11 off, as much as float16 outputs are rounded; 64 sequences 57 us instead of 63.) p's reference is
-//   kept such that the largest is below 2^15. Their sum is not rounded. The elements reach down to 2^-24, so that positions and
-//   groups keep these bits while their p_t s_t are within 2^17 of the largest, and lose one with each power of 2 below.
+//   kept such that the largest is below 2^15. Their sum is not rounded. The elements reach down to 2^-24: positions and
+//   groups lose bits, one for each power of 2, whose p_t s_t are below 2^-16 of what the largest scale so far makes the largest.
 // - Products of subnormal numbers keep fewer of their low bits beside large sums, the fewer the smaller they are: codes in bits 0 to
 //   3, as n 2^-24, were 2e-6 to 5e-6 of the values off (64 sequences 63 us instead of 65). float32 takes other
 //   codes: less 8, as normal numbers (two operations more each), whose sums stay small; and joins steps outside the products.

@@ -109,3 +109,24 @@ def test_scores_are_float32_sums(gpu, dtype, d):
     size = float((q[0].double().cpu().abs() @ sizes[0, 0]).max()) * d**-0.5
     u = 2.0**-24
     assert float((lse[0].double().cpu() - want).abs().max()) <= 4 * (size / d**0.5 + 8) * u + 8 * u * float(want.abs().max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [128, 192, 256, 96])
+@pytest.mark.parametrize("high, low", [(1.0, 2.0**-10), (2.0**-10, 1.0), (2.0**12, 2.0**-8), (2.0**-8, 2.0**12)])
+def test_groups_of_different_sizes(gpu, dtype, d, high, low):
+    """Values of one group of 64 elements are as precise as if the others were not there, though those are up to 2^20 times as large: as in
+    test_weights_enter_whole, for each group by itself."""
+    n, heads = 40, 32
+    k, v = rand(n, 2, d, dtype=dtype), rand(n, 2, d, dtype=dtype, seed=1)
+    for group in range(-(-d // 64)):
+        v[..., 64 * group : 64 * group + 64] *= high if group % 2 == 0 else low
+    q, slopes = torch.zeros(1, heads, d, dtype=dtype, device="cuda"), torch.linspace(0.001, 0.1, heads, device="cuda")
+    pages = certex.PackedPages(-(-n // 16), 16, 2, d)
+    table = torch.arange(-(-n // 16), dtype=torch.int32, device="cuda").flip(0)[None]
+    positions = torch.arange(n, device="cuda")
+    pages.append(k, v, table, positions, sequences=torch.zeros_like(positions))
+    out, lse = pages.attend(q, table, ints([n]), return_lse=True, slopes=slopes)
+    (keys, key_sizes), (values, value_sizes) = pack.stored(k), pack.stored(v)
+    ref.check(out, lse, ref.attend(q, torch.tensor([n - 1]), keys, values, d**-0.5, weight=2.0**-21 + 2.0**-24, key_sizes=key_sizes,
+                                   value_sizes=value_sizes, slopes=slopes))
