@@ -191,8 +191,8 @@ class PackedPages:
 
     def attend(self, q, page_table, lengths, scale=None, window=None, return_lse=False, cap=None, slopes=None):
         """As paged_attention: q (n_sequences, n_heads, head_dim) of any element type gives (n_sequences, n_heads, value_dim)
-        of the same. Groups of 64 values that are
-        more than 2^14 times smaller than others of their head lose precision: at 2^26 float16's is left."""
+        of the same. Groups of 64 values that are more than 2^14 times smaller than others of their head lose precision: at 2^26
+        float16's is left."""
         return C.operators().attend_packed(self.head_dim, self.value_dim, q, self.data, page_table, lengths, scale, window, cap,
                                            slopes, return_lse)
 
